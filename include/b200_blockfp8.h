@@ -431,6 +431,40 @@ int b200_moe_sum_reduce(const void* rows, const int32_t* topk_ids, void* out, in
                         int topk, int E, int64_t H, float scale, int skip_unrouted,
                         int poison_on_status, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * 8-bit rows with scales from what precedes a quantised linear, in one pass over the rows.
+ *
+ * b200_rmsnorm_quant: h = x (+ residual), y = h * weight / sqrt(mean(h^2) + eps) in fp32, never rounded to 16 bits;
+ *   residual_out [M,H] = h rounded to the input type (NULL without residual). The sum is normalised unrounded.
+ *   replaces: the pair fused_add_rmsnorm / rmsnorm (python/sglang/srt/layers/layernorm.py) -> quantiser of the linear.
+ * b200_per_token_quant_int8: y = x, or with fuse_silu_and_mul y = silu(gate) * up in fp32 of rows [gate | up] (x is [M,2K]).
+ *   replaces: python/sglang/srt/layers/quantization/int8_kernel.py (per_token_quant_int8), with silu_and_mul before it.
+ * x and residual: rows x_ld / residual_ld elements apart, elements of a row contiguous, of `dtype` like weight [H].
+ * kind, with amax floored at 1e-10:
+ *   B200_ROW_INT8       s[m] = amax(row) / 127, q = y / s rounded to the nearest integer, ties to even (s_stride_* unused);
+ *                       a NaN in the row makes s[m] NaN
+ *   B200_ROW_FP8        per 128 columns (H % 128 == 0): s[m*s_stride_m + g*s_stride_g] = amax / 448, q = e4m3(y / s)
+ *   B200_ROW_FP8_UE8M0  the same with s = 2^ceil(log2(amax / 448)), its biased exponent in byte (g % 4) of word
+ *                       [g/4 * s_stride_g + m]; bytes past the last group are written as 0
+ * q [M,H] contiguous, 16-byte aligned for the FP8 kinds. Any H (int8) up to 2^24, any element alignment of x. */
+enum { B200_ROW_INT8 = 0, B200_ROW_FP8 = 1, B200_ROW_FP8_UE8M0 = 2 };
+int b200_rmsnorm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
+                       const void* weight, int dtype, int kind, void* q, void* s, int64_t s_stride_m,
+                       int64_t s_stride_g, void* residual_out, int64_t M, int64_t H, float eps,
+                       void* stream);
+int b200_per_token_quant_int8(const void* x, int64_t x_ld, int dtype, void* q, float* s, int64_t M,
+                              int64_t K, int fuse_silu_and_mul, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * int8_scaled_mm
+ * replaces: torch.ops.sgl_kernel.int8_scaled_mm (sgl-kernel/csrc/gemm/int8_gemm_kernel.cu)
+ * C[m,n] = (sum_k A[m,k]*B[n,k]) * sa[m] * sb[n] (+ bias[n]): exact 32-bit integer sums, then fp32, rounded once.
+ * A [M,K] and B [N,K] signed 8-bit, rows lda / ldb bytes apart; bias [N] of C's type or NULL; C [M,N] contiguous.
+ * Requirements: K, lda and ldb multiples of 16, A, B and C 16-byte aligned, N % 8 == 0, 0 < K <= 131071. No workspace. */
+int b200_int8_scaled_mm(const void* A, int64_t lda, const float* sa, const void* B, int64_t ldb,
+                        const float* sb, const void* bias, void* C, int c_dtype, int64_t M, int64_t N,
+                        int64_t K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

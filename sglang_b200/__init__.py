@@ -29,5 +29,7 @@ from .topk import (  # noqa: F401,E402
     topk_sigmoid,
     topk_softmax,
 )
+from .int8_kernel import int8_scaled_mm, per_token_quant_int8, w8a8_int8_linear  # noqa: F401,E402
+from .layernorm import rmsnorm_quant_fp8, rmsnorm_quant_int8  # noqa: F401,E402
 from . import fp8  # noqa: F401,E402
 from . import custom_ops  # noqa: F401,E402  (registers torch.ops.sglang_b200.*)

@@ -123,6 +123,20 @@ SIGNATURES = {
         [c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
          c_void_p, c_void_p, c_void_p],
     ),
+    "b200_rmsnorm_quant": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+         c_int64, c_int64, c_float, c_void_p],
+    ),
+    "b200_per_token_quant_int8": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p],
+    ),
+    "b200_int8_scaled_mm": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
+         c_void_p],
+    ),
     "b200_route_topk_softmax_capped": (
         c_int,
         [c_void_p, c_int, c_float, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],

@@ -18,7 +18,8 @@ CSRC = os.path.join(PKG, "csrc")
 OUT_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(OUT_DIR, "libb200_blockfp8.so")
 HOST_EXT = os.path.join(OUT_DIR, "_host.so")  # CPython extension: the operators' host path (csrc/host_ext.cpp)
-SOURCES = ["status.cu", "quant.cu", "align.cu", "gemm.cu", "moe.cu", "topk.cu", "comm.cu", "ep.cu"]
+SOURCES = ["status.cu", "quant.cu", "align.cu", "gemm.cu", "moe.cu", "topk.cu", "comm.cu", "ep.cu",
+           "row_quant.cu", "int8_gemm.cu"]
 
 NVCC_FLAGS = [
     "-std=c++17",

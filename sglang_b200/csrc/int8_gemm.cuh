@@ -1,0 +1,205 @@
+// Product of 8-bit integers with a scale per token and per output channel:
+//     C[m, n] = (sum_k A[m, k] * B[n, k]) * sa[m] * sb[n] (+ bias[n])
+// tcgen05.mma kind::i8 adds up in 32-bit integers, exactly, so the sum stays in TMEM for all of K, the order of the additions does
+// not matter, and one pass over it at the end applies both scales: three roundings in fp32 and the last one to the output type.
+#pragma once
+
+#include "gemm_pair.cuh"
+
+namespace b200 {
+
+namespace ptx {
+__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor for kind::i8, signed x signed -> int32 (no saturation), both operands K-major.
+//   bits 4-5 D format (2 = s32)  7-9 A format (1 = signed)  10-12 B format  17-22 N >> 3  24-28 M >> 4
+__host__ __device__ constexpr uint32_t idesc_s8_s32(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+}  // namespace ptx
+
+struct Int8Params {
+  const float *sa, *sb;  // [M], [N]
+  const void* bias;      // [N] of the output's type, or null
+  void* C;               // [M, N], contiguous
+  const int8_t* w;       // B, for prefetches
+  int64_t w_ld;
+  int M, N, num_kb;
+  int n_tiles, t_tiles;
+  int* status;
+};
+
+// The roles of the operands are swapped: 128 rows of B fill the lanes of the tensor-core tile, NT tokens are its columns, so that
+// few tokens waste nothing and a thread of the epilogue owns one output channel.
+template <int NT>
+struct Int8StreamCfg {
+  static constexpr int kStageW = 128 * kBK, kStageX = NT * kBK;
+  static constexpr int kStages = 5;
+  static constexpr int kThreads = 192;  // 4 epilogue warps, producer, MMA issuer
+  static constexpr int kTmemCols = NT < 32 ? 32 : NT;
+  static constexpr size_t kSmemBytes = (size_t)kStages * (kStageW + kStageX) + NT * 4 + 1024 + 256;
+};
+
+template <int NT, typename OutT>
+__global__ void __launch_bounds__(Int8StreamCfg<NT>::kThreads)
+int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8Params p) {
+  using Cfg = Int8StreamCfg<NT>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t sW = smem_base, sX = smem_base + S * Cfg::kStageW;
+  float* sa = reinterpret_cast<float*>(smem_al + (size_t)S * (Cfg::kStageW + Cfg::kStageX));  // [NT]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sa + NT);
+  const uint32_t bar0 = ptx::smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
+  const uint32_t done_bar = bar0 + 8u * 2 * S;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kProducerWarp = 4, kMmaWarp = 5;
+  const int nt = blockIdx.x / p.t_tiles, tt = blockIdx.x - nt * p.t_tiles;
+  const int n0 = nt * 128, m0 = tt * NT;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    ptx::mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    ptx::prefetch_tensormap(&tmap_w);
+    ptx::prefetch_tensormap(&tmap_x);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_wait();
+
+  if (warp == kProducerWarp) {
+    if (ptx::elect_one()) {
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        const int s = kb % S;
+        if (!ptx::mbar_wait(empty_bar(s), ((kb / S) & 1) ^ 1, abort_flag)) break;
+        ptx::mbar_expect_tx(full_bar(s), Cfg::kStageW + Cfg::kStageX);
+        ptx::tma_load_2d(sW + s * Cfg::kStageW, &tmap_w, kb * kBK, n0, full_bar(s));
+        ptx::tma_load_2d(sX + s * Cfg::kStageX, &tmap_x, kb * kBK, m0, full_bar(s));
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (ptx::elect_one()) {
+      constexpr uint32_t idesc = ptx::idesc_s8_s32(128, NT);
+      bool ok = true;
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        const int s = kb % S;
+        ok = ptx::mbar_wait(full_bar(s), (kb / S) & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint64_t dw = ptx::smem_desc_sw128(sW + s * Cfg::kStageW), dx = ptx::smem_desc_sw128(sX + s * Cfg::kStageX);
+#pragma unroll
+        for (int k = 0; k < kBK / 32; ++k) ptx::mma_i8(tmem_base, dw + 2 * k, dx + 2 * k, idesc, kb > 0 || k > 0);
+        ptx::mma_commit(empty_bar(s));
+      }
+      if (ok) ptx::mma_commit(done_bar);
+    }
+    __syncwarp();
+  } else {  // epilogue: a lane is an output channel, a column a token
+    for (int t = threadIdx.x; t < NT; t += 128) sa[t] = m0 + t < p.M ? __ldg(p.sa + m0 + t) : 0.f;
+    const int n = n0 + (int)threadIdx.x;
+    const float sb = n < p.N ? __ldg(p.sb + n) : 0.f;
+    const float bias = p.bias != nullptr && n < p.N ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (ptx::mbar_wait(done_bar, 0, abort_flag)) {
+      ptx::tc_fence_after();
+      const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
+      OutT* out = static_cast<OutT*>(p.C) + (int64_t)m0 * p.N + n;
+#pragma unroll 1
+      for (int c = 0; c < NT; c += 16) {
+        uint32_t v[32];
+        ptx::tmem_ld16(lane_base + c, v);
+        ptx::tmem_ld_wait16(v);
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+          if (m0 + c + t < p.M && n < p.N)
+            out[(int64_t)(c + t) * p.N] = from_f32<OutT>(fmaf((float)(int)v[t] * sa[c + t], sb, bias));
+      }
+    }
+  }
+
+  if (*abort_flag) {  // a wait gave up: copies that are still under way land before the shared memory goes
+    const unsigned long long t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicCAS(p.status, 0, 1);
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+// Row-major [rows, cols] matrix of `es`-byte elements, `ld` elements between rows, box [box_rows x box_cols] with the swizzle that fits
+// its width. Encoded for every call.
+inline int encode_tmap(CUtensorMap* m, CUtensorMapDataType type, int es, const void* base, int64_t rows, int64_t cols, int64_t ld,
+                       int box_rows, int box_cols, CUtensorMapL2promotion promotion, const char* what) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) {
+    set_error_detail("cuTensorMapEncodeTiled is not available from the driver");
+    return B200_E_LAUNCH;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * es)};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const int w = box_cols * es;
+  CUresult r = enc(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   w == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                   : w == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                             : CU_TENSOR_MAP_SWIZZLE_NONE,
+                   promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error_detail("cuTensorMapEncodeTiled(%s: rows=%lld cols=%lld ld=%lld box=%dx%d) failed with CUresult %d", what, (long long)rows,
+                     (long long)cols, (long long)ld, box_rows, box_cols, (int)r);
+    return B200_E_LAUNCH;
+  }
+  return B200_OK;
+}
+inline int encode_tmap_s8(CUtensorMap* m, const void* base, int64_t rows, int64_t k, int64_t ld, int box_rows, const char* what) {
+  return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, k, ld, box_rows, kBK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
+}
+
+template <int NT, typename OutT>
+inline int launch_int8_stream(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
+  using Cfg = Int8StreamCfg<NT>;
+  p.n_tiles = (int)cdiv(p.N, 128);
+  p.t_tiles = (int)cdiv(p.M, NT);
+  CUtensorMap tw, tx;
+  if (int rc = encode_tmap_s8(&tw, B, p.N, K, ldb, 128, "B")) return rc;
+  if (int rc = encode_tmap_s8(&tx, A, p.M, K, lda, NT, "A")) return rc;
+  auto k = int8_stream_kernel<NT, OutT>;
+  if (int rc = allow_smem(k, Cfg::kSmemBytes, "int8_stream_kernel")) return rc;
+  return launch_dependent(k, dim3((unsigned)(p.n_tiles * p.t_tiles)), Cfg::kThreads, Cfg::kSmemBytes, st, 1, "int8_stream_kernel", tw,
+                          tx, p);
+}
+
+}  // namespace b200
