@@ -71,7 +71,9 @@ int b200_read_device_status(int* out, void* stream);
  * single-CTA / CTA-pair block-scaled kernel), "linear_decode_fused" (0 = never a kernel that quantises its own input, 2 = the
  * linear takes the decode kernel that does wherever that runs; 9 to 16 rows: B200_E_UNSUPPORTED), "moe_decode"
  * (0 = never the weight-streaming MoE kernels, 1 = always, 16 / 32 / 64 = always with that row block), "moe_down_splitk" (0 = never),
- * "moe_zero_pads" (0 / 1), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
+ * "moe_zero_pads" (0 / 1), "int8_tile" (16 .. 256 in steps of 16 = always the int8 stream kernel with
+ * tiles of that many tokens at most, 1128 / 1256 = always the int8 pair kernel of that width), "int8_splits" (1 .. 8 = K splits of the
+ * int8 stream kernel), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
  * No counterpart in the reference (its Triton launchers read tuned JSON configs instead,
  * python/sglang/srt/layers/moe/fused_moe_triton/fused_moe_triton_config.py). Not thread-safe
  * against concurrent launches: set knobs before the calls they affect. */
@@ -464,6 +466,14 @@ int b200_per_token_quant_int8(const void* x, int64_t x_ld, int dtype, void* q, f
 int b200_int8_scaled_mm(const void* A, int64_t lda, const float* sa, const void* B, int64_t ldb,
                         const float* sb, const void* bias, void* C, int c_dtype, int64_t M, int64_t N,
                         int64_t K, void* stream);
+
+/* b200_w8a8_int8_linear: per_token_quant_int8 of x [M,K] (bf16 / f16, rows x_ld elements apart), then int8_scaled_mm with the weight
+ * w [N,K]; out [M,N] of x's type. Replaces W8A8Int8LinearMethod.apply (python/sglang/srt/layers/quantization/w8a8_int8.py).
+ * workspace: the quantised rows and their scales, 16-byte aligned, the caller's until the kernels are done. */
+size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, const void* w, int64_t ldw,
+                          const float* sw, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -137,6 +137,12 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
          c_void_p],
     ),
+    "b200_w8a8_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "b200_w8a8_int8_linear": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t,
+         c_void_p],
+    ),
     "b200_route_topk_softmax_capped": (
         c_int,
         [c_void_p, c_int, c_float, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],

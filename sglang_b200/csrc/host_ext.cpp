@@ -46,6 +46,11 @@ struct Abi {
   decltype(&b200_fused_experts_fp8_workspace_bytes) experts_ws;
   decltype(&b200_fused_experts_fp8) experts;
   decltype(&b200_route_topk) route;
+  decltype(&b200_rmsnorm_quant) norm_quant;
+  decltype(&b200_per_token_quant_int8) quant_int8;
+  decltype(&b200_int8_scaled_mm) int8_mm;
+  decltype(&b200_w8a8_int8_linear_workspace_bytes) int8_linear_ws;
+  decltype(&b200_w8a8_int8_linear) int8_linear;
 } abi;
 
 PyObject* fail(int status, const char* what) {
@@ -381,6 +386,163 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------ norms and int8
+// Rows whose elements are contiguous: any contiguous tensor, or a 2-D one with its rows at any distance.
+bool rows_of(const Tensor& t, int64_t& rows, int64_t& cols, int64_t& ld) {
+  if (t.dim() < 1 || t.numel() == 0) return false;
+  cols = t.size(-1), rows = t.numel() / cols;
+  ld = t.dim() == 2 && rows > 1 ? t.stride(0) : cols;
+  return t.is_contiguous() || (t.dim() == 2 && t.stride(1) == 1);
+}
+// No device is asked for before an argument on one is seen.
+bool is_cuda(PyObject* o) { return THPVariable_CheckExact(o) && THPVariable_Unpack(o).is_cuda(); }
+c10::SmallVector<int64_t, 4> with_last(const Tensor& t, int64_t last) {
+  c10::SmallVector<int64_t, 4> shape(t.sizes().begin(), t.sizes().end());
+  shape.back() = last;
+  return shape;
+}
+
+// norm_quant(x, weight, eps, residual or None, layout) -> (x_q, x_s[, residual_out]); layout 0: int8, 1 to 4: FP8 with row-major,
+// column-major, padded column-major and packed power-of-two scales
+PyObject* norm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor *x = plain(args[0], dev), *w = plain(args[1], dev);
+  const double eps = PyFloat_AsDouble(args[2]);
+  const bool add = args[3] != Py_None;
+  const Tensor* r = add ? plain(args[3], dev) : nullptr;
+  const long layout = PyLong_AsLong(args[4]);
+  int64_t rows, H, ld, r_rows = 0, r_cols = 0, r_ld = 0;
+  if (PyErr_Occurred() || !x || !w || (add && !r) || !rows_of(*x, rows, H, ld) || (add && !rows_of(*r, r_rows, r_cols, r_ld))) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const auto type = x->scalar_type();
+  const int code = dtype_code(type);
+  if (code < 0 || w->scalar_type() != type || w->dim() != 1 || w->size(0) != H || !w->is_contiguous() ||
+      (add && (r->scalar_type() != type || r->sizes() != x->sizes())) || layout < 0 || layout > 4 || (layout > 0 && H % 128) ||
+      (layout > 1 && x->dim() != 2))
+    Py_RETURN_NONE;
+  const int64_t groups = H / 128, padded = cdiv(rows, 4) * 4, pitch = layout >= 3 ? padded : rows;
+  Tensor q, s, out;
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    q = empty_on(dev, x->sizes(), layout == 0 ? at::kChar : kFp8);
+    s = layout == 0   ? empty_on(dev, with_last(*x, 1), at::kFloat)
+        : layout == 1 ? empty_on(dev, with_last(*x, groups), at::kFloat)
+        : layout == 4 ? empty_on(dev, {cdiv(groups, 4), padded}, at::kInt)
+                      : empty_on(dev, {groups, pitch}, at::kFloat);
+    if (add) out = empty_on(dev, x->sizes(), type);
+    rc = abi.norm_quant(x->data_ptr(), ld, add ? r->data_ptr() : nullptr, r_ld, w->data_ptr(), code,
+                        layout == 0   ? B200_ROW_INT8
+                        : layout == 4 ? B200_ROW_FP8_UE8M0
+                                      : B200_ROW_FP8,
+                        q.data_ptr(), s.data_ptr(), layout == 1 ? groups : 1, layout == 1 ? 1 : pitch, add ? out.data_ptr() : nullptr, rows,
+                        H, (float)eps, stream_of(dev));
+  }
+  if (rc) return fail(rc, "rmsnorm_quant");
+  if (layout > 1) row_contiguous(s, rows, layout == 4 ? cdiv(groups, 4) : groups, pitch);
+  if (!add) return pair(std::move(q), std::move(s));
+  PyObject* t = PyTuple_New(3);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(q)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(s)));
+  PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(std::move(out)));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// quant_int8(x, fuse_silu_and_mul) -> (x_q, x_s)
+PyObject* quant_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 2 || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor* x = plain(args[0], dev);
+  const bool silu = args[1] == Py_True;
+  int64_t rows, width, ld;
+  if (!x || dtype_code(x->scalar_type()) < 0 || !rows_of(*x, rows, width, ld) || (silu && width % 2)) Py_RETURN_NONE;
+  const int64_t K = silu ? width / 2 : width;
+  Tensor q, s;
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    q = empty_on(dev, with_last(*x, K), at::kChar);
+    s = empty_on(dev, with_last(*x, 1), at::kFloat);
+    rc = abi.quant_int8(x->data_ptr(), ld, dtype_code(x->scalar_type()), q.data_ptr(), s.data_ptr<float>(), rows, K, silu, stream_of(dev));
+  }
+  if (rc) return fail(rc, "per_token_quant_int8");
+  return pair(std::move(q), std::move(s));
+  END_HANDLE_TH_ERRORS
+}
+
+bool is_vector(const Tensor* t, int64_t n, at::ScalarType type) {
+  return t && t->scalar_type() == type && t->numel() == n && t->is_contiguous();
+}
+
+// int8_mm(mat_a, mat_b, scales_a, scales_b, out_dtype_code, bias or None): mat_b a transposed [N, K] weight
+PyObject* int8_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6 || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor *a = plain(args[0], dev), *b = plain(args[1], dev), *sa = plain(args[2], dev), *sb = plain(args[3], dev);
+  const long code = PyLong_AsLong(args[4]);
+  const bool biased = args[5] != Py_None;
+  const Tensor* bias = biased ? plain(args[5], dev) : nullptr;
+  if (!a || !b || a->dim() != 2 || b->dim() != 2 || a->scalar_type() != at::kChar || b->scalar_type() != at::kChar ||
+      code < B200_BF16 || code > B200_F32)
+    Py_RETURN_NONE;
+  const int64_t M = a->size(0), K = a->size(1), N = b->size(1);
+  const auto type = dtype_of_code(code);
+  if (M == 0 || N == 0 || K < 2 || b->size(0) != K || a->stride(1) != 1 || b->stride(0) != 1 || !is_vector(sa, M, at::kFloat) ||
+      !is_vector(sb, N, at::kFloat) || (biased && !is_vector(bias, N, type)))
+    Py_RETURN_NONE;
+  Tensor out;
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    out = empty_on(dev, {M, N}, type);
+    rc = abi.int8_mm(a->data_ptr(), M > 1 ? a->stride(0) : K, sa->data_ptr<float>(), b->data_ptr(), N > 1 ? b->stride(1) : K,
+                     sb->data_ptr<float>(), biased ? bias->data_ptr() : nullptr, out.data_ptr(), (int)code, M, N, K, stream_of(dev));
+  }
+  if (rc) return fail(rc, "int8_scaled_mm");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_linear(x, weight, weight_scale, bias or None). The quantised rows live in a block of the caching allocator, not in the
+// stream's scratch: calls captured into two graphs may be replayed at the same time.
+PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 4 || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor *x = plain(args[0], dev), *w = plain(args[1], dev), *sw = plain(args[2], dev);
+  const bool biased = args[3] != Py_None;
+  const Tensor* bias = biased ? plain(args[3], dev) : nullptr;
+  int64_t M, K, ld;
+  if (!x || !w || w->dim() != 2 || w->scalar_type() != at::kChar || !rows_of(*x, M, K, ld)) Py_RETURN_NONE;
+  const auto type = x->scalar_type();
+  const int code = dtype_code(type);
+  const int64_t N = w->size(0);
+  if ((code != B200_BF16 && code != B200_F16) || N == 0 || K < 2 || w->size(1) != K || w->stride(1) != 1 ||
+      !is_vector(sw, N, at::kFloat) || (biased && !is_vector(bias, N, type)))
+    Py_RETURN_NONE;
+  Tensor out;
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    out = empty_on(dev, with_last(*x, N), type);
+    const size_t need = abi.int8_linear_ws(M, N, K);
+    const Tensor ws = empty_on(dev, {(int64_t)need}, at::kByte);
+    rc = abi.int8_linear(x->data_ptr(), ld, code, w->data_ptr(), N > 1 ? w->stride(0) : K, sw->data_ptr<float>(),
+                         biased ? bias->data_ptr() : nullptr, out.data_ptr(), M, N, K, ws.data_ptr(), need, stream_of(dev));
+  }
+  if (rc) return fail(rc, "w8a8_int8_linear");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // scratch(device, bytes): the current stream's scratch buffer as a uint8 tensor of at least that size
 PyObject* scratch_tensor(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -453,6 +615,11 @@ PyObject* bind(PyObject*, PyObject* arg) {
   get(abi.experts_ws, "b200_fused_experts_fp8_workspace_bytes");
   get(abi.experts, "b200_fused_experts_fp8");
   get(abi.route, "b200_route_topk");
+  get(abi.norm_quant, "b200_rmsnorm_quant");
+  get(abi.quant_int8, "b200_per_token_quant_int8");
+  get(abi.int8_mm, "b200_int8_scaled_mm");
+  get(abi.int8_linear_ws, "b200_w8a8_int8_linear_workspace_bytes");
+  get(abi.int8_linear, "b200_w8a8_int8_linear");
   if (!ok) return PyErr_Format(PyExc_ImportError, "%s lacks a symbol of its header", path);
   Py_RETURN_NONE;
 }
@@ -464,6 +631,8 @@ PyMethodDef methods[] = {
     {"matmul_ue8m0", FAST(matmul_ue8m0), nullptr}, {"experts", FAST(experts), nullptr},
     {"route", FAST(route), nullptr},          {"scratch", FAST(scratch_tensor), nullptr},
     {"acquire", FAST(acquire), nullptr},      {"release", release, METH_O, nullptr},
+    {"norm_quant", FAST(norm_quant), nullptr}, {"quant_int8", FAST(quant_int8), nullptr},
+    {"int8_mm", FAST(int8_mm), nullptr},      {"int8_linear", FAST(int8_linear), nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the block-FP8 operators.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

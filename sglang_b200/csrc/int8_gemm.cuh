@@ -19,6 +19,9 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 // Instruction descriptor for kind::i8, signed x signed -> int32 (no saturation), both operands K-major.
 //   bits 4-5 D format (2 = s32)  7-9 A format (1 = signed)  10-12 B format  17-22 N >> 3  24-28 M >> 4
 __host__ __device__ constexpr uint32_t idesc_s8_s32(int M, int N) {
@@ -34,18 +37,27 @@ struct Int8Params {
   int64_t w_ld;
   int M, N, num_kb;
   int n_tiles, t_tiles;
+  int nt, k_splits, kb_per_split;           // stream kernel: tokens of a tile, K splits of an item (one cluster)
+  int m_tiles, group_m;                     // pair kernel
+  FastDiv per_group_div;
   int* status;
 };
 
-// The roles of the operands are swapped: 128 rows of B fill the lanes of the tensor-core tile, NT tokens are its columns, so that
-// few tokens waste nothing and a thread of the epilogue owns one output channel.
+// Few tokens. The roles of the operands are swapped: 128 rows of B fill the lanes of the tensor-core tile, nt tokens (a multiple of
+// 16, at most NT) are its columns, so that few tokens waste little and a thread of the epilogue owns one output channel.
+// Work item = (128 rows of B, nt tokens, K split); one CTA each. The K splits of an item are one cluster: they exchange their integer
+// sums through distributed shared memory, every one of them adding up and storing its share of the tokens.
 template <int NT>
 struct Int8StreamCfg {
   static constexpr int kStageW = 128 * kBK, kStageX = NT * kBK;
-  static constexpr int kStages = 5;
+  static constexpr int kCtasPerSm = NT <= 64 ? 2 : 1;
+  static constexpr int kStages = NT == 16 ? 5 : NT == 32 ? 4 : NT == 64 ? 4 : NT == 128 ? 6 : 4;
   static constexpr int kThreads = 192;  // 4 epilogue warps, producer, MMA issuer
   static constexpr int kTmemCols = NT < 32 ? 32 : NT;
-  static constexpr size_t kSmemBytes = (size_t)kStages * (kStageW + kStageX) + NT * 4 + 1024 + 256;
+  // sums of the splits, [split][tokens of this CTA][128]; with many tokens they go to the ring once it is idle
+  static constexpr int kSumBytes = NT <= 32 ? (NT + 8) * 512 : 0;
+  static constexpr size_t kSmemBytes = (size_t)kStages * (kStageW + kStageX) + kSumBytes + NT * 4 + 1024 + 256;
+  static_assert(kSumBytes > 0 || (NT + 8) * 512 <= kStages * (kStageW + kStageX), "the sums fit the ring");
 };
 
 template <int NT, typename OutT>
@@ -57,7 +69,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
   const uint32_t sW = smem_base, sX = smem_base + S * Cfg::kStageW;
-  float* sa = reinterpret_cast<float*>(smem_al + (size_t)S * (Cfg::kStageW + Cfg::kStageX));  // [NT]
+  constexpr uint32_t kRing = S * (Cfg::kStageW + Cfg::kStageX), kSums = Cfg::kSumBytes ? kRing : 0;
+  float* sa = reinterpret_cast<float*>(smem_al + kRing + Cfg::kSumBytes);  // [NT]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sa + NT);
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -68,8 +81,10 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kProducerWarp = 4, kMmaWarp = 5;
-  const int nt = blockIdx.x / p.t_tiles, tt = blockIdx.x - nt * p.t_tiles;
-  const int n0 = nt * 128, m0 = tt * NT;
+  const int splits = p.k_splits, tile = blockIdx.x / splits, ks = blockIdx.x - tile * splits;
+  const int n_tile = tile / p.t_tiles, n0 = n_tile * 128, m0 = (tile - n_tile * p.t_tiles) * p.nt;
+  const int kb0 = ks * p.kb_per_split, kb1 = min(p.num_kb, kb0 + p.kb_per_split);
+  const int rows = min(p.nt, p.M - m0);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -92,14 +107,27 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // "I have started", waited for before another CTA's shared memory is written at the very end
+  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // This grid is launched as a programmatic dependent: every operand, and at the end the output, belongs to the kernels before it
+  // in the stream, which may still run. Until then the weights are only asked for, as a prefetch into L2, a row each.
+  if (warp < 4 && n0 + (int)threadIdx.x < p.N)
+    prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)(n0 + threadIdx.x) * p.w_ld + kb0 * kBK, min(kPrefetchKb, kb1 - kb0));
   grid_dependency_wait();
 
+  bool ok = true;
+  float sb = 0.f, bias = 0.f;
+  const int n = n0 + (int)threadIdx.x;  // of an epilogue thread
+  const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
+  OutT* const out = static_cast<OutT*>(p.C) + (int64_t)m0 * p.N + n;
   if (warp == kProducerWarp) {
     if (ptx::elect_one()) {
-      for (int kb = 0; kb < p.num_kb; ++kb) {
-        const int s = kb % S;
-        if (!ptx::mbar_wait(empty_bar(s), ((kb / S) & 1) ^ 1, abort_flag)) break;
-        ptx::mbar_expect_tx(full_bar(s), Cfg::kStageW + Cfg::kStageX);
+      const uint32_t bytes = Cfg::kStageW + p.nt * kBK;
+      uint32_t it = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % S;
+        if (!ptx::mbar_wait(empty_bar(s), ((it / S) & 1) ^ 1, abort_flag)) break;
+        ptx::mbar_expect_tx(full_bar(s), bytes);
         ptx::tma_load_2d(sW + s * Cfg::kStageW, &tmap_w, kb * kBK, n0, full_bar(s));
         ptx::tma_load_2d(sX + s * Cfg::kStageX, &tmap_x, kb * kBK, m0, full_bar(s));
       }
@@ -107,40 +135,73 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     __syncwarp();
   } else if (warp == kMmaWarp) {
     if (ptx::elect_one()) {
-      constexpr uint32_t idesc = ptx::idesc_s8_s32(128, NT);
-      bool ok = true;
-      for (int kb = 0; kb < p.num_kb; ++kb) {
-        const int s = kb % S;
-        ok = ptx::mbar_wait(full_bar(s), (kb / S) & 1, abort_flag);
+      const uint32_t idesc = ptx::idesc_s8_s32(128, p.nt);
+      uint32_t it = 0;
+      for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+        const int s = it % S;
+        ok = ptx::mbar_wait(full_bar(s), (it / S) & 1, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
         const uint64_t dw = ptx::smem_desc_sw128(sW + s * Cfg::kStageW), dx = ptx::smem_desc_sw128(sX + s * Cfg::kStageX);
 #pragma unroll
-        for (int k = 0; k < kBK / 32; ++k) ptx::mma_i8(tmem_base, dw + 2 * k, dx + 2 * k, idesc, kb > 0 || k > 0);
+        for (int k = 0; k < kBK / 32; ++k) ptx::mma_i8(tmem_base, dw + 2 * k, dx + 2 * k, idesc, it > 0 || k > 0);
         ptx::mma_commit(empty_bar(s));
       }
       if (ok) ptx::mma_commit(done_bar);
     }
     __syncwarp();
-  } else {  // epilogue: a lane is an output channel, a column a token
-    for (int t = threadIdx.x; t < NT; t += 128) sa[t] = m0 + t < p.M ? __ldg(p.sa + m0 + t) : 0.f;
-    const int n = n0 + (int)threadIdx.x;
-    const float sb = n < p.N ? __ldg(p.sb + n) : 0.f;
-    const float bias = p.bias != nullptr && n < p.N ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f;
+  } else {
+    for (int t = threadIdx.x; t < rows; t += 128) sa[t] = __ldg(p.sa + m0 + t);
+    if (n < p.N) {
+      sb = __ldg(p.sb + n);
+      if (p.bias != nullptr) bias = to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]);
+    }
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (ptx::mbar_wait(done_bar, 0, abort_flag)) {
-      ptx::tc_fence_after();
-      const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
-      OutT* out = static_cast<OutT*>(p.C) + (int64_t)m0 * p.N + n;
+    ok = ptx::mbar_wait(done_bar, 0, abort_flag);
+    grid_launch_dependents();  // as this grid drains
+    ptx::tc_fence_after();
+    if (splits == 1 && ok) {
 #pragma unroll 1
-      for (int c = 0; c < NT; c += 16) {
+      for (int c = 0; c < rows; c += 16) {
         uint32_t v[32];
         ptx::tmem_ld16(lane_base + c, v);
         ptx::tmem_ld_wait16(v);
 #pragma unroll
         for (int t = 0; t < 16; ++t)
-          if (m0 + c + t < p.M && n < p.N)
-            out[(int64_t)(c + t) * p.N] = from_f32<OutT>(fmaf((float)(int)v[t] * sa[c + t], sb, bias));
+          if (c + t < rows && n < p.N) out[(int64_t)(c + t) * p.N] = from_f32<OutT>(fmaf((float)(int)v[t] * sa[c + t], sb, bias));
+      }
+    }
+  }
+
+  if (splits > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (Cfg::kSumBytes == 0) ptx::cluster_sync();  // every ring is idle: done_bar completes behind the last product
+    const int r = threadIdx.x & 127, per = (rows + splits - 1) / splits;  // token t belongs to split t / per
+    if (warp < 4) {
+      int owner = 0, j = 0;
+#pragma unroll 1
+      for (int c = 0; c < rows; c += 16) {
+        uint32_t v[32];
+        ptx::tmem_ld16(lane_base + c, v);
+        ptx::tmem_ld_wait16(v);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          if (c + t < rows)
+            ptx::st_cluster_u32(ptx::mapa(smem_base + kSums, owner) + ((ks * per + j) * 128 + r) * 4, v[t]);
+          if (++j == per) j = 0, ++owner;
+        }
+      }
+    }
+    __syncwarp();
+    ptx::cluster_sync();
+    if (warp < 4 && ok && n < p.N) {
+      const int* src = reinterpret_cast<const int*>(smem_al + kSums) + r;
+      const int t0 = ks * per, mine = min(per, rows - t0);
+      for (int j = 0; j < mine; ++j) {
+        int sum = 0;
+        for (int c = 0; c < splits; ++c) sum += src[(c * per + j) * 128];
+        out[(int64_t)(t0 + j) * p.N] = from_f32<OutT>(fmaf((float)sum * sa[t0 + j], sb, bias));
       }
     }
   }
@@ -188,18 +249,20 @@ inline int encode_tmap_s8(CUtensorMap* m, const void* base, int64_t rows, int64_
   return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, k, ld, box_rows, kBK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
 }
 
+// p.nt tokens per tile (at most NT), p.k_splits splits.
 template <int NT, typename OutT>
 inline int launch_int8_stream(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
   using Cfg = Int8StreamCfg<NT>;
   p.n_tiles = (int)cdiv(p.N, 128);
-  p.t_tiles = (int)cdiv(p.M, NT);
+  p.t_tiles = (int)cdiv(p.M, p.nt);
+  p.kb_per_split = (int)cdiv(p.num_kb, p.k_splits);
   CUtensorMap tw, tx;
   if (int rc = encode_tmap_s8(&tw, B, p.N, K, ldb, 128, "B")) return rc;
-  if (int rc = encode_tmap_s8(&tx, A, p.M, K, lda, NT, "A")) return rc;
+  if (int rc = encode_tmap_s8(&tx, A, p.M, K, lda, p.nt, "A")) return rc;
   auto k = int8_stream_kernel<NT, OutT>;
   if (int rc = allow_smem(k, Cfg::kSmemBytes, "int8_stream_kernel")) return rc;
-  return launch_dependent(k, dim3((unsigned)(p.n_tiles * p.t_tiles)), Cfg::kThreads, Cfg::kSmemBytes, st, 1, "int8_stream_kernel", tw,
-                          tx, p);
+  return launch_dependent(k, dim3((unsigned)(p.n_tiles * p.t_tiles * p.k_splits)), Cfg::kThreads, Cfg::kSmemBytes, st, (unsigned)p.k_splits,
+                          "int8_stream_kernel", tw, tx, p);
 }
 
 }  // namespace b200

@@ -1,0 +1,279 @@
+// Many tokens (see int8_gemm.cuh): persistent CTA pairs (tcgen05 cta_group::2), a 256 x BN output tile per pair. Each CTA loads its own
+// 128 rows of A and half of the B tile: with 256 columns 32 KB per 128 of K, which at 128 B/clk in and out of shared memory
+// fit the 512 clocks of its products. Two accumulators of up to 256 columns in TMEM, so that the epilogue of a tile runs under the
+// products of the next. Roles per CTA (320 threads):
+//   warps 0-7  epilogue: warp w owns TMEM lanes 32 (w % 4).. and half w / 4 of the columns; 32 x 32 boxes leave through bulk tensor stores
+//   warp  8    TMA producer (no multicast)      warp 9  MMA issuer (leader CTA only)
+// Cross-CTA protocol (rank 0 = leader):
+//   full[s]   (leader's)  2 arrivals (one expect_tx per producer) + the bytes of both CTAs' loads
+//   empty[s]  (each CTA)  arrival from the leader's commit       tfull[b] (each CTA)  likewise, when a tile's sums are complete
+//   tempty[b] (leader's)  16 arrivals: the epilogue warps of both CTAs
+#pragma once
+
+#include "int8_gemm.cuh"
+
+namespace b200 {
+
+namespace ptx {
+__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(m), "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+// All but the newest store that this thread committed have finished reading shared memory.
+__device__ __forceinline__ void tma_store_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+}  // namespace ptx
+
+template <int BN, typename OutT>
+struct Int8PairCfg {
+  static constexpr int kStageA = kBM * kBK, kStageB = BN / 2 * kBK;
+  static constexpr int kEpiWarps = 8, kProducerWarp = 8, kMmaWarp = 9, kThreads = 320;
+  static constexpr int kCols = BN / 2;                                // columns of an epilogue warp
+  static constexpr int kBoxBytes = 32 * 32 * (int)sizeof(OutT);       // its 32 rows of 32 columns
+  static constexpr int kStaging = kEpiWarps * 2 * kBoxBytes;          // two boxes a warp
+  static constexpr int kScales = kEpiWarps * 2 * kCols * 4;           // sb and bias of its columns: no warp waits for another
+  static constexpr int kFixed = kStaging + kScales + 1024 + 256;
+  static constexpr int kFit = (232448 - kFixed) / (kStageA + kStageB), kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kTmemCols = BN == 256 ? 512 : 256, kAccStride = BN == 256 ? 256 : 128;
+  static constexpr size_t kSmemBytes = (size_t)kStages * (kStageA + kStageB) + kFixed;
+};
+
+template <int BN, typename OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Int8PairCfg<BN, OutT>::kThreads, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_c, const Int8Params p) {
+  using Cfg = Int8PairCfg<BN, OutT>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t sA = smem_base, sB = smem_base + S * Cfg::kStageA;
+  constexpr uint32_t kRing = S * (Cfg::kStageA + Cfg::kStageB);
+  const uint32_t staging = smem_base + kRing;
+  float* cols = reinterpret_cast<float*>(smem_al + kRing + Cfg::kStaging);  // [warp][2][kCols]: sb, bias
+  uint64_t* bars = reinterpret_cast<uint64_t*>(cols + Cfg::kScales / 4);
+  const uint32_t bar0 = ptx::smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
+  auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * S + b); };
+  auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * S + 2 + b); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 5);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(full_bar(s), 2);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(tfull_bar(b), 1);
+      ptx::mbar_init(tempty_bar(b), 2 * Cfg::kEpiWarps);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == Cfg::kMmaWarp) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
+    ptx::tmem_relinquish_pair();
+  }
+  if (warp == Cfg::kProducerWarp && lane == 0) {
+    ptx::prefetch_tensormap(&tmap_a);
+    ptx::prefetch_tensormap(&tmap_b);
+    ptx::prefetch_tensormap(&tmap_c);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();  // the peer's barriers are initialised before anything signals them
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  grid_launch_dependents();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1, tiles = p.m_tiles * p.n_tiles, num_kb = p.num_kb;
+  auto coords = [&](int t, int& mt, int& nt) { tile_coords(t, p.m_tiles, p.n_tiles, p.group_m, p.per_group_div, mt, nt); };
+  // What is read and overwritten below belongs to the kernels before, which may still run; the weights of the first K blocks are
+  // asked for all the same, as a prefetch into L2, a row each.
+  if ((int)threadIdx.x < BN / 2) {
+    int mt, nt;
+    coords(pair, mt, nt);
+    const int row = nt * BN + (int)rank * (BN / 2) + (int)threadIdx.x;
+    if (row < p.N) prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)row * p.w_ld, min(kPrefetchKb, num_kb));
+  }
+  grid_dependency_wait();
+
+  if (warp == Cfg::kProducerWarp) {
+    if (ptx::elect_one()) {
+      int s = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += npairs) {
+        int mt, nt;
+        coords(t, mt, nt);
+        const int a_row = mt * 2 * kBM + (int)rank * kBM, b_row = nt * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          ok = ptx::mbar_wait(empty_bar(s), phase, abort_flag);
+          if (!ok) break;
+          const uint32_t lf = ptx::mapa(full_bar(s), 0);
+          ptx::mbar_expect_tx_cluster(lf, Cfg::kStageA + Cfg::kStageB);
+          ptx::tma_load_2d_pair(sA + s * Cfg::kStageA, &tmap_a, kb * kBK, a_row, lf);
+          ptx::tma_load_2d_pair(sB + s * Cfg::kStageB, &tmap_b, kb * kBK, b_row, lf);
+          if (++s == S) s = 0, phase ^= 1;
+        }
+      }
+      // the leader's last arrivals on this CTA's empty barriers, before its shared memory may go
+      for (int i = 0; i < S && ok; ++i) {
+        ok = ptx::mbar_wait(empty_bar(s), phase, abort_flag);
+        if (++s == S) s = 0, phase ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp == Cfg::kMmaWarp) {
+    if (leader && ptx::elect_one()) {
+      constexpr uint32_t idesc = ptx::idesc_s8_s32(2 * kBM, BN);
+      const uint64_t da0 = ptx::smem_desc_sw128(sA), db0 = ptx::smem_desc_sw128(sB);
+      int s = 0, b = 0;
+      uint32_t phase = 0, tphase = 1;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += npairs) {
+        ok = ptx::mbar_wait(tempty_bar(b), tphase, abort_flag);
+        const uint32_t d = tmem_base + b * Cfg::kAccStride;
+#pragma unroll 1
+        for (int kb = 0; kb < num_kb && ok; ++kb) {
+          ok = ptx::mbar_wait(full_bar(s), phase, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          // a stage further = its bytes >> 4 in the address field, which does not overflow: shared memory ends below 2^18
+          const uint64_t da = da0 + (uint32_t)(s * (Cfg::kStageA >> 4)), db = db0 + (uint32_t)(s * (Cfg::kStageB >> 4));
+#pragma unroll
+          for (int k = 0; k < kBK / 32; ++k) ptx::mma_i8_pair(d, da + 2 * k, db + 2 * k, idesc, kb > 0 || k > 0);
+          ptx::mma_commit_pair_multicast(empty_bar(s), (uint16_t)3);
+          if (++s == S) s = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        ptx::mma_commit_pair_multicast(tfull_bar(b), (uint16_t)3);
+        if (++b == 2) b = 0, tphase ^= 1;
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t leader_tempty = ptx::mapa(tempty_bar(0), 0);
+    float* my_cols = cols + warp * 2 * Cfg::kCols;
+    const uint32_t boxes = staging + warp * 2 * Cfg::kBoxBytes;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * Cfg::kCols;
+    int b = 0;
+    uint32_t phase = 0;
+    for (int t = pair; t < tiles; t += npairs) {
+      int mt, nt;
+      coords(t, mt, nt);
+      const int row0 = mt * 2 * kBM + (int)rank * kBM + quarter * 32, row = row0 + lane;
+      const float sa = row < p.M ? __ldg(p.sa + row) : 0.f;
+      const int col0 = nt * BN + half * Cfg::kCols;
+      __syncwarp();  // the last tile's columns have been read
+#pragma unroll
+      for (int c = 0; c < Cfg::kCols; c += 32) {
+        const int n = col0 + c + lane;
+        my_cols[c + lane] = n < p.N ? __ldg(p.sb + n) : 0.f;
+        my_cols[Cfg::kCols + c + lane] = n < p.N && p.bias != nullptr ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f;
+      }
+      __syncwarp();
+      if (!ptx::mbar_wait(tfull_bar(b), phase, abort_flag)) break;
+      ptx::tc_fence_after();
+      const uint32_t ta = lane_base + b * Cfg::kAccStride;
+#pragma unroll 1
+      for (int c = 0; c < Cfg::kCols; c += 32) {
+        uint32_t v[32];
+        ptx::tmem_ld32(ta + c, v);
+        ptx::tmem_ld_wait(v);
+        if (c + 32 == Cfg::kCols) {  // the accumulator is in registers
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster(leader_tempty + 8 * b);
+        }
+        const uint32_t box = boxes + ((c >> 5) & 1) * Cfg::kBoxBytes;
+        if (lane == 0) ptx::tma_store_wait_read_but_one();  // the box before the last has left this half of the staging area
+        __syncwarp();
+        const float* sb = my_cols + c;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const float4 s4 = ld_shared_f4(sb + 8 * g + i), b4 = ld_shared_f4(sb + Cfg::kCols + 8 * g + i);
+            f[i + 0] = fmaf((float)(int)v[8 * g + i + 0] * sa, s4.x, b4.x);
+            f[i + 1] = fmaf((float)(int)v[8 * g + i + 1] * sa, s4.y, b4.y);
+            f[i + 2] = fmaf((float)(int)v[8 * g + i + 2] * sa, s4.z, b4.z);
+            f[i + 3] = fmaf((float)(int)v[8 * g + i + 3] * sa, s4.w, b4.w);
+          }
+          // rows of 64 bytes (16-bit types) or 128, in the swizzle of the tensor map
+          if constexpr (sizeof(OutT) == 2) {
+            const uint4 o = pack8<OutT>(f);
+            const uint32_t at = box + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const uint32_t at = box + lane * 128 + (((2 * g + i / 4) ^ (lane & 7)) << 4);
+              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(f[i]), "f"(f[i + 1]), "f"(f[i + 2]), "f"(f[i + 3]) : "memory");
+            }
+          }
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (row0 < p.M && col0 + c < p.N) ptx::tma_store_2d(&tmap_c, box, col0 + c, row0);
+          ptx::tma_store_commit();
+        }
+      }
+      if (++b == 2) b = 0, phase ^= 1;
+    }
+    if (lane == 0) ptx::tma_store_wait_all();
+  }
+
+  if (*abort_flag) {
+    const unsigned long long t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();  // neither CTA leaves while the other may still signal its barriers or read its shared memory
+  if (threadIdx.x == 0 && *abort_flag) atomicCAS(p.status, 0, 1);
+  if (warp == Cfg::kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+template <int BN, typename OutT>
+inline int launch_int8_pair(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
+  using Cfg = Int8PairCfg<BN, OutT>;
+  p.m_tiles = (int)cdiv(p.M, 2 * kBM);
+  p.n_tiles = (int)cdiv(p.N, BN);
+  p.group_m = row_group(p.M, K, 2 * kBM);
+  p.per_group_div = make_fastdiv(p.group_m * p.n_tiles);
+  CUtensorMap ta, tb, tc;
+  if (int rc = encode_tmap_s8(&ta, A, p.M, K, lda, kBM, "A")) return rc;
+  if (int rc = encode_tmap_s8(&tb, B, p.N, K, ldb, BN / 2, "B")) return rc;
+  const CUtensorMapDataType type = sizeof(OutT) == 4                                ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<OutT, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (int rc = encode_tmap(&tc, type, (int)sizeof(OutT), p.C, p.M, p.N, p.N, 32, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE, "C")) return rc;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int slots = sm_count() / 2, pairs = (int)(tiles < slots ? tiles : slots);
+  auto k = int8_pair_kernel<BN, OutT>;
+  if (int rc = allow_smem(k, Cfg::kSmemBytes, "int8_pair_kernel")) return rc;
+  return launch_dependent(k, dim3((unsigned)(2 * pairs)), Cfg::kThreads, Cfg::kSmemBytes, st, 1, "int8_pair_kernel", ta, tb, tc, p);
+}
+
+}  // namespace b200

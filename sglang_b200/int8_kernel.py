@@ -39,6 +39,10 @@ def per_token_quant_int8(
     """
     if scale_dtype != torch.float32 or cal_sum:
         raise NotImplementedError("per_token_quant_int8: only fp32 scales without row sums are built")
+    N.load()
+    pair = N.host.quant_int8(x, fuse_silu_and_mul)
+    if pair is not None:
+        return pair
     assert x.dtype in (torch.bfloat16, torch.float16, torch.float32), f"unsupported input dtype {x.dtype}"
     x, ld = rows_of(x, "x")
     width = x.shape[-1]
@@ -73,6 +77,10 @@ def int8_scaled_mm(
     reference's: rows of ``mat_a`` and columns of ``mat_b`` start at multiples of 16 bytes, ``K`` is a multiple of 16, ``N`` of 8;
     beyond ``K`` = 131071 a 32-bit sum could overflow and the call is refused.
     """
+    N.load()
+    out = N.host.int8_mm(mat_a, mat_b, scales_a, scales_b, N.DTYPE_CODE.get(out_dtype, -1), bias)
+    if out is not None:
+        return out
     assert mat_a.dim() == 2 and mat_b.dim() == 2, "mat_a and mat_b must be 2D tensors"
     M, K = mat_a.shape
     Nn = mat_b.shape[1]
@@ -115,6 +123,10 @@ def w8a8_int8_linear(
     """Quantise the activation per token, multiply, apply the scales and the bias: what the reference's
     ``W8A8Int8LinearMethod.apply`` runs. ``input [.., K]`` bf16 or fp16, ``weight [N, K]`` int8, ``weight_scale`` fp32 with ``N``
     elements, ``bias [N]`` of the input's type; the result has the input's type."""
+    N.load()
+    out = N.host.int8_linear(input, weight, weight_scale, bias)
+    if out is not None:
+        return out
     assert input.dtype in (torch.bfloat16, torch.float16), f"unsupported input dtype {input.dtype}"
     assert weight.dim() == 2, "weight must be a 2D tensor"
     input_2d = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])

@@ -52,6 +52,10 @@ def rmsnorm_quant_int8(
     ``h = x + residual`` (or ``x``), ``y = h * weight / sqrt(mean(h^2) + eps)``, all in fp32; ``y`` is quantised unrounded.
     Returns ``(x_q [.., H] int8, x_s [.., 1] fp32)`` and, with ``residual``, ``h`` rounded to the input type as a new tensor.
     ``x`` and ``residual`` are contiguous, or 2-D with contiguous rows at any distance; ``weight [H]``; one dtype for all."""
+    N.load()
+    out = N.host.norm_quant(x, weight, eps, residual, 0)
+    if out is not None:
+        return out
     assert x.shape[-1] > 0, "rows without elements have no scale"
     _check(x, weight, residual)
     x_q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
@@ -75,8 +79,12 @@ def rmsnorm_quant_fp8(
     powers of two) as for ``per_token_group_quant_fp8``. Only ``group_size`` 128, the K block of the GEMM, is built."""
     if group_size != 128:
         raise NotImplementedError("rmsnorm_quant_fp8: only group_size 128 is built")
-    assert x.shape[-1] % group_size == 0, "the last dimension of `x` cannot be divisible by `group_size`"
     assert not scale_ue8m0 or (column_major_scales and scale_tma_aligned), "packed scales are column-major and padded"
+    N.load()
+    out = N.host.norm_quant(x, weight, eps, residual, 4 if scale_ue8m0 else 1 if not column_major_scales else 3 if scale_tma_aligned else 2)
+    if out is not None:
+        return out
+    assert x.shape[-1] % group_size == 0, "the last dimension of `x` cannot be divisible by `group_size`"
     assert x.dim() == 2 or not column_major_scales, "column-major scales need a 2-D input"
     _check(x, weight, residual)
     x_q = torch.empty(x.shape, dtype=fp8_dtype, device=x.device)

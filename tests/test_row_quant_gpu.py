@@ -162,14 +162,20 @@ def test_leading_dimensions_and_empty_inputs():
 @pytest.mark.parametrize("offset", [0, 8, 16, 3])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_wider_tensors(offset, dtype):
-    """Slices of wider rows, aligned to 16 bytes or not, give what their copies give."""
+    """Slices of wider rows, aligned to 16 bytes or not."""
     wide = draw(9, 2 * 1152 + 40, dtype, 3)
     x, r, w = wide[:, offset : offset + 1152], wide[:, offset + 1152 : offset + 2304], draw(1, 1152, dtype, 4)[0]
-    for fn in (lambda a, b: S.rmsnorm_quant_int8(a, w, residual=b), lambda a, b: S.rmsnorm_quant_fp8(a, w, residual=b),
-               lambda a, b: S.per_token_quant_int8(a), lambda a, b: S.per_token_quant_int8(a, fuse_silu_and_mul=True)):
-        for got, want in zip(fn(x, r), fn(x.contiguous(), r.contiguous())):
-            assert torch.equal(got.view(torch.uint8) if got.dtype == torch.float8_e4m3fn else got,
-                               want.view(torch.uint8) if want.dtype == torch.float8_e4m3fn else want)
+    y, h = normed(x, r, w, 1e-6)
+    q, s, res = S.rmsnorm_quant_int8(x, w, residual=r)
+    check_int8(q, s, y)
+    check_residual(res, h, dtype)
+    q, s, res = S.rmsnorm_quant_fp8(x, w, residual=r)
+    check_fp8(q.float(), s, y, False)
+    check_residual(res, h, dtype)
+    for got, want in zip(S.per_token_quant_int8(x), S.per_token_quant_int8(x.contiguous())):
+        assert torch.equal(got, want)
+    gate, up = x.double().chunk(2, -1)
+    check_int8(*S.per_token_quant_int8(x, fuse_silu_and_mul=True), gate / (1 + (-gate).exp()) * up, extra=2.0**-16)
 
 
 @pytest.mark.parametrize("width", [128, 1000, 4096, 16384, 33024])
@@ -191,6 +197,27 @@ def test_zero_rows_nan_and_infinity(width):
         q, s = S.rmsnorm_quant_fp8(x, w)
         f = q.float()
         assert (f[0] == 0).all() and f[1].isnan().all() and f[4].isnan().all() and f[2, 0].isnan() and f[[3, 5]].isfinite().all()
+
+
+@pytest.mark.parametrize("vectors", [1, 2, 4, 8])
+@pytest.mark.parametrize("width", [8, 128, 264, 1024, 4096, 8192, 16384, 24576])
+def test_every_number_of_vectors_per_thread(vectors, width):
+    from sglang_b200 import _native as N
+
+    x, r, w = draw(6, width, torch.bfloat16, 1), draw(6, width, torch.bfloat16, 2), draw(1, width, torch.bfloat16, 3)[0]
+    y, h = normed(x, r, w, 1e-6)
+    with N.tuning(row_vectors=vectors):
+        q, s, res = S.rmsnorm_quant_int8(x, w, residual=r)
+        check_int8(q, s, y)
+        check_residual(res, h, torch.bfloat16)
+        if width % 128 == 0:
+            q, s, res = S.rmsnorm_quant_fp8(x, w, residual=r, column_major_scales=True)
+            check_fp8(q.float(), s, y, False)
+        gate, up = x.double().chunk(2, -1)
+        if width % 16 == 0:
+            check_int8(*S.per_token_quant_int8(x, fuse_silu_and_mul=True), gate / (1 + (-gate).exp()) * up, extra=2.0**-16)
+        q, s = S.per_token_quant_int8(x)
+    assert torch.equal(q.float().cpu(), (x.float().cpu() / s.cpu()).round())
 
 
 def test_many_rows_and_repeats():
