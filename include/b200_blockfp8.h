@@ -72,8 +72,8 @@ int b200_read_device_status(int* out, void* stream);
  * linear takes the decode kernel that does wherever that runs; 9 to 16 rows: B200_E_UNSUPPORTED), "moe_decode"
  * (0 = never the weight-streaming MoE kernels, 1 = always, 16 / 32 / 64 = always with that row block), "moe_down_splitk" (0 = never),
  * "moe_zero_pads" (0 / 1), "int8_tile" (16 .. 256 in steps of 16 = always the int8 stream kernel with
- * tiles of that many tokens at most, 1128 / 1256 = always the int8 pair kernel of that width), "int8_splits" (1 .. 8 = K splits of the
- * int8 stream kernel), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
+ * tiles of that many tokens at most, 1032 .. 1256 in steps of 32 = always the int8 pair kernel with tiles of 32 .. 256
+ * columns), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
  * No counterpart in the reference (its Triton launchers read tuned JSON configs instead,
  * python/sglang/srt/layers/moe/fused_moe_triton/fused_moe_triton_config.py). Not thread-safe
  * against concurrent launches: set knobs before the calls they affect. */

@@ -34,8 +34,13 @@ static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
   const Tuning& t = tuning();
   const int64_t num_kb = cdiv(K, kBK);
   if (M > 256) pl.pair_n = 256;
-  if (t.int8_tile > 0) pl.pair_n = t.int8_tile > 256 ? (t.int8_tile == 1128 ? 128 : 256) : 0;
-  if (pl.pair_n) return pl;
+  if (t.int8_tile > 0) pl.pair_n = t.int8_tile > 1000 ? (int)t.int8_tile - 1000 : 0;
+  if (pl.pair_n) {
+    pl.pair_n = pl.pair_n < 32 ? 32 : pl.pair_n > 256 ? 256 : pl.pair_n / 32 * 32;
+    pl.splits = t.int8_splits == 2 || t.int8_splits == 4 ? (int)t.int8_splits : 1;
+    if (pl.splits > num_kb || cdiv(num_kb, cdiv(num_kb, pl.splits)) != pl.splits) pl.splits = 1;  // no empty split
+    return pl;
+  }
   const int cap = t.int8_tile > 0 ? (int)t.int8_tile : 256;
   const int64_t t_tiles = cdiv(M, cap);
   pl.nt = (int)align_up(cdiv(M, t_tiles), 16);
@@ -50,9 +55,9 @@ static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
 template <typename OutT>
 static int run_int8(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
   const Int8Plan pl = plan_int8(p.M, p.N, K, sm_count());
-  if (pl.pair_n == 256) return launch_int8_pair<256, OutT>(a, lda, b, ldb, K, p, st);
-  if (pl.pair_n == 128) return launch_int8_pair<128, OutT>(a, lda, b, ldb, K, p, st);
-  p.nt = pl.nt, p.k_splits = pl.splits;
+  p.nt = pl.pair_n ? pl.pair_n : pl.nt, p.k_splits = pl.splits;
+  if (pl.pair_n)
+    return pl.pair_n > 128 ? launch_int8_pair<256, OutT>(a, lda, b, ldb, K, p, st) : launch_int8_pair<128, OutT>(a, lda, b, ldb, K, p, st);
   return pl.nt <= 16    ? launch_int8_stream<16, OutT>(a, lda, b, ldb, K, p, st)
          : pl.nt <= 32  ? launch_int8_stream<32, OutT>(a, lda, b, ldb, K, p, st)
          : pl.nt <= 64  ? launch_int8_stream<64, OutT>(a, lda, b, ldb, K, p, st)

@@ -1,10 +1,14 @@
-// Many tokens (see int8_gemm.cuh): persistent CTA pairs (tcgen05 cta_group::2), a 256 x BN output tile per pair. Each CTA loads its own
-// 128 rows of A and half of the B tile: with 256 columns 32 KB per 128 of K, which at 128 B/clk in and out of shared memory
-// fit the 512 clocks of its products. Two accumulators of up to 256 columns in TMEM, so that the epilogue of a tile runs under the
-// products of the next. Roles per CTA (320 threads):
-//   warps 0-7  epilogue: warp w owns TMEM lanes 32 (w % 4).. and half w / 4 of the columns; 32 x 32 boxes leave through bulk tensor stores
+// Many tokens (see int8_gemm.cuh): persistent CTA pairs (tcgen05 cta_group::2), a tile of 256 rows and up to BN columns per pair.
+// Each CTA loads its own 128 rows of A and half of the B tile: with 256 columns 32 KB per 128 of K, which at 128 B/clk in and
+// out of shared memory fit the 512 clocks of its products. Two accumulators of BN columns in TMEM, so that the epilogue of a tile
+// runs under the products of the next. The width of a tile is any multiple of 32: the launch takes the one that fills its waves.
+// Few tiles: the K splits of a tile, 2 or 4, are one cluster; every one of them sums and stores its share of the 32-column chunks,
+// the others hand theirs over through distributed shared memory, into the ring, which is idle by then.
+// Roles per CTA (320 threads):
+//   warps 0-7  epilogue: warp w owns TMEM lanes 32 (w % 4).. and every second chunk of 32 columns; 32 x 32 boxes leave through bulk
+//              tensor stores
 //   warp  8    TMA producer (no multicast)      warp 9  MMA issuer (leader CTA only)
-// Cross-CTA protocol (rank 0 = leader):
+// Protocol of a pair (rank 0 = leader):
 //   full[s]   (leader's)  2 arrivals (one expect_tx per producer) + the bytes of both CTAs' loads
 //   empty[s]  (each CTA)  arrival from the leader's commit       tfull[b] (each CTA)  likewise, when a tile's sums are complete
 //   tempty[b] (leader's)  16 arrivals: the epilogue warps of both CTAs
@@ -33,11 +37,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, uint32_t src,
 __device__ __forceinline__ void tma_store_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 }  // namespace ptx
 
+// BN: the widest tile
 template <int BN, typename OutT>
 struct Int8PairCfg {
   static constexpr int kStageA = kBM * kBK, kStageB = BN / 2 * kBK;
   static constexpr int kEpiWarps = 8, kProducerWarp = 8, kMmaWarp = 9, kThreads = 320;
-  static constexpr int kCols = BN / 2;                                // columns of an epilogue warp
+  static constexpr int kCols = BN / 2;                                // columns of an epilogue warp at most
   static constexpr int kBoxBytes = 32 * 32 * (int)sizeof(OutT);       // its 32 rows of 32 columns
   static constexpr int kStaging = kEpiWarps * 2 * kBoxBytes;          // two boxes a warp
   static constexpr int kScales = kEpiWarps * 2 * kCols * 4;           // sb and bias of its columns: no warp waits for another
@@ -45,10 +50,11 @@ struct Int8PairCfg {
   static constexpr int kFit = (232448 - kFixed) / (kStageA + kStageB), kStages = kFit < 8 ? kFit : 8;
   static constexpr int kTmemCols = BN == 256 ? 512 : 256, kAccStride = BN == 256 ? 256 : 128;
   static constexpr size_t kSmemBytes = (size_t)kStages * (kStageA + kStageB) + kFixed;
+  static_assert(kStages * (kStageA + kStageB) >= 6 * 16384, "the sums of the other splits fit the ring");
 };
 
 template <int BN, typename OutT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Int8PairCfg<BN, OutT>::kThreads, 1)
+__global__ void __launch_bounds__(Int8PairCfg<BN, OutT>::kThreads, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const __grid_constant__ CUtensorMap tmap_c, const Int8Params p) {
   using Cfg = Int8PairCfg<BN, OutT>;
@@ -70,8 +76,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 5);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_ctarank();
+  const uint32_t cluster_rank = ptx::cluster_ctarank(), rank = cluster_rank & 1, leader_rank = cluster_rank - rank;
   const bool leader = rank == 0;
+  const int bn = p.nt, splits = p.k_splits;  // columns of the tile
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -100,32 +107,37 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1, tiles = p.m_tiles * p.n_tiles, num_kb = p.num_kb;
+  // a cluster takes one tile where K is split, else as many as there are
+  const int cluster_pairs = splits, ks = (int)cluster_rank >> 1;
+  const int pair = (blockIdx.x >> 1) / cluster_pairs, npairs = (gridDim.x >> 1) / cluster_pairs, tiles = p.m_tiles * p.n_tiles;
+  const int kb0 = ks * p.kb_per_split, kb1 = min(p.num_kb, kb0 + p.kb_per_split);
   auto coords = [&](int t, int& mt, int& nt) { tile_coords(t, p.m_tiles, p.n_tiles, p.group_m, p.per_group_div, mt, nt); };
   // What is read and overwritten below belongs to the kernels before, which may still run; the weights of the first K blocks are
   // asked for all the same, as a prefetch into L2, a row each.
-  if ((int)threadIdx.x < BN / 2) {
+  if ((int)threadIdx.x < bn / 2) {
     int mt, nt;
     coords(pair, mt, nt);
-    const int row = nt * BN + (int)rank * (BN / 2) + (int)threadIdx.x;
-    if (row < p.N) prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)row * p.w_ld, min(kPrefetchKb, num_kb));
+    const int row = nt * bn + (int)rank * (bn / 2) + (int)threadIdx.x;
+    if (row < p.N)
+      prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)row * p.w_ld + kb0 * kBK, min(kPrefetchKb, kb1 - kb0));
   }
   grid_dependency_wait();
 
   if (warp == Cfg::kProducerWarp) {
     if (ptx::elect_one()) {
+      const uint32_t bytes = Cfg::kStageA + bn / 2 * kBK;
       int s = 0;
       uint32_t phase = 1;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += npairs) {
         int mt, nt;
         coords(t, mt, nt);
-        const int a_row = mt * 2 * kBM + (int)rank * kBM, b_row = nt * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < num_kb; ++kb) {
+        const int a_row = mt * 2 * kBM + (int)rank * kBM, b_row = nt * bn + (int)rank * (bn / 2);
+        for (int kb = kb0; kb < kb1; ++kb) {
           ok = ptx::mbar_wait(empty_bar(s), phase, abort_flag);
           if (!ok) break;
-          const uint32_t lf = ptx::mapa(full_bar(s), 0);
-          ptx::mbar_expect_tx_cluster(lf, Cfg::kStageA + Cfg::kStageB);
+          const uint32_t lf = ptx::mapa(full_bar(s), leader_rank);
+          ptx::mbar_expect_tx_cluster(lf, bytes);
           ptx::tma_load_2d_pair(sA + s * Cfg::kStageA, &tmap_a, kb * kBK, a_row, lf);
           ptx::tma_load_2d_pair(sB + s * Cfg::kStageB, &tmap_b, kb * kBK, b_row, lf);
           if (++s == S) s = 0, phase ^= 1;
@@ -140,7 +152,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     __syncwarp();
   } else if (warp == Cfg::kMmaWarp) {
     if (leader && ptx::elect_one()) {
-      constexpr uint32_t idesc = ptx::idesc_s8_s32(2 * kBM, BN);
+      const uint32_t idesc = ptx::idesc_s8_s32(2 * kBM, bn);
+      const uint16_t both = (uint16_t)(3u << leader_rank);
       const uint64_t da0 = ptx::smem_desc_sw128(sA), db0 = ptx::smem_desc_sw128(sB);
       int s = 0, b = 0;
       uint32_t phase = 0, tphase = 1;
@@ -149,62 +162,89 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         ok = ptx::mbar_wait(tempty_bar(b), tphase, abort_flag);
         const uint32_t d = tmem_base + b * Cfg::kAccStride;
 #pragma unroll 1
-        for (int kb = 0; kb < num_kb && ok; ++kb) {
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
           ok = ptx::mbar_wait(full_bar(s), phase, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
           // a stage further = its bytes >> 4 in the address field, which does not overflow: shared memory ends below 2^18
           const uint64_t da = da0 + (uint32_t)(s * (Cfg::kStageA >> 4)), db = db0 + (uint32_t)(s * (Cfg::kStageB >> 4));
 #pragma unroll
-          for (int k = 0; k < kBK / 32; ++k) ptx::mma_i8_pair(d, da + 2 * k, db + 2 * k, idesc, kb > 0 || k > 0);
-          ptx::mma_commit_pair_multicast(empty_bar(s), (uint16_t)3);
+          for (int k = 0; k < kBK / 32; ++k) ptx::mma_i8_pair(d, da + 2 * k, db + 2 * k, idesc, kb > kb0 || k > 0);
+          ptx::mma_commit_pair_multicast(empty_bar(s), both);
           if (++s == S) s = 0, phase ^= 1;
         }
         if (!ok) break;
-        ptx::mma_commit_pair_multicast(tfull_bar(b), (uint16_t)3);
+        ptx::mma_commit_pair_multicast(tfull_bar(b), both);
         if (++b == 2) b = 0, tphase ^= 1;
       }
     }
     __syncwarp();
   } else {
     const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t leader_tempty = ptx::mapa(tempty_bar(0), 0);
+    const uint32_t leader_tempty = ptx::mapa(tempty_bar(0), leader_rank);
     float* my_cols = cols + warp * 2 * Cfg::kCols;
     const uint32_t boxes = staging + warp * 2 * Cfg::kBoxBytes;
-    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * Cfg::kCols;
-    int b = 0;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const int chunks = bn / 32;
+    int b = 0, box_no = 0;
     uint32_t phase = 0;
     for (int t = pair; t < tiles; t += npairs) {
       int mt, nt;
       coords(t, mt, nt);
       const int row0 = mt * 2 * kBM + (int)rank * kBM + quarter * 32, row = row0 + lane;
       const float sa = row < p.M ? __ldg(p.sa + row) : 0.f;
-      const int col0 = nt * BN + half * Cfg::kCols;
       __syncwarp();  // the last tile's columns have been read
-#pragma unroll
-      for (int c = 0; c < Cfg::kCols; c += 32) {
-        const int n = col0 + c + lane;
-        my_cols[c + lane] = n < p.N ? __ldg(p.sb + n) : 0.f;
-        my_cols[Cfg::kCols + c + lane] = n < p.N && p.bias != nullptr ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f;
+      for (int j = half; j < chunks; j += 2) {
+        const int n = nt * bn + j * 32 + lane;
+        my_cols[(j >> 1) * 32 + lane] = n < p.N ? __ldg(p.sb + n) : 0.f;
+        my_cols[Cfg::kCols + (j >> 1) * 32 + lane] = n < p.N && p.bias != nullptr ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f;
       }
       __syncwarp();
-      if (!ptx::mbar_wait(tfull_bar(b), phase, abort_flag)) break;
+      bool ok = ptx::mbar_wait(tfull_bar(b), phase, abort_flag);
+      if (!ok && splits == 1) break;
       ptx::tc_fence_after();
       const uint32_t ta = lane_base + b * Cfg::kAccStride;
-#pragma unroll 1
-      for (int c = 0; c < Cfg::kCols; c += 32) {
-        uint32_t v[32];
-        ptx::tmem_ld32(ta + c, v);
-        ptx::tmem_ld_wait(v);
-        if (c + 32 == Cfg::kCols) {  // the accumulator is in registers
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(leader_tempty + 8 * b);
+      // K splits: the chunks of both halves go round. Slot of a sum: [chunk of its owner][source][4 columns][row], 16 bytes
+      auto owner_of = [&](int j) { return (j >> 1) & (splits - 1); };
+      auto slot = [&](int j, int src) {
+        const int mine = (j >> 1) / splits * 2 + half;
+        return (uint32_t)(((mine * (splits - 1) + src) * 8 * kBM + quarter * 32 + lane) * 16);
+      };
+      if (splits > 1) {
+        __syncwarp();
+        ptx::cluster_sync();  // every ring is idle
+        for (int j = half; j < chunks; j += 2) {
+          const int owner = owner_of(j);
+          if (owner == ks) continue;
+          uint32_t v[32];
+          ptx::tmem_ld32(ta + j * 32, v);
+          ptx::tmem_ld_wait(v);
+          const uint32_t dst = ptx::mapa(smem_base, (uint32_t)owner * 2 + rank) + slot(j, ks < owner ? ks : ks - 1);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) ptx::st_cluster_v4(dst + g * kBM * 16, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         }
-        const uint32_t box = boxes + ((c >> 5) & 1) * Cfg::kBoxBytes;
+        __syncwarp();
+        ptx::cluster_sync();
+      }
+#pragma unroll 1
+      for (int j = half; j < chunks; j += 2) {
+        if (splits > 1 && (owner_of(j) != ks || !ok)) continue;
+        uint32_t v[32];
+        ptx::tmem_ld32(ta + j * 32, v);
+        ptx::tmem_ld_wait(v);
+        for (int src = 0; src < splits - 1; ++src) {
+          const uint32_t from = smem_base + slot(j, src);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const int4 o = ptx::ld_shared_i4(from + g * kBM * 16);
+            v[4 * g] += o.x, v[4 * g + 1] += o.y, v[4 * g + 2] += o.z, v[4 * g + 3] += o.w;
+          }
+        }
+        const uint32_t box = boxes + (box_no & 1) * Cfg::kBoxBytes;
+        ++box_no;
         if (lane == 0) ptx::tma_store_wait_read_but_one();  // the box before the last has left this half of the staging area
         __syncwarp();
-        const float* sb = my_cols + c;
+        const float* sb = my_cols + (j >> 1) * 32;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float f[8];
@@ -232,13 +272,22 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (row0 < p.M && col0 + c < p.N) ptx::tma_store_2d(&tmap_c, box, col0 + c, row0);
+          const int col0 = nt * bn + j * 32;
+          if (row0 < p.M && col0 < p.N) ptx::tma_store_2d(&tmap_c, box, col0, row0);
           ptx::tma_store_commit();
         }
       }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(leader_tempty + 8 * b);  // the accumulator is in registers
       if (++b == 2) b = 0, phase ^= 1;
     }
     if (lane == 0) ptx::tma_store_wait_all();
+  }
+  if (splits > 1 && warp >= Cfg::kEpiWarps) {  // the other warps' share of the two cluster barriers above
+    __syncwarp();
+    ptx::cluster_sync();
+    ptx::cluster_sync();
   }
 
   if (*abort_flag) {
@@ -255,25 +304,28 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   }
 }
 
+// p.nt columns per tile (a multiple of 32, at most BN), p.k_splits 1, 2 or 4.
 template <int BN, typename OutT>
 inline int launch_int8_pair(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
   using Cfg = Int8PairCfg<BN, OutT>;
   p.m_tiles = (int)cdiv(p.M, 2 * kBM);
-  p.n_tiles = (int)cdiv(p.N, BN);
+  p.n_tiles = (int)cdiv(p.N, p.nt);
+  p.kb_per_split = (int)cdiv(p.num_kb, p.k_splits);
   p.group_m = row_group(p.M, K, 2 * kBM);
   p.per_group_div = make_fastdiv(p.group_m * p.n_tiles);
   CUtensorMap ta, tb, tc;
   if (int rc = encode_tmap_s8(&ta, A, p.M, K, lda, kBM, "A")) return rc;
-  if (int rc = encode_tmap_s8(&tb, B, p.N, K, ldb, BN / 2, "B")) return rc;
+  if (int rc = encode_tmap_s8(&tb, B, p.N, K, ldb, p.nt / 2, "B")) return rc;
   const CUtensorMapDataType type = sizeof(OutT) == 4                                ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : std::is_same<OutT, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (int rc = encode_tmap(&tc, type, (int)sizeof(OutT), p.C, p.M, p.N, p.N, 32, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE, "C")) return rc;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  const int slots = sm_count() / 2, pairs = (int)(tiles < slots ? tiles : slots);
+  const int slots = sm_count() / 2, pairs = (int)(p.k_splits > 1 || tiles < slots ? tiles : slots);
   auto k = int8_pair_kernel<BN, OutT>;
   if (int rc = allow_smem(k, Cfg::kSmemBytes, "int8_pair_kernel")) return rc;
-  return launch_dependent(k, dim3((unsigned)(2 * pairs)), Cfg::kThreads, Cfg::kSmemBytes, st, 1, "int8_pair_kernel", ta, tb, tc, p);
+  return launch_dependent(k, dim3((unsigned)(2 * pairs * p.k_splits)), Cfg::kThreads, Cfg::kSmemBytes, st, 2u * p.k_splits,
+                          "int8_pair_kernel", ta, tb, tc, p);
 }
 
 }  // namespace b200
