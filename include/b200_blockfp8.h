@@ -467,6 +467,10 @@ int b200_int8_scaled_mm(const void* A, int64_t lda, const float* sa, const void*
                         const float* sb, const void* bias, void* C, int c_dtype, int64_t M, int64_t N,
                         int64_t K, void* stream);
 
+/* Which kernel a product of this size takes under the present knobs: host arithmetic, for tests and sweeps. *pair != 0: CTA pairs with
+ * tiles of *tile columns, else the stream kernel with tiles of *tile tokens; sms = 0: for the current device. */
+int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* pair, int* tile, int* splits);
+
 /* b200_w8a8_int8_linear: per_token_quant_int8 of x [M,K] (bf16 / f16, rows x_ld elements apart), then int8_scaled_mm with the weight
  * w [N,K]; out [M,N] of x's type. Replaces W8A8Int8LinearMethod.apply (python/sglang/srt/layers/quantization/w8a8_int8.py).
  * workspace: the quantised rows and their scales, 16-byte aligned, the caller's until the kernels are done. */

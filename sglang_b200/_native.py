@@ -137,6 +137,7 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
          c_void_p],
     ),
+    "b200_plan_int8": (c_int, [c_int64, c_int64, c_int64, c_int, POINTER(c_int), POINTER(c_int), POINTER(c_int)]),
     "b200_w8a8_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "b200_w8a8_int8_linear": (
         c_int,
@@ -301,6 +302,19 @@ def plan_dense(entry: str, M: int, N: int, K: int, sms: int = 0) -> DensePlan:
     check(load().b200_plan_dense(PLAN_ENTRIES[entry], M, N, K, sms, *map(ctypes.byref, v)), "plan_dense")
     kernel, tile_n, splits, total = (x.value for x in v)
     return DensePlan(KERNELS[kernel], tile_n, splits, SUMS[total])
+
+
+class Int8Plan(NamedTuple):
+    kernel: str  # "stream": tile tokens by 128 channels, "pair": 256 tokens by tile channels
+    tile: int
+    splits: int
+
+
+def plan_int8(M: int, N: int, K: int, sms: int = 0) -> Int8Plan:
+    """The kernel that an int8 product of this size takes (``b200_plan_int8``); sms = 0: on the current device."""
+    v = [c_int(0) for _ in range(3)]
+    check(load().b200_plan_int8(M, N, K, sms, *map(ctypes.byref, v)), "plan_int8")
+    return Int8Plan("pair" if v[0].value else "stream", v[1].value, v[2].value)
 
 
 def read_device_status() -> int:

@@ -66,7 +66,9 @@ struct Int8StreamCfg {
   static constexpr int kStageW = 128 * kBK, kStageX = NT * kBK;
   static constexpr int kCtasPerSm = NT <= 64 ? 2 : 1;
   static constexpr int kStages = NT == 16 ? 5 : NT == 32 ? 4 : NT == 64 ? 4 : NT == 128 ? 6 : 4;
-  static constexpr int kThreads = 192;  // 4 epilogue warps, producer, MMA issuer
+  // With many tokens two epilogue warps share 32 channels and take every second 16 tokens each
+  static constexpr int kEpiWarps = NT <= 32 ? 4 : 8, kEpiThreads = kEpiWarps * 32;
+  static constexpr int kProducerWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1, kThreads = kEpiThreads + 64;
   static constexpr int kTmemCols = NT < 32 ? 32 : NT;
   // sums of the splits, [split][tokens of this CTA / 4][128][4]; with many tokens they go to the ring once it is idle
   static constexpr int kSumBytes = NT <= 32 ? int8_sum_rows(NT) * 512 : 0;
@@ -94,7 +96,7 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kProducerWarp = 4, kMmaWarp = 5;
+  constexpr int kProducerWarp = Cfg::kProducerWarp, kMmaWarp = Cfg::kMmaWarp;
   const int splits = p.k_splits, tile = blockIdx.x / splits, ks = blockIdx.x - tile * splits;
   const int n_tile = tile / p.t_tiles, n0 = n_tile * 128, m0 = (tile - n_tile * p.t_tiles) * p.nt;
   const int kb0 = ks * p.kb_per_split, kb1 = min(p.num_kb, kb0 + p.kb_per_split);
@@ -131,9 +133,22 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 
   bool ok = true;
   float sb = 0.f, bias = 0.f;
-  const int n = n0 + (int)threadIdx.x;  // of an epilogue thread
-  const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
+  const int r = threadIdx.x & 127, half = warp >> 2, n = n0 + r;  // of an epilogue thread
+  constexpr int kStep = Cfg::kEpiWarps * 4;                       // tokens until its next 16
+  const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
   OutT* const out = static_cast<OutT*>(p.C) + (int64_t)m0 * p.N + n;
+  // Four tokens of this thread's channel. The values come first and the stores are all that a predicate guards: with a branch around
+  // each token's arithmetic the epilogue of 256 tokens took 10 us.
+  auto store4 = [&](int t, int a, int b, int c, int d) {
+    const float4 s4 = ld_shared_f4(sa + t);
+    const OutT o[4] = {from_f32<OutT>(fmaf((float)a * s4.x, sb, bias)), from_f32<OutT>(fmaf((float)b * s4.y, sb, bias)),
+                       from_f32<OutT>(fmaf((float)c * s4.z, sb, bias)), from_f32<OutT>(fmaf((float)d * s4.w, sb, bias))};
+    const int here = n < p.N ? rows - t : 0;
+    OutT* to = out + (int64_t)t * p.N;
+#pragma unroll
+    for (int i = 0; i < 4; ++i, to += p.N)
+      if (i < here) *to = o[i];
+  };
   if (warp == kProducerWarp) {
     if (ptx::elect_one()) {
       const uint32_t bytes = Cfg::kStageW + p.nt * kBK;
@@ -165,24 +180,23 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     }
     __syncwarp();
   } else {
-    for (int t = threadIdx.x; t < rows; t += 128) sa[t] = __ldg(p.sa + m0 + t);
+    for (int t = threadIdx.x; t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? __ldg(p.sa + m0 + t) : 0.f;
     if (n < p.N) {
       sb = __ldg(p.sb + n);
       if (p.bias != nullptr) bias = to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]);
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(Cfg::kEpiThreads) : "memory");
     ok = ptx::mbar_wait(done_bar, 0, abort_flag);
     grid_launch_dependents();  // as this grid drains
     ptx::tc_fence_after();
     if (splits == 1 && ok) {
 #pragma unroll 1
-      for (int c = 0; c < rows; c += 16) {
+      for (int c = half * 16; c < rows; c += kStep) {
         uint32_t v[32];
         ptx::tmem_ld16(lane_base + c, v);
         ptx::tmem_ld_wait16(v);
 #pragma unroll
-        for (int t = 0; t < 16; ++t)
-          if (c + t < rows && n < p.N) out[(int64_t)(c + t) * p.N] = from_f32<OutT>(fmaf((float)(int)v[t] * sa[c + t], sb, bias));
+        for (int t = 0; t < 16; t += 4) store4(c + t, (int)v[t], (int)v[t + 1], (int)v[t + 2], (int)v[t + 3]);
       }
     }
   }
@@ -191,41 +205,36 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (Cfg::kSumBytes == 0) ptx::cluster_sync();  // every ring is idle: done_bar completes behind the last product
-    const int r = threadIdx.x & 127, share = int8_share(rows, splits), groups = share / 4;  // token t belongs to split t / share
-    if (warp < 4) {
-      int owner = 0, g = 0;
+    const int share = int8_share(rows, splits), groups = share / 4;  // token t belongs to split t / share
+    if (warp < Cfg::kEpiWarps) {
 #pragma unroll 1
-      for (int c = 0; c < rows; c += 16) {
+      for (int c = half * 16; c < rows; c += kStep) {
         uint32_t v[32];
         ptx::tmem_ld16(lane_base + c, v);
+        int owner = c / share, g = (c - owner * share) / 4;
         ptx::tmem_ld_wait16(v);
 #pragma unroll
         for (int t = 0; t < 16; t += 4) {
-          if (c + t < rows)
-            ptx::st_cluster_v4(ptx::mapa(smem_base + kSums, owner) + ((ks * groups + g) * 128 + r) * 16, v[t], v[t + 1], v[t + 2], v[t + 3]);
+          const uint32_t to = ptx::mapa(smem_base + kSums, min(owner, splits - 1)) + ((ks * groups + g) * 128 + r) * 16;
+          if (c + t < rows) ptx::st_cluster_v4(to, v[t], v[t + 1], v[t + 2], v[t + 3]);
           if (++g == groups) g = 0, ++owner;
         }
       }
     }
     __syncwarp();
     ptx::cluster_sync();
-    if (warp < 4 && ok) {
+    if (warp < Cfg::kEpiWarps && ok) {
       const uint32_t src = smem_base + kSums + r * 16;
       const int t0 = ks * share, mine = min(share, rows - t0);
 #pragma unroll 2
-      for (int g = 0; 4 * g < mine; ++g) {
-        int sum[4] = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int c = 0; c < splits; ++c) {
+      for (int g = half; 4 * g < mine; g += Cfg::kEpiWarps / 4) {
+        int4 sum = ptx::ld_shared_i4(src + g * 2048);
+#pragma unroll 3
+        for (int c = 1; c < splits; ++c) {
           const int4 v = ptx::ld_shared_i4(src + (c * groups + g) * 2048);
-          sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (4 * g + i < mine && n < p.N) {
-            const int t = t0 + 4 * g + i;
-            out[(int64_t)t * p.N] = from_f32<OutT>(fmaf((float)sum[i] * sa[t], sb, bias));
-          }
+        store4(t0 + 4 * g, sum.x, sum.y, sum.z, sum.w);
       }
     }
   }

@@ -105,3 +105,27 @@ def test_codes_as_the_kernels_round_them():
         q = fma(rest, r, q)
         whole = (q + f(12582912)).view(np.uint32).astype(np.uint8).view(np.int8)
         assert np.array_equal(whole, np.rint(x / s).astype(np.int8))
+
+
+def test_plan():
+    """Every size, known or odd, gets a kernel that can run it: no empty split, tiles within the kernels' limits, and few rows stream."""
+    import random
+
+    rng = random.Random(0)
+    for _ in range(3000):
+        M, n, K = (int(2 ** rng.uniform(0, 13)), int(2 ** rng.uniform(3, 16)) // 8 * 8, int(2 ** rng.uniform(4, 17)) // 16 * 16)
+        K = min(K, 131056)
+        pl = N.plan_int8(M, n, K, rng.choice([148, 148, 132, 16, 1]))
+        kbs = -(-K // 128)
+        assert 1 <= pl.splits <= 8 and -(-kbs // -(-kbs // pl.splits)) == pl.splits, (M, n, K, pl)
+        if pl.kernel == "pair":
+            assert pl.tile in range(32, 257, 32) and pl.splits in (1, 2, 4) and M > 32
+        else:
+            assert pl.tile in range(16, 257, 16) and pl.tile < M + 16
+    assert N.plan_int8(1, 4096, 4096, 148) == ("stream", 16, 4)
+    assert N.plan_int8(8192, 28672, 4096, 148) == ("pair", 256, 1)
+    with N.tuning(int8_tile=64, int8_splits=8):
+        assert N.plan_int8(100, 4096, 256, 148) == ("stream", 64, 2)
+    with N.tuning(int8_tile=1128, int8_splits=3):
+        assert N.plan_int8(100, 4096, 4096, 148) == ("pair", 128, 1)
+    assert N.load().b200_plan_int8(0, 8, 16, 148, None, None, None) == N.E_BAD_ARG
