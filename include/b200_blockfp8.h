@@ -72,8 +72,8 @@ int b200_read_device_status(int* out, void* stream);
  * linear takes the decode kernel that does wherever that runs; 9 to 16 rows: B200_E_UNSUPPORTED), "moe_decode"
  * (0 = never the weight-streaming MoE kernels, 1 = always, 16 / 32 / 64 = always with that row block), "moe_down_splitk" (0 = never),
  * "moe_zero_pads" (0 / 1), "int8_tile" (16 .. 256 in steps of 16 = always the int8 stream kernel with
- * tiles of that many tokens at most, 1032 .. 1256 in steps of 32 = always the int8 pair kernel with tiles of 32 .. 256
- * columns), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
+ * tiles of that many tokens at most, 1032 .. 1256 and 2032 .. 2256 in steps of 32 = always the int8 pair kernel, the
+ * latter with swapped operands, with tiles of 32 .. 256 columns), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
  * No counterpart in the reference (its Triton launchers read tuned JSON configs instead,
  * python/sglang/srt/layers/moe/fused_moe_triton/fused_moe_triton_config.py). Not thread-safe
  * against concurrent launches: set knobs before the calls they affect. */
@@ -467,9 +467,10 @@ int b200_int8_scaled_mm(const void* A, int64_t lda, const float* sa, const void*
                         const float* sb, const void* bias, void* C, int c_dtype, int64_t M, int64_t N,
                         int64_t K, void* stream);
 
-/* Which kernel a product of this size takes under the present knobs: host arithmetic, for tests and sweeps. *pair != 0: CTA pairs with
- * tiles of *tile columns, else the stream kernel with tiles of *tile tokens; sms = 0: for the current device. */
-int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* pair, int* tile, int* splits);
+/* Which kernel a product of this size takes under the present knobs: host arithmetic, for tests and sweeps. *kernel: 0 the stream
+ * kernel (128 channels by *tile tokens), 1 CTA pairs (256 tokens by *tile channels), 2 swapped pairs (256 channels by *tile tokens);
+ * sms = 0: for the current device. */
+int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* kernel, int* tile, int* splits);
 
 /* b200_w8a8_int8_linear: per_token_quant_int8 of x [M,K] (bf16 / f16, rows x_ld elements apart), then int8_scaled_mm with the weight
  * w [N,K]; out [M,N] of x's type. Replaces W8A8Int8LinearMethod.apply (python/sglang/srt/layers/quantization/w8a8_int8.py).

@@ -305,7 +305,7 @@ def plan_dense(entry: str, M: int, N: int, K: int, sms: int = 0) -> DensePlan:
 
 
 class Int8Plan(NamedTuple):
-    kernel: str  # "stream": tile tokens by 128 channels, "pair": 256 tokens by tile channels
+    kernel: str  # "stream": tile tokens by 128 channels, "pair": 256 tokens by tile channels, "swapped": tile tokens by 256 channels
     tile: int
     splits: int
 
@@ -314,7 +314,7 @@ def plan_int8(M: int, N: int, K: int, sms: int = 0) -> Int8Plan:
     """The kernel that an int8 product of this size takes (``b200_plan_int8``); sms = 0: on the current device."""
     v = [c_int(0) for _ in range(3)]
     check(load().b200_plan_int8(M, N, K, sms, *map(ctypes.byref, v)), "plan_int8")
-    return Int8Plan("pair" if v[0].value else "stream", v[1].value, v[2].value)
+    return Int8Plan(("stream", "pair", "swapped")[v[0].value], v[1].value, v[2].value)
 
 
 def read_device_status() -> int:

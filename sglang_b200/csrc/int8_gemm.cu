@@ -26,9 +26,11 @@ static int check_int8(const char* what, const void* a, int64_t lda, const void* 
   return B200_OK;
 }
 
+enum Int8Kernel { INT8_STREAM = 0, INT8_PAIR = 1, INT8_PAIR_SWAPPED = 2 };
+
 struct Int8Plan {
-  bool pair;   // the pair kernel (tile = columns), else the stream kernel (tile = tokens)
-  int tile, splits;
+  int kernel;
+  int tile, splits;  // tile: tokens (stream, swapped pair) or channels (pair)
   float us;    // what the model expects
 };
 
@@ -65,8 +67,8 @@ static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int 
   const float sum = splits > 1 ? c.sum + c.sum_nt * nt * (splits - 1) / splits : 0.f;
   return c.start + join(per * kbs * rate, memory) + (c.store_nt * nt + sum) * waves + c.cta * items * splits / sms + c.wave * (waves - 1);
 }
-static float pair_us(int64_t M, int64_t N, int64_t K, int bn, int splits, int sms) {
-  const int64_t tiles = cdiv(N, bn) * cdiv(M, 2 * kBM), kbs = cdiv(cdiv(K, kBK), splits);
+static float pair_us(int64_t M, int64_t N, int64_t K, bool swap, int bn, int splits, int sms) {
+  const int64_t tiles = swap ? cdiv(M, bn) * cdiv(N, 2 * kBM) : cdiv(N, bn) * cdiv(M, 2 * kBM), kbs = cdiv(cdiv(K, kBK), splits);
   const int64_t waves = cdiv(tiles, clusters_at_once(2 * splits, sms));
   const float loop = kbs * (0.0898f + 0.0009f * bn), epilogue = 1.01f + 0.0084f * bn;
   const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 5.0e6f;
@@ -80,22 +82,24 @@ static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
   const int forced = t.int8_splits > 0 ? (int)t.int8_splits : 0;
   // no split without a K block
   auto whole = [&](int splits) { return splits <= num_kb && cdiv(num_kb, cdiv(num_kb, splits)) == splits; };
-  Int8Plan best = {false, 16, 1, 1e30f};
-  auto consider = [&](bool pair, int tile, int splits) {
+  Int8Plan best = {INT8_STREAM, 16, 1, 1e30f};
+  auto consider = [&](int kernel, int tile, int splits) {
     if (!whole(splits)) return;
-    const float us = pair ? pair_us(M, N, K, tile, splits, sms) : stream_us(M, N, K, tile, splits, sms);
-    if (us < best.us) best = {pair, tile, splits, us};
+    const float us = kernel == INT8_STREAM ? stream_us(M, N, K, tile, splits, sms)
+                                           : pair_us(M, N, K, kernel == INT8_PAIR_SWAPPED, tile, splits, sms);
+    if (us < best.us) best = {kernel, tile, splits, us};
   };
   if (t.int8_tile > 1000) {
-    const int bn = (int)(t.int8_tile - 1000) / 32 * 32;
-    consider(true, bn < 32 ? 32 : bn > 256 ? 256 : bn, (forced == 2 || forced == 4) && whole(forced) ? forced : 1);
+    const int bn = (int)(t.int8_tile % 1000) / 32 * 32;
+    consider(t.int8_tile > 2000 ? INT8_PAIR_SWAPPED : INT8_PAIR, bn < 32 ? 32 : bn > 256 ? 256 : bn,
+             (forced == 2 || forced == 4) && whole(forced) ? forced : 1);
     return best;
   }
   if (t.int8_tile > 0) {
     const int cap = t.int8_tile < 16 ? 16 : t.int8_tile > 256 ? 256 : (int)t.int8_tile / 16 * 16;
     int splits = forced > kInt8MaxSplits ? kInt8MaxSplits : forced > 0 ? forced : 1;
     while (!whole(splits)) --splits;
-    consider(false, (int)align_up(cdiv(M, cdiv(M, cap)), 16), splits);
+    consider(INT8_STREAM, (int)align_up(cdiv(M, cdiv(M, cap)), 16), splits);
     return best;
   }
   // the tokens in up to eight tiles of equal size
@@ -104,13 +108,15 @@ static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
     if (nt == last) continue;
     last = nt;
     for (int splits = 1; splits <= kInt8MaxSplits; ++splits)
-      if (splits == 1 || cdiv(N, 128) * cdiv(M, nt) * splits <= 2 * sms) consider(false, (int)nt, splits);
+      if (splits == 1 || cdiv(N, 128) * cdiv(M, nt) * splits <= 2 * sms) consider(INT8_STREAM, (int)nt, splits);
     if (nt == 16) break;
   }
   if (M > 32)
     for (int bn = 64; bn <= 256; bn += 32)
-      for (int splits = 1; splits <= 4; splits *= 2)
-        if (splits == 1 || cdiv(N, bn) * cdiv(M, 2 * kBM) * splits <= sms / 2) consider(true, bn, splits);
+      for (int splits = 1; splits <= 4; splits *= 2) {
+        if (splits == 1 || cdiv(N, bn) * cdiv(M, 2 * kBM) * splits <= sms / 2) consider(INT8_PAIR, bn, splits);
+        if (splits == 1 || cdiv(M, bn) * cdiv(N, 2 * kBM) * splits <= sms / 2) consider(INT8_PAIR_SWAPPED, bn, splits);
+      }
   return best;
 }
 
@@ -118,7 +124,12 @@ template <typename OutT>
 static int run_int8(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
   const Int8Plan pl = plan_int8(p.M, p.N, K, sm_count());
   p.nt = pl.tile, p.k_splits = pl.splits;
-  if (pl.pair) return pl.tile > 128 ? launch_int8_pair<256, OutT>(a, lda, b, ldb, K, p, st) : launch_int8_pair<128, OutT>(a, lda, b, ldb, K, p, st);
+  if (pl.kernel == INT8_PAIR)
+    return pl.tile > 128 ? launch_int8_pair<256, false, OutT>(a, lda, b, ldb, K, p, st)
+                         : launch_int8_pair<128, false, OutT>(a, lda, b, ldb, K, p, st);
+  if (pl.kernel == INT8_PAIR_SWAPPED)
+    return pl.tile > 128 ? launch_int8_pair<256, true, OutT>(a, lda, b, ldb, K, p, st)
+                         : launch_int8_pair<128, true, OutT>(a, lda, b, ldb, K, p, st);
   return pl.tile <= 16    ? launch_int8_stream<16, OutT>(a, lda, b, ldb, K, p, st)
          : pl.tile <= 32  ? launch_int8_stream<32, OutT>(a, lda, b, ldb, K, p, st)
          : pl.tile <= 64  ? launch_int8_stream<64, OutT>(a, lda, b, ldb, K, p, st)
@@ -147,11 +158,11 @@ static int run_int8(const void* a, int64_t lda, const float* sa, const void* b, 
 
 }  // namespace b200
 
-extern "C" int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* pair, int* tile, int* splits) {
+extern "C" int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* kernel, int* tile, int* splits) {
   using namespace b200;
-  B200_CHECK_ARG(M > 0 && N > 0 && K > 0 && sms >= 0 && pair && tile && splits, "plan_int8: empty shape or null pointer");
+  B200_CHECK_ARG(M > 0 && N > 0 && K > 0 && sms >= 0 && kernel && tile && splits, "plan_int8: empty shape or null pointer");
   const Int8Plan pl = plan_int8(M, N, K, sms > 0 ? sms : sm_count());
-  *pair = pl.pair, *tile = pl.tile, *splits = pl.splits;
+  *kernel = pl.kernel, *tile = pl.tile, *splits = pl.splits;
   return B200_OK;
 }
 

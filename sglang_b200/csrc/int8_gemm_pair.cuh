@@ -2,6 +2,8 @@
 // Each CTA loads its own 128 rows of A and half of the B tile: with 256 columns 32 KB per 128 of K, which at 128 B/clk in and
 // out of shared memory fit the 512 clocks of its products. Two accumulators of BN columns in TMEM, so that the epilogue of a tile
 // runs under the products of the next. The width of a tile is any multiple of 32: the launch takes the one that fills its waves.
+// SWAP: the 256 rows are rows of B, output channels, and the columns are tokens, so that a tile's width divides their number evenly:
+// 1027 tokens are multiplied as 5 x 224 and not as 5 x 256. A thread then owns a channel and its boxes are written by columns.
 // Few tiles: the K splits of a tile, 2 or 4, are one cluster; every one of them sums and stores its share of the 32-column chunks,
 // the others hand theirs over through distributed shared memory, into the ring, which is idle by then.
 // Roles per CTA (320 threads):
@@ -53,7 +55,7 @@ struct Int8PairCfg {
   static_assert(kStages * (kStageA + kStageB) >= 6 * 16384, "the sums of the other splits fit the ring");
 };
 
-template <int BN, typename OutT>
+template <int BN, bool SWAP, typename OutT>
 __global__ void __launch_bounds__(Int8PairCfg<BN, OutT>::kThreads, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const __grid_constant__ CUtensorMap tmap_c, const Int8Params p) {
@@ -114,10 +116,10 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   auto coords = [&](int t, int& mt, int& nt) { tile_coords(t, p.m_tiles, p.n_tiles, p.group_m, p.per_group_div, mt, nt); };
   // What is read and overwritten below belongs to the kernels before, which may still run; the weights of the first K blocks are
   // asked for all the same, as a prefetch into L2, a row each.
-  if ((int)threadIdx.x < bn / 2) {
+  if ((int)threadIdx.x < (SWAP ? kBM : bn / 2)) {
     int mt, nt;
     coords(pair, mt, nt);
-    const int row = nt * bn + (int)rank * (bn / 2) + (int)threadIdx.x;
+    const int row = (SWAP ? mt * 2 * kBM + (int)rank * kBM : nt * bn + (int)rank * (bn / 2)) + (int)threadIdx.x;
     if (row < p.N)
       prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)row * p.w_ld + kb0 * kBK, min(kPrefetchKb, kb1 - kb0));
   }
@@ -192,12 +194,19 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       int mt, nt;
       coords(t, mt, nt);
       const int row0 = mt * 2 * kBM + (int)rank * kBM + quarter * 32, row = row0 + lane;
-      const float sa = row < p.M ? __ldg(p.sa + row) : 0.f;
+      // scale (and bias) of this thread's row and of the tile's columns
+      auto load_bias = [&](int n) { return p.bias != nullptr ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f; };
+      float own = 0.f, own_bias = 0.f;
+      if (row < (SWAP ? p.N : p.M)) {
+        own = __ldg((SWAP ? p.sb : p.sa) + row);
+        if (SWAP) own_bias = load_bias(row);
+      }
       __syncwarp();  // the last tile's columns have been read
       for (int j = half; j < chunks; j += 2) {
-        const int n = nt * bn + j * 32 + lane;
-        my_cols[(j >> 1) * 32 + lane] = n < p.N ? __ldg(p.sb + n) : 0.f;
-        my_cols[Cfg::kCols + (j >> 1) * 32 + lane] = n < p.N && p.bias != nullptr ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f;
+        const int n = nt * bn + j * 32 + lane, at = (j >> 1) * 32 + lane;
+        const bool inside = n < (SWAP ? p.M : p.N);
+        my_cols[at] = inside ? __ldg((SWAP ? p.sa : p.sb) + n) : 0.f;
+        if (!SWAP) my_cols[Cfg::kCols + at] = inside ? load_bias(n) : 0.f;
       }
       __syncwarp();
       bool ok = ptx::mbar_wait(tfull_bar(b), phase, abort_flag);
@@ -244,27 +253,48 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         ++box_no;
         if (lane == 0) ptx::tma_store_wait_read_but_one();  // the box before the last has left this half of the staging area
         __syncwarp();
-        const float* sb = my_cols + (j >> 1) * 32;
+        const float* col = my_cols + (j >> 1) * 32;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float f[8];
 #pragma unroll
           for (int i = 0; i < 8; i += 4) {
-            const float4 s4 = ld_shared_f4(sb + 8 * g + i), b4 = ld_shared_f4(sb + Cfg::kCols + 8 * g + i);
-            f[i + 0] = fmaf((float)(int)v[8 * g + i + 0] * sa, s4.x, b4.x);
-            f[i + 1] = fmaf((float)(int)v[8 * g + i + 1] * sa, s4.y, b4.y);
-            f[i + 2] = fmaf((float)(int)v[8 * g + i + 2] * sa, s4.z, b4.z);
-            f[i + 3] = fmaf((float)(int)v[8 * g + i + 3] * sa, s4.w, b4.w);
+            const uint32_t* q = v + 8 * g + i;
+            const float4 c4 = ld_shared_f4(col + 8 * g + i);
+            if constexpr (SWAP) {
+              f[i + 0] = fmaf((float)(int)q[0] * c4.x, own, own_bias);
+              f[i + 1] = fmaf((float)(int)q[1] * c4.y, own, own_bias);
+              f[i + 2] = fmaf((float)(int)q[2] * c4.z, own, own_bias);
+              f[i + 3] = fmaf((float)(int)q[3] * c4.w, own, own_bias);
+            } else {
+              const float4 b4 = ld_shared_f4(col + Cfg::kCols + 8 * g + i);
+              f[i + 0] = fmaf((float)(int)q[0] * own, c4.x, b4.x);
+              f[i + 1] = fmaf((float)(int)q[1] * own, c4.y, b4.y);
+              f[i + 2] = fmaf((float)(int)q[2] * own, c4.z, b4.z);
+              f[i + 3] = fmaf((float)(int)q[3] * own, c4.w, b4.w);
+            }
           }
-          // rows of 64 bytes (16-bit types) or 128, in the swizzle of the tensor map
-          if constexpr (sizeof(OutT) == 2) {
+          // the box has rows of 64 bytes (16-bit types) or 128, tokens, in the swizzle of the tensor map
+          constexpr int kRow = 32 * (int)sizeof(OutT), kXor = kRow / 16 - 1, kShift = kRow == 64 ? 1 : 0;
+          if constexpr (SWAP) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int t = 8 * g + i, byte = lane * (int)sizeof(OutT);
+              const OutT o = from_f32<OutT>(f[i]);
+              const uint32_t at = box + t * kRow + (((byte >> 4) ^ ((t >> kShift) & kXor)) << 4) + (byte & 15);
+              if constexpr (sizeof(OutT) == 2)
+                asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(*reinterpret_cast<const uint16_t*>(&o)) : "memory");
+              else
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(o) : "memory");
+            }
+          } else if constexpr (sizeof(OutT) == 2) {
             const uint4 o = pack8<OutT>(f);
-            const uint32_t at = box + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4);
+            const uint32_t at = box + lane * kRow + ((g ^ ((lane >> kShift) & kXor)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w) : "memory");
           } else {
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
-              const uint32_t at = box + lane * 128 + (((2 * g + i / 4) ^ (lane & 7)) << 4);
+              const uint32_t at = box + lane * kRow + (((2 * g + i / 4) ^ (lane & kXor)) << 4);
               asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(f[i]), "f"(f[i + 1]), "f"(f[i + 2]), "f"(f[i + 3]) : "memory");
             }
           }
@@ -273,7 +303,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         __syncwarp();
         if (lane == 0) {
           const int col0 = nt * bn + j * 32;
-          if (row0 < p.M && col0 < p.N) ptx::tma_store_2d(&tmap_c, box, col0, row0);
+          const int channel = SWAP ? row0 : col0, token = SWAP ? col0 : row0;
+          if (token < p.M && channel < p.N) ptx::tma_store_2d(&tmap_c, box, channel, token);
           ptx::tma_store_commit();
         }
       }
@@ -305,24 +336,25 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 }
 
 // p.nt columns per tile (a multiple of 32, at most BN), p.k_splits 1, 2 or 4.
-template <int BN, typename OutT>
+template <int BN, bool SWAP, typename OutT>
 inline int launch_int8_pair(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
   using Cfg = Int8PairCfg<BN, OutT>;
-  p.m_tiles = (int)cdiv(p.M, 2 * kBM);
-  p.n_tiles = (int)cdiv(p.N, p.nt);
+  const int64_t rows = SWAP ? p.N : p.M, cols = SWAP ? p.M : p.N;
+  p.m_tiles = (int)cdiv(rows, 2 * kBM);
+  p.n_tiles = (int)cdiv(cols, p.nt);
   p.kb_per_split = (int)cdiv(p.num_kb, p.k_splits);
-  p.group_m = row_group(p.M, K, 2 * kBM);
+  p.group_m = row_group(rows, K, 2 * kBM);
   p.per_group_div = make_fastdiv(p.group_m * p.n_tiles);
   CUtensorMap ta, tb, tc;
-  if (int rc = encode_tmap_s8(&ta, A, p.M, K, lda, kBM, "A")) return rc;
-  if (int rc = encode_tmap_s8(&tb, B, p.N, K, ldb, p.nt / 2, "B")) return rc;
+  if (int rc = encode_tmap_s8(&ta, SWAP ? B : A, rows, K, SWAP ? ldb : lda, kBM, "rows")) return rc;
+  if (int rc = encode_tmap_s8(&tb, SWAP ? A : B, cols, K, SWAP ? lda : ldb, p.nt / 2, "columns")) return rc;
   const CUtensorMapDataType type = sizeof(OutT) == 4                                ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : std::is_same<OutT, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (int rc = encode_tmap(&tc, type, (int)sizeof(OutT), p.C, p.M, p.N, p.N, 32, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE, "C")) return rc;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   const int slots = sm_count() / 2, pairs = (int)(p.k_splits > 1 || tiles < slots ? tiles : slots);
-  auto k = int8_pair_kernel<BN, OutT>;
+  auto k = int8_pair_kernel<BN, SWAP, OutT>;
   if (int rc = allow_smem(k, Cfg::kSmemBytes, "int8_pair_kernel")) return rc;
   return launch_dependent(k, dim3((unsigned)(2 * pairs * p.k_splits)), Cfg::kThreads, Cfg::kSmemBytes, st, 2u * p.k_splits,
                           "int8_pair_kernel", ta, tb, tc, p);

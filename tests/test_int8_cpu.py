@@ -118,7 +118,7 @@ def test_plan():
         pl = N.plan_int8(M, n, K, rng.choice([148, 148, 132, 16, 1]))
         kbs = -(-K // 128)
         assert 1 <= pl.splits <= 8 and -(-kbs // -(-kbs // pl.splits)) == pl.splits, (M, n, K, pl)
-        if pl.kernel == "pair":
+        if pl.kernel != "stream":
             assert pl.tile in range(32, 257, 32) and pl.splits in (1, 2, 4) and M > 32
         else:
             assert pl.tile in range(16, 257, 16) and pl.tile < M + 16
@@ -128,4 +128,6 @@ def test_plan():
         assert N.plan_int8(100, 4096, 256, 148) == ("stream", 64, 2)
     with N.tuning(int8_tile=1128, int8_splits=3):
         assert N.plan_int8(100, 4096, 4096, 148) == ("pair", 128, 1)
+    with N.tuning(int8_tile=2224):
+        assert N.plan_int8(100, 4096, 4096, 148) == ("swapped", 224, 1)
     assert N.load().b200_plan_int8(0, 8, 16, 148, None, None, None) == N.E_BAD_ARG

@@ -96,7 +96,7 @@ def test_the_same_bits_on_every_run_and_for_every_batch():
             assert torch.equal(S.int8_scaled_mm(a[:m], b.t(), sa[:m], sb, torch.bfloat16, bias.bfloat16()), full[:m]), m
 
 
-@pytest.mark.parametrize("tile", [16, 32, 48, 64, 96, 128, 208, 256, 1032, 1064, 1096, 1128, 1160, 1192, 1224, 1256])
+@pytest.mark.parametrize("tile", [16, 32, 48, 64, 96, 128, 208, 256, 1032, 1064, 1096, 1128, 1160, 1192, 1224, 1256, 2032, 2064, 2096, 2128, 2160, 2192, 2224, 2256])
 @pytest.mark.parametrize("splits", [1, 2, 3, 4, 5, 7, 8])
 def test_every_tile_and_split(tile, splits):
     """The kernels that the plan chooses from, each at sizes that it would not be chosen for, too."""
