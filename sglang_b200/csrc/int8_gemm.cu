@@ -47,16 +47,16 @@ static float join(float a, float b) {  // near the larger of the two, a little a
   return sqrtf(sqrtf(a * a + b * b));
 }
 
-// Time of one call in us, back to back with others. The constants are fitted to 2269 sizes (1 to 4096 rows, N 256 to 57344, K 256 to 28672),
-// each measured with every tile and split below: the choice is 1.5 % behind the best of them on average, 5 % at the 90th percentile.
+// Time of one call in us, back to back with others. The constants are fitted to 4727 sizes (1 to 4096 rows, N 256 to 57344, K 256 to 28672),
+// each measured with every tile and split below: the choice is 1.7 % behind the best of them on average, 6 % at the 90th percentile.
 struct StreamCost {
   float start, alone, alone_nt, shared, shared_nt;  // a K block of a CTA that has its SM to itself, of one of several on an SM
   float bandwidth, store_nt, sum, sum_nt, cta, wave;
 };
 static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int sms) {
-  static const StreamCost few = {1.96f, 0.220f, 0.0012f, 0.130f, 0.0034f, 6.30e6f, 0.f, 0.27f, 0.f, 1.13f, 0.29f};
-  static const StreamCost some = {1.61f, 0.1855f, 0.0023f, 0.1205f, 0.0015f, 6.06e6f, 0.0098f, 0.38f, 0.0121f, 1.13f, 0.22f};
-  static const StreamCost many = {1.61f, 0.1854f, 0.0006f, 0.1117f, 0.0010f, 5.84e6f, 0.0106f, 0.53f, 0.0210f, 1.09f, 0.68f};
+  static const StreamCost few = {1.89f, 0.220f, 0.0010f, 0.130f, 0.0031f, 6.26e6f, 0.0061f, 0.27f, 0.f, 1.10f, 0.36f};
+  static const StreamCost some = {1.76f, 0.1816f, 0.0023f, 0.1177f, 0.0017f, 5.98e6f, 0.0084f, 0.38f, 0.0109f, 1.03f, 0.10f};
+  static const StreamCost many = {1.61f, 0.1835f, 0.0006f, 0.1088f, 0.0010f, 5.83e6f, 0.0109f, 0.49f, 0.0204f, 1.09f, 0.79f};
   const StreamCost& c = M <= 16 ? few : M <= 64 ? some : many;
   const int per_sm = nt <= 64 ? 2 : 1;
   const int64_t items = cdiv(N, 128) * cdiv(M, nt), kbs = cdiv(cdiv(K, kBK), splits);
@@ -70,10 +70,10 @@ static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int 
 static float pair_us(int64_t M, int64_t N, int64_t K, bool swap, int bn, int splits, int sms) {
   const int64_t tiles = swap ? cdiv(M, bn) * cdiv(N, 2 * kBM) : cdiv(N, bn) * cdiv(M, 2 * kBM), kbs = cdiv(cdiv(K, kBK), splits);
   const int64_t waves = cdiv(tiles, clusters_at_once(2 * splits, sms));
-  const float loop = kbs * (0.0898f + 0.0009f * bn), epilogue = 1.01f + 0.0084f * bn;
-  const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 5.0e6f;
-  const float sum = splits > 1 ? 1.36f + 0.0178f * bn * (splits - 1) / splits : 0.f;
-  return 3.52f + join((waves - 1) * (loop > epilogue ? loop : epilogue) + loop, memory) + 0.0045f * bn + sum * waves;
+  const float loop = kbs * (0.0891f + 0.0009f * bn), epilogue = 0.96f + (swap ? 0.009f : 0.0082f) * bn;
+  const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 5.07e6f;
+  const float sum = splits > 1 ? 1.35f + 0.017f * bn * (splits - 1) / splits : 0.f;
+  return 3.52f + join((waves - 1) * (loop > epilogue ? loop : epilogue) + loop, memory) + (swap ? 0.0055f : 0.005f) * bn + sum * waves;
 }
 
 static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
