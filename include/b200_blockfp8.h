@@ -73,7 +73,8 @@ int b200_read_device_status(int* out, void* stream);
  * (0 = never the weight-streaming MoE kernels, 1 = always, 16 / 32 / 64 = always with that row block), "moe_down_splitk" (0 = never),
  * "moe_zero_pads" (0 / 1), "int8_tile" (16 .. 256 in steps of 16 = always the int8 stream kernel with
  * tiles of that many tokens at most, 1032 .. 1256 and 2032 .. 2256 in steps of 32 = always the int8 pair kernel, the
- * latter with swapped operands, with tiles of 32 .. 256 columns), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
+ * latter with swapped operands, with tiles of 32 .. 256 columns), "int8_linear_fused" (0 / 1 = the int8 linear never / up to 4 rows always
+ * quantises in the product's kernel), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
  * No counterpart in the reference (its Triton launchers read tuned JSON configs instead,
  * python/sglang/srt/layers/moe/fused_moe_triton/fused_moe_triton_config.py). Not thread-safe
  * against concurrent launches: set knobs before the calls they affect. */
@@ -474,8 +475,9 @@ int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* kernel, int* t
 
 /* b200_w8a8_int8_linear: per_token_quant_int8 of x [M,K] (bf16 / f16, rows x_ld elements apart), then int8_scaled_mm with the weight
  * w [N,K]; out [M,N] of x's type. Replaces W8A8Int8LinearMethod.apply (python/sglang/srt/layers/quantization/w8a8_int8.py).
- * workspace: the quantised rows and their scales, 16-byte aligned, the caller's until the kernels are done. */
-size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ * workspace: the quantised rows and their scales, 16-byte aligned, the caller's until the kernels are done; none where a few short
+ * rows (M <= 4, K <= 6144, M*K <= 8192) that start at multiples of 16 bytes (x_aligned) are quantised by the product's own kernel. The result is the same. */
+size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_aligned);
 int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, const void* w, int64_t ldw,
                           const float* sw, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
                           void* workspace, size_t workspace_bytes, void* stream);

@@ -138,7 +138,7 @@ SIGNATURES = {
          c_void_p],
     ),
     "b200_plan_int8": (c_int, [c_int64, c_int64, c_int64, c_int, POINTER(c_int), POINTER(c_int), POINTER(c_int)]),
-    "b200_w8a8_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "b200_w8a8_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
     "b200_w8a8_int8_linear": (
         c_int,
         [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t,

@@ -533,10 +533,11 @@ PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   {
     WithoutInterpreterLock unlocked;
     out = empty_on(dev, with_last(*x, N), type);
-    const size_t need = abi.int8_linear_ws(M, N, K);
-    const Tensor ws = empty_on(dev, {(int64_t)need}, at::kByte);
+    const bool aligned = reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0 && (M == 1 || ld % 8 == 0);
+    const size_t need = abi.int8_linear_ws(M, N, K, aligned);
+    const Tensor ws = need ? empty_on(dev, {(int64_t)need}, at::kByte) : Tensor();
     rc = abi.int8_linear(x->data_ptr(), ld, code, w->data_ptr(), N > 1 ? w->stride(0) : K, sw->data_ptr<float>(),
-                         biased ? bias->data_ptr() : nullptr, out.data_ptr(), M, N, K, ws.data_ptr(), need, stream_of(dev));
+                         biased ? bias->data_ptr() : nullptr, out.data_ptr(), M, N, K, need ? ws.data_ptr() : nullptr, need, stream_of(dev));
   }
   if (rc) return fail(rc, "w8a8_int8_linear");
   return THPVariable_Wrap(std::move(out));

@@ -130,25 +130,30 @@ static int run_int8(const void* a, int64_t lda, const void* b, int64_t ldb, int6
   if (pl.kernel == INT8_PAIR_SWAPPED)
     return pl.tile > 128 ? launch_int8_pair<256, true, OutT>(a, lda, b, ldb, K, p, st)
                          : launch_int8_pair<128, true, OutT>(a, lda, b, ldb, K, p, st);
-  return pl.tile <= 16    ? launch_int8_stream<16, OutT>(a, lda, b, ldb, K, p, st)
-         : pl.tile <= 32  ? launch_int8_stream<32, OutT>(a, lda, b, ldb, K, p, st)
-         : pl.tile <= 64  ? launch_int8_stream<64, OutT>(a, lda, b, ldb, K, p, st)
-         : pl.tile <= 128 ? launch_int8_stream<128, OutT>(a, lda, b, ldb, K, p, st)
-                        : launch_int8_stream<256, OutT>(a, lda, b, ldb, K, p, st);
+  return pl.tile <= 16    ? launch_int8_stream<16, false, OutT>(a, lda, b, ldb, K, p, st)
+         : pl.tile <= 32  ? launch_int8_stream<32, false, OutT>(a, lda, b, ldb, K, p, st)
+         : pl.tile <= 64  ? launch_int8_stream<64, false, OutT>(a, lda, b, ldb, K, p, st)
+         : pl.tile <= 128 ? launch_int8_stream<128, false, OutT>(a, lda, b, ldb, K, p, st)
+                        : launch_int8_stream<256, false, OutT>(a, lda, b, ldb, K, p, st);
+}
+
+static int fill_int8(Int8Params& p, const float* sa, const void* b, int64_t ldb, const float* sb, const void* bias, void* c, int64_t M,
+                     int64_t N, int64_t K) {
+  p = {};
+  p.sa = sa, p.sb = sb, p.bias = bias, p.C = c;
+  p.w = static_cast<const int8_t*>(b), p.w_ld = ldb;
+  p.M = (int)M, p.N = (int)N, p.num_kb = (int)cdiv(K, kBK);
+  p.status = device_status_word();
+  if (p.status) return B200_OK;
+  set_error_detail("cannot resolve the device status word");
+  return B200_E_LAUNCH;
 }
 
 // Checked operands.
 static int run_int8(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, const void* bias, void* c,
                     int c_dtype, int64_t M, int64_t N, int64_t K, cudaStream_t st) {
-  Int8Params p = {};
-  p.sa = sa, p.sb = sb, p.bias = bias, p.C = c;
-  p.w = static_cast<const int8_t*>(b), p.w_ld = ldb;
-  p.M = (int)M, p.N = (int)N, p.num_kb = (int)cdiv(K, kBK);
-  p.status = device_status_word();
-  if (!p.status) {
-    set_error_detail("cannot resolve the device status word");
-    return B200_E_LAUNCH;
-  }
+  Int8Params p;
+  if (int rc = fill_int8(p, sa, b, ldb, sb, bias, c, M, N, K)) return rc;
   switch (c_dtype) {
     case B200_BF16: return run_int8<__nv_bfloat16>(a, lda, b, ldb, K, p, st);
     case B200_F16: return run_int8<__half>(a, lda, b, ldb, K, p, st);
@@ -175,9 +180,30 @@ extern "C" int b200_int8_scaled_mm(const void* a, int64_t lda, const float* sa, 
   return run_int8(a, lda, sa, b, ldb, sb, bias, c, c_dtype, M, N, K, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+namespace b200 {
+
+// One launch for the layer, where the rows are few and short enough that every CTA may look for their largest magnitudes itself, and
+// start at multiples of 16 bytes. Two launches and one, replayed from a graph, 1 row: 6144 x 4096 9.06, 8.87 us; 28672 x 2048 14.4, 13.1;
+// past the limits 4096 x 14336 14.3, 15.0, and 4 rows 6144 x 4096 9.2, 9.2; launched from Python 7.0, 5.2 us of host time.
+static bool linear_fuses(int64_t M, int64_t K, int aligned) {
+  if (!aligned || M > Int8StreamCfg<16, true>::kQuantRows || tuning().int8_linear_fused == 0) return false;
+  return tuning().int8_linear_fused > 0 || (K <= 6144 && M * K <= 8192);
+}
+
+template <typename T>
+static int run_int8_linear_fused(const void* x, int64_t x_ld, const void* w, int64_t ldw, int64_t K, Int8Params p, cudaStream_t st) {
+  const Int8Plan pl = plan_int8(p.M, p.N, K, sm_count());  // 16 tokens: the stream kernel
+  p.x = x, p.x_ld = x_ld;
+  p.nt = 16, p.k_splits = pl.kernel == INT8_STREAM ? pl.splits : 1;
+  return launch_int8_stream<16, true, T>(nullptr, 0, w, ldw, K, p, st);
+}
+
+}  // namespace b200
+
+extern "C" size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_aligned) {
   (void)N;
-  return M > 0 && K > 0 ? b200::align_up((size_t)M * K, 16) + (size_t)M * 4 : 0;
+  if (M <= 0 || K <= 0 || b200::linear_fuses(M, K, x_aligned)) return 0;
+  return b200::align_up((size_t)M * K, 16) + (size_t)M * 4;
 }
 
 extern "C" int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, const void* w, int64_t ldw, const float* sw,
@@ -186,14 +212,25 @@ extern "C" int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, c
   using namespace b200;
   B200_CHECK_ARG(M >= 0 && N >= 0 && K >= 0, "w8a8_int8_linear: negative shape");
   if (M == 0 || N == 0) return B200_OK;
+  B200_CHECK_ARG(x && (uintptr_t)x % 2 == 0, "w8a8_int8_linear: null or misaligned input");
   B200_CHECK_ARG(x_dtype == B200_BF16 || x_dtype == B200_F16, "w8a8_int8_linear: input dtype code %d", x_dtype);
-  if (workspace == nullptr || workspace_bytes < b200_w8a8_int8_linear_workspace_bytes(M, N, K)) {
-    set_error_detail("w8a8_int8_linear: workspace of %zu bytes, %zu needed", workspace_bytes, b200_w8a8_int8_linear_workspace_bytes(M, N, K));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int aligned = (uintptr_t)x % 16 == 0 && (M == 1 || x_ld % 8 == 0);
+  if (linear_fuses(M, K, aligned)) {
+    if (int rc = check_int8("w8a8_int8_linear", w, ldw, w, ldw, sw, sw, out, x_dtype, M, N, K)) return rc;
+    Int8Params p;
+    if (int rc = fill_int8(p, nullptr, w, ldw, sw, bias, out, M, N, K)) return rc;
+    return x_dtype == B200_BF16 ? run_int8_linear_fused<__nv_bfloat16>(x, x_ld, w, ldw, K, p, st)
+                                : run_int8_linear_fused<__half>(x, x_ld, w, ldw, K, p, st);
+  }
+  const size_t need = b200_w8a8_int8_linear_workspace_bytes(M, N, K, 0);
+  if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0) {
+    set_error_detail("w8a8_int8_linear: workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, need);
     return B200_E_WORKSPACE;
   }
   void* q = workspace;
   float* s = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align_up((size_t)M * K, 16));
   if (int rc = check_int8("w8a8_int8_linear", q, K, w, ldw, s, sw, out, x_dtype, M, N, K)) return rc;
   if (int rc = b200_per_token_quant_int8(x, x_ld, x_dtype, q, s, M, K, 0, stream)) return rc;
-  return run_int8(q, K, s, w, ldw, sw, bias, out, x_dtype, M, N, K, static_cast<cudaStream_t>(stream));
+  return run_int8(q, K, s, w, ldw, sw, bias, out, x_dtype, M, N, K, st);
 }

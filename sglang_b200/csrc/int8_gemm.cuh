@@ -5,6 +5,7 @@
 #pragma once
 
 #include "gemm_pair.cuh"
+#include "int8_round.cuh"
 
 namespace b200 {
 
@@ -36,11 +37,13 @@ __host__ __device__ constexpr uint32_t idesc_s8_s32(int M, int N) {
 
 struct Int8Params {
   const float *sa, *sb;  // [M], [N]
+  const void* x;         // QUANT: 16-bit rows [M, K], x_ld elements apart
+  int64_t x_ld;
   const void* bias;      // [N] of the output's type, or null
   void* C;               // [M, N], contiguous
   const int8_t* w;       // B, for prefetches
   int64_t w_ld;
-  int M, N, num_kb;
+  int M, N, K, num_kb;
   int n_tiles, t_tiles;
   int nt, k_splits, kb_per_split;           // stream kernel: tokens of a tile, K splits of an item (one cluster)
   int m_tiles, group_m;                     // pair kernel
@@ -52,7 +55,7 @@ struct Int8Params {
 // 16, at most NT) are its columns, so that few tokens waste little and a thread of the epilogue owns one output channel.
 // Work item = (128 rows of B, nt tokens, K split); one CTA each. The K splits of an item are one cluster: they exchange their integer
 // sums through distributed shared memory, every one of them adding up and storing its share of the tokens.
-// Sums of four tokens travel as one 16-byte store per lane: 203 x 4096 x 14336 in four splits went from 25 us, a word at a time, to XX.
+// Sums of four tokens travel as one 16-byte store per lane: 203 x 4096 x 14336 in four splits 25.3 us a word at a time, 22.9 so.
 constexpr int kInt8MaxSplits = 8;
 __host__ __device__ constexpr int int8_share(int rows, int splits) { return ((rows + splits - 1) / splits + 3) / 4 * 4; }  // tokens per split
 constexpr int int8_sum_rows(int nt) {
@@ -61,25 +64,30 @@ constexpr int int8_sum_rows(int nt) {
   return most;
 }
 
-template <int NT>
+template <int NT, bool QUANT>
 struct Int8StreamCfg {
   static constexpr int kStageW = 128 * kBK, kStageX = NT * kBK;
   static constexpr int kCtasPerSm = NT <= 64 ? 2 : 1;
   static constexpr int kStages = NT == 16 ? 5 : NT == 32 ? 4 : NT == 64 ? 4 : NT == 128 ? 6 : 4;
   // With many tokens two epilogue warps share 32 channels and take every second 16 tokens each
   static constexpr int kEpiWarps = NT <= 32 ? 4 : 8, kEpiThreads = kEpiWarps * 32;
-  static constexpr int kProducerWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1, kThreads = kEpiThreads + 64;
+  static constexpr int kProducerWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1;
+  static constexpr int kQuantRows = 4, kQuantWarps = 4;  // QUANT: rows that the quantiser warps cover
+  static constexpr int kThreads = kEpiThreads + 64 + (QUANT ? kQuantWarps * 32 : 0);
   static constexpr int kTmemCols = NT < 32 ? 32 : NT;
   // sums of the splits, [split][tokens of this CTA / 4][128][4]; with many tokens they go to the ring once it is idle
   static constexpr int kSumBytes = NT <= 32 ? int8_sum_rows(NT) * 512 : 0;
-  static constexpr size_t kSmemBytes = (size_t)kStages * (kStageW + kStageX) + kSumBytes + NT * 4 + 1024 + 256;
+  static constexpr size_t kSmemBytes = (size_t)kStages * (kStageW + kStageX) + kSumBytes + NT * 4 + (QUANT ? 32 : 0) + 1024 + 256;
   static_assert(kSumBytes > 0 || int8_sum_rows(NT) * 512 <= kStages * (kStageW + kStageX), "the sums fit the ring");
 };
 
-template <int NT, typename OutT>
-__global__ void __launch_bounds__(Int8StreamCfg<NT>::kThreads)
+// QUANT: A is the 16-bit input of a linear layer, up to four rows. While the weights fill the ring, every CTA finds the rows' largest
+// magnitudes (the epilogue warps and four more, a whole row from L2), then the four quantise the K blocks of the CTA into the ring,
+// bit for bit as the stand-alone quantiser does: one launch for the layer instead of two.
+template <int NT, bool QUANT, typename OutT>
+__global__ void __launch_bounds__(Int8StreamCfg<NT, QUANT>::kThreads)
 int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8Params p) {
-  using Cfg = Int8StreamCfg<NT>;
+  using Cfg = Int8StreamCfg<NT, QUANT>;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -87,7 +95,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const uint32_t sW = smem_base, sX = smem_base + S * Cfg::kStageW;
   constexpr uint32_t kRing = S * (Cfg::kStageW + Cfg::kStageX), kSums = Cfg::kSumBytes ? kRing : 0;
   float* sa = reinterpret_cast<float*>(smem_al + kRing + Cfg::kSumBytes);  // [NT]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sa + NT);
+  float* tops = sa + NT;                                                   // QUANT: [rows][parts of a row], one a warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tops + (QUANT ? 8 : 0));
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
@@ -101,10 +110,15 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const int n_tile = tile / p.t_tiles, n0 = n_tile * 128, m0 = (tile - n_tile * p.t_tiles) * p.nt;
   const int kb0 = ks * p.kb_per_split, kb1 = min(p.num_kb, kb0 + p.kb_per_split);
   const int rows = min(p.nt, p.M - m0);
+  // QUANT: 16 groups of eight lanes take four rows of four K blocks side by side. Four K blocks are fewer than the ring's stages: with more
+  // under way a group would wait for a phase of a stage's barrier that is two ahead of it, which the parity does not tell
+  // from the one before.
+  constexpr int kQuantRows = Cfg::kQuantRows;
+  static_assert(!QUANT || (NT == 16 && S > 4), "the K blocks under way fit the ring");
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(full_bar(s), QUANT ? 1 + kQuantRows : 1);
       ptx::mbar_init(empty_bar(s), 1);
     }
     ptx::mbar_init(done_bar, 1);
@@ -117,7 +131,7 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   }
   if (warp == kProducerWarp && lane == 0) {
     ptx::prefetch_tensormap(&tmap_w);
-    ptx::prefetch_tensormap(&tmap_x);
+    if (!QUANT) ptx::prefetch_tensormap(&tmap_x);
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -132,9 +146,9 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   grid_dependency_wait();
 
   bool ok = true;
-  float sb = 0.f, bias = 0.f;
+  float sb = 0.f, bias = 0.f, scale_of_lane = 0.f;
   const int r = threadIdx.x & 127, half = warp >> 2, n = n0 + r;  // of an epilogue thread
-  constexpr int kStep = Cfg::kEpiWarps * 4;                       // tokens until its next 16
+  constexpr int kNext = Cfg::kEpiWarps * 4;                       // tokens until its next 16
   const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
   OutT* const out = static_cast<OutT*>(p.C) + (int64_t)m0 * p.N + n;
   // Four tokens of this thread's channel. The values come first and the stores are all that a predicate guards: with a branch around
@@ -149,16 +163,64 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     for (int i = 0; i < 4; ++i, to += p.N)
       if (i < here) *to = o[i];
   };
+  // QUANT: eight lanes hold the 128 values of one (row, K block), 16 each; the groups of a warp have the same K block
+  constexpr int kStep = 4 * Cfg::kQuantWarps / kQuantRows, kAhead = 4;  // K blocks side by side, and in flight per group
+  const int q_tid = threadIdx.x - (kMmaWarp + 1) * 32, chunk = q_tid & 7, q_row = (q_tid >> 3) & (kQuantRows - 1);
+  const int first = (q_tid >> 3) / kQuantRows, nkb = kb1 - kb0;
+  uint4 raw[kAhead][2];
+  auto request = [&](int j, int u) {
+    const int k = (kb0 + j) * kBK + chunk * 16;  // K is a multiple of 16
+    const OutT* src = static_cast<const OutT*>(p.x) + (m0 + min(q_row, rows - 1)) * p.x_ld + k;
+    const bool inside = j < nkb && k < p.K;
+    raw[u][0] = inside ? ld_nc_16(src) : make_uint4(0, 0, 0, 0);
+    raw[u][1] = inside ? ld_nc_16(src + 8) : make_uint4(0, 0, 0, 0);
+  };
+  if constexpr (QUANT) {
+    if (warp > kMmaWarp)
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) request(first + u * kStep, u);
+    // largest magnitudes: the eight warps that do not drive the pipeline share the rows evenly, 16 bytes a lane
+    if (warp < kProducerWarp || warp > kMmaWarp) {
+      const int w = warp < kProducerWarp ? warp : warp - 2;
+      const int per_row = rows <= 1 ? 8 : rows <= 2 ? 4 : 2, row = w / per_row, part = w - row * per_row;
+      float top = 0.f;
+      if (row < rows) {
+        const OutT* x = static_cast<const OutT*>(p.x) + (m0 + row) * p.x_ld;
+        const int nvec = p.K >> 3, step = per_row * 32;
+        for (int i = part * 32 + lane; i < nvec; i += 8 * step) {
+          uint4 part8[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) part8[u] = i + u * step < nvec ? ld_nc_16(x + (i + u * step) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(to_f32<OutT>(reinterpret_cast<const OutT*>(part8 + u)[e])));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
+      if (lane == 0) tops[w] = top;
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      // every warp on its own: no second barrier before the scales are used
+      if (lane < kQuantRows) {
+        float m = 0.f;
+        for (int i = 0; i < per_row && lane < rows; ++i) m = max_nan(m, tops[lane * per_row + i]);
+        scale_of_lane = int8_scale(m);
+      }
+      if (warp == 0 && lane < NT) sa[lane] = lane < rows ? scale_of_lane : 0.f;
+    }
+  }
+
   if (warp == kProducerWarp) {
     if (ptx::elect_one()) {
-      const uint32_t bytes = Cfg::kStageW + p.nt * kBK;
+      const uint32_t bytes = Cfg::kStageW + (QUANT ? 0 : p.nt * kBK);
       uint32_t it = 0;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % S;
         if (!ptx::mbar_wait(empty_bar(s), ((it / S) & 1) ^ 1, abort_flag)) break;
         ptx::mbar_expect_tx(full_bar(s), bytes);
         ptx::tma_load_2d(sW + s * Cfg::kStageW, &tmap_w, kb * kBK, n0, full_bar(s));
-        ptx::tma_load_2d(sX + s * Cfg::kStageX, &tmap_x, kb * kBK, m0, full_bar(s));
+        if (!QUANT) ptx::tma_load_2d(sX + s * Cfg::kStageX, &tmap_x, kb * kBK, m0, full_bar(s));
       }
     }
     __syncwarp();
@@ -179,8 +241,37 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (ok) ptx::mma_commit(done_bar);
     }
     __syncwarp();
+  } else if (QUANT && warp > kMmaWarp) {
+    if constexpr (QUANT) {
+      const unsigned group = 0xffu << (lane & 24);
+      const float scale = __shfl_sync(0xffffffffu, scale_of_lane, min(q_row, rows - 1)), inv = __frcp_rn(scale);
+      for (int j0 = 0; j0 < nkb; j0 += kAhead * kStep) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (j0 + u * kStep >= nkb) break;  // the same for the whole warp
+          const int j = j0 + u * kStep + first;
+          uint32_t c[2][8];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            c[e >> 3][e & 7] = rint_bits(div_by(to_f32<OutT>(reinterpret_cast<const OutT*>(raw[u])[e]), scale, inv));
+          const uint2 lo = pack8_s8(c[0]), hi = pack8_s8(c[1]);
+          request(j + kAhead * kStep, u);
+          if (j >= nkb) continue;
+          const int s = j % S;
+          ok = ok && ptx::mbar_wait(empty_bar(s), ((j / S) & 1) ^ 1, abort_flag);
+          if (ok && q_row < rows) {
+            const uint32_t dst = sX + s * Cfg::kStageX + q_row * 128 + ((chunk ^ q_row) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(lo.x), "r"(lo.y), "r"(hi.x), "r"(hi.y) : "memory");
+            ptx::fence_proxy_async_smem();  // generic-proxy writes -> the tensor core's reads
+          }
+          __syncwarp(group);
+          if (ok && chunk == 0) ptx::mbar_arrive(full_bar(s));
+        }
+      }
+    }
+    __syncwarp();
   } else {
-    for (int t = threadIdx.x; t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? __ldg(p.sa + m0 + t) : 0.f;
+    for (int t = threadIdx.x; !QUANT && t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? __ldg(p.sa + m0 + t) : 0.f;
     if (n < p.N) {
       sb = __ldg(p.sb + n);
       if (p.bias != nullptr) bias = to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]);
@@ -191,7 +282,7 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     ptx::tc_fence_after();
     if (splits == 1 && ok) {
 #pragma unroll 1
-      for (int c = half * 16; c < rows; c += kStep) {
+      for (int c = half * 16; c < rows; c += kNext) {
         uint32_t v[32];
         ptx::tmem_ld16(lane_base + c, v);
         ptx::tmem_ld_wait16(v);
@@ -208,7 +299,7 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     const int share = int8_share(rows, splits), groups = share / 4;  // token t belongs to split t / share
     if (warp < Cfg::kEpiWarps) {
 #pragma unroll 1
-      for (int c = half * 16; c < rows; c += kStep) {
+      for (int c = half * 16; c < rows; c += kNext) {
         uint32_t v[32];
         ptx::tmem_ld16(lane_base + c, v);
         int owner = c / share, g = (c - owner * share) / 4;
@@ -282,17 +373,19 @@ inline int encode_tmap_s8(CUtensorMap* m, const void* base, int64_t rows, int64_
   return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, k, ld, box_rows, kBK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
 }
 
-// p.nt tokens per tile (at most NT), p.k_splits splits.
-template <int NT, typename OutT>
+// p.nt tokens per tile (at most NT), p.k_splits splits. QUANT: p.x is quantised, A is null.
+template <int NT, bool QUANT, typename OutT>
 inline int launch_int8_stream(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t K, Int8Params p, cudaStream_t st) {
-  using Cfg = Int8StreamCfg<NT>;
+  using Cfg = Int8StreamCfg<NT, QUANT>;
   p.n_tiles = (int)cdiv(p.N, 128);
   p.t_tiles = (int)cdiv(p.M, p.nt);
   p.kb_per_split = (int)cdiv(p.num_kb, p.k_splits);
+  p.K = (int)K;
   CUtensorMap tw, tx;
   if (int rc = encode_tmap_s8(&tw, B, p.N, K, ldb, 128, "B")) return rc;
-  if (int rc = encode_tmap_s8(&tx, A, p.M, K, lda, p.nt, "A")) return rc;
-  auto k = int8_stream_kernel<NT, OutT>;
+  if (QUANT) tx = tw;
+  else if (int rc = encode_tmap_s8(&tx, A, p.M, K, lda, p.nt, "A")) return rc;
+  auto k = int8_stream_kernel<NT, QUANT, OutT>;
   if (int rc = allow_smem(k, Cfg::kSmemBytes, "int8_stream_kernel")) return rc;
   return launch_dependent(k, dim3((unsigned)(p.n_tiles * p.t_tiles * p.k_splits)), Cfg::kThreads, Cfg::kSmemBytes, st, (unsigned)p.k_splits,
                           "int8_stream_kernel", tw, tx, p);

@@ -7,7 +7,7 @@
 //   fp8 ue8m0 s = 2^ceil(log2(max|y| / 448)) likewise, exponent bytes packed four groups per int32 word, rows contiguous
 // Sums and maxima are fp32; the floor of a maximum is 1e-10 as in the group quantiser. A row or group with a NaN in it gets a NaN
 // (int8: as its scale, there is no NaN code; fp8: as codes).
-#include "common.cuh"
+#include "int8_round.cuh"
 
 namespace b200 {
 
@@ -27,13 +27,6 @@ struct RowParams {
   int H;
   float eps;
 };
-
-// max that keeps a NaN: a row must not hide one behind its other values
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 // Sum and maximum over a row's threads (of a warp, or of the whole block); every thread gets both. red: 64 floats of shared memory.
 template <bool SUM, bool MAX>
@@ -59,15 +52,6 @@ __device__ __forceinline__ void row_sum_max(float& sum, float& top, int warps, f
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
-
-// The nearest whole number of |v| < 2^22, ties to even, in the low bits of the result: adding 1.5 * 2^23 leaves no room for a fraction.
-__device__ __forceinline__ uint32_t rint_bits(float v) { return __float_as_uint(v + 12582912.f); }
-
-// x / s rounded to the nearest float, r = 1 / s rounded: one residual step (Markstein)
-__device__ __forceinline__ float div_by(float x, float s, float r) {
-  const float q = x * r;
-  return fmaf(fmaf(-q, s, x), r, q);
-}
 
 struct Ue8m0 {
   uint32_t byte;
@@ -120,7 +104,7 @@ __global__ void __launch_bounds__(256) row_quant_any_kernel(const RowParams p) {
   row_sum_max<true, true>(sum, top, 8, red);
   const float rstd = SRC >= ROW_NORM ? rsqrtf(sum / (float)H + p.eps) : 1.f;
   if constexpr (KIND == B200_ROW_INT8) {
-    const float s = __fdiv_rn(max_nan(top * rstd, 1e-10f), 127.f), inv = __frcp_rn(s);
+    const float s = int8_scale(top * rstd), inv = __frcp_rn(s);
     if (threadIdx.x == 0) static_cast<float*>(p.s)[row] = s;
     for (int i = threadIdx.x; i < H; i += 256)
       p.q[row * H + i] = (uint8_t)rint_bits(div_by(value(i) * weight(i) * rstd, s, inv));
@@ -241,7 +225,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
   row_sum_max<kNorm, KIND == B200_ROW_INT8>(sum, top, blockDim.x >> 5, red);
   const float rstd = kNorm ? rsqrtf(sum / (float)H + p.eps) : 1.f;
   if constexpr (KIND == B200_ROW_INT8) {
-    const float s = __fdiv_rn(max_nan(top * rstd, 1e-10f), 127.f), inv = kNorm ? rstd / s : __frcp_rn(s);
+    const float s = int8_scale(top * rstd), inv = kNorm ? rstd / s : __frcp_rn(s);
     if (threadIdx.x == 0) static_cast<float*>(p.s)[row] = s;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -253,10 +237,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
         else if (SRC == ROW_PLAIN) c[i] = rint_bits(div_by(a[j].get(i), s, inv));
         else c[i] = __float_as_uint(fmaf(y[SRC == ROW_PLAIN ? 0 : j][i], inv, 12582912.f));
       }
-      uint2 out;
-      out.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-      out.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-      if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = out;
+      if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = pack8_s8(c);
     }
   } else {
 #pragma unroll

@@ -161,6 +161,34 @@ def test_linear_is_quantiser_and_product():
             assert torch.equal(S.w8a8_int8_linear(x, b, sb, bias.to(dtype)), want)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("N,K", [(8, 16), (128, 128), (136, 272), (1000, 1040), (4096, 4096), (6144, 2064), (264, 14336), (28672, 512), (2048, 28672)])
+def test_linear_in_one_launch_equals_two(M, N, K):
+    from sglang_b200 import _native
+
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    for dtype, splits in ((torch.bfloat16, 0), (torch.float16, 0), (torch.bfloat16, 1), (torch.bfloat16, 3), (torch.float16, 8)):
+        wide = torch.randn(M, K + 64, generator=g, device="cuda").to(dtype)
+        x = wide[:, 8 : 8 + K] if splits else wide[:, :K].contiguous()
+        if M > 2:
+            x[1, K // 2], x[2] = float("nan"), 0
+        _, b, _, sb, bias = operands(1, N, K)
+        with _native.tuning(int8_splits=splits, int8_tile=16 if splits else -1, int8_linear_fused=1):
+            got = S.w8a8_int8_linear(x, b, sb, bias.to(dtype))
+            with _native.tuning(int8_linear_fused=0):
+                want = S.w8a8_int8_linear(x, b, sb, bias.to(dtype))
+        assert torch.equal(got.nan_to_num(7e4), want.nan_to_num(7e4)) and torch.equal(got.isnan(), want.isnan())
+        q, s = S.per_token_quant_int8(x)
+        keep = [i for i in range(M) if M <= 2 or i != 1]
+        check(got[keep], q[keep], b, s[keep], sb, bias.to(dtype))
+
+
+def test_linear_rows_at_odd_addresses():
+    x = torch.randn(3, 1032, device="cuda").bfloat16()[:, 3 : 3 + 1024]
+    _, b, _, sb, _ = operands(1, 512, 1024)
+    assert torch.equal(S.w8a8_int8_linear(x, b, sb), S.w8a8_int8_linear(x.contiguous(), b, sb))
+
+
 def test_device_status_is_clear():
     from sglang_b200 import _native as N
 
