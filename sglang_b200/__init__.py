@@ -1,4 +1,5 @@
-"""sglang_b200: the block-FP8 W8A8 linear + fused-MoE hot path of SGLang on B200 (sm_100a).
+"""sglang_b200: the block-FP8 W8A8 linear + fused-MoE hot path of SGLang on B200 (sm_100a), with the int8 W8A8 linear and the
+norms that feed either.
 
 Operators keep the reference's names and signatures; all compute is hand-written CUDA
 behind the C ABI of ``include/b200_blockfp8.h``."""
@@ -32,4 +33,5 @@ from .topk import (  # noqa: F401,E402
 from .int8_kernel import int8_scaled_mm, per_token_quant_int8, w8a8_int8_linear  # noqa: F401,E402
 from .layernorm import rmsnorm_quant_fp8, rmsnorm_quant_int8  # noqa: F401,E402
 from . import fp8  # noqa: F401,E402
+from . import int8  # noqa: F401,E402
 from . import custom_ops  # noqa: F401,E402  (registers torch.ops.sglang_b200.*)

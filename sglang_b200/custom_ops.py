@@ -19,6 +19,8 @@ import torch
 
 from . import _native as N
 from . import fp8_kernel as _q
+from . import int8_kernel as _i8
+from . import layernorm as _norm
 from . import topk as _topk
 from .fused_moe import fused_experts_impl as _experts
 from .moe_align_block_size import sgl_moe_align_block_size as _align_into
@@ -33,6 +35,12 @@ SCHEMAS = {
     "float eps, float fp8_min, float fp8_max, bool scale_ue8m0, bool fuse_silu_and_mul, Tensor? masked_m) -> ()",
     "fp8_blockwise_scaled_mm": "(Tensor mat_a, Tensor mat_b, Tensor scales_a, Tensor scales_b, ScalarType out_dtype) "
     "-> Tensor",
+    "int8_scaled_mm": "(Tensor mat_a, Tensor mat_b, Tensor scales_a, Tensor scales_b, ScalarType out_dtype, Tensor? bias) "
+    "-> Tensor",
+    "per_token_quant_int8": "(Tensor x, bool fuse_silu_and_mul=False) -> (Tensor, Tensor)",
+    "rmsnorm_quant_int8": "(Tensor x, Tensor weight, float eps, Tensor? residual=None) -> Tensor[]",
+    "rmsnorm_quant_fp8": "(Tensor x, Tensor weight, int group_size, float eps, Tensor? residual=None, "
+    "bool column_major_scales=False, bool scale_tma_aligned=False, bool scale_ue8m0=False) -> Tensor[]",
     "moe_align_block_size": "(Tensor topk_ids, int num_experts, int block_size, Tensor(a!) sorted_token_ids, "
     "Tensor(b!) experts_ids, Tensor(c!) num_tokens_post_pad, Tensor(d!) cumsum_buffer, bool pad_sorted_token_ids) "
     "-> ()",
@@ -165,6 +173,54 @@ def _mm(mat_a, mat_b, scales_a, scales_b, out_dtype):
 def _mm_fake(mat_a, mat_b, scales_a, scales_b, out_dtype):
     _mm_checks(mat_a, mat_b, scales_a, scales_b, out_dtype)
     return mat_a.new_empty((mat_a.shape[0], mat_b.shape[1]), dtype=out_dtype)
+
+
+# ------------------------------------------------------------------------------- int8 and norms
+
+@_impl("int8_scaled_mm")
+def _int8_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias):
+    return _i8.int8_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias)
+
+
+@_fake("int8_scaled_mm")
+def _int8_mm_fake(mat_a, mat_b, scales_a, scales_b, out_dtype, bias):
+    return mat_a.new_empty((mat_a.shape[0], mat_b.shape[1]), dtype=out_dtype)
+
+
+@_impl("per_token_quant_int8")
+def _int8_quant(x, fuse_silu_and_mul=False):
+    return _i8.per_token_quant_int8(x, fuse_silu_and_mul=fuse_silu_and_mul)
+
+
+@_fake("per_token_quant_int8")
+def _int8_quant_fake(x, fuse_silu_and_mul=False):
+    k = x.shape[-1] // (2 if fuse_silu_and_mul else 1)
+    return x.new_empty((*x.shape[:-1], k), dtype=torch.int8), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)
+
+
+@_impl("rmsnorm_quant_int8")
+def _norm_int8(x, weight, eps, residual=None):
+    return list(_norm.rmsnorm_quant_int8(x, weight, eps, residual))
+
+
+@_fake("rmsnorm_quant_int8")
+def _norm_int8_fake(x, weight, eps, residual=None):
+    out = [x.new_empty(x.shape, dtype=torch.int8), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)]
+    return out if residual is None else out + [x.new_empty(x.shape)]
+
+
+@_impl("rmsnorm_quant_fp8")
+def _norm_fp8(x, weight, group_size, eps, residual=None, column_major_scales=False, scale_tma_aligned=False, scale_ue8m0=False):
+    return list(_norm.rmsnorm_quant_fp8(x, weight, group_size, eps, residual, column_major_scales, scale_tma_aligned, scale_ue8m0))
+
+
+@_fake("rmsnorm_quant_fp8")
+def _norm_fp8_fake(x, weight, group_size, eps, residual=None, column_major_scales=False, scale_tma_aligned=False,
+                   scale_ue8m0=False):
+    out = [x.new_empty(x.shape, dtype=_q.fp8_dtype),
+           _q.create_per_token_group_quant_fp8_output_scale(x.shape, x.device, group_size, column_major_scales, scale_tma_aligned,
+                                                            scale_ue8m0)]
+    return out if residual is None else out + [x.new_empty(x.shape)]
 
 
 # ------------------------------------------------------------------------------------------ align

@@ -51,6 +51,47 @@ def test_norm_and_quantiser_refuse():
         S.per_token_quant_int8(x, scale_dtype=torch.bfloat16)
 
 
+def test_dispatcher_ops_describe_their_results():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    ops = torch.ops.sglang_b200
+    schema = ops.int8_scaled_mm.default._schema
+    assert [(a.name, str(a.type)) for a in schema.arguments] == [
+        ("mat_a", "Tensor"), ("mat_b", "Tensor"), ("scales_a", "Tensor"), ("scales_b", "Tensor"), ("out_dtype", "int"), ("bias", "Optional[Tensor]")]
+    with FakeTensorMode():
+        x, w = torch.empty(6, 512, dtype=torch.bfloat16, device="cuda"), torch.empty(512, dtype=torch.bfloat16, device="cuda")
+        q, s, r = ops.rmsnorm_quant_int8(x, w, 1e-6, x)
+        assert (q.dtype, q.shape, s.shape, r.dtype) == (torch.int8, (6, 512), (6, 1), torch.bfloat16)
+        q, s = ops.rmsnorm_quant_fp8(x, w, 128, 1e-6, None, True, True, True)
+        assert (q.dtype, s.dtype, s.shape, s.stride()) == (torch.float8_e4m3fn, torch.int32, (6, 1), (1, 8))
+        q, s = ops.per_token_quant_int8(x, True)
+        assert q.shape == (6, 256) and s.shape == (6, 1)
+        out = ops.int8_scaled_mm(q, torch.empty(64, 256, dtype=torch.int8, device="cuda").t(), s, torch.empty(64, 1, device="cuda"),
+                                 torch.float16, None)
+        assert out.shape == (6, 64) and out.dtype == torch.float16
+    with pytest.raises(NotImplementedError):
+        ops.per_token_quant_int8(torch.zeros(2, 16))
+
+
+def test_linear_method_loads_a_checkpoint():
+    from sglang_b200.int8 import W8A8Int8Config, W8A8Int8LinearMethod, quant_weight_int8
+
+    cfg = W8A8Int8Config.from_config({"quant_method": "w8a8_int8", "ignore": ["lm_head"]})
+    assert cfg.get_name() == "w8a8_int8" and cfg.is_layer_skipped("lm_head") and not cfg.is_layer_skipped("model.layers.0.mlp")
+    with pytest.raises(NotImplementedError):
+        W8A8Int8Config.from_config({"is_dynamic": False})
+    method, layer = W8A8Int8LinearMethod(cfg), torch.nn.Module()
+    method.create_weights(layer, 64, [32, 16], 64, 48, torch.bfloat16)
+    with pytest.raises(AssertionError):
+        method.process_weights_after_loading(layer)  # nothing loaded
+    w = torch.randn(48, 64, generator=torch.Generator().manual_seed(0))
+    q, s = quant_weight_int8(w)
+    assert ((q.float() * s - w).abs() <= s / 2 * (1 + 2.0**-20)).all() and (q.abs().amax(1) == 127).all()
+    layer.load_state_dict({"weight": q, "weight_scale": s})
+    method.process_weights_after_loading(layer)
+    assert torch.equal(layer.weight, q) and torch.equal(layer.weight_scale, s)
+
+
 FAKE = 1 << 20  # an aligned address that no refused call reads
 
 
