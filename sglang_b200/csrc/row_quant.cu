@@ -405,9 +405,9 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
   // Few rows: latency counts, and the fewer values a thread has the sooner it is done, but a plain maximum is so quick that fewer
   // warps to join win. Many rows: four vectors in flight. us for 1 / 2 / 4 / 8 vectors, 203 and 16384 rows of 8192:
   //   FP8, residual   3.8 / 4.1 / 5.4 / 6.4, 170 / 147 / 145 / 188      int8, residual  4.0 / 3.9 / 4.5 / 4.7, 170 / 189 / 140 / 162
-  //   plain           2.9 / 3.2 / 2.9 / 2.6, 128 / 77 / 69 / 80
+  //   plain           2.9 / 3.2 / 2.9 / 2.6, 128 / 77 / 69 / 80                gated           3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 110 / 148
   const bool few = p.rows < 1024;
-  int vpt = SRC == ROW_PLAIN ? (few ? 8 : 4) : SRC == ROW_SILU ? (few ? 1 : 2) : KIND == B200_ROW_INT8 ? 4 : few ? 1 : 4;
+  int vpt = SRC == ROW_PLAIN ? (few ? 8 : 4) : SRC == ROW_SILU ? (few ? 1 : 4) : KIND == B200_ROW_INT8 ? 4 : few ? 1 : 4;
   if (tuning().row_vectors > 0) vpt = tuning().row_vectors < 8 ? (int)tuning().row_vectors : 8;
   while (vpt > 1 && nvec < 32 * vpt) vpt /= 2;
   while (vpt < 8 && cdiv(nvec, vpt) > (vpt <= 2 ? 1024 : 512)) vpt *= 2;
