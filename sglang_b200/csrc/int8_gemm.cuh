@@ -23,6 +23,40 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// 16 bytes to another CTA's shared memory, counted on a barrier there: whoever waits for the bytes sees them, without a barrier of
+// the whole cluster (0.75 us with the release of everything written before it)
+__device__ __forceinline__ void st_async_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "r"(a),
+               "r"(b), "r"(c), "r"(d), "r"(bar)
+               : "memory");
+}
+// As mbar_wait, for bytes that another CTA of the cluster wrote
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (uint32_t spin = 1;; ++spin) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((spin & 63u) == 0u) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+// Cluster barrier that orders nothing but the CTAs' progress: 0.35 us, with release and acquire 0.75
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ int4 ld_shared_i4(uint32_t addr) {
   int4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -78,6 +112,9 @@ struct Int8StreamCfg {
   // sums of the splits, [split][tokens of this CTA / 4][128][4]; with many tokens they go to the ring once it is idle
   static constexpr int kSumBytes = NT <= 32 ? int8_sum_rows(NT) * 512 : 0;
   static constexpr size_t kSmemBytes = (size_t)kStages * (kStageW + kStageX) + kSumBytes + NT * 4 + (QUANT ? 32 : 0) + 1024 + 256;
+  // Few sums travel as stores that count themselves (1 x 6144 x 4096 in four splits 7.7 -> 7.1 us), many as plain ones with one barrier
+  // behind them, which are faster by the byte (203 x 4096 x 14336 22.4 against 19.9)
+  static constexpr bool kCounted = NT <= 64;
   static_assert(kSumBytes > 0 || int8_sum_rows(NT) * 512 <= kStages * (kStageW + kStageX), "the sums fit the ring");
 };
 
@@ -100,9 +137,9 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
-  const uint32_t done_bar = bar0 + 8u * 2 * S;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 2);
+  const uint32_t done_bar = bar0 + 8u * 2 * S, sum_bar = done_bar + 8u;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 3);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kProducerWarp = Cfg::kProducerWarp, kMmaWarp = Cfg::kMmaWarp;
@@ -110,6 +147,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const int n_tile = tile / p.t_tiles, n0 = n_tile * 128, m0 = (tile - n_tile * p.t_tiles) * p.nt;
   const int kb0 = ks * p.kb_per_split, kb1 = min(p.num_kb, kb0 + p.kb_per_split);
   const int rows = min(p.nt, p.M - m0);
+  // K splits: token t belongs to split t / share, this one's are t0 .. t0 + mine
+  const int share = int8_share(rows, splits), groups = share / 4, t0 = ks * share, mine = min(share, rows - t0);
   // QUANT: 16 groups of eight lanes take four rows of four K blocks side by side. Four K blocks are fewer than the ring's stages: with more
   // under way a group would wait for a phase of a stage's barrier that is two ahead of it, which the parity does not tell
   // from the one before.
@@ -122,8 +161,11 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       ptx::mbar_init(empty_bar(s), 1);
     }
     ptx::mbar_init(done_bar, 1);
+    ptx::mbar_init(sum_bar, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
+    // sums of every split for this CTA's tokens, four tokens of 128 channels at a time
+    if (Cfg::kCounted && splits > 1) ptx::mbar_expect_tx(sum_bar, (uint32_t)(splits * ((max(mine, 0) + 3) / 4) * 2048));
   }
   if (warp == kMmaWarp) {
     ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
@@ -137,8 +179,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // "I have started", waited for before another CTA's shared memory is written at the very end
-  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // "I have started, my barriers are initialised", waited for before another CTA's shared memory is written at the very end
+  if (splits > 1) ptx::cluster_arrive_relaxed();
   // This grid is launched as a programmatic dependent: every operand, and at the end the output, belongs to the kernels before it
   // in the stream, which may still run. Until then the weights are only asked for, as a prefetch into L2, a row each.
   if (warp < 4 && n0 + (int)threadIdx.x < p.N)
@@ -294,9 +336,11 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 
   if (splits > 1) {
     __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (Cfg::kSumBytes == 0) ptx::cluster_sync();  // every ring is idle: done_bar completes behind the last product
-    const int share = int8_share(rows, splits), groups = share / 4;  // token t belongs to split t / share
+    ptx::cluster_wait();
+    if (Cfg::kSumBytes == 0) {  // every ring is idle: done_bar completes behind the last product
+      ptx::cluster_arrive_relaxed();
+      ptx::cluster_wait();
+    }
     if (warp < Cfg::kEpiWarps) {
 #pragma unroll 1
       for (int c = half * 16; c < rows; c += kNext) {
@@ -306,28 +350,37 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         ptx::tmem_ld_wait16(v);
 #pragma unroll
         for (int t = 0; t < 16; t += 4) {
-          const uint32_t to = ptx::mapa(smem_base + kSums, min(owner, splits - 1)) + ((ks * groups + g) * 128 + r) * 16;
-          if (c + t < rows) ptx::st_cluster_v4(to, v[t], v[t + 1], v[t + 2], v[t + 3]);
+          const int cta = min(owner, splits - 1);
+          const uint32_t to = ptx::mapa(smem_base + kSums + ((ks * groups + g) * 128 + r) * 16, cta);
+          if (c + t < rows) {
+            if (Cfg::kCounted) ptx::st_async_v4(to, v[t], v[t + 1], v[t + 2], v[t + 3], ptx::mapa(sum_bar, cta));
+            else ptx::st_cluster_v4(to, v[t], v[t + 1], v[t + 2], v[t + 3]);
+          }
           if (++g == groups) g = 0, ++owner;
         }
       }
     }
     __syncwarp();
-    ptx::cluster_sync();
-    if (warp < Cfg::kEpiWarps && ok) {
-      const uint32_t src = smem_base + kSums + r * 16;
-      const int t0 = ks * share, mine = min(share, rows - t0);
+    // "I have sent everything": counted sums are waited for by their bytes, and for this only before the CTA leaves
+    if (Cfg::kCounted) ptx::cluster_arrive_relaxed();
+    else ptx::cluster_sync();
+    if (warp < Cfg::kEpiWarps) {
+      if (ok && mine > 0 && (!Cfg::kCounted || ptx::mbar_wait_cluster(sum_bar, 0, abort_flag))) {
+        const uint32_t src = smem_base + kSums + r * 16;
 #pragma unroll 2
-      for (int g = half; 4 * g < mine; g += Cfg::kEpiWarps / 4) {
-        int4 sum = ptx::ld_shared_i4(src + g * 2048);
+        for (int g = half; 4 * g < mine; g += Cfg::kEpiWarps / 4) {
+          int4 sum = ptx::ld_shared_i4(src + g * 2048);
 #pragma unroll 3
-        for (int c = 1; c < splits; ++c) {
-          const int4 v = ptx::ld_shared_i4(src + (c * groups + g) * 2048);
-          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+          for (int c = 1; c < splits; ++c) {
+            const int4 v = ptx::ld_shared_i4(src + (c * groups + g) * 2048);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+          }
+          store4(t0 + 4 * g, sum.x, sum.y, sum.z, sum.w);
         }
-        store4(t0 + 4 * g, sum.x, sum.y, sum.z, sum.w);
       }
     }
+    __syncwarp();
+    if (Cfg::kCounted) ptx::cluster_wait();
   }
 
   if (*abort_flag) {  // a wait gave up: copies that are still under way land before the shared memory goes

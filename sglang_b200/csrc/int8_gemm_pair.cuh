@@ -74,13 +74,15 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
   auto tfull_bar = [&](int b) { return bar0 + 8u * (2 * S + b); };
   auto tempty_bar = [&](int b) { return bar0 + 8u * (2 * S + 2 + b); };
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 4);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 5);
+  const uint32_t sum_bar = bar0 + 8u * (2 * S + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 6);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t cluster_rank = ptx::cluster_ctarank(), rank = cluster_rank & 1, leader_rank = cluster_rank - rank;
   const bool leader = rank == 0;
-  const int bn = p.nt, splits = p.k_splits;  // columns of the tile
+  const int bn = p.nt, splits = p.k_splits, ks = (int)cluster_rank >> 1;  // columns of the tile
+  auto owner_of = [&](int chunk) { return (chunk >> 1) & (splits - 1); };  // K splits: the chunks of both halves go round
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -91,8 +93,14 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       ptx::mbar_init(tfull_bar(b), 1);
       ptx::mbar_init(tempty_bar(b), 2 * Cfg::kEpiWarps);
     }
+    ptx::mbar_init(sum_bar, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
+    if (splits > 1) {  // the other splits' sums of this CTA's chunks
+      int mine = 0;
+      for (int j = 0; j < bn / 32; ++j) mine += owner_of(j) == ks;
+      ptx::mbar_expect_tx(sum_bar, (uint32_t)(mine * (splits - 1) * 32 * kBM * 4));
+    }
   }
   if (warp == Cfg::kMmaWarp) {
     ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
@@ -105,13 +113,12 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   }
   ptx::tc_fence_before();
   __syncthreads();
-  ptx::cluster_sync();  // the peer's barriers are initialised before anything signals them
+  ptx::cluster_arrive_relaxed();  // waited for below: the peer's barriers are initialised before anything signals them
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();
   // a cluster takes one tile where K is split, else as many as there are
-  const int cluster_pairs = splits, ks = (int)cluster_rank >> 1;
-  const int pair = (blockIdx.x >> 1) / cluster_pairs, npairs = (gridDim.x >> 1) / cluster_pairs, tiles = p.m_tiles * p.n_tiles;
+  const int pair = (blockIdx.x >> 1) / splits, npairs = (gridDim.x >> 1) / splits, tiles = p.m_tiles * p.n_tiles;
   const int kb0 = ks * p.kb_per_split, kb1 = min(p.num_kb, kb0 + p.kb_per_split);
   auto coords = [&](int t, int& mt, int& nt) { tile_coords(t, p.m_tiles, p.n_tiles, p.group_m, p.per_group_div, mt, nt); };
   // What is read and overwritten below belongs to the kernels before, which may still run; the weights of the first K blocks are
@@ -123,6 +130,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     if (row < p.N)
       prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)row * p.w_ld + kb0 * kBK, min(kPrefetchKb, kb1 - kb0));
   }
+  __syncwarp();
+  ptx::cluster_wait();
   grid_dependency_wait();
 
   if (warp == Cfg::kProducerWarp) {
@@ -213,27 +222,28 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       if (!ok && splits == 1) break;
       ptx::tc_fence_after();
       const uint32_t ta = lane_base + b * Cfg::kAccStride;
-      // K splits: the chunks of both halves go round. Slot of a sum: [chunk of its owner][source][4 columns][row], 16 bytes
-      auto owner_of = [&](int j) { return (j >> 1) & (splits - 1); };
+      // K splits. Slot of a sum: [chunk of its owner][source][4 columns][row], 16 bytes
       auto slot = [&](int j, int src) {
         const int mine = (j >> 1) / splits * 2 + half;
         return (uint32_t)(((mine * (splits - 1) + src) * 8 * kBM + quarter * 32 + lane) * 16);
       };
       if (splits > 1) {
         __syncwarp();
-        ptx::cluster_sync();  // every ring is idle
+        ptx::cluster_arrive_relaxed();
+        ptx::cluster_wait();  // every ring is idle
         for (int j = half; j < chunks; j += 2) {
           const int owner = owner_of(j);
           if (owner == ks) continue;
           uint32_t v[32];
           ptx::tmem_ld32(ta + j * 32, v);
           ptx::tmem_ld_wait(v);
-          const uint32_t dst = ptx::mapa(smem_base, (uint32_t)owner * 2 + rank) + slot(j, ks < owner ? ks : ks - 1);
+          const uint32_t cta = (uint32_t)owner * 2 + rank, dst = ptx::mapa(smem_base + slot(j, ks < owner ? ks : ks - 1), cta),
+                         bar = ptx::mapa(sum_bar, cta);
 #pragma unroll
-          for (int g = 0; g < 8; ++g) ptx::st_cluster_v4(dst + g * kBM * 16, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+          for (int g = 0; g < 8; ++g)
+            ptx::st_async_v4(dst + g * kBM * 16, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3], bar);
         }
-        __syncwarp();
-        ptx::cluster_sync();
+        ok = ok && ptx::mbar_wait_cluster(sum_bar, 0, abort_flag);
       }
 #pragma unroll 1
       for (int j = half; j < chunks; j += 2) {
@@ -315,10 +325,10 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     }
     if (lane == 0) ptx::tma_store_wait_all();
   }
-  if (splits > 1 && warp >= Cfg::kEpiWarps) {  // the other warps' share of the two cluster barriers above
+  if (splits > 1 && warp >= Cfg::kEpiWarps) {  // the other warps' share of the cluster barrier above
     __syncwarp();
-    ptx::cluster_sync();
-    ptx::cluster_sync();
+    ptx::cluster_arrive_relaxed();
+    ptx::cluster_wait();
   }
 
   if (*abort_flag) {
@@ -327,7 +337,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   }
   ptx::tc_fence_before();
   __syncthreads();
-  ptx::cluster_sync();  // neither CTA leaves while the other may still signal its barriers or read its shared memory
+  ptx::cluster_arrive_relaxed();
+  ptx::cluster_wait();  // neither CTA leaves while the other may still signal its barriers or read its shared memory
   if (threadIdx.x == 0 && *abort_flag) atomicCAS(p.status, 0, 1);
   if (warp == Cfg::kMmaWarp) {
     ptx::tc_fence_after();
