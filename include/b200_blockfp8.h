@@ -74,8 +74,7 @@ int b200_read_device_status(int* out, void* stream);
  * "moe_zero_pads" (0 / 1), "int8_tile" (16 .. 256 in steps of 16 = always the int8 stream kernel with
  * tiles of that many tokens at most, 1032 .. 1256 and 2032 .. 2256 in steps of 32 = always the int8 pair kernel, the
  * latter with swapped operands, with tiles of 32 .. 256 columns), "int8_linear_fused" (0 / 1 = the int8 linear never / up to 4 rows always
- * quantises in the product's kernel), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_ring" (0 / 1 = the plain row quantiser never /
- * always keeps a ring of rows in shared memory where they are aligned), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
+ * quantises in the product's kernel), "int8_splits" (K splits of the int8 product, 1 .. 8, of the pair kernel 1, 2 or 4), "row_vectors" (1 / 2 / 4 / 8 = vectors of eight elements per thread of the row quantisers), "peer_wait_ms" (limit of a device-side wait for another GPU, 100 .. 60000).
  * No counterpart in the reference (its Triton launchers read tuned JSON configs instead,
  * python/sglang/srt/layers/moe/fused_moe_triton/fused_moe_triton_config.py). Not thread-safe
  * against concurrent launches: set knobs before the calls they affect. */

@@ -62,7 +62,6 @@ struct Tuning {
   long moe_zero_pads = -1;      // 0 / 1: whether the gather pass zeroes pad rows
   long int8_tile = -1;          // 16 .. 256 (a multiple of 16): tokens of a tile of the int8 stream kernel; 1032 .. 1256, 2032 .. 2256: int8 pairs, swapped pairs, columns + 1000 / 2000
   long int8_splits = -1;        // 1 .. 8: K splits of the int8 stream kernel; 1, 2, 4: of the pairs
-  long row_ring = -1;           // 0 / 1: the plain row quantiser never / always keeps a ring of rows in shared memory
   long int8_linear_fused = -1;  // 0 / 1: the int8 linear never / always (up to 4 rows) quantises in the product's kernel
   long row_vectors = -1;        // 1, 2, 4, 8: vectors of eight elements per thread of the row quantisers
   long peer_wait_ms = -1;       // limit of a device-side wait for another GPU

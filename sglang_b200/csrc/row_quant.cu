@@ -7,19 +7,11 @@
 //   fp8 ue8m0 s = 2^ceil(log2(max|y| / 448)) likewise, exponent bytes packed four groups per int32 word, rows contiguous
 // Sums and maxima are fp32; the floor of a maximum is 1e-10 as in the group quantiser. A row or group with a NaN in it gets a NaN
 // (int8: as its scale, there is no NaN code; fp8: as codes).
-#include "gemm_host.cuh"
+#include <type_traits>
+
 #include "int8_round.cuh"
 
 namespace b200 {
-
-namespace ptx {
-// Untiled bulk copy global -> shared, completion on an mbarrier: both addresses 16-byte aligned, bytes a multiple of 16.
-__device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
-               "r"(bar)
-               : "memory");
-}
-}  // namespace ptx
 
 enum RowSource { ROW_PLAIN = 0, ROW_SILU = 1, ROW_NORM = 2, ROW_ADD_NORM = 3 };
 
@@ -38,18 +30,17 @@ struct RowParams {
   float eps;
 };
 
-template <bool SUM, bool MAX>
-__device__ __forceinline__ void warp_sum_max(float& sum, float& top) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (MAX) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  }
-}
 // Sum and maximum over a row's threads (of a warp, or of the whole block); every thread gets both. red: 64 floats of shared memory.
 template <bool SUM, bool MAX>
 __device__ __forceinline__ void row_sum_max(float& sum, float& top, int warps, float* red) {
-  warp_sum_max<SUM, MAX>(sum, top);
+  auto warp_reduce = [&] {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (MAX) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  };
+  warp_reduce();
   if (warps == 1) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) {
@@ -59,7 +50,7 @@ __device__ __forceinline__ void row_sum_max(float& sum, float& top, int warps, f
   __syncthreads();
   if (SUM) sum = lane < warps ? red[lane] : 0.f;
   if (MAX) top = lane < warps ? red[32 + lane] : 0.f;
-  warp_sum_max<SUM, MAX>(sum, top);
+  warp_reduce();
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
@@ -152,13 +143,23 @@ struct Raw8 {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   }
-  __device__ __forceinline__ void shared(const T* p) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  // largest magnitude, a NaN if there is one
+  __device__ __forceinline__ float amax() const {
+    if constexpr (sizeof(T) == 2) {
+      using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+      const T2* p = reinterpret_cast<const T2*>(v);
+      const T2 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+      return max_nan(to_f32<T>(m.x), to_f32<T>(m.y));
+    } else {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(get(i)));
+      return m;
+    }
   }
   __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T*>(v)[i]); }
   __device__ __forceinline__ void set(int i, float f) { reinterpret_cast<T*>(v)[i] = from_f32<T>(f); }
@@ -168,9 +169,9 @@ struct Raw8 {
   }
 };
 
-// Rows in flight decide: a block loads, then reduces, and only other blocks' loads keep the memory busy meanwhile. Registers capped
-// to 40 (plain, four vectors): 16384 x 8192 bf16 73.4 -> 68.8 us.
-constexpr int row_min_blocks(int src, int vpt) { return src == ROW_PLAIN && vpt == 4 ? 3 : src == ROW_SILU && vpt <= 4 ? 2 : 1; }
+// Rows in flight decide: a block loads, then reduces, and only other blocks' loads keep the memory busy meanwhile. So registers are
+// capped where it costs no spills (16384 x 1024 plain 9.2 -> 8.4 us).
+constexpr int row_min_blocks(int src, int vpt) { return vpt > 4 ? 1 : src == ROW_SILU ? 2 : src == ROW_PLAIN && vpt == 4 ? 3 : 1; }
 
 // A row in the registers of a block, or of a warp (blockDim.y rows per block): one pass over memory. A thread has VPT vectors of eight
 // elements, blockDim.x vectors apart, so loads are 16 bytes per lane without gaps, and all of them are under way before the
@@ -204,8 +205,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     if constexpr (SRC == ROW_PLAIN) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(a[j].get(i)));
+      top = max_nan(top, a[j].amax());
       continue;
     }
     const int v = threadIdx.x + j * blockDim.x;
@@ -241,16 +241,19 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
   const float rstd = kNorm ? rsqrtf(sum / (float)H + p.eps) : 1.f;
   if constexpr (KIND == B200_ROW_INT8) {
     const float s = int8_scale(top * rstd), inv = kNorm ? rstd / s : __frcp_rn(s);
+    const DivTwo div(s, inv);
     if (threadIdx.x == 0) static_cast<float*>(p.s)[row] = s;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int v = threadIdx.x + j * blockDim.x;
       uint32_t c[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (kNorm) c[i] = __float_as_uint(fmaf(y[j][i], inv, 12582912.f));
-        else if (SRC == ROW_PLAIN) c[i] = rint_bits(div_by(a[j].get(i), s, inv));
-        else c[i] = __float_as_uint(fmaf(y[SRC == ROW_PLAIN ? 0 : j][i], inv, 12582912.f));
+      for (int i = 0; i < 8; i += 2) {
+        if constexpr (SRC == ROW_PLAIN) {
+          div.rint_bits(a[j].get(i), a[j].get(i + 1), c[i], c[i + 1]);
+        } else {
+          rint_scaled_two(y[j][i], y[j][i + 1], twice(inv), c[i], c[i + 1]);
+        }
       }
       if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = pack8_s8(c);
     }
@@ -277,101 +280,6 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       }
     }
   }
-}
-
-// Long prefills of wide plain rows: persistent blocks with a ring of rows in shared memory, which bulk copies keep full, so that the memory
-// never waits for a reduction. A slot is free as soon as the barrier of its row's reduction is passed: by then every thread has it in
-// registers. One row a block (above) and this, bf16: 16384 x 14336 126 -> 112 us (6.3 TB/s), 8192 x 14336 66.0 -> 60.8, 16384 x 8192 70.5 ->
-// 68.8, but 16384 x 4096 36.4 -> 37.4; gated rows 16384 x 14336 216 -> 222.
-template <typename T, int VPT>
-__global__ void __launch_bounds__(512) row_quant_ring_kernel(const RowParams p, int stages, int slot_bytes, int* status) {
-  constexpr int kMaxStages = 8;
-  extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ float red[2][64];
-  __shared__ uint64_t full[kMaxStages];
-  __shared__ int abort_flag;
-  const int H = p.H, nvec = H >> 3, tid = threadIdx.x, warps = blockDim.x >> 5;
-  const uint32_t row_bytes = (uint32_t)(H * (int)sizeof(T)), bar0 = ptx::smem_u32(full), ring0 = ptx::smem_u32(ring);
-  if (tid == 0) {
-    for (int s = 0; s < stages; ++s) ptx::mbar_init(bar0 + 8 * s, 1);
-    abort_flag = 0;
-    ptx::fence_mbar_init();
-  }
-  __syncthreads();
-  grid_launch_dependents();
-  grid_dependency_wait();
-  auto fetch = [&](int64_t row, int s) {
-    if (row >= p.rows) return;
-    ptx::mbar_expect_tx(bar0 + 8 * s, row_bytes);
-    ptx::bulk_load_1d(ring0 + s * slot_bytes, static_cast<const T*>(p.x) + row * p.x_ld, row_bytes, bar0 + 8 * s);
-  };
-  if (tid == 0)
-    for (int s = 0; s < stages; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
-  int s = 0, side = 0;
-  uint32_t phase = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const bool ok = ptx::mbar_wait(bar0 + 8 * s, phase, &abort_flag);
-    const T* x = reinterpret_cast<const T*>(ring + s * slot_bytes);
-    Raw8<T> a[VPT];
-    float none = 0.f, top = 0.f;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int v = tid + j * blockDim.x;
-      if (v < nvec) a[j].shared(x + v * 8);
-      else a[j].zero();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(a[j].get(i)));
-    }
-    warp_sum_max<false, true>(none, top);
-    if ((tid & 31) == 0) red[side][tid >> 5] = top;
-    if (!__syncthreads_and(ok)) break;  // the next row uses the other side of red: nobody is two barriers ahead
-    if (tid == 0) fetch(row + (int64_t)stages * gridDim.x, s);
-    top = (tid & 31) < warps ? red[side][tid & 31] : 0.f;
-    warp_sum_max<false, true>(none, top);
-    const float scale = int8_scale(top), inv = __frcp_rn(scale);
-    if (tid == 0) static_cast<float*>(p.s)[row] = scale;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int v = tid + j * blockDim.x;
-      uint32_t c[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = rint_bits(div_by(a[j].get(i), scale, inv));
-      if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = pack8_s8(c);
-    }
-    side ^= 1;
-    if (++s == stages) s = 0, phase ^= 1;
-  }
-  if (abort_flag) {  // a copy did not arrive: those that are still under way land before the shared memory goes
-    const unsigned long long t0 = ptx::globaltimer_ns();
-    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
-    if (tid == 0) atomicCAS(status, 0, 1);
-  }
-}
-
-// vpt: 4 or 8. Blocks of about 1024 threads per SM share its memory.
-template <typename T>
-static int launch_row_ring(const RowParams& p, int vpt, cudaStream_t st, const char* what) {
-  constexpr int kShared = 220000;
-  const unsigned threads = (unsigned)align_up(cdiv(p.H / 8, vpt), 32);
-  const int slot = (int)align_up((size_t)p.H * sizeof(T), 128);
-  int blocks = 1024 / (int)threads;
-  while (blocks > 1 && kShared / blocks / slot < 2) --blocks;
-  const int stages = kShared / blocks / slot < 8 ? kShared / blocks / slot : 8;
-  if (stages < 1) {
-    set_error_detail("%s: a row of %d elements does not fit shared memory", what, p.H);
-    return B200_E_UNSUPPORTED;
-  }
-  int* status = device_status_word();
-  if (!status) {
-    set_error_detail("cannot resolve the device status word");
-    return B200_E_LAUNCH;
-  }
-  const int64_t grid = (int64_t)blocks * sm_count();
-  auto go = [&](auto k) {
-    if (int rc = allow_smem(k, kShared, what)) return rc;
-    return launch_dependent(k, dim3((unsigned)(grid < p.rows ? grid : p.rows)), threads, (size_t)stages * slot, st, 1, what, p, stages, slot, status);
-  };
-  return vpt <= 4 ? go(row_quant_ring_kernel<T, 4>) : go(row_quant_ring_kernel<T, 8>);
 }
 
 template <typename T, int SRC, int KIND, int VPT>
@@ -403,18 +311,15 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
                        (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.q % 8 == 0;
   if (!vectors) return launch_dependent(row_quant_any_kernel<T, SRC, KIND>, dim3((unsigned)p.rows), 256, 0, st, 1, what, p);
   // Few rows: latency counts, and the fewer values a thread has the sooner it is done, but a plain maximum is so quick that fewer
-  // warps to join win. Many rows: four vectors in flight. us for 1 / 2 / 4 / 8 vectors, 203 and 16384 rows of 8192:
-  //   FP8, residual   3.8 / 4.1 / 5.4 / 6.4, 170 / 147 / 145 / 188      int8, residual  4.0 / 3.9 / 4.5 / 4.7, 170 / 189 / 140 / 162
-  //   plain           2.9 / 3.2 / 2.9 / 2.6, 128 / 77 / 69 / 80                gated           3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 110 / 148
+  // warps to join win. Many rows: the vectors in flight. us for 1 / 2 / 4 / 8 vectors, 203 and 16384 rows of 8192 bf16:
+  //   FP8, residual   3.8 / 4.1 / 5.4 / 6.4, 170 / 147 / 145 / 188 (6.5 TB/s)   int8, residual  4.0 / 3.9 / 4.5 / 4.7, 170 / 189 / 140 / 162 (6.7)
+  //   plain           2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5)           gated           3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
+  // Blocks that go through many rows, with a ring of them in shared memory that bulk copies fill, were no faster (plain 69 to 73 us).
   const bool few = p.rows < 1024;
-  int vpt = SRC == ROW_PLAIN ? (few ? 8 : 4) : SRC == ROW_SILU ? (few ? 1 : 4) : KIND == B200_ROW_INT8 ? 4 : few ? 1 : 4;
+  int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (few ? 1 : 4) : KIND == B200_ROW_INT8 ? 4 : few ? 1 : 4;
   if (tuning().row_vectors > 0) vpt = tuning().row_vectors < 8 ? (int)tuning().row_vectors : 8;
   while (vpt > 1 && nvec < 32 * vpt) vpt /= 2;
   while (vpt < 8 && cdiv(nvec, vpt) > (vpt <= 2 ? 1024 : 512)) vpt *= 2;
-  if constexpr (SRC == ROW_PLAIN) {
-    const bool wide = p.H > 4096 && p.rows * p.H * (int64_t)sizeof(T) >= (128 << 20);
-    if (vpt >= 4 && (tuning().row_ring >= 0 ? tuning().row_ring > 0 : wide)) return launch_row_ring<T>(p, vpt, st, what);
-  }
   const unsigned threads = (unsigned)align_up(cdiv(nvec, vpt), 32), rpb = threads == 32 ? 4 : 1;
   switch (vpt) {
     case 1: return launch_row_regs<T, SRC, KIND, 1>(p, threads, rpb, st, what);

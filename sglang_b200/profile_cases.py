@@ -4,6 +4,9 @@
     python -m sglang_b200.profile_cases gemm_ue8m0 M N K [calls]          (packed power-of-two scales: block-scaled kernel)
     python -m sglang_b200.profile_cases linear_decode M N K [calls]       (one-launch quantise + GEMM + split-K sum)
     python -m sglang_b200.profile_cases quant M K [calls]
+    python -m sglang_b200.profile_cases int8_mm M N K [calls]             (rotates over three weights)
+    python -m sglang_b200.profile_cases quant_int8 M K plain|silu [calls]
+    python -m sglang_b200.profile_cases norm M H int8|fp8 [calls]         (RMSNorm with the residual's addition)
     python -m sglang_b200.profile_cases align T topk E [calls]
     python -m sglang_b200.profile_cases route T E topk grouped|softmax [calls]
     python -m sglang_b200.profile_cases moe deepseek|mixtral T [calls]
@@ -69,6 +72,26 @@ def main(argv) -> int:
         for _ in range(calls(2)):
             out, _ = S.per_token_group_quant_fp8(x, 128, column_major_scales=True)
         out = out.view(torch.uint8)
+    elif case == "int8_mm":
+        M, Nn, K = (int(a) for a in args[:3])
+        a = torch.randint(-100, 100, (M, K), device=dev, generator=g, dtype=torch.int8)
+        ws = [torch.randint(-100, 100, (Nn, K), device=dev, generator=g, dtype=torch.int8) for _ in range(3)]
+        sa, sb = torch.rand(M, device=dev, generator=g) * 1e-3, torch.rand(Nn, device=dev, generator=g) * 1e-3
+        for i in range(calls(3)):
+            out = S.int8_scaled_mm(a, ws[i % 3].t(), sa, sb, torch.bfloat16)
+    elif case == "quant_int8":
+        silu = args[2] == "silu"
+        x = torch.randn(int(args[0]), int(args[1]) * (2 if silu else 1), device=dev, generator=g).bfloat16()
+        for _ in range(calls(3)):
+            out, _ = S.per_token_quant_int8(x, fuse_silu_and_mul=silu)
+    elif case == "norm":
+        x, r = (torch.randn(int(args[0]), int(args[1]), device=dev, generator=g).bfloat16() for _ in range(2))
+        w = torch.ones(int(args[1]), device=dev).bfloat16()
+        for _ in range(calls(3)):
+            if args[2] == "int8":
+                out, *_ = S.rmsnorm_quant_int8(x, w, residual=r)
+            else:
+                out, *_ = S.rmsnorm_quant_fp8(x, w, residual=r, column_major_scales=True)
     elif case == "align":
         T, topk, E = (int(a) for a in args[:3])
         ids = torch.randint(0, E, (T, topk), device=dev, generator=g, dtype=torch.int32)
