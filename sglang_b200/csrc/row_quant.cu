@@ -169,15 +169,19 @@ struct Raw8 {
   }
 };
 
-// Rows in flight decide: a block loads, then reduces, and only other blocks' loads keep the memory busy meanwhile. So registers are
-// capped where it costs no spills (16384 x 1024 plain 9.2 -> 8.4 us).
-constexpr int row_min_blocks(int src, int vpt) { return vpt > 4 ? 1 : src == ROW_SILU ? 2 : src == ROW_PLAIN && vpt == 4 ? 3 : 1; }
+// Many rows: what counts are the rows in flight, as a block loads, then reduces, and only other blocks' loads keep the memory busy
+// meanwhile, so registers are held down (0: as the compiler sees fit, 62 for a norm with four vectors; plain 16384 x 1024 9.2 -> 8.4 us
+// at three blocks). Few rows: a block is alone, and with all the registers it likes (86) it has everything requested at once: 203 x 8192
+// int8 with residual 4.5 -> 2.6 us, but 16384 rows 140 -> 160.
+constexpr int row_min_blocks(int src, int vpt, bool few) {
+  return few || vpt > 4 ? 1 : src == ROW_SILU ? 2 : src == ROW_PLAIN && vpt == 4 ? 3 : 0;
+}
 
 // A row in the registers of a block, or of a warp (blockDim.y rows per block): one pass over memory. A thread has VPT vectors of eight
 // elements, blockDim.x vectors apart, so loads are 16 bytes per lane without gaps, and all of them are under way before the
 // first is used. The codes of a norm need no 1/rms: it cancels in y / s, so only the scales wait for the sum of squares.
-template <typename T, int SRC, int KIND, int VPT>
-__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT)) row_quant_kernel(const RowParams p) {
+template <typename T, int SRC, int KIND, int VPT, bool FEW>
+__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT, FEW)) row_quant_kernel(const RowParams p) {
   constexpr bool kNorm = SRC >= ROW_NORM, kTwo = SRC == ROW_SILU || SRC == ROW_ADD_NORM;
   __shared__ float red[64];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -248,12 +252,12 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       const int v = threadIdx.x + j * blockDim.x;
       uint32_t c[8];
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        if constexpr (SRC == ROW_PLAIN) {
-          div.rint_bits(a[j].get(i), a[j].get(i + 1), c[i], c[i + 1]);
-        } else {
-          rint_scaled_two(y[j][i], y[j][i + 1], twice(inv), c[i], c[i + 1]);
-        }
+      for (int i = 0; i < 8; ++i)
+        if constexpr (kNorm) c[i] = __float_as_uint(fmaf(y[j][i], inv, 12582912.f));
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {  // packed the norm's registers grow and it is slower
+        if constexpr (SRC == ROW_PLAIN) div.rint_bits(a[j].get(i), a[j].get(i + 1), c[i], c[i + 1]);
+        if constexpr (SRC == ROW_SILU) rint_scaled_two(y[j][i], y[j][i + 1], twice(inv), c[i], c[i + 1]);
       }
       if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = pack8_s8(c);
     }
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
   }
 }
 
-template <typename T, int SRC, int KIND, int VPT>
+template <typename T, int SRC, int KIND, int VPT, bool FEW = false>
 static int launch_row_regs(const RowParams& p, unsigned threads, unsigned rows_per_block, cudaStream_t st, const char* what) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cdiv(p.rows, rows_per_block));
@@ -293,7 +297,7 @@ static int launch_row_regs(const RowParams& p, unsigned threads, unsigned rows_p
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, row_quant_kernel<T, SRC, KIND, VPT>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, row_quant_kernel<T, SRC, KIND, VPT, FEW>, p);
   if (e != cudaSuccess) {
     set_error_detail("%s: %s", what, cudaGetErrorString(e));
     return B200_E_LAUNCH;
@@ -310,21 +314,23 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
                        (SRC != ROW_ADD_NORM || (even(p.r, p.rows == 1 ? 0 : p.r_ld) && (uintptr_t)p.r_out % 16 == 0)) &&
                        (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.q % 8 == 0;
   if (!vectors) return launch_dependent(row_quant_any_kernel<T, SRC, KIND>, dim3((unsigned)p.rows), 256, 0, st, 1, what, p);
-  // Few rows: latency counts, and the fewer values a thread has the sooner it is done, but a plain maximum is so quick that fewer
-  // warps to join win. Many rows: the vectors in flight. us for 1 / 2 / 4 / 8 vectors, 203 and 16384 rows of 8192 bf16:
-  //   FP8, residual   3.8 / 4.1 / 5.4 / 6.4, 170 / 147 / 145 / 188 (6.5 TB/s)   int8, residual  4.0 / 3.9 / 4.5 / 4.7, 170 / 189 / 140 / 162 (6.7)
+  // us for 1 / 2 / 4 / 8 vectors a thread, 203 and 16384 rows of 8192 bf16:
+  //   FP8, residual   3.8 / 3.7 / 3.6 / 6.4, 170 / 147 / 145 / 188 (6.5 TB/s)   int8, residual  4.0 / 3.7 / 2.6 / 4.7, 170 / 189 / 140 / 162 (6.7)
   //   plain           2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5)           gated           3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
   // Blocks that go through many rows, with a ring of them in shared memory that bulk copies fill, were no faster (plain 69 to 73 us).
-  const bool few = p.rows < 1024;
-  int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (few ? 1 : 4) : KIND == B200_ROW_INT8 ? 4 : few ? 1 : 4;
+  int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (p.rows < 1024 ? 1 : 4) : KIND == B200_ROW_INT8 || nvec >= 512 || p.rows >= 1024 ? 4 : 1;
   if (tuning().row_vectors > 0) vpt = tuning().row_vectors < 8 ? (int)tuning().row_vectors : 8;
   while (vpt > 1 && nvec < 32 * vpt) vpt /= 2;
   while (vpt < 8 && cdiv(nvec, vpt) > (vpt <= 2 ? 1024 : 512)) vpt *= 2;
   const unsigned threads = (unsigned)align_up(cdiv(nvec, vpt), 32), rpb = threads == 32 ? 4 : 1;
+  const bool few = p.rows <= 148 * (740 / (int)threads);  // one wave of blocks with all the registers they like
   switch (vpt) {
     case 1: return launch_row_regs<T, SRC, KIND, 1>(p, threads, rpb, st, what);
     case 2: return launch_row_regs<T, SRC, KIND, 2>(p, threads, rpb, st, what);
-    case 4: return launch_row_regs<T, SRC, KIND, 4>(p, threads, rpb, st, what);
+    case 4:
+      if constexpr (SRC >= ROW_NORM)
+        if (few) return launch_row_regs<T, SRC, KIND, 4, true>(p, threads, rpb, st, what);
+      return launch_row_regs<T, SRC, KIND, 4>(p, threads, rpb, st, what);
     default: return launch_row_regs<T, SRC, KIND, 8>(p, threads, rpb, st, what);
   }
 }
