@@ -449,7 +449,7 @@ int b200_moe_sum_reduce(const void* rows, const int32_t* topk_ids, void* out, in
  *   B200_ROW_FP8        per 128 columns (H % 128 == 0): s[m*s_stride_m + g*s_stride_g] = amax / 448, q = e4m3(y / s)
  *   B200_ROW_FP8_UE8M0  the same with s = 2^ceil(log2(amax / 448)), its biased exponent in byte (g % 4) of word
  *                       [g/4 * s_stride_g + m]; bytes past the last group are written as 0
- * q [M,H] contiguous, 16-byte aligned for the FP8 kinds. Any H (int8) up to 2^24, any element alignment of x. */
+ * No output overlaps an input. q [M,H] contiguous, 16-byte aligned for the FP8 kinds. Any H (int8) up to 2^24, any element alignment of x. */
 enum { B200_ROW_INT8 = 0, B200_ROW_FP8 = 1, B200_ROW_FP8_UE8M0 = 2 };
 int b200_rmsnorm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,
                        const void* weight, int dtype, int kind, void* q, void* s, int64_t s_stride_m,

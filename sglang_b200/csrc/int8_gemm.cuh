@@ -185,7 +185,7 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   // in the stream, which may still run. Until then the weights are only asked for, as a prefetch into L2, a row each.
   if (warp < 4 && n0 + (int)threadIdx.x < p.N)
     prefetch_weight_row(reinterpret_cast<const uint8_t*>(p.w) + (int64_t)(n0 + threadIdx.x) * p.w_ld + kb0 * kBK, min(kPrefetchKb, kb1 - kb0));
-  grid_dependency_wait();
+  const int64_t zero = grid_dependency_zero();
 
   bool ok = true;
   float sb = 0.f, bias = 0.f, scale_of_lane = 0.f;
@@ -212,10 +212,10 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   uint4 raw[kAhead][2];
   auto request = [&](int j, int u) {
     const int k = (kb0 + j) * kBK + chunk * 16;  // K is a multiple of 16
-    const OutT* src = static_cast<const OutT*>(p.x) + (m0 + min(q_row, rows - 1)) * p.x_ld + k;
+    const OutT* src = static_cast<const OutT*>(p.x) + (m0 + min(q_row, rows - 1)) * p.x_ld + k + zero;
     const bool inside = j < nkb && k < p.K;
-    raw[u][0] = inside ? ld_nc_16(src) : make_uint4(0, 0, 0, 0);
-    raw[u][1] = inside ? ld_nc_16(src + 8) : make_uint4(0, 0, 0, 0);
+    raw[u][0] = inside ? ld_stream_16(src) : make_uint4(0, 0, 0, 0);
+    raw[u][1] = inside ? ld_stream_16(src + 8) : make_uint4(0, 0, 0, 0);
   };
   if constexpr (QUANT) {
     if (warp > kMmaWarp)
@@ -227,12 +227,12 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       const int per_row = rows <= 1 ? 8 : rows <= 2 ? 4 : 2, row = w / per_row, part = w - row * per_row;
       float top = 0.f;
       if (row < rows) {
-        const OutT* x = static_cast<const OutT*>(p.x) + (m0 + row) * p.x_ld;
+        const OutT* x = static_cast<const OutT*>(p.x) + (m0 + row) * p.x_ld + zero;
         const int nvec = p.K >> 3, step = per_row * 32;
         for (int i = part * 32 + lane; i < nvec; i += 8 * step) {
           uint4 part8[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) part8[u] = i + u * step < nvec ? ld_nc_16(x + (i + u * step) * 8) : make_uint4(0, 0, 0, 0);
+          for (int u = 0; u < 8; ++u) part8[u] = i + u * step < nvec ? ld_stream_16(x + (i + u * step) * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
           for (int u = 0; u < 8; ++u)
 #pragma unroll
@@ -313,9 +313,9 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     }
     __syncwarp();
   } else {
-    for (int t = threadIdx.x; !QUANT && t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? __ldg(p.sa + m0 + t) : 0.f;
+    for (int t = threadIdx.x; !QUANT && t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? __ldcg(p.sa + m0 + t) : 0.f;
     if (n < p.N) {
-      sb = __ldg(p.sb + n);
+      sb = __ldcg(p.sb + n);
       if (p.bias != nullptr) bias = to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]);
     }
     asm volatile("bar.sync 1, %0;" ::"n"(Cfg::kEpiThreads) : "memory");

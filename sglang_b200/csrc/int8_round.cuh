@@ -5,6 +5,25 @@
 
 namespace b200 {
 
+// griddepcontrol.wait, and a zero that is known only behind it: added to an operand's address it keeps the loads there, which the compiler
+// may otherwise move as it likes. They are ordinary loads, which the wait covers, and not from the read-only path: an earlier kernel of
+// the stream may have written the operand while this one was already resident.
+__device__ __forceinline__ int64_t grid_dependency_zero() {
+  int64_t zero;
+  asm volatile("griddepcontrol.wait;\n\tmov.b64 %0, 0;" : "=l"(zero)::"memory");
+  return zero;
+}
+__device__ __forceinline__ uint4 ld_stream_16(const void* p) {  // read once, and requested here
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_again_16(const void* p) {  // read by every row
+  uint4 v;
+  asm("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // max that keeps a NaN: a row must not hide one behind its other values
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;

@@ -137,11 +137,11 @@ struct Raw8 {
   uint4 v[kLoads];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) v[i] = ld_nc_16(p + i * (16 / sizeof(T)));
+    for (int i = 0; i < kLoads; ++i) v[i] = ld_stream_16(p + i * (16 / sizeof(T)));
   }
   __device__ __forceinline__ void cached(const T* p) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < kLoads; ++i) v[i] = ld_again_16(p + i * (16 / sizeof(T)));
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -169,28 +169,28 @@ struct Raw8 {
   }
 };
 
-// Many rows: what counts are the rows in flight, as a block loads, then reduces, and only other blocks' loads keep the memory busy
-// meanwhile, so registers are held down (0: as the compiler sees fit, 62 for a norm with four vectors; plain 16384 x 1024 9.2 -> 8.4 us
-// at three blocks). Few rows: a block is alone, and with all the registers it likes (86) it has everything requested at once: 203 x 8192
-// int8 with residual 4.5 -> 2.6 us, but 16384 rows 140 -> 160.
-constexpr int row_min_blocks(int src, int vpt, bool few) {
-  return few || vpt > 4 ? 1 : src == ROW_SILU ? 2 : src == ROW_PLAIN && vpt == 4 ? 3 : 0;
+// What counts for many rows are the rows in flight, as a block loads, then reduces, and only other blocks' loads keep the memory busy
+// meanwhile: registers are held down (0: as the compiler sees fit; plain 16384 x 1024 9.2 -> 8.4 us at three blocks). For few rows it is a
+// block's own latency: `ahead`, the norm's weights are requested together with the row, whatever registers that takes.
+constexpr int row_min_blocks(int src, int vpt, bool ahead) {
+  return ahead || vpt > 4 ? 1 : src == ROW_SILU ? 2 : src == ROW_PLAIN && vpt == 4 ? 3 : 0;
 }
 
 // A row in the registers of a block, or of a warp (blockDim.y rows per block): one pass over memory. A thread has VPT vectors of eight
 // elements, blockDim.x vectors apart, so loads are 16 bytes per lane without gaps, and all of them are under way before the
 // first is used. The codes of a norm need no 1/rms: it cancels in y / s, so only the scales wait for the sum of squares.
-template <typename T, int SRC, int KIND, int VPT, bool FEW>
-__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT, FEW)) row_quant_kernel(const RowParams p) {
+template <typename T, int SRC, int KIND, int VPT, bool AHEAD>
+__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT, AHEAD)) row_quant_kernel(const RowParams p) {
   constexpr bool kNorm = SRC >= ROW_NORM, kTwo = SRC == ROW_SILU || SRC == ROW_ADD_NORM;
   __shared__ float red[64];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= p.rows) return;  // a whole warp: several rows to a block only where each has one
   const int H = p.H, nvec = H >> 3;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-  const T* second = SRC == ROW_SILU ? x + H : static_cast<const T*>(p.r) + row * p.r_ld;
   grid_launch_dependents();
-  grid_dependency_wait();
+  const int64_t zero = grid_dependency_zero();
+  const T* x = static_cast<const T*>(p.x) + row * p.x_ld + zero;
+  const T* second = SRC == ROW_SILU ? x + H : static_cast<const T*>(p.r) + row * p.r_ld + zero;
+  const T* weight = static_cast<const T*>(p.w) + zero;
   Raw8<T> a[VPT], b[kTwo ? VPT : 1];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
@@ -203,6 +203,16 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       if (kTwo) b[j].zero();
     }
   }
+  Raw8<T> w[kNorm && AHEAD ? VPT : 1];
+  auto load_weights = [&](int j, Raw8<T>& to) {
+    const int v = threadIdx.x + j * blockDim.x;
+    if (v < nvec) to.cached(weight + v * 8);
+    else to.zero();
+  };
+  if constexpr (kNorm && AHEAD) {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) load_weights(j, w[j]);
+  }
   // y as it is quantised; a plain row stays in its own type and is converted twice instead, which leaves registers for more rows
   float y[SRC == ROW_PLAIN ? 1 : VPT][8], sum = 0.f, top = 0.f;
   float amax[KIND == B200_ROW_INT8 ? 1 : VPT];
@@ -213,11 +223,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       continue;
     }
     const int v = threadIdx.x + j * blockDim.x;
-    Raw8<T> w;
-    if (kNorm) {
-      if (v < nvec) w.cached(static_cast<const T*>(p.w) + v * 8);
-      else w.zero();
-    }
+    if (kNorm && !AHEAD) load_weights(j, w[0]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float h = a[j].get(i);
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       }
       if (kNorm) {
         sum = fmaf(h, h, sum);
-        h *= w.get(i);
+        h *= w[AHEAD ? j : 0].get(i);
       }
       y[j][i] = h;
       if constexpr (KIND == B200_ROW_INT8) top = max_nan(top, fabsf(h));
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
   }
 }
 
-template <typename T, int SRC, int KIND, int VPT, bool FEW = false>
+template <typename T, int SRC, int KIND, int VPT, bool AHEAD = false>
 static int launch_row_regs(const RowParams& p, unsigned threads, unsigned rows_per_block, cudaStream_t st, const char* what) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cdiv(p.rows, rows_per_block));
@@ -297,7 +303,7 @@ static int launch_row_regs(const RowParams& p, unsigned threads, unsigned rows_p
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, row_quant_kernel<T, SRC, KIND, VPT, FEW>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, row_quant_kernel<T, SRC, KIND, VPT, AHEAD>, p);
   if (e != cudaSuccess) {
     set_error_detail("%s: %s", what, cudaGetErrorString(e));
     return B200_E_LAUNCH;
@@ -315,21 +321,25 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
                        (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.q % 8 == 0;
   if (!vectors) return launch_dependent(row_quant_any_kernel<T, SRC, KIND>, dim3((unsigned)p.rows), 256, 0, st, 1, what, p);
   // us for 1 / 2 / 4 / 8 vectors a thread, 203 and 16384 rows of 8192 bf16:
-  //   FP8, residual   3.8 / 3.7 / 3.6 / 6.4, 170 / 147 / 145 / 188 (6.5 TB/s)   int8, residual  4.0 / 3.7 / 2.6 / 4.7, 170 / 189 / 140 / 162 (6.7)
-  //   plain           2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5)           gated           3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
+  //   plain  2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5 TB/s)           gated  3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
+  // and for 1 / 2 / 4, with the weights requested ahead and (in brackets) as they are used:
+  //   FP8, residual   3.8 / 3.7 / 4.3 (3.8 / 4.2 / 5.4), 167 / 161 / 157 (170 / 160 / 153, 6.1 TB/s)
+  //   int8, residual  4.1 / 3.6 / 3.8 (4.0 / 3.8 / 5.1), 172 / 159 / 164 (171 / 189 / 142, 6.6)      16384 x 4096: 84 / 73 / 76 (84 / 85 / 74)
+  // and 400 x 14336: FP8 at 4 vectors 8.5 (9.6), int8 9.8 (9.5), whose registers then leave one block fewer.
   // Blocks that go through many rows, with a ring of them in shared memory that bulk copies fill, were no faster (plain 69 to 73 us).
-  int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (p.rows < 1024 ? 1 : 4) : KIND == B200_ROW_INT8 || nvec >= 512 || p.rows >= 1024 ? 4 : 1;
+  const bool short_or_few = nvec <= 512 || (p.rows <= 512 && nvec <= 1024);
+  int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (p.rows < 1024 ? 1 : 4) : short_or_few ? 2 : 4;
   if (tuning().row_vectors > 0) vpt = tuning().row_vectors < 8 ? (int)tuning().row_vectors : 8;
   while (vpt > 1 && nvec < 32 * vpt) vpt /= 2;
   while (vpt < 8 && cdiv(nvec, vpt) > (vpt <= 2 ? 1024 : 512)) vpt *= 2;
   const unsigned threads = (unsigned)align_up(cdiv(nvec, vpt), 32), rpb = threads == 32 ? 4 : 1;
-  const bool few = p.rows <= 148 * (740 / (int)threads);  // one wave of blocks with all the registers they like
+  constexpr bool kNorm = SRC >= ROW_NORM;
   switch (vpt) {
-    case 1: return launch_row_regs<T, SRC, KIND, 1>(p, threads, rpb, st, what);
-    case 2: return launch_row_regs<T, SRC, KIND, 2>(p, threads, rpb, st, what);
+    case 1: return launch_row_regs<T, SRC, KIND, 1, kNorm>(p, threads, rpb, st, what);
+    case 2: return launch_row_regs<T, SRC, KIND, 2, kNorm>(p, threads, rpb, st, what);
     case 4:
-      if constexpr (SRC >= ROW_NORM)
-        if (few) return launch_row_regs<T, SRC, KIND, 4, true>(p, threads, rpb, st, what);
+      if constexpr (kNorm && KIND != B200_ROW_INT8)
+        if (nvec > 1024) return launch_row_regs<T, SRC, KIND, 4, true>(p, threads, rpb, st, what);
       return launch_row_regs<T, SRC, KIND, 4>(p, threads, rpb, st, what);
     default: return launch_row_regs<T, SRC, KIND, 8>(p, threads, rpb, st, what);
   }

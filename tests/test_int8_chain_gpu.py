@@ -142,6 +142,34 @@ def test_side_stream_waits_for_its_inputs():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("rows", [1, 3, 40, 300])
+def test_long_chain_equals_step_by_step(rows):
+    """Layer after layer without a pause, every kernel resident before the one ahead has finished and buffers given out again at once:
+    the same bits as with a synchronisation behind every operator."""
+    mlps = [MLP(1024, 640, torch.bfloat16, seed=i) for i in range(3)]
+    lin = [quant_weight_int8(0.05 * torch.randn(1024, 1024, generator=torch.Generator().manual_seed(i)).cuda()) for i in range(3)]
+
+    def run(pause):
+        x, r = inputs(rows, 1024, torch.bfloat16, 9)
+        for k in range(60):
+            m, (w, s) = mlps[k % 3], lin[k % 3]
+            q, sc, r = S.rmsnorm_quant_int8(x, m.norm, 1e-6, residual=r)
+            pause()
+            mid = S.int8_scaled_mm(q, m.w1.t(), sc, m.s1, m.dtype)
+            pause()
+            q, sc = S.per_token_quant_int8(mid, fuse_silu_and_mul=True)
+            pause()
+            x = S.int8_scaled_mm(q, m.w2.t(), sc, m.s2, m.dtype)
+            pause()
+            x = S.w8a8_int8_linear(x, w, s)
+            pause()
+        return x, r
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(run(lambda: None), want))
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_threads_share_a_stream(rows):
     mlps = [MLP(1024, 512, torch.bfloat16, seed=i) for i in range(4)]

@@ -135,6 +135,17 @@ def test_quant_int8_every_pair_of_mantissas(dtype):
         assert torch.equal(q.cpu(), (x.float() / want).round().to(torch.int8))
 
 
+@pytest.mark.parametrize("width", [64, 100, 4096])
+def test_smallest_and_largest_values(width):
+    """Rows of nothing but subnormal fp16 numbers, and of the largest that each type has."""
+    g = torch.Generator().manual_seed(width)
+    for dtype, size in ((torch.float16, 2.0**-17), (torch.float16, 60000.0), (torch.bfloat16, 3e38), (torch.float32, 3e38), (torch.bfloat16, 1e-9)):
+        x = ((torch.rand(3, width, generator=g) * 2 - 1) * size).to(dtype)
+        q, s = S.per_token_quant_int8(x.cuda())
+        want = x.float().abs().amax(-1, keepdim=True).clamp_min(1e-10) / torch.tensor(127.0)
+        assert torch.equal(s.cpu(), want) and torch.equal(q.cpu(), (x.float() / want).round().to(torch.int8))
+
+
 @pytest.mark.parametrize("width", [1, 7, 8, 100, 128, 1000, 2048, 3584, 14336, 14337, 28672, 33000])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_silu_quant_int8(width, dtype):
