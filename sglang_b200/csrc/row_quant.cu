@@ -244,7 +244,25 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       amax[j] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) amax[j] = fmaxf(amax[j], fabsf(y[j][i]));
-      amax[j] = group_max<16>(amax[j]);
+    }
+  }
+  // 16 lanes hold VPT groups of 128 columns, one per vector: each step halves the values a lane still has, so that lane l ends with the
+  // maximum, and then the scale, of group l % VPT (16384 x 8192 144 us, with every group's maximum and scale in every lane 153)
+  if constexpr (KIND != B200_ROW_INT8) {
+    int n = VPT;
+#pragma unroll
+    for (int bit = 1; bit < 16; bit <<= 1) {
+      const bool upper = (threadIdx.x & bit) != 0;
+      if (n > 1) {
+        n /= 2;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float other = __shfl_xor_sync(0xffffffffu, upper ? amax[2 * i] : amax[2 * i + 1], bit);
+          amax[i] = fmaxf(upper ? amax[2 * i + 1] : amax[2 * i], other);
+        }
+      } else {
+        amax[0] = fmaxf(amax[0], __shfl_xor_sync(0xffffffffu, amax[0], bit));
+      }
     }
   }
   row_sum_max<kNorm, KIND == B200_ROW_INT8>(sum, top, blockDim.x >> 5, red);
@@ -268,26 +286,26 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512, row_min_blocks(SRC, VPT
       if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = pack8_s8(c);
     }
   } else {
+    const float m = fmaxf(amax[0] * rstd, 1e-10f);
+    Ue8m0 e = {};
+    float s = 0.f, inv;
+    if constexpr (KIND == B200_ROW_FP8) {
+      s = m * (1.f / 448.f);
+      inv = rstd * __fdividef(448.f, m);
+    } else {
+      e = ue8m0_of(m);
+      inv = rstd * e.inv;
+    }
+    const int own = threadIdx.x & 15, first = (threadIdx.x & ~15) + own * blockDim.x;
+    if (own < VPT && first < nvec) put_group_scale<KIND>(p, row, first >> 4, s, e.byte);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int v = threadIdx.x + j * blockDim.x;
-      const float m = fmaxf(amax[j] * rstd, 1e-10f);
-      Ue8m0 e = {};
-      float s = 0.f, inv;
-      if constexpr (KIND == B200_ROW_FP8) {
-        s = m * (1.f / 448.f);
-        inv = rstd * __fdividef(448.f, m);
-      } else {
-        e = ue8m0_of(m);
-        inv = rstd * e.inv;
-      }
+      const float f = __shfl_sync(0xffffffffu, inv, j, 16);
       uint2 out;
-      out.x = pack4_e4m3(y[j][0] * inv, y[j][1] * inv, y[j][2] * inv, y[j][3] * inv);
-      out.y = pack4_e4m3(y[j][4] * inv, y[j][5] * inv, y[j][6] * inv, y[j][7] * inv);
-      if (v < nvec) {
-        *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = out;
-        if ((threadIdx.x & 15) == 0) put_group_scale<KIND>(p, row, v >> 4, s, e.byte);
-      }
+      out.x = pack4_e4m3(y[j][0] * f, y[j][1] * f, y[j][2] * f, y[j][3] * f);
+      out.y = pack4_e4m3(y[j][4] * f, y[j][5] * f, y[j][6] * f, y[j][7] * f);
+      if (v < nvec) *reinterpret_cast<uint2*>(p.q + row * H + v * 8) = out;
     }
   }
 }
@@ -322,10 +340,9 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
   if (!vectors) return launch_dependent(row_quant_any_kernel<T, SRC, KIND>, dim3((unsigned)p.rows), 256, 0, st, 1, what, p);
   // us for 1 / 2 / 4 / 8 vectors a thread, 203 and 16384 rows of 8192 bf16:
   //   plain  2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5 TB/s)           gated  3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
-  // and for 1 / 2 / 4, with the weights requested ahead and (in brackets) as they are used:
-  //   FP8, residual   3.8 / 3.7 / 4.3 (3.8 / 4.2 / 5.4), 167 / 161 / 157 (170 / 160 / 153, 6.1 TB/s)
-  //   int8, residual  4.1 / 3.6 / 3.8 (4.0 / 3.8 / 5.1), 172 / 159 / 164 (171 / 189 / 142, 6.6)      16384 x 4096: 84 / 73 / 76 (84 / 85 / 74)
-  // and 400 x 14336: FP8 at 4 vectors 8.5 (9.6), int8 9.8 (9.5), whose registers then leave one block fewer.
+  // norms with a residual for 1 / 2 / 4, the first two with `ahead` (203 x 8192 at 2 vectors without it 4.2 FP8, 3.8 int8):
+  //   203 x 8192   FP8 3.9 / 3.5 / 5.1, int8 4.1 / 3.6 / 5.1         8192 x 8192  FP8 89 / 82 / 76 (6.2 TB/s), int8 90 / 83 / 74 (6.3)
+  //   2048 x 4096  FP8 11.4 / 9.6 / 10.7, int8 11.7 / 9.6 / 10.8     8192 x 4096  FP8 43 / 39 / 40, int8 44 / 39 / 40
   // Blocks that go through many rows, with a ring of them in shared memory that bulk copies fill, were no faster (plain 69 to 73 us).
   const bool short_or_few = nvec <= 512 || (p.rows <= 512 && nvec <= 1024);
   int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (p.rows < 1024 ? 1 : 4) : short_or_few ? 2 : 4;
@@ -337,10 +354,7 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
   switch (vpt) {
     case 1: return launch_row_regs<T, SRC, KIND, 1, kNorm>(p, threads, rpb, st, what);
     case 2: return launch_row_regs<T, SRC, KIND, 2, kNorm>(p, threads, rpb, st, what);
-    case 4:
-      if constexpr (kNorm && KIND != B200_ROW_INT8)
-        if (nvec > 1024) return launch_row_regs<T, SRC, KIND, 4, true>(p, threads, rpb, st, what);
-      return launch_row_regs<T, SRC, KIND, 4>(p, threads, rpb, st, what);
+    case 4: return launch_row_regs<T, SRC, KIND, 4>(p, threads, rpb, st, what);
     default: return launch_row_regs<T, SRC, KIND, 8>(p, threads, rpb, st, what);
   }
 }
