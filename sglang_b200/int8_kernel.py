@@ -1,7 +1,5 @@
-"""W8A8 int8 operators with the reference's names, arguments and error behaviour: the per-token quantiser
-(python/sglang/srt/layers/quantization/int8_kernel.py), the product with scales per token and per output channel
-(sgl-kernel/csrc/gemm/int8_gemm_kernel.cu, sgl-kernel/python/sgl_kernel/gemm.py) and the linear layer that runs both
-(python/sglang/srt/layers/quantization/w8a8_int8.py). CUDA tensors only; no fallback.
+"""W8A8 int8 operators: the per-token quantiser, the product with scales per token and per output channel, and the linear layer
+that runs both. CUDA tensors only; no fallback.
 """
 from __future__ import annotations
 
@@ -40,7 +38,7 @@ def per_token_quant_int8(
     if scale_dtype != torch.float32 or cal_sum:
         raise NotImplementedError("per_token_quant_int8: only fp32 scales without row sums are built")
     N.load()
-    pair = N.host.quant_int8(x, fuse_silu_and_mul)
+    pair = N.host.quant_int8(x, bool(fuse_silu_and_mul))
     if pair is not None:
         return pair
     assert x.dtype in (torch.bfloat16, torch.float16, torch.float32), f"unsupported input dtype {x.dtype}"
@@ -73,8 +71,7 @@ def int8_scaled_mm(
 
     ``mat_a [M, K]`` int8 with contiguous rows, ``mat_b [K, N]`` int8 column-major (a transposed ``[N, K]`` weight), ``scales_a``
     fp32 with ``M`` elements, ``scales_b`` fp32 with ``N``, ``bias [N]`` of ``out_dtype`` (bf16, fp16; fp32 is built, too). The
-    integer sums are exact; scales and bias are applied in fp32 and the result is rounded once. The preconditions are the
-    reference's: rows of ``mat_a`` and columns of ``mat_b`` start at multiples of 16 bytes, ``K`` is a multiple of 16, ``N`` of 8;
+    integer sums are exact; scales and bias are applied in fp32 and the result is rounded once. Preconditions: rows of ``mat_a`` and columns of ``mat_b`` start at multiples of 16 bytes, ``K`` is a multiple of 16, ``N`` of 8;
     beyond ``K`` = 131071 a 32-bit sum could overflow and the call is refused.
     """
     N.load()
@@ -120,8 +117,7 @@ def w8a8_int8_linear(
     weight_scale: torch.Tensor,
     bias: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """Quantise the activation per token, multiply, apply the scales and the bias: what the reference's
-    ``W8A8Int8LinearMethod.apply`` runs. ``input [.., K]`` bf16 or fp16, ``weight [N, K]`` int8, ``weight_scale`` fp32 with ``N``
+    """Quantise the activation per token, multiply, apply the scales and the bias. ``input [.., K]`` bf16 or fp16, ``weight [N, K]`` int8, ``weight_scale`` fp32 with ``N``
     elements, ``bias [N]`` of the input's type; the result has the input's type."""
     N.load()
     out = N.host.int8_linear(input, weight, weight_scale, bias)

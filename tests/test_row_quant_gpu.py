@@ -156,6 +156,12 @@ def test_silu_quant_int8(width, dtype):
         check_int8(q, s, gate / (1 + (-gate).exp()) * up, extra=2.0**-16)
 
 
+@pytest.mark.parametrize("flag", [1, "gate"])
+def test_any_true_value_fuses_the_gate(flag):
+    x = draw(3, 512, torch.bfloat16, 4)
+    assert all(torch.equal(a, b) for a, b in zip(S.per_token_quant_int8(x, fuse_silu_and_mul=flag), S.per_token_quant_int8(x, fuse_silu_and_mul=True)))
+
+
 def test_leading_dimensions_and_empty_inputs():
     x, w = draw(6, 256, torch.bfloat16, 1).view(2, 3, 256), draw(1, 256, torch.bfloat16, 2)[0]
     q, s, r = S.rmsnorm_quant_int8(x, w, residual=x)
