@@ -10,7 +10,7 @@ namespace b200 {
 constexpr int64_t kInt8MaxK = 131071;
 
 static int check_int8(const char* what, const void* a, int64_t lda, const void* b, int64_t ldb, const void* sa, const void* sb,
-                      const void* c, int c_dtype, int64_t M, int64_t N, int64_t K) {
+                      const void* bias, const void* c, int c_dtype, int64_t M, int64_t N, int64_t K) {
   B200_CHECK_ARG(a && b && sa && sb && c, "%s: null pointer", what);
   B200_CHECK_ARG(c_dtype == B200_BF16 || c_dtype == B200_F16 || c_dtype == B200_F32, "%s: unknown dtype code %d", what, c_dtype);
   B200_CHECK_ARG(K > 0, "%s: K is zero", what);
@@ -22,7 +22,9 @@ static int check_int8(const char* what, const void* a, int64_t lda, const void* 
   B200_UNSUPPORTED(N % 8 != 0, "%s: N=%lld is not a multiple of 8", what, (long long)N);
   B200_UNSUPPORTED(K > kInt8MaxK, "%s: K=%lld, 32-bit sums hold %lld products", what, (long long)K, (long long)kInt8MaxK);
   B200_UNSUPPORTED(M > 0x7fffff00LL || N > 0x7fffff00LL || cdiv(M, 16) * cdiv(N, 128) > 0x7fffffffLL / 8, "%s: too many tiles", what);
-  B200_CHECK_ARG((uintptr_t)c % 16 == 0 && (uintptr_t)sa % 4 == 0 && (uintptr_t)sb % 4 == 0, "%s: misaligned pointer", what);
+  B200_CHECK_ARG((uintptr_t)c % 16 == 0 && (uintptr_t)sa % 4 == 0 && (uintptr_t)sb % 4 == 0 &&
+                     (uintptr_t)bias % (c_dtype == B200_F32 ? 4 : 2) == 0,
+                 "%s: misaligned pointer", what);
   return B200_OK;
 }
 
@@ -177,7 +179,7 @@ extern "C" int b200_int8_scaled_mm(const void* a, int64_t lda, const float* sa, 
   using namespace b200;
   B200_CHECK_ARG(M >= 0 && N >= 0 && K >= 0, "int8_scaled_mm: negative shape");
   if (M == 0 || N == 0) return B200_OK;
-  if (int rc = check_int8("int8_scaled_mm", a, lda, b, ldb, sa, sb, c, c_dtype, M, N, K)) return rc;
+  if (int rc = check_int8("int8_scaled_mm", a, lda, b, ldb, sa, sb, bias, c, c_dtype, M, N, K)) return rc;
   return run_int8(a, lda, sa, b, ldb, sb, bias, c, c_dtype, M, N, K, static_cast<cudaStream_t>(stream));
 }
 
@@ -218,7 +220,7 @@ extern "C" int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, c
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int aligned = (uintptr_t)x % 16 == 0 && (M == 1 || x_ld % 8 == 0);
   if (linear_fuses(M, K, aligned)) {
-    if (int rc = check_int8("w8a8_int8_linear", w, ldw, w, ldw, sw, sw, out, x_dtype, M, N, K)) return rc;
+    if (int rc = check_int8("w8a8_int8_linear", w, ldw, w, ldw, sw, sw, bias, out, x_dtype, M, N, K)) return rc;
     Int8Params p;
     if (int rc = fill_int8(p, nullptr, w, ldw, sw, bias, out, M, N, K)) return rc;
     return x_dtype == B200_BF16 ? run_int8_linear_fused<__nv_bfloat16>(x, x_ld, w, ldw, K, p, st)
@@ -231,7 +233,7 @@ extern "C" int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, c
   }
   void* q = workspace;
   float* s = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align_up((size_t)M * K, 16));
-  if (int rc = check_int8("w8a8_int8_linear", q, K, w, ldw, s, sw, out, x_dtype, M, N, K)) return rc;
+  if (int rc = check_int8("w8a8_int8_linear", q, K, w, ldw, s, sw, bias, out, x_dtype, M, N, K)) return rc;
   if (int rc = b200_per_token_quant_int8(x, x_ld, x_dtype, q, s, M, K, 0, stream)) return rc;
   return run_int8(q, K, s, w, ldw, sw, bias, out, x_dtype, M, N, K, st);
 }

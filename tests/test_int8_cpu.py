@@ -95,13 +95,14 @@ def test_linear_method_loads_a_checkpoint():
 FAKE = 1 << 20  # an aligned address that no refused call reads
 
 
-def mm(a=FAKE, lda=64, b=FAKE, ldb=64, sa=FAKE, sb=FAKE, c=FAKE, dtype=0, M=4, n=64, K=64):
-    return N.load().b200_int8_scaled_mm(a, lda, sa, b, ldb, sb, 0, c, dtype, M, n, K, None)
+def mm(a=FAKE, lda=64, b=FAKE, ldb=64, sa=FAKE, sb=FAKE, c=FAKE, dtype=0, M=4, n=64, K=64, bias=0):
+    return N.load().b200_int8_scaled_mm(a, lda, sa, b, ldb, sb, bias, c, dtype, M, n, K, None)
 
 
 @pytest.mark.parametrize("kw,status", [
     (dict(a=None), N.E_BAD_ARG), (dict(sb=None), N.E_BAD_ARG), (dict(dtype=3), N.E_BAD_ARG), (dict(M=-1), N.E_BAD_ARG),
     (dict(K=0), N.E_BAD_ARG), (dict(lda=32), N.E_BAD_ARG), (dict(ldb=48), N.E_BAD_ARG), (dict(c=FAKE + 8), N.E_BAD_ARG), (dict(sa=FAKE + 2), N.E_BAD_ARG),
+    (dict(bias=FAKE + 1), N.E_BAD_ARG), (dict(bias=FAKE + 2, dtype=2), N.E_BAD_ARG),
     (dict(K=72, lda=80, ldb=80), N.E_UNSUPPORTED), (dict(lda=72), N.E_UNSUPPORTED), (dict(ldb=65), N.E_UNSUPPORTED),
     (dict(a=FAKE + 8), N.E_UNSUPPORTED), (dict(b=FAKE + 1), N.E_UNSUPPORTED), (dict(n=65), N.E_UNSUPPORTED), (dict(n=4), N.E_UNSUPPORTED),
     (dict(K=131072, lda=131072, ldb=131072), N.E_UNSUPPORTED), (dict(M=1 << 40), N.E_UNSUPPORTED), (dict(M=0, a=None), 0), (dict(n=0), 0)])
