@@ -439,9 +439,7 @@ int b200_moe_sum_reduce(const void* rows, const int32_t* topk_ids, void* out, in
  *
  * b200_rmsnorm_quant: h = x (+ residual), y = h * weight / sqrt(mean(h^2) + eps) in fp32, never rounded to 16 bits;
  *   residual_out [M,H] = h rounded to the input type (NULL without residual). The sum is normalised unrounded.
- *   replaces: the pair fused_add_rmsnorm / rmsnorm (python/sglang/srt/layers/layernorm.py) -> quantiser of the linear.
  * b200_per_token_quant_int8: y = x, or with fuse_silu_and_mul y = silu(gate) * up in fp32 of rows [gate | up] (x is [M,2K]).
- *   replaces: python/sglang/srt/layers/quantization/int8_kernel.py (per_token_quant_int8), with silu_and_mul before it.
  * x and residual: rows x_ld / residual_ld elements apart, elements of a row contiguous, of `dtype` like weight [H].
  * kind, with amax floored at 1e-10:
  *   B200_ROW_INT8       s[m] = amax(row) / 127, q = y / s rounded to the nearest integer, ties to even (s_stride_* unused);
@@ -460,7 +458,6 @@ int b200_per_token_quant_int8(const void* x, int64_t x_ld, int dtype, void* q, f
 
 /* ---------------------------------------------------------------------------------------
  * int8_scaled_mm
- * replaces: torch.ops.sgl_kernel.int8_scaled_mm (sgl-kernel/csrc/gemm/int8_gemm_kernel.cu)
  * C[m,n] = (sum_k A[m,k]*B[n,k]) * sa[m] * sb[n] (+ bias[n]): exact 32-bit integer sums, then fp32, rounded once.
  * A [M,K] and B [N,K] signed 8-bit, rows lda / ldb bytes apart; bias [N] of C's type or NULL; C [M,N] contiguous.
  * Requirements: K, lda and ldb multiples of 16, A, B and C 16-byte aligned, N % 8 == 0, 0 < K <= 131071. No workspace. */
@@ -474,7 +471,7 @@ int b200_int8_scaled_mm(const void* A, int64_t lda, const float* sa, const void*
 int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* kernel, int* tile, int* splits);
 
 /* b200_w8a8_int8_linear: per_token_quant_int8 of x [M,K] (bf16 / f16, rows x_ld elements apart), then int8_scaled_mm with the weight
- * w [N,K]; out [M,N] of x's type. Replaces W8A8Int8LinearMethod.apply (python/sglang/srt/layers/quantization/w8a8_int8.py).
+ * w [N,K]; out [M,N] of x's type.
  * workspace: the quantised rows and their scales, 16-byte aligned, the caller's until the kernels are done; none where a few short
  * rows (M <= 4, K <= 6144, M*K <= 8192) that start at multiples of 16 bytes (x_aligned) are quantised by the product's own kernel. The result is the same. */
 size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_aligned);

@@ -1,9 +1,8 @@
 """Weight-side objects of the W8A8 int8 path: the quantisation config and the linear "quant method" that create the parameters
 of a checkpoint with int8 weights and one scale per output channel, and call the operators.
 
-They mirror python/sglang/srt/layers/quantization/w8a8_int8.py (``W8A8Int8Config``, ``W8A8Int8LinearMethod``) with the same
-parameter names (``weight`` int8 ``[N, K]``, ``weight_scale`` fp32 ``[N, 1]``), so that a state dict of such a checkpoint loads as
-is. Dynamic symmetric activations only; expert weights are not built.
+The parameters are ``weight`` int8 ``[N, K]`` and ``weight_scale`` fp32 ``[N, 1]``, the names that such checkpoints use, so that a
+state dict loads as is. Dynamic symmetric activations only; expert weights are not built.
 """
 from __future__ import annotations
 

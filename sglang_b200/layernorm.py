@@ -1,6 +1,5 @@
 """RMSNorm in front of a quantised linear, with the residual's addition and the linear's quantiser in the same pass over the
-rows: what ``RMSNorm.forward`` (python/sglang/srt/layers/layernorm.py) and the activation quantiser of the linear behind it
-compute one after the other, without the 16-bit tensor in between. CUDA tensors only; no fallback.
+rows, without the 16-bit tensor in between. CUDA tensors only; no fallback.
 """
 from __future__ import annotations
 
