@@ -50,16 +50,16 @@ static float join(float a, float b) {  // near the larger of the two, a little a
 }
 
 // Time of one call in us, back to back with others: started from a least-squares fit, the constants were then moved until the choice
-// among 3435 measured sizes (1 to 4096 rows, N 256 to 57344, K 256 to 28672, each with every tile and split below) was as near the
-// best of them as it would come: 0.4 % behind on average up to 16 rows, 1.2 % above, 4 % at the 90th percentile.
+// among 10468 measured sizes (1 to 4096 rows, N 256 to 57344, K 256 to 28672, each with every tile and split below) was as near the
+// best of them as it would come: 0.5 % behind on average up to 16 rows, 0.7 to 1.8 % above, 2 and 5 % at the 90th percentile.
 struct StreamCost {
   float start, alone, alone_nt, shared, shared_nt;  // a K block of a CTA that has its SM to itself, of one of several on an SM
   float bandwidth, store_nt, sum, sum_nt, cta, wave;
 };
 static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int sms) {
-  static const StreamCost few = {1.53f, 0.270f, 0.0020f, 0.206f, 0.f, 9.64e6f, 0.0037f, 0.193f, 0.f, 0.548f, 0.64f};
-  static const StreamCost some = {1.98f, 0.210f, 0.0020f, 0.1184f, 0.0016f, 7.81e6f, 0.0125f, 0.166f, 0.0084f, 0.775f, 0.48f};
-  static const StreamCost many = {1.68f, 0.2024f, 0.0009f, 0.0993f, 0.0018f, 8.21e6f, 0.0114f, 0.253f, 0.0211f, 0.887f, 0.84f};
+  static const StreamCost few = {1.34f, 0.2743f, 0.0026f, 0.1973f, 0.f, 5.91e6f, 0.0034f, 0.435f, 0.f, 0.682f, 0.63f};
+  static const StreamCost some = {2.17f, 0.2018f, 0.0018f, 0.1200f, 0.0016f, 8.20e6f, 0.0125f, 0.199f, 0.0120f, 0.751f, 0.39f};
+  static const StreamCost many = {1.98f, 0.2025f, 0.0010f, 0.1134f, 0.0021f, 9.14e6f, 0.0112f, 0.305f, 0.0178f, 0.688f, 1.02f};
   const StreamCost& c = M <= 16 ? few : M <= 64 ? some : many;
   const int per_sm = nt <= 64 ? 2 : 1;
   const int64_t items = cdiv(N, 128) * cdiv(M, nt), kbs = cdiv(cdiv(K, kBK), splits);
@@ -73,10 +73,10 @@ static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int 
 static float pair_us(int64_t M, int64_t N, int64_t K, bool swap, int bn, int splits, int sms) {
   const int64_t tiles = swap ? cdiv(M, bn) * cdiv(N, 2 * kBM) : cdiv(N, bn) * cdiv(M, 2 * kBM), kbs = cdiv(cdiv(K, kBK), splits);
   const int64_t waves = cdiv(tiles, clusters_at_once(2 * splits, sms));
-  const float loop = kbs * (0.1114f + 0.0009f * bn), epilogue = 0.89f + (swap ? 0.0089f : 0.0082f) * bn;
-  const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 7.61e6f;
-  const float sum = splits > 1 ? 0.98f + 0.0177f * bn * (splits - 1) / splits : 0.f;
-  return (swap ? 3.54f : 3.48f) + join((waves - 1) * (loop > epilogue ? loop : epilogue) + loop, memory) + (swap ? 0.004f : 0.0035f) * bn + sum * waves;
+  const float loop = kbs * (0.1238f + 0.0009f * bn), epilogue = 1.04f + (swap ? 0.0092f : 0.0078f) * bn;
+  const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 8.23e6f;
+  const float sum = splits > 1 ? 1.19f + 0.0187f * bn * (splits - 1) / splits : 0.f;
+  return (swap ? 3.55f : 3.47f) + join((waves - 1) * (loop > epilogue ? loop : epilogue) + loop, memory) + (swap ? 0.0042f : 0.0037f) * bn + sum * waves;
 }
 
 static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
@@ -115,10 +115,10 @@ static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
     if (nt == 16) break;
   }
   if (M > 32)
-    for (int bn = 64; bn <= 256; bn += 32)
+    for (int bn = 32; bn <= 256; bn += 32)
       for (int splits = 1; splits <= 4; splits *= 2) {
         if (splits == 1 || cdiv(N, bn) * cdiv(M, 2 * kBM) * splits <= sms / 2) consider(INT8_PAIR, bn, splits);
-        if (splits == 1 || cdiv(M, bn) * cdiv(N, 2 * kBM) * splits <= sms / 2) consider(INT8_PAIR_SWAPPED, bn, splits);
+        if (bn > 32 && (splits == 1 || cdiv(M, bn) * cdiv(N, 2 * kBM) * splits <= sms / 2)) consider(INT8_PAIR_SWAPPED, bn, splits);
       }
   return best;
 }
