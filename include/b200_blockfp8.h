@@ -473,7 +473,7 @@ int b200_plan_int8(int64_t M, int64_t N, int64_t K, int sms, int* kernel, int* t
 /* b200_w8a8_int8_linear: per_token_quant_int8 of x [M,K] (bf16 / f16, rows x_ld elements apart), then int8_scaled_mm with the weight
  * w [N,K]; out [M,N] of x's type.
  * workspace: the quantised rows and their scales, 16-byte aligned, the caller's until the kernels are done; none where a few short
- * rows (M <= 4, K <= 6144, M*K <= 8192) that start at multiples of 16 bytes (x_aligned) are quantised by the product's own kernel. The result is the same. */
+ * rows (M <= 4, M*K <= 16384) that start at multiples of 16 bytes (x_aligned) are quantised by the product's own kernel. The result is the same. */
 size_t b200_w8a8_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_aligned);
 int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, const void* w, int64_t ldw,
                           const float* sw, const void* bias, void* out, int64_t M, int64_t N, int64_t K,

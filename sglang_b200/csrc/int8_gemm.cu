@@ -186,11 +186,12 @@ extern "C" int b200_int8_scaled_mm(const void* a, int64_t lda, const float* sa, 
 namespace b200 {
 
 // One launch for the layer, where the rows are few and short enough that every CTA may look for their largest magnitudes itself, and
-// start at multiples of 16 bytes. Two launches and one, replayed from a graph, 1 row: 6144 x 4096 9.06, 8.87 us; 28672 x 2048 14.4, 13.1;
-// past the limits 4096 x 14336 14.3, 15.0, and 4 rows 6144 x 4096 9.2, 9.2; launched from Python 7.0, 5.2 us of host time.
+// start at multiples of 16 bytes. Two launches and one, replayed from a graph: 1 x 6144 x 4096 8.5, 6.9 us, 1 x 28672 x 4096 23.1, 21.7,
+// 1 x 4096 x 14336 13.5, 13.5, 4 x 6144 x 4096 8.4, 8.0; past the limit 4 x 4096 x 6144 8.1, 9.3, 2 x 4096 x 14336 13.7, 14.3; launched from
+// Python 7.0, 5.2 us of host time.
 static bool linear_fuses(int64_t M, int64_t K, int aligned) {
   if (!aligned || M > Int8StreamCfg<16, true>::kQuantRows || tuning().int8_linear_fused == 0) return false;
-  return tuning().int8_linear_fused > 0 || (K <= 6144 && M * K <= 8192);
+  return tuning().int8_linear_fused > 0 || M * K <= 16384;
 }
 
 template <typename T>
