@@ -79,16 +79,21 @@ __device__ __forceinline__ void put_group_scale(const RowParams& p, int64_t row,
   }
 }
 
-// A row per block, one element per thread and step, read twice: any width and alignment.
-template <typename T, int SRC, int KIND>
-__global__ void __launch_bounds__(256) row_quant_any_kernel(const RowParams p) {
+// A row per block, element by element, some of them under way at once: any width and alignment. KEEP: the values wait in shared memory, as
+// fp32, for the row's scale (gated 8192 x 5001 69 us, computed twice 79 with one element at a time, 112 with four). A plain row is read again
+// instead, 43 against 45. Bound by the instructions per element: 2.8 to 3 TB/s.
+constexpr int kKeepWidth = 12000;  // beside the reductions' 256 bytes it stays below the 48 KB of any launch
+template <typename T, int SRC, int KIND, int BLOCK, bool KEEP>
+__global__ void __launch_bounds__(BLOCK) row_quant_any_kernel(const RowParams p) {
   __shared__ float red[64];
+  extern __shared__ float kept[];
   grid_dependency_wait();
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* r = static_cast<const T*>(p.r) + row * p.r_ld;
   const T* w = static_cast<const T*>(p.w);
   const int H = p.H;
+  constexpr int kAtOnce = SRC == ROW_PLAIN || SRC == ROW_NORM ? 8 : 4;  // elements under way
   auto value = [&](int i) {
     const float v = to_f32<T>(x[i]);
     if constexpr (SRC == ROW_SILU) return silu_mul(v, to_f32<T>(x[H + i]));
@@ -97,26 +102,47 @@ __global__ void __launch_bounds__(256) row_quant_any_kernel(const RowParams p) {
   };
   auto weight = [&](int i) { return SRC >= ROW_NORM ? to_f32<T>(w[i]) : 1.f; };
   float sum = 0.f, top = 0.f;
-  for (int i = threadIdx.x; i < H; i += 256) {
-    const float h = value(i);
-    sum = fmaf(h, h, sum);
-    if constexpr (KIND == B200_ROW_INT8) top = max_nan(top, fabsf(h * weight(i)));
-    if constexpr (SRC == ROW_ADD_NORM) static_cast<T*>(p.r_out)[row * H + i] = from_f32<T>(h);
+  for (int i0 = threadIdx.x; i0 < H; i0 += kAtOnce * BLOCK) {
+    float h[kAtOnce], y[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * BLOCK;
+      h[u] = i < H ? value(i) : 0.f;
+      if (KEEP || KIND == B200_ROW_INT8) y[u] = i < H ? h[u] * weight(i) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * BLOCK;
+      sum = fmaf(h[u], h[u], sum);
+      if (KIND == B200_ROW_INT8) top = max_nan(top, fabsf(y[u]));
+      if (KEEP && i < H) kept[i] = y[u];
+      if (SRC == ROW_ADD_NORM && i < H) static_cast<T*>(p.r_out)[row * H + i] = from_f32<T>(h[u]);
+    }
   }
-  row_sum_max<true, true>(sum, top, 8, red);
+  row_sum_max<true, true>(sum, top, BLOCK / 32, red);
   const float rstd = SRC >= ROW_NORM ? rsqrtf(sum / (float)H + p.eps) : 1.f;
+  auto normed = [&](int i) { return (KEEP ? kept[i] : value(i) * weight(i)) * rstd; };
   if constexpr (KIND == B200_ROW_INT8) {
     const float s = int8_scale(top * rstd), inv = __frcp_rn(s);
     if (threadIdx.x == 0) static_cast<float*>(p.s)[row] = s;
-    for (int i = threadIdx.x; i < H; i += 256)
-      p.q[row * H + i] = (uint8_t)rint_bits(div_by(value(i) * weight(i) * rstd, s, inv));
+    for (int i0 = threadIdx.x; i0 < H; i0 += kAtOnce * BLOCK) {
+      float y[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = i0 + u * BLOCK;
+        y[u] = i < H ? normed(i) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (i0 + u * BLOCK < H) p.q[row * H + i0 + u * BLOCK] = (uint8_t)rint_bits(div_by(y[u], s, inv));
+    }
   } else {  // 128 columns: four per lane of a warp
-    for (int g = threadIdx.x >> 5; g * 128 < H; g += 8) {
+    for (int g = threadIdx.x >> 5; g * 128 < H; g += BLOCK / 32) {
       const int i0 = g * 128 + (threadIdx.x & 31) * 4;
       float y[4], amax = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        y[k] = value(i0 + k) * weight(i0 + k) * rstd;
+        y[k] = normed(i0 + k);
         amax = fmaxf(amax, fabsf(y[k]));
       }
       amax = fmaxf(group_max<32>(amax), 1e-10f);
@@ -337,7 +363,16 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
   const bool vectors = p.H % 8 == 0 && nvec <= 4096 && (p.rows == 1 || p.x_ld % (16 / (int)sizeof(T)) == 0) && (uintptr_t)p.x % 16 == 0 &&
                        (SRC != ROW_ADD_NORM || (even(p.r, p.rows == 1 ? 0 : p.r_ld) && (uintptr_t)p.r_out % 16 == 0)) &&
                        (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.q % 8 == 0;
-  if (!vectors) return launch_dependent(row_quant_any_kernel<T, SRC, KIND>, dim3((unsigned)p.rows), 256, 0, st, 1, what, p);
+  if (!vectors) {
+    const dim3 grid((unsigned)p.rows);
+    const size_t keep = (size_t)p.H * 4;
+    constexpr bool kKeep = SRC != ROW_PLAIN;
+    if (p.H <= 1024)  // 16384 x 701: 18 us; with 256 threads, an element at a time, 39
+      return launch_dependent(row_quant_any_kernel<T, SRC, KIND, 128, kKeep>, grid, 128, kKeep ? keep : 0, st, 1, what, p);
+    if (kKeep && p.H <= kKeepWidth)
+      return launch_dependent(row_quant_any_kernel<T, SRC, KIND, 256, kKeep>, grid, 256, keep, st, 1, what, p);
+    return launch_dependent(row_quant_any_kernel<T, SRC, KIND, 256, false>, grid, 256, 0, st, 1, what, p);
+  }
   // us for 1 / 2 / 4 / 8 vectors a thread, 203 and 16384 rows of 8192 bf16:
   //   plain  2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5 TB/s)           gated  3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
   // norms with a residual for 1 / 2 / 4, the first two with `ahead` (203 x 8192 at 2 vectors without it 4.2 FP8, 3.8 int8):
