@@ -58,8 +58,8 @@ struct StreamCost {
 };
 static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int sms) {
   static const StreamCost few = {1.34f, 0.2743f, 0.0026f, 0.1973f, 0.f, 5.91e6f, 0.0034f, 0.435f, 0.f, 0.682f, 0.63f};
-  static const StreamCost some = {2.17f, 0.2018f, 0.0018f, 0.1200f, 0.0016f, 8.20e6f, 0.0125f, 0.199f, 0.0120f, 0.751f, 0.39f};
-  static const StreamCost many = {1.98f, 0.2025f, 0.0010f, 0.1134f, 0.0021f, 9.14e6f, 0.0112f, 0.305f, 0.0178f, 0.688f, 1.02f};
+  static const StreamCost some = {2.28f, 0.2091f, 0.0017f, 0.1168f, 0.0016f, 10.62e6f, 0.0148f, 0.482f, 0.0127f, 0.770f, 0.42f};
+  static const StreamCost many = {1.97f, 0.2161f, 0.0010f, 0.1137f, 0.0022f, 9.43e6f, 0.0109f, 0.350f, 0.0177f, 0.722f, 0.73f};
   const StreamCost& c = M <= 16 ? few : M <= 64 ? some : many;
   const int per_sm = nt <= 64 ? 2 : 1;
   const int64_t items = cdiv(N, 128) * cdiv(M, nt), kbs = cdiv(cdiv(K, kBK), splits);
@@ -73,10 +73,10 @@ static float stream_us(int64_t M, int64_t N, int64_t K, int nt, int splits, int 
 static float pair_us(int64_t M, int64_t N, int64_t K, bool swap, int bn, int splits, int sms) {
   const int64_t tiles = swap ? cdiv(M, bn) * cdiv(N, 2 * kBM) : cdiv(N, bn) * cdiv(M, 2 * kBM), kbs = cdiv(cdiv(K, kBK), splits);
   const int64_t waves = cdiv(tiles, clusters_at_once(2 * splits, sms));
-  const float loop = kbs * (0.1238f + 0.0009f * bn), epilogue = 1.04f + (swap ? 0.0092f : 0.0078f) * bn;
-  const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 8.23e6f;
-  const float sum = splits > 1 ? 1.19f + 0.0187f * bn * (splits - 1) / splits : 0.f;
-  return (swap ? 3.55f : 3.47f) + join((waves - 1) * (loop > epilogue ? loop : epilogue) + loop, memory) + (swap ? 0.0042f : 0.0037f) * bn + sum * waves;
+  const float loop = kbs * (0.1221f + 0.0009f * bn), epilogue = 1.04f + (swap ? 0.0088f : 0.0074f) * bn;
+  const float memory = ((float)N * K + (float)M * K + 2.f * M * N) / 8.27e6f;
+  const float sum = splits > 1 ? 1.15f + 0.0197f * bn * (splits - 1) / splits : 0.f;
+  return (swap ? 3.57f : 3.47f) + join((waves - 1) * (loop > epilogue ? loop : epilogue) + loop, memory) + (swap ? 0.0040f : 0.0036f) * bn + sum * waves;
 }
 
 static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, int sms) {
