@@ -271,6 +271,25 @@ def test_long_prefills(rows, width, pad, dtype):
             check_int8(q[part], s[part], gate / (1 + (-gate).exp()) * up, extra=2.0**-16)
 
 
+@pytest.mark.parametrize("width", [128, 512, 1024, 1152, 8192, 11904, 12032, 14336])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_unaligned_rows_of_every_width(width, dtype):
+    """Rows that start off the 16-byte boundaries: narrow ones, those whose values are kept and those too wide for that."""
+    wide = draw(3, 2 * width + 2, dtype, width)
+    x, r, w = wide[:, 1 : 1 + width], wide[:, 1 + width : 1 + 2 * width], draw(1, width, dtype, 5, outliers=False)[0]
+    y, h = normed(x, r, w, 1e-6)
+    q, s, out = S.rmsnorm_quant_int8(x, w, 1e-6, residual=r)
+    check_int8(q, s, y)
+    check_residual(out, h, dtype)
+    for ue8m0 in (False, True):
+        q, s, out = S.rmsnorm_quant_fp8(x, w, 128, 1e-6, residual=r, column_major_scales=ue8m0, scale_tma_aligned=ue8m0, scale_ue8m0=ue8m0)
+        check_fp8(q.float(), s, y, ue8m0)
+        check_residual(out, h, dtype)
+    q, s = S.per_token_quant_int8(wide[:, 1 : 1 + 2 * width], fuse_silu_and_mul=True)
+    gate, up = x.double(), r.double()
+    check_int8(q, s, gate / (1 + (-gate).exp()) * up, extra=2.0**-16)
+
+
 def test_offsets_past_31_bits():
     """Rows that lie more than 2^31 elements into their tensors."""
     rows, width = 270000, 8192
