@@ -13,7 +13,7 @@
 // Protocol of a pair (rank 0 = leader):
 //   full[s]   (leader's)  2 arrivals (one expect_tx per producer) + the bytes of both CTAs' loads
 //   empty[s]  (each CTA)  arrival from the leader's commit       tfull[b] (each CTA)  likewise, when a tile's sums are complete
-//   tempty[b] (leader's)  16 arrivals: the epilogue warps of both CTAs
+//   tempty[b] (leader's)  16 arrivals: the epilogue warps of both CTAs, where a later tile of the pair uses the accumulator
 #pragma once
 
 #include "int8_gemm.cuh"
@@ -320,7 +320,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(leader_tempty + 8 * b);  // the accumulator is in registers
+      // The accumulator is in registers. Only for a tile that waits for it: nobody would wait for the last ones, and the follower's could
+      // then reach the leader's shared memory after the leader has left it.
+      if (lane == 0 && t + 2 * npairs < tiles) ptx::mbar_arrive_cluster(leader_tempty + 8 * b);
       if (++b == 2) b = 0, phase ^= 1;
     }
     if (lane == 0) ptx::tma_store_wait_all();
@@ -338,7 +340,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   ptx::tc_fence_before();
   __syncthreads();
   ptx::cluster_arrive_relaxed();
-  ptx::cluster_wait();  // neither CTA leaves while the other may still signal its barriers or read its shared memory
+  // Neither CTA leaves while the other may still signal its barriers or read its shared memory: every such signal has been waited for by
+  // then (this barrier itself orders nothing), and it holds a CTA back until its peer's waits are done, too.
+  ptx::cluster_wait();
   if (threadIdx.x == 0 && *abort_flag) atomicCAS(p.status, 0, 1);
   if (warp == Cfg::kMmaWarp) {
     ptx::tc_fence_after();
