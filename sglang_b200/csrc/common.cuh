@@ -160,12 +160,28 @@ __device__ __forceinline__ int fast_div(int n, FastDiv f) {
   return f.mul == 0u ? n : (int)(__umulhi((uint32_t)n, f.mul) >> f.shr);
 }
 
-// 16-byte read-only global load (bypasses L1 allocation: streamed once).
-__device__ __forceinline__ uint4 ld_nc_16(const void* p) {
+// Loads of operands. A kernel launched as a programmatic dependent may be resident while an earlier kernel of the stream still writes what it
+// will read; it waits (grid_dependency_wait) and reads then. The read-only path (ld.global.nc, __ldg, whatever the compiler makes of a
+// const __restrict__ parameter) is defined only for data that nobody writes while the kernel lives, so a line of it may be stale behind the
+// wait. These are ordinary loads, which the wait covers, and volatile, so that the compiler leaves them behind it.
+__device__ __forceinline__ float ld_operand(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int32_t ld_operand(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ld_operand(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_stream_16(const void* p) {  // read once: no line in L1
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -206,7 +222,7 @@ template <>
 struct Vec16<__nv_bfloat16> {
   static constexpr int kLoads = 2;  // 16-byte loads per 16 elements
   __device__ static void load(const __nv_bfloat16* p, float (&f)[16]) {
-    uint4 r[2] = {ld_nc_16(p), ld_nc_16(p + 8)};
+    uint4 r[2] = {ld_stream_16(p), ld_stream_16(p + 8)};
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -219,7 +235,7 @@ struct Vec16<__nv_bfloat16> {
 template <>
 struct Vec16<__half> {
   __device__ static void load(const __half* p, float (&f)[16]) {
-    uint4 r[2] = {ld_nc_16(p), ld_nc_16(p + 8)};
+    uint4 r[2] = {ld_stream_16(p), ld_stream_16(p + 8)};
     const __half2* h = reinterpret_cast<const __half2*>(r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -234,7 +250,7 @@ struct Vec16<float> {
   __device__ static void load(const float* p, float (&f)[16]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint4 r = ld_nc_16(p + 4 * i);
+      uint4 r = ld_stream_16(p + 4 * i);
       f[4 * i] = __uint_as_float(r.x);
       f[4 * i + 1] = __uint_as_float(r.y);
       f[4 * i + 2] = __uint_as_float(r.z);

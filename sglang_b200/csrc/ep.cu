@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(128) ep_dispatch_kernel(const EpDispatchParams
     if (!need) continue;  // uniform over the block
     const uint4* src = reinterpret_cast<const uint4*>(a.x_q + t * a.H);
     uint4* dst = reinterpret_cast<uint4*>(a.recv_q[d] + slot * a.H);
-    for (int64_t c = threadIdx.x; c < chunks; c += blockDim.x) dst[c] = ld_nc_16(src + c);
+    for (int64_t c = threadIdx.x; c < chunks; c += blockDim.x) dst[c] = ld_stream_16(src + c);
     for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) a.recv_s[d][slot * groups + g] = a.x_s[t * groups + g];
   }
 }

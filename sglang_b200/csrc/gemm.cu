@@ -18,7 +18,7 @@ struct FanOut {
 // C[m, n] = sum over splits of the fp32 partials; 8 elements per thread. With a fan-out the sum
 // goes to every destination buffer (or to the owner of the 128-row block) instead of C.
 template <typename OutT>
-__global__ void __launch_bounds__(256) splitk_reduce_kernel(const float* __restrict__ partial, OutT* __restrict__ C,
+__global__ void __launch_bounds__(256) splitk_reduce_kernel(const float* partial, OutT* C,
                                                             int64_t mn, int splits, const FanOut fan, int64_t N) {
   const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
   // launched with programmatic stream serialisation: this grid may start while the GEMM that
@@ -28,8 +28,8 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const float* __restr
   if (i >= mn) return;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < splits; ++s) {
-    const float4 a = *reinterpret_cast<const float4*>(partial + (int64_t)s * mn + i);
-    const float4 b = *reinterpret_cast<const float4*>(partial + (int64_t)s * mn + i + 4);
+    const float4 a = ld_operand(reinterpret_cast<const float4*>(partial + (int64_t)s * mn + i));
+    const float4 b = ld_operand(reinterpret_cast<const float4*>(partial + (int64_t)s * mn + i + 4));
     acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
     acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
   }
@@ -586,9 +586,9 @@ extern "C" int b200_w8a8_block_fp8_gemm_ue8m0(const void* A, const int32_t* sfa,
 namespace b200 {
 // Packed exponent words -> the fp32 scales of the promotion kernels (exact): As column-major [num_kb][M], Bs
 // [n_blocks][num_kb]. One thread per word of four K blocks.
-__global__ void __launch_bounds__(256) unpack_scales_kernel(const int32_t* __restrict__ sfa, int64_t sfa_ld,
-                                                            const int32_t* __restrict__ sfb, int64_t sfb_ld, int sfb_step,
-                                                            float* __restrict__ as, float* __restrict__ bs, int M, int n_blocks,
+__global__ void __launch_bounds__(256) unpack_scales_kernel(const int32_t* sfa, int64_t sfa_ld,
+                                                            const int32_t* sfb, int64_t sfb_ld, int sfb_step,
+                                                            float* as, float* bs, int M, int n_blocks,
                                                             int num_kb) {
   grid_launch_dependents();
   grid_dependency_wait();
@@ -596,11 +596,11 @@ __global__ void __launch_bounds__(256) unpack_scales_kernel(const int32_t* __res
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i < (int64_t)M * words) {
     const int w = (int)(i / M), m = (int)(i - (int64_t)w * M);
-    const uint32_t e = (uint32_t)__ldg(sfa + w * sfa_ld + m);
+    const uint32_t e = (uint32_t)ld_operand(sfa + w * sfa_ld + m);
     for (int k = 0; k < 4 && 4 * w + k < num_kb; ++k) as[(int64_t)(4 * w + k) * M + m] = __uint_as_float((e >> (8 * k) & 0xffu) << 23);
   } else if (i - (int64_t)M * words < (int64_t)n_blocks * words) {
     const int j = (int)(i - (int64_t)M * words), w = j / n_blocks, n = j - w * n_blocks;
-    const uint32_t e = (uint32_t)__ldg(sfb + w * sfb_ld + (int64_t)n * sfb_step);
+    const uint32_t e = (uint32_t)ld_operand(sfb + w * sfb_ld + (int64_t)n * sfb_step);
     for (int k = 0; k < 4 && 4 * w + k < num_kb; ++k) bs[(int64_t)n * num_kb + 4 * w + k] = __uint_as_float((e >> (8 * k) & 0xffu) << 23);
   }
 }

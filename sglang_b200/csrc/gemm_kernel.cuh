@@ -412,13 +412,13 @@ block_fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         c.bs_ptr = p.Bs + ((int64_t)c.expert * bs_rows + nb) * num_kb;
         c.bs2_ptr = c.bs_ptr + (int64_t)p.n_blocks * num_kb;
         c.flat = 0;
-        if (MODE == GEMM_GROUPED_SCATTER) c.flat = c.row_ok ? __ldg(p.sorted_ids + c.row) : p.numel;
+        if (MODE == GEMM_GROUPED_SCATTER) c.flat = c.row_ok ? ld_operand(p.sorted_ids + c.row) : p.numel;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           const bool in = c.row_ok && c.kb0 + d < c.kb1;
-          c.a_pf[d] = in ? __ldg(c.as_ptr + (int64_t)(c.kb0 + d) * p.as_sk) : 0.f;
-          c.b_pf[d] = in ? __ldg(c.bs_ptr + c.kb0 + d) : 0.f;
-          if (MODE == GEMM_GROUPED_SILU_QUANT) c.b2_pf[d] = in ? __ldg(c.bs2_ptr + c.kb0 + d) : 0.f;
+          c.a_pf[d] = in ? ld_operand(c.as_ptr + (int64_t)(c.kb0 + d) * p.as_sk) : 0.f;
+          c.b_pf[d] = in ? ld_operand(c.bs_ptr + c.kb0 + d) : 0.f;
+          if (MODE == GEMM_GROUPED_SILU_QUANT) c.b2_pf[d] = in ? ld_operand(c.bs2_ptr + c.kb0 + d) : 0.f;
         }
         return true;
       }
@@ -436,7 +436,7 @@ block_fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       if (MODE != GEMM_DENSE && hint_item < total_items) {
         int hmt, hnt;
         tile_coords(fast_div(hint_item, p.k_splits_div), m_tiles, p.n_tiles, p.group_m, p.per_group_div, hmt, hnt);
-        hint_expert = __ldg(p.expert_ids + hmt);
+        hint_expert = ld_operand(p.expert_ids + hmt);
       }
       float acc[128];
 #pragma unroll
@@ -445,7 +445,7 @@ block_fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       // ahead) and used only in the epilogue
       float row_weight = 1.f;
       if (MODE == GEMM_GROUPED_SCATTER && p.topk_weights != nullptr && cur.flat < p.numel)
-        row_weight = __ldg(p.topk_weights + cur.flat);
+        row_weight = ld_operand(p.topk_weights + cur.flat);
 
       // The scale registers form a ring of four: K block kb uses slot (kb - kb0) % 4 and refills it
       // for kb + 4. The loop is unrolled by four so the slots are fixed registers (a rotating
@@ -461,9 +461,9 @@ block_fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           const float sc2 = MODE == GEMM_GROUPED_SILU_QUANT ? cur.a_pf[j] * cur.b2_pf[j] : sc;
           {
             const bool in = cur.row_ok && kb + 4 < cur.kb1;
-            cur.a_pf[j] = in ? __ldg(cur.as_ptr + (int64_t)(kb + 4) * p.as_sk) : 0.f;
-            cur.b_pf[j] = in ? __ldg(cur.bs_ptr + kb + 4) : 0.f;
-            if (MODE == GEMM_GROUPED_SILU_QUANT) cur.b2_pf[j] = in ? __ldg(cur.bs2_ptr + kb + 4) : 0.f;
+            cur.a_pf[j] = in ? ld_operand(cur.as_ptr + (int64_t)(kb + 4) * p.as_sk) : 0.f;
+            cur.b_pf[j] = in ? ld_operand(cur.bs_ptr + kb + 4) : 0.f;
+            if (MODE == GEMM_GROUPED_SILU_QUANT) cur.b2_pf[j] = in ? ld_operand(cur.bs2_ptr + kb + 4) : 0.f;
           }
           ok = ptx::mbar_wait(tfull_bar(b), (it >> 1) & 1, abort_flag);
           if (!ok) break;
@@ -525,7 +525,7 @@ block_fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           // router weight applied to the gate_up product in fp32, before the activation (where
           // the reference's first grouped GEMM applies it when apply_router_weight_on_input is set)
           const int flat = row_ok ? p.sorted_ids[row] : p.numel;
-          const float w = flat < p.numel ? __ldg(p.topk_weights + flat) : 0.f;
+          const float w = flat < p.numel ? ld_operand(p.topk_weights + flat) : 0.f;
 #pragma unroll
           for (int j = 0; j < 128; ++j) acc[j] *= w;
         }

@@ -330,11 +330,11 @@ block_fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __g
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int kb = min(kbase + j, c.kb1 - 1);
-            a[j][0] = __ldg(as0 + (int64_t)kb * p.as_sk);
-            a[j][1] = __ldg(as1 + (int64_t)kb * p.as_sk);
+            a[j][0] = ld_operand(as0 + (int64_t)kb * p.as_sk);
+            a[j][1] = ld_operand(as1 + (int64_t)kb * p.as_sk);
 #pragma unroll
             for (int n = 0; n < Cfg::kBlocks; ++n)
-              b[j][n] = __ldg(p.Bs + (int64_t)min(blk0 + n, p.n_blocks - 1) * num_kb + kb);
+              b[j][n] = ld_operand(p.Bs + (int64_t)min(blk0 + n, p.n_blocks - 1) * num_kb + kb);
           }
           ok = ptx::mbar_wait(sempty_bar(q), phase, abort_flag);
           if (!ok) break;

@@ -145,10 +145,10 @@ block_fp8_gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const _
       float s = 0.f;
       if (m < p.M) {
         if (p.As != nullptr) {
-          s = __ldg(p.As + (int64_t)m * p.as_sm + (int64_t)kb * p.as_sk) * __ldg(bs_row + kb);
+          s = ld_operand(p.As + (int64_t)m * p.as_sm + (int64_t)kb * p.as_sk) * ld_operand(bs_row + kb);
         } else {  // exponent byte -> power of two
-          const uint32_t a = (uint32_t)__ldg(p.sfa + (kb >> 2) * p.sfa_ld + m) >> (8 * (kb & 3));
-          const uint32_t b = (uint32_t)__ldg(p.sfb + (kb >> 2) * p.sfb_ld + (int64_t)nt * p.sfb_step) >> (8 * (kb & 3));
+          const uint32_t a = (uint32_t)ld_operand(p.sfa + (kb >> 2) * p.sfa_ld + m) >> (8 * (kb & 3));
+          const uint32_t b = (uint32_t)ld_operand(p.sfb + (kb >> 2) * p.sfb_ld + (int64_t)nt * p.sfb_step) >> (8 * (kb & 3));
           s = __uint_as_float((a & 0xffu) << 23) * __uint_as_float((b & 0xffu) << 23);
         }
       }
@@ -209,9 +209,9 @@ block_fp8_gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const _
       float b[D];
       auto request = [&](int j, int u) {
         j = min(j, nkb - 1);
-        raw[u][0] = ld_nc_16(src + (int64_t)j * kBK);
-        raw[u][1] = ld_nc_16(src + (int64_t)j * kBK + 8);
-        b[u] = __ldg(bs + j);
+        raw[u][0] = ld_stream_16(src + (int64_t)j * kBK);
+        raw[u][1] = ld_stream_16(src + (int64_t)j * kBK + 8);
+        b[u] = ld_operand(bs + j);
       };
       grid_dependency_wait();
 #pragma unroll

@@ -301,17 +301,17 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       const float* as = p.As + (int64_t)kb0 * p.as_ld + blk * NT;
 #pragma unroll 8
       for (int i = tid; i < nkb * V; i += 64)
-        table[i] = __ldg(reinterpret_cast<const float4*>(as + (int64_t)(i / V) * p.as_ld) + i % V);
+        table[i] = ld_operand(reinterpret_cast<const float4*>(as + (int64_t)(i / V) * p.as_ld) + i % V);
       float* bs_tab = bs_tab_of(tb);
 #pragma unroll 4
       for (int i = tid; i < 2 * nkb; i += 64) {
         const int h = i >= nkb, kb = i - h * nkb;
-        bs_tab[h * p.table_kb + kb] = __ldg(p.Bs + (int64_t)scale_row(e, nt, h) * p.num_kb + kb0 + kb);
+        bs_tab[h * p.table_kb + kb] = ld_operand(p.Bs + (int64_t)scale_row(e, nt, h) * p.num_kb + kb0 + kb);
       }
       if (tid < NT) {
         const int flat = p.sorted_ids[blk * NT + tid];
         row_id_of(tb)[tid] = flat;
-        row_w_of(tb)[tid] = p.topk_weights == nullptr ? 1.f : flat < p.numel ? __ldg(p.topk_weights + flat) : 0.f;
+        row_w_of(tb)[tid] = p.topk_weights == nullptr ? 1.f : flat < p.numel ? ld_operand(p.topk_weights + flat) : 0.f;
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(tab_full_bar(tb));

@@ -152,12 +152,12 @@ block_fp8_gemm_ue8m0_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, con
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = m0 + 32 * j + lane;
-        wa[j] = r < p.M ? __ldg(ga + r) : kOne;
+        wa[j] = r < p.M ? ld_operand(ga + r) : kOne;
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = n0 + 32 * j + lane;
-        wb[j] = (32 * j < BN && r < p.N) ? __ldg(gb + (p.sfb_rows_per_word == 1 ? r : r / 128)) : kOne;
+        wb[j] = (32 * j < BN && r < p.N) ? ld_operand(gb + (p.sfb_rows_per_word == 1 ? r : r / 128)) : kOne;
       }
     };
     advance(0);

@@ -316,9 +316,9 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     }
     __syncwarp();
   } else {
-    for (int t = threadIdx.x; !QUANT && t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? __ldcg(p.sa + m0 + t) : 0.f;
+    for (int t = threadIdx.x; !QUANT && t < NT; t += Cfg::kEpiThreads) sa[t] = t < rows ? ld_operand(p.sa + m0 + t) : 0.f;
     if (n < p.N) {
-      sb = __ldcg(p.sb + n);
+      sb = ld_operand(p.sb + n);
       if (p.bias != nullptr) bias = to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]);
     }
     asm volatile("bar.sync 1, %0;" ::"n"(Cfg::kEpiThreads) : "memory");

@@ -207,14 +207,14 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       auto load_bias = [&](int n) { return p.bias != nullptr ? to_f32<OutT>(static_cast<const OutT*>(p.bias)[n]) : 0.f; };
       float own = 0.f, own_bias = 0.f;
       if (row < (SWAP ? p.N : p.M)) {
-        own = __ldcg((SWAP ? p.sb : p.sa) + row);
+        own = ld_operand((SWAP ? p.sb : p.sa) + row);
         if (SWAP) own_bias = load_bias(row);
       }
       __syncwarp();  // the last tile's columns have been read
       for (int j = half; j < chunks; j += 2) {
         const int n = nt * bn + j * 32 + lane, at = (j >> 1) * 32 + lane;
         const bool inside = n < (SWAP ? p.M : p.N);
-        my_cols[at] = inside ? __ldcg((SWAP ? p.sa : p.sb) + n) : 0.f;
+        my_cols[at] = inside ? ld_operand((SWAP ? p.sa : p.sb) + n) : 0.f;
         if (!SWAP) my_cols[Cfg::kCols + at] = inside ? load_bias(n) : 0.f;
       }
       __syncwarp();

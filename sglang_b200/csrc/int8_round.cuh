@@ -13,11 +13,6 @@ __device__ __forceinline__ int64_t grid_dependency_zero() {
   asm volatile("griddepcontrol.wait;\n\tmov.b64 %0, 0;" : "=l"(zero)::"memory");
   return zero;
 }
-__device__ __forceinline__ uint4 ld_stream_16(const void* p) {  // read once, and requested here
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint4 ld_again_16(const void* p) {  // read by every row
   uint4 v;
   asm("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));

@@ -198,8 +198,8 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
           row[u] = g - kb[u] * p.M;
           const bool in = kb[u] >= 0 && (kb0 + kb[u]) * 128 + chunk * 16 < p.K;  // K is a multiple of 16
           const T* src = static_cast<const T*>(p.x) + (int64_t)row[u] * p.K + (int64_t)(kb0 + kb[u]) * 128 + chunk * 16;
-          raw[u][0] = in ? ld_nc_16(src) : make_uint4(0, 0, 0, 0);
-          raw[u][1] = in ? ld_nc_16(src + 8) : make_uint4(0, 0, 0, 0);
+          raw[u][0] = in ? ld_stream_16(src) : make_uint4(0, 0, 0, 0);
+          raw[u][1] = in ? ld_stream_16(src + 8) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int u = 0; u < R; ++u) {
@@ -227,13 +227,13 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       named_bar_sync(1, 256);  // every warp is done with the last item's tables
       for (int i = threadIdx.x; i < 2 * nkb; i += 256) {
         const int h = i >= nkb, kb = i - h * nkb;
-        bs_tab[h * cap + kb] = __ldg(p.Bs + (int64_t)min(nt * 2 + h, row_blocks - 1) * p.num_kb + kb0 + kb);
+        bs_tab[h * cap + kb] = ld_operand(p.Bs + (int64_t)min(nt * 2 + h, row_blocks - 1) * p.num_kb + kb0 + kb);
       }
       if (!QUANT) {
 #pragma unroll 4
         for (int i = threadIdx.x; i < nkb * NT; i += 256) {
           const int j = i / NT, m = min(m0 + i % NT, p.M - 1);
-          table[i] = __ldg(p.As + (int64_t)m * p.as_sm + (int64_t)(kb0 + j) * p.as_sk);
+          table[i] = ld_operand(p.As + (int64_t)m * p.as_sm + (int64_t)(kb0 + j) * p.as_sk);
         }
       }
       named_bar_sync(1, 256);

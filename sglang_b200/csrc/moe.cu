@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(512) moe_scatter_quant_kernel(
     const int64_t slot0 = ((int64_t)blockIdx.x - T_tokens) * kPadSlots;
     // every warp looks at the slots at once (kPadSlots == 32) and then only at the pads among them
     const int64_t slot = slot0 + (threadIdx.x & 31);
-    unsigned pads = __ballot_sync(0xffffffffu, slot < *num_post_pad && __ldg(sorted_ids + slot) >= numel);
+    unsigned pads = __ballot_sync(0xffffffffu, slot < *num_post_pad && ld_operand(sorted_ids + slot) >= numel);
     for (; pads; pads &= pads - 1) {
       const int r = __ffs(pads) - 1;
       for (int chunk = threadIdx.x; chunk < H / 16; chunk += blockDim.x) {
@@ -52,10 +52,10 @@ __global__ void __launch_bounds__(512) moe_scatter_quant_kernel(
   __shared__ int pos[64];
   __shared__ float row_s[kRowScales];
   const int64_t tok = blockIdx.x;
-  for (int j = threadIdx.x; j < min(topk, 64); j += blockDim.x) pos[j] = __ldg(position + tok * topk + j);
+  for (int j = threadIdx.x; j < min(topk, 64); j += blockDim.x) pos[j] = ld_operand(position + tok * topk + j);
   __syncthreads();
   // more than 64 slots per token: the scatter entry point takes them (fused_experts and the slot sum refuse)
-  auto position_of = [&](int j) { return j < 64 ? pos[j] : __ldg(position + tok * topk + j); };
+  auto position_of = [&](int j) { return j < 64 ? pos[j] : ld_operand(position + tok * topk + j); };
   const int groups = (int)(H / 128);
   for (int c0 = threadIdx.x & ~31; c0 < H / 16; c0 += blockDim.x) {  // whole warps
     const int chunk = c0 + (threadIdx.x & 31);
@@ -63,12 +63,12 @@ __global__ void __launch_bounds__(512) moe_scatter_quant_kernel(
     uint4 out;
     float scale;
     if (hidden_q != nullptr) {
-      out = active ? ld_nc_16(hidden_q + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
-      scale = active && (chunk & 7) == 0 ? __ldg(hidden_s + tok * (H / 128) + chunk / 8) : 0.f;
+      out = active ? ld_stream_16(hidden_q + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
+      scale = active && (chunk & 7) == 0 ? ld_operand(hidden_s + tok * (H / 128) + chunk / 8) : 0.f;
     } else {
       uint4 raw[2];
-      raw[0] = active ? ld_nc_16(hidden + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
-      raw[1] = active ? ld_nc_16(hidden + tok * H + chunk * 16 + 8) : make_uint4(0, 0, 0, 0);
+      raw[0] = active ? ld_stream_16(hidden + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
+      raw[1] = active ? ld_stream_16(hidden + tok * H + chunk * 16 + 8) : make_uint4(0, 0, 0, 0);
       scale = quant_chunk<T>(raw, 1e-10f, out);
     }
     if (!active) continue;
@@ -97,11 +97,11 @@ __global__ void __launch_bounds__(512) moe_scatter_quant_kernel(
 // plus two launch gaps -> one of 5 us.
 constexpr int kPrepMaxPairs = 1024;
 template <typename T>
-__global__ void __launch_bounds__(256) moe_prep_kernel(const T* __restrict__ hidden, const uint8_t* __restrict__ hidden_q,
-                                                       const float* __restrict__ hidden_s, const int32_t* __restrict__ topk_ids,
-                                                       int32_t* __restrict__ sorted, int32_t* __restrict__ expert_ids,
-                                                       int32_t* __restrict__ npp, uint8_t* __restrict__ q,
-                                                       float* __restrict__ s, int64_t H, int E, int numel, int topk, int block_m,
+__global__ void __launch_bounds__(256) moe_prep_kernel(const T* hidden, const uint8_t* hidden_q,
+                                                       const float* hidden_s, const int32_t* topk_ids,
+                                                       int32_t* sorted, int32_t* expert_ids,
+                                                       int32_t* npp, uint8_t* q,
+                                                       float* s, int64_t H, int E, int numel, int topk, int block_m,
                                                        int64_t cap) {
   __shared__ int cnt[1024];
   __shared__ int part[3][8];
@@ -110,12 +110,12 @@ __global__ void __launch_bounds__(256) moe_prep_kernel(const T* __restrict__ hid
   grid_dependency_wait();
   grid_launch_dependents();
   __syncthreads();
-  const int mine = __ldg(topk_ids + i);
+  const int mine = ld_operand(topk_ids + i);
   const bool valid = mine >= 0 && mine < E;
   if (!valid && i != 0) return;
   int rank = 0;
   for (int j = tid; j < numel; j += 256) {
-    const int e = __ldg(topk_ids + j);
+    const int e = ld_operand(topk_ids + j);
     if (e >= 0 && e < E) {
       atomicAdd(&cnt[e], 1);
       rank += (e == mine && j < i) ? 1 : 0;
@@ -152,12 +152,12 @@ __global__ void __launch_bounds__(256) moe_prep_kernel(const T* __restrict__ hid
     uint4 out;
     float scale;
     if (hidden_q != nullptr) {
-      out = active ? ld_nc_16(hidden_q + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
-      scale = active && (chunk & 7) == 0 ? __ldg(hidden_s + tok * (H / 128) + chunk / 8) : 0.f;
+      out = active ? ld_stream_16(hidden_q + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
+      scale = active && (chunk & 7) == 0 ? ld_operand(hidden_s + tok * (H / 128) + chunk / 8) : 0.f;
     } else {
       uint4 raw[2];
-      raw[0] = active ? ld_nc_16(hidden + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
-      raw[1] = active ? ld_nc_16(hidden + tok * H + chunk * 16 + 8) : make_uint4(0, 0, 0, 0);
+      raw[0] = active ? ld_stream_16(hidden + tok * H + chunk * 16) : make_uint4(0, 0, 0, 0);
+      raw[1] = active ? ld_stream_16(hidden + tok * H + chunk * 16 + 8) : make_uint4(0, 0, 0, 0);
       scale = quant_chunk<T>(raw, 1e-10f, out);
     }
     if (!active) continue;
@@ -172,9 +172,9 @@ __global__ void __launch_bounds__(256) moe_prep_kernel(const T* __restrict__ hid
 // are in flight per thread and six blocks fit an SM; the sum stays in slot order.
 constexpr int kSumReduceMaxSlots = 64;
 template <typename T>
-__global__ void __launch_bounds__(256, 6) moe_sum_reduce_kernel(const T* __restrict__ y, const int32_t* __restrict__ topk_ids,
-                                                                T* __restrict__ out, int topk, int E, int64_t H, float scale,
-                                                                int skip_unrouted, const int* __restrict__ poison_status) {
+__global__ void __launch_bounds__(256, 6) moe_sum_reduce_kernel(const T* y, const int32_t* topk_ids,
+                                                                T* out, int topk, int E, int64_t H, float scale,
+                                                                int skip_unrouted, const int* poison_status) {
   __shared__ int s_slot[kSumReduceMaxSlots];
   __shared__ int s_n;
   const int64_t t = blockIdx.x;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(256, 6) moe_sum_reduce_kernel(const T* __restr
     int n = 0;
     for (int j0 = 0; j0 < topk; j0 += 32) {
       const int j = j0 + (int)threadIdx.x;
-      const int e = j < topk ? __ldg(topk_ids + t * topk + j) : -1;
+      const int e = j < topk ? ld_operand(topk_ids + t * topk + j) : -1;
       const bool ok = e >= 0 && e < E;
       const unsigned m = __ballot_sync(0xffffffffu, ok);
       if (ok) s_slot[n + __popc(m & ((1u << threadIdx.x) - 1u))] = j;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256, 6) moe_sum_reduce_kernel(const T* __restr
       uint4 r[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k0 + k < n) r[k] = ld_nc_16(base + (int64_t)s_slot[k0 + k] * H + v * 8);
+        if (k0 + k < n) r[k] = ld_stream_16(base + (int64_t)s_slot[k0 + k] * H + v * 8);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (k0 + k < n) {
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(256) moe_sum_reduce_splits_kernel(const float*
     any = true;
     for (int sp = 0; sp < splits; ++sp) {
       const float* src = y + sp * split_stride + (r * slots + j) * H + v * 8;
-      const uint4 a = ld_nc_16(src), b = ld_nc_16(src + 4);
+      const uint4 a = ld_stream_16(src), b = ld_stream_16(src + 4);
       acc[0] += __uint_as_float(a.x); acc[1] += __uint_as_float(a.y);
       acc[2] += __uint_as_float(a.z); acc[3] += __uint_as_float(a.w);
       acc[4] += __uint_as_float(b.x); acc[5] += __uint_as_float(b.y);

@@ -10,8 +10,8 @@ namespace b200 {
 // Row of a chunk by a multiplication: the division of 64-bit numbers was a good part of the instructions (8192 x 14336 bf16
 // 66.0 -> 63.2 us, 203 x 4096 2.03 -> 1.95). Two chunks per thread, both loaded ahead, are slower (78 us).
 template <typename T, int LPG, int FORMULA>
-__global__ void __launch_bounds__(256) quant_group_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
-                                                          float* __restrict__ s, int64_t total_chunks,
+__global__ void __launch_bounds__(256) quant_group_kernel(const T* x, uint8_t* q,
+                                                          float* s, int64_t total_chunks,
                                                           int chunks_per_row, FastDiv row_div, int64_t s_stride_m,
                                                           int64_t s_stride_g, float eps, int early) {
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -101,10 +101,10 @@ int quant_for_linear(const void* x, int x_dtype, void* q, float* s, int64_t M, i
 // gate | up (2K wide) and the quantised value is T(silu(gate)) * up in the input type T.
 // masked_m: rows t >= masked_m[expert] of a [E][rows_per_expert] input are skipped.
 template <typename T, int LPG, bool SILU>
-__global__ void __launch_bounds__(256) quant_group_ue8m0_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
-                                                                uint8_t* __restrict__ s, int64_t total_chunks,
+__global__ void __launch_bounds__(256) quant_group_ue8m0_kernel(const T* x, uint8_t* q,
+                                                                uint8_t* s, int64_t total_chunks,
                                                                 int chunks_per_row, int64_t aligned_mn,
-                                                                const int32_t* __restrict__ masked_m,
+                                                                const int32_t* masked_m,
                                                                 int64_t rows_per_expert) {
   grid_dependency_wait();  // x, and the readers of the buffers overwritten below
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
       if (j < vpl && e0 + j < E) {
         float v = s[j];
         if (p.softcap != 0.f) v = tanhf(v / p.softcap) * p.softcap;
-        if (p.logit_bias != nullptr) v += __ldg(p.logit_bias + e0 + j);
+        if (p.logit_bias != nullptr) v += ld_operand(p.logit_bias + e0 + j);
         s[j] = v;
       }
     }
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
 #pragma unroll
   for (int j = 0; j < VMAX; ++j) {
     const bool valid = j < vpl && e0 + j < E;
-    c[j] = valid ? s[j] + (p.bias ? __ldg(p.bias + e0 + j) : 0.f) : kNegInf;
+    c[j] = valid ? s[j] + (p.bias ? ld_operand(p.bias + e0 + j) : 0.f) : kNegInf;
   }
 
   if (p.n_group > 1) {
