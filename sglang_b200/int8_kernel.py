@@ -31,7 +31,9 @@ def per_token_quant_int8(
 
     ``x_s = max(|x|, 1e-10) / 127`` over the row, ``x_q = x / x_s`` rounded to the nearest integer, ties to even (both IEEE
     divisions, in fp32). ``x`` (bf16, fp16 or fp32) is contiguous, or 2-D with contiguous rows at any distance.
-    ``fuse_silu_and_mul``: ``x`` is ``[.., 2K]`` = gate | up and ``silu(gate) * up``, in fp32, is quantised. A NaN or an
+    ``fuse_silu_and_mul``: ``x`` is ``[.., 2K]`` = gate | up and ``y = silu(gate) * up``, in fp32, is quantised: ``x_s = max(|y|, 1e-10) / 127``,
+    ``x_q`` the integer nearest to the unrounded product of ``y`` and ``127 / max(|y|, 1e-10)``, a quotient rounded once. The bits are the same
+    for every alignment and number of rows. A NaN or an
     infinity in a row leaves the row's scale NaN or infinite. ``scale_dtype`` other than fp32 and ``cal_sum`` (row sums for
     asymmetric weights) are not built.
     """
