@@ -447,10 +447,11 @@ int b200_moe_sum_reduce(const void* rows, const int32_t* topk_ids, void* out, in
  *   B200_ROW_FP8        per 128 columns (H % 128 == 0): s[m*s_stride_m + g*s_stride_g] = amax / 448, q = e4m3(y / s)
  *   B200_ROW_FP8_UE8M0  the same with s = 2^ceil(log2(amax / 448)), its biased exponent in byte (g % 4) of word
  *                       [g/4 * s_stride_g + m]; bytes past the last group are written as 0
- * Plain int8 rows: scale and quotient are IEEE divisions. Gated and normed ones: the code of y = v * c (v = silu(gate) * up, c = 1, or v = h * weight, c
- * = 1/rms, which cancels) is the whole number nearest to v * f or e4m3(v * f), f = 127 or 448 over max|v| rounded once (amax below the floor: f = c
- * times 127 or 448 over the floor). So the codes do not depend on the alignment or the number of the rows. The order of the sum of squares does: the last
- * bits of a norm's fp32 scales, and the few codes that a power-of-two scale or the floor leaves next to a tie, may differ between such calls.
+ * Codes come from v and its largest magnitude, where y = v * c: v = x or h * weight or silu(gate) * up in fp32, c = 1 or 1/rms, which cancels. Plain
+ * and normed int8 rows: the whole number nearest to v / t, t = max|v| / 127, both quotients rounded once (IEEE); gated ones: nearest to v * f, f = 127 /
+ * max|v| rounded once; FP8: e4m3(v * f), f = 448 / max|v| likewise; power-of-two scales: e4m3(v * (c / s)). Where amax is below the floor, t and f are the
+ * floor's, with c. So the codes do not depend on the alignment or the number of the rows. The order of the sum of squares does: the last bits of a norm's
+ * fp32 scales, and the few codes that a power-of-two scale or the floor leaves next to a tie, may differ between such calls.
  * No output overlaps an input. q [M,H] contiguous, 16-byte aligned for the FP8 kinds. Any H (int8) up to 2^24, any element alignment of x. */
 enum { B200_ROW_INT8 = 0, B200_ROW_FP8 = 1, B200_ROW_FP8_UE8M0 = 2 };
 int b200_rmsnorm_quant(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld,

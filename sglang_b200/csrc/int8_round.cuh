@@ -41,7 +41,8 @@ __device__ __forceinline__ uint64_t twice(float v) {
   return p;
 }
 
-// rint_bits of two products at once
+// rint_bits of a product that is not rounded before, and of two at once
+__device__ __forceinline__ uint32_t rint_scaled(float y, float scale) { return __float_as_uint(fmaf(y, scale, 12582912.f)); }
 __device__ __forceinline__ void rint_scaled_two(float y0, float y1, uint64_t scale, uint32_t& c0, uint32_t& c1) {
   asm("{.reg .b64 y; mov.b64 y, {%2, %3}; fma.rn.f32x2 y, y, %4, %5; mov.b64 {%0, %1}, y;}"
       : "=r"(c0), "=r"(c1)
@@ -76,7 +77,10 @@ __device__ __forceinline__ uint2 pack8_s8(const uint32_t (&c)[8]) {
   return out;
 }
 
+// m / 127 as IEEE rounds it: one residual step does so for every mantissa; infinities and NaN stay
+__device__ __forceinline__ float over_127(float m) { return m < INFINITY ? div_by(m, 127.f, 1.f / 127.f) : m; }
+
 // Scale of 8-bit integers for a largest magnitude
-__device__ __forceinline__ float int8_scale(float amax) { return __fdiv_rn(max_nan(amax, 1e-10f), 127.f); }
+__device__ __forceinline__ float int8_scale(float amax) { return over_127(max_nan(amax, 1e-10f)); }
 
 }  // namespace b200

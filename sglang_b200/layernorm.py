@@ -49,7 +49,7 @@ def rmsnorm_quant_int8(
     """RMSNorm, then 8-bit integers with one scale per row (``per_token_quant_int8``): the input of ``int8_scaled_mm``.
 
     ``h = x + residual`` (or ``x``), ``y = h * weight / sqrt(mean(h^2) + eps)``, all in fp32; ``y`` is quantised unrounded. The root
-    cancels in a code, the integer nearest to ``h * weight`` times ``127 / max|h * weight|``, so codes do not depend on the alignment or the number of
+    cancels in a code, the integer nearest to ``v / (max|v| / 127)``, ``v = h * weight`` (IEEE divisions), so codes do not depend on the alignment or the number of
     rows; the last bits of the scales may, with the order of the sum of squares.
     Returns ``(x_q [.., H] int8, x_s [.., 1] fp32)`` and, with ``residual``, ``h`` rounded to the input type as a new tensor.
     ``x`` and ``residual`` are contiguous, or 2-D with contiguous rows at any distance; ``weight [H]``; one dtype for all."""
@@ -76,8 +76,8 @@ def rmsnorm_quant_fp8(
 ) -> Tuple[torch.Tensor, ...]:
     """RMSNorm, then FP8 E4M3 with one scale per row and ``group_size`` columns: the input of ``w8a8_block_fp8_matmul``.
 
-    Norm, residual and result as for ``rmsnorm_quant_int8`` (codes ``e4m3(h * weight * f)``, ``f = 448 / max|h * weight|`` of the group; a power-of-two
-    scale does not cancel the root); scales and their layouts (row-major, column-major, padded, packed
+    Norm, residual and result as for ``rmsnorm_quant_int8`` (codes ``e4m3(v * f)``, ``f = 448 / max|v|`` of the group; a power-of-two scale does not
+    cancel the root); scales and their layouts (row-major, column-major, padded, packed
     powers of two) as for ``per_token_group_quant_fp8``. Only ``group_size`` 128, the K block of the GEMM, is built."""
     if group_size != 128:
         raise NotImplementedError("rmsnorm_quant_fp8: only group_size 128 is built")

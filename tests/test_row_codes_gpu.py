@@ -2,7 +2,7 @@
 number or on how many vectors a thread takes, and those of the norms are what IEEE arithmetic in fp32 gives.
 
 1/rms cancels in y / s, so the codes of a norm come from v = h * w alone (h and v rounded once each): e4m3(v * f), f = 448 / max|v| of the group
-rounded once, and the whole number nearest to the unrounded product v * f, f = 127 / max|v| of the row. Nothing in them depends on the order of the sum of
+rounded once, and the whole number nearest to v / t, t = max|v| / 127 of the row, both quotients rounded once. Nothing in them depends on the order of the sum of
 squares; it may move the last bits of the scales, by less than 2^-17 as everywhere."""
 import pytest
 import torch
@@ -43,8 +43,8 @@ def test_codes_of_the_norms_by_the_formula(width, dtype):
         x, w = rows_at(rows, width, dtype, 1, 0), rows_at(1, width, dtype, 2, 0)[0]
         r = rows_at(rows, width, dtype, 3, 0) if with_res else None
         v = (x.float() + r.float() if with_res else x.float()) * w.float()
-        f = over(v.abs().amax(-1, keepdim=True), 127.0)
-        assert torch.equal(S.rmsnorm_quant_int8(x, w, residual=r)[0], (v.double() * f.double()).round().to(torch.int8))
+        t = v.abs().amax(-1, keepdim=True) / torch.full((), 127.0, device="cuda")
+        assert torch.equal(S.rmsnorm_quant_int8(x, w, residual=r)[0], (v / t).round().to(torch.int8))
         g = v.view(rows, -1, 128)
         want = (g * over(g.abs().amax(-1, keepdim=True), 448.0)).to(torch.float8_e4m3fn).view(rows, width)
         assert torch.equal(S.rmsnorm_quant_fp8(x, w, residual=r)[0].view(torch.uint8), want.view(torch.uint8))
@@ -103,3 +103,29 @@ def test_rows_below_the_floor():
             off = (q.double().view(g.shape) - g / step).abs()
             half = 0.5 if top == 127 else 2.0 ** ((g / step).abs().clamp_min(2.0**-6).log2().floor() - 4)
             assert (off <= half * (1 + 2.0**-12) + top * 2.0**-17).all()
+
+
+@pytest.mark.parametrize("width", [1024, 1023, 8192, 14336])
+def test_ties_go_to_even(width):
+    """Quotients that lie halfway between two whole numbers: max|v| = 127 * 2^k makes them exact."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    halves = torch.randint(-252, 253, (4, width), generator=g, device="cuda").float() / 2
+    halves[:, width // 3] = 127
+    want = halves.round().to(torch.int8)  # ties to even
+    for dtype in DTYPES:
+        x = (halves * torch.tensor([[1.0], [0.25], [8.0], [2.0**-7]], device="cuda")).to(dtype)
+        assert torch.equal(x.float(), halves * torch.tensor([[1.0], [0.25], [8.0], [2.0**-7]], device="cuda"))
+        w = torch.ones(width, dtype=dtype, device="cuda")
+        assert torch.equal(S.rmsnorm_quant_int8(x, w)[0], want)
+        assert torch.equal(S.rmsnorm_quant_int8(x, w, residual=torch.zeros_like(x))[0], want)
+        assert torch.equal(S.per_token_quant_int8(x)[0], want)
+
+
+def test_a_sum_past_the_largest_float_leaves_zeros():
+    """mean(h^2) is infinite in fp32, so y is zero: codes are zeros and the scale is that of the floor, at every alignment."""
+    for offset in (0, 1):
+        x = rows_at(2, 1024, torch.bfloat16, 11, offset, scale=1e25)
+        w = torch.ones(1024, dtype=torch.bfloat16, device="cuda")
+        for top, fn in ((127.0, S.rmsnorm_quant_int8), (448.0, S.rmsnorm_quant_fp8)):
+            q, s = fn(x, w)
+            assert (q.float() == 0).all() and torch.equal(s, torch.full_like(s, 1e-10) / torch.full_like(s, top))
