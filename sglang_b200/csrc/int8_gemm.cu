@@ -51,7 +51,9 @@ static float join(float a, float b) {  // near the larger of the two, a little a
 
 // Time of one call in us, back to back with others: started from a least-squares fit, the constants were then moved until the choice
 // among 10468 measured sizes (1 to 4096 rows, N 256 to 57344, K 256 to 28672, each with every tile and split below) was as near the
-// best of them as it would come: 0.5 % behind on average up to 16 rows, 0.7 to 1.8 % above, 2 and 5 % at the 90th percentile.
+// best of them as it would come. The sizes of the served models and their shards, half of them all, weigh three times as much as the others, and what is
+// more than 5 % behind counts double. Behind the best on 5521 other sizes: 0.5 % on average up to 16 rows, 0.6 to 1.9 % above; 2 and 6 %
+// at the 90th percentile, 6 and 8 to 21 % at the 99th; at worst 18 %, and 54 % between 33 and 64 rows.
 struct StreamCost {
   float start, alone, alone_nt, shared, shared_nt;  // a K block of a CTA that has its SM to itself, of one of several on an SM
   float bandwidth, store_nt, sum, sum_nt, cta, wave;

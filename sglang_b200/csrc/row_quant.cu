@@ -86,7 +86,7 @@ __device__ __forceinline__ RowScale int8_row_scale(float top, float rstd) {
 __device__ __forceinline__ float over_448(float m) { return m < INFINITY ? div_by(m, 448.f, 1.f / 448.f) : m; }
 
 // Likewise of a group of FP8 values, code e4m3(v * factor). A power of two does not hold the maximum, so there the factor holds rstd.
-// quotient: 448 / amax, which need not wait for rstd. With approximate quotients, 203 x 4096 takes 2.94 us instead of 3.02 and more codes
+// quotient: 448 / amax, which need not wait for rstd. With approximate quotients 203 x 4096 takes 2.94 us instead of 3.03, and more codes
 // lie on the other side of a tie than in the plain form.
 struct GroupScale {
   float top;      // s = top / 448
@@ -120,7 +120,7 @@ __device__ __forceinline__ void put_group_scale(const RowParams& p, int64_t row,
 }
 
 // A row per block, element by element, some of them under way at once: any width and alignment. KEEP: the values wait in shared memory, as
-// fp32, for the row's scale (gated 8192 x 5001 69 us, computed twice 79 with one element at a time, 112 with four). A plain row is read again
+// fp32, for the row's scale (gated 8192 x 5001 65 us, computed twice 79 with one element at a time, 112 with four). A plain row is read again
 // instead, 43 against 45. Bound by the instructions per element: 2.8 to 3 TB/s.
 constexpr int kKeepWidth = 12000;  // beside the reductions' 256 bytes it stays below the 48 KB of any launch
 template <typename T, int SRC, int KIND, int BLOCK, bool KEEP>
@@ -402,11 +402,11 @@ static int launch_rows(const RowParams& p, cudaStream_t st, const char* what) {
       return launch_dependent(row_quant_any_kernel<T, SRC, KIND, 256, kKeep>, grid, 256, keep, st, 1, what, p);
     return launch_dependent(row_quant_any_kernel<T, SRC, KIND, 256, false>, grid, 256, 0, st, 1, what, p);
   }
-  // us for 1 / 2 / 4 / 8 vectors a thread, 203 and 16384 rows of 8192 bf16:
-  //   plain  2.9 / 3.2 / 2.9 / 2.6, 128 / 90 / 64 / 62 (6.5 TB/s)           gated  3.8 / 5.2 / 5.4 / 6.1, 151 / 114 / 109 / 148 (6.2)
-  // norms with a residual for 1 / 2 / 4, the first two with `ahead` (203 x 8192 at 2 vectors without it 4.2 FP8, 3.8 int8):
-  //   203 x 8192   FP8 3.9 / 3.5 / 5.1, int8 4.1 / 3.6 / 5.1         8192 x 8192  FP8 89 / 82 / 76 (6.2 TB/s), int8 90 / 83 / 74 (6.3)
-  //   2048 x 4096  FP8 11.4 / 9.6 / 10.7, int8 11.7 / 9.6 / 10.8     8192 x 4096  FP8 43 / 39 / 40, int8 44 / 39 / 40
+  // us in a graph for 1 / 2 / 4 / 8 vectors a thread, 203 and 16384 rows of 8192 bf16:
+  //   plain  2.4 / 2.8 / 3.2 / 3.2, 125 / 77 / 62 / 61 (6.6 TB/s)           gated  3.0 / 4.5 / 4.4 / 5.0, 135 / 112 / 106 / 132 (6.3)
+  // norms with a residual for 1 / 2 / 4, the first two with `ahead`:
+  //   203 x 8192   FP8 3.6 / 3.0 / 4.7, int8 3.8 / 3.1 / 4.9         8192 x 8192  FP8 88 / 81 / 74 (6.4 TB/s), int8 92 / 83 / 72 (6.5)
+  //   2048 x 4096  FP8 11.0 / 9.1 / 10.3, int8 11.6 / 9.4 / 10.4     8192 x 4096  FP8 42 / 37 / 39, int8 43 / 37 / 39
   // Blocks that go through many rows, with a ring of them in shared memory that bulk copies fill, were no faster (plain 69 to 73 us).
   const bool short_or_few = nvec <= 512 || (p.rows <= 512 && nvec <= 1024);
   int vpt = SRC == ROW_PLAIN ? 8 : SRC == ROW_SILU ? (p.rows < 1024 ? 1 : 4) : short_or_few ? 2 : 4;
