@@ -484,6 +484,43 @@ int b200_w8a8_int8_linear(const void* x, int64_t x_ld, int x_dtype, const void* 
                           const float* sw, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * qk_norm_rope: heads of q, k and v between the qkv linear and attention.
+ * q [rows,q_heads,dim] and k, v [rows,kv_heads,dim] of `dtype` (bf16, f16, f32): tokens *_token and heads *_head elements apart, elements of a head
+ * contiguous. Per head of q and k, in fp32 and rounded once:
+ *   y = x * weight / sqrt(mean(x^2) + eps)      where its weight [dim] is not NULL
+ *   the first `rotated` elements turn: pair j (elements j and j + rotated/2 with neox, else 2j and 2j + 1) becomes (a c - b s, b c + a s),
+ *   c = cos_sin[p * cos_sin_ld + j], s = cos_sin[p * cos_sin_ld + rotated/2 + j], p = positions[axis(j) * positions_ld + token]
+ *   axis(j): 0 with one axis; else runs of sections[0], sections[1], .. pairs, or with sections_interleaved axis j % axes where that is not 0 and
+ *   j < axes * sections[j % axes], else 0. The sections sum to rotated/2. A position outside [0, table_rows) makes the pairs that take it NaN.
+ * q (NULL: none) goes to q_out [rows,q_heads,dim]. k goes to k_out [rows,kv_heads,dim], or, where k_cache is not NULL, with v into the caches: the
+ * token's slot is token `slots % page_size` of page `slots / page_size`, pages, tokens and heads *_cache_page, *_cache_token and *_cache_head elements
+ * apart. cache_dtype: dtype, or B200_E4M3: e4m3(y / scale) of the IEEE quotient, saturated at +-448 (a NaN stays one), with k_scale / v_scale of one
+ * element or one per kv head (k_scales, v_scales), NULL: 1. A slot outside [0, pages * page_size) leaves its token out; slots are distinct.
+ * No output overlaps an input. positions and slots: B200_I32 or B200_I64. Without rotation (rotated = 0) positions and table may be NULL. */
+enum { B200_E4M3 = 5 };
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  const void *q_weight, *k_weight;
+  void *q_out, *k_out;
+  const void* positions;
+  int64_t positions_ld;
+  const float* cos_sin;
+  int64_t cos_sin_ld, table_rows;
+  void *k_cache, *v_cache;
+  int64_t k_cache_page, k_cache_token, k_cache_head, v_cache_page, v_cache_token, v_cache_head;
+  int64_t pages;
+  const void* slots;
+  const float *k_scale, *v_scale;
+  int64_t rows;
+  int q_heads, kv_heads, dim, dtype, rotated, neox;
+  int axes, sections[4], sections_interleaved, positions_dtype;
+  int page_size, cache_dtype, slots_dtype, k_scales, v_scales;
+  float eps;
+} b200_rope_args;
+int b200_qk_norm_rope(const b200_rope_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,107 @@
+"""Calls that the operators between qkv and attention refuse (no GPU: a refusal comes before any launch)."""
+import ctypes
+
+import pytest
+import torch
+
+import sglang_b200 as S
+from sglang_b200 import _native as N
+from sglang_b200.rotary import RopeArgs
+
+BF, FP8 = torch.bfloat16, torch.float8_e4m3fn
+
+
+def good():
+    """Arguments of qk_norm_rope_append that only lack a GPU."""
+    return dict(qkv=torch.zeros(3, 12 * 64, dtype=BF), num_heads=8, num_kv_heads=2, positions=torch.arange(3), cos_sin_cache=torch.zeros(9, 64),
+                k_cache=torch.zeros(4, 4, 2, 64, dtype=BF), v_cache=torch.zeros(4, 4, 2, 64, dtype=BF), slots=torch.arange(3),
+                q_weight=torch.ones(64, dtype=BF), k_weight=torch.ones(64, dtype=BF))
+
+
+def test_a_good_call_lacks_only_the_gpu():
+    a = good()
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        S.qk_norm_rope_append(**a)
+    for n in ("k_cache", "v_cache", "slots"):
+        del a[n]
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        S.qk_norm_rope(**a)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        S.append_paged_kv(torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF), *(torch.zeros(4, 4, 2, 64, dtype=BF),) * 2, torch.arange(3))
+
+
+BAD = {
+    "double": dict(qkv=torch.zeros(3, 12 * 64, dtype=torch.float64)),
+    "width": dict(qkv=torch.zeros(3, 12 * 64 + 1, dtype=BF)),
+    "columns apart": dict(qkv=torch.zeros(3, 24 * 64, dtype=BF)[:, ::2]),
+    "no heads": dict(num_kv_heads=0),
+    "weight size": dict(q_weight=torch.ones(65, dtype=BF)),
+    "weight type": dict(k_weight=torch.ones(64)),
+    "float positions": dict(positions=torch.zeros(3)),
+    "positions of another length": dict(positions=torch.arange(4)),
+    "positions without a table": dict(cos_sin_cache=None),
+    "16-bit table": dict(cos_sin_cache=torch.zeros(9, 64, dtype=BF)),
+    "table wider than a head": dict(cos_sin_cache=torch.zeros(9, 66)),
+    "odd table": dict(cos_sin_cache=torch.zeros(9, 63)),
+    "one axis of positions for three": dict(mrope_section=[10, 11, 11]),
+    "sections of another sum": dict(mrope_section=[10, 11, 10], positions=torch.zeros(3, 3, dtype=torch.int64)),
+    "a negative section": dict(mrope_section=[40, -8], positions=torch.zeros(2, 3, dtype=torch.int64)),
+    "an interleaved section that does not fit": dict(mrope_section=[6, 13, 13], mrope_interleaved=True,
+                                                     positions=torch.zeros(3, 3, dtype=torch.int64)),
+    "cache heads": dict(k_cache=torch.zeros(4, 4, 3, 64, dtype=BF)),
+    "cache type": dict(k_cache=torch.zeros(4, 4, 2, 64, dtype=torch.float16), v_cache=torch.zeros(4, 4, 2, 64, dtype=torch.float16)),
+    "caches of two types": dict(v_cache=torch.zeros(4, 4, 2, 64).to(FP8)),
+    "caches of two sizes": dict(v_cache=torch.zeros(5, 4, 2, 64, dtype=BF)),
+    "heads of a cache apart": dict(k_cache=torch.zeros(4, 4, 2, 128, dtype=BF)[..., ::2]),
+    "float slots": dict(slots=torch.zeros(3)),
+    "too few slots": dict(slots=torch.arange(2)),
+    "scale of a 16-bit cache": dict(k_scale=torch.ones(1)),
+    "16-bit scale": dict(k_cache=torch.zeros(4, 4, 2, 64).to(FP8), v_cache=torch.zeros(4, 4, 2, 64).to(FP8), k_scale=torch.ones(1, dtype=BF)),
+    "scales per token": dict(k_cache=torch.zeros(4, 4, 2, 64).to(FP8), v_cache=torch.zeros(4, 4, 2, 64).to(FP8), v_scale=torch.ones(3)),
+}
+
+
+@pytest.mark.parametrize("what", BAD)
+def test_refused(what):
+    with pytest.raises(AssertionError):
+        S.qk_norm_rope_append(**{**good(), **BAD[what]})
+
+
+def test_five_axes_are_not_built():
+    with pytest.raises(NotImplementedError):
+        S.qk_norm_rope_append(**{**good(), "mrope_section": [8, 8, 8, 4, 4], "positions": torch.zeros(5, 3, dtype=torch.int64)})
+
+
+def test_keys_and_values_have_to_match():
+    c = torch.zeros(4, 4, 2, 64, dtype=BF)
+    k = torch.zeros(3, 2, 64, dtype=BF)
+    for a, b in ((k, k[:2]), (k, k.half()), (k[0], k[0]), (k.transpose(1, 2), k.transpose(1, 2))):
+        with pytest.raises(AssertionError):
+            S.append_paged_kv(a, b, c, c, torch.arange(3))
+
+
+def test_abi_refuses_before_a_launch():
+    lib = N.load()
+
+    def call(**fields):
+        sections = fields.pop("sections", [])
+        a = RopeArgs(rows=3, q_heads=2, kv_heads=1, dim=64, **{**dict(dtype=N.BF16, q=64, k=64, q_out=64, k_out=64, axes=1), **fields})
+        for i, n in enumerate(sections):
+            a.sections[i] = n
+        return lib.b200_qk_norm_rope(ctypes.addressof(a), None)
+
+    bad = N.E_BAD_ARG
+    assert lib.b200_qk_norm_rope(None, None) == bad
+    assert call(rotated=7) == bad and call(rotated=66) == bad and call(rotated=64) == bad
+    table = dict(rotated=64, positions=64, cos_sin=64, positions_dtype=N.I64, table_rows=4, cos_sin_ld=64)
+    assert call(**{**table, "positions_dtype": N.F32}) == bad
+    assert call(**{**table, "axes": 1, "cos_sin": 65}) == bad
+    assert call(k_cache=64) == bad and call(slots=64) == bad
+    cache = dict(k_cache=64, v_cache=64, slots=64, v=64, pages=4, page_size=4, slots_dtype=N.I64, cache_dtype=5)
+    assert call(**{**cache, "cache_dtype": N.F16}) == bad and call(**{**cache, "page_size": 0}) == bad
+    assert call(**{**cache, "k_scale": 64, "k_scales": 3}) == bad
+    assert call(**{**cache, "cache_dtype": N.BF16, "k_scale": 64, "k_scales": 1}) == bad
+    a = RopeArgs(rows=3, q_heads=2, kv_heads=1, dim=64, dtype=9, q=64, k=64, q_out=64, k_out=64)
+    assert lib.b200_qk_norm_rope(ctypes.addressof(a), None) == bad
+    a = RopeArgs(rows=0, q_heads=2, kv_heads=1, dim=64, dtype=N.BF16)
+    assert lib.b200_qk_norm_rope(ctypes.addressof(a), None) == 0
