@@ -521,6 +521,40 @@ typedef struct {
 } b200_rope_args;
 int b200_qk_norm_rope(const b200_rope_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * tree_attention: the newest tokens of every sequence over a paged cache that already holds them.
+ * q, out [tokens,q_heads,dim] of `dtype` (bf16, f16; dim 64, 128, 256); q's tokens and heads q_token and q_head elements apart, out contiguous.
+ * Sequence b has the tokens q_starts[b] .. q_starts[b+1] - 1 (n of them; NULL: token b) and seq_lens[b] keys, the last n of which are its own. Key j is
+ * token j % page_size of page page_table[b * page_table_ld + j / page_size] of k_cache and v_cache, pages, tokens and heads k_page, k_token, k_head (v_*)
+ * elements apart, of `dtype` or B200_E4M3 with scales as for b200_qk_norm_rope, positive. Head i reads kv head i / (q_heads / kv_heads).
+ *   o = sum_j softmax_j(scale q . k_j k_scale) v_j v_scale over the keys that the token sees, rounded once; weights are multiplied in `dtype`
+ *   lse [tokens,q_heads] fp32 or NULL: the logarithm of the sum of the exponentials
+ * Token i of a sequence sees every key before the sequence's own n, and of those key j where byte mask[(q_starts[b] + i) * mask_ld + j] is not 0 (j <
+ * mask_width), or without a mask those up to itself. A token that sees nothing: o = 0, lse = -infinity. Tokens of no sequence keep what
+ * out and lse held. A key of a page outside [0, pages) makes the rows that see it NaN; seq_lens are capped at max_pages * page_size.
+ * Pointers of q, out and the caches and all strides: multiples of 16 bytes. Workspace: 16-byte aligned, contents immaterial, one per call under way. */
+typedef struct {
+  const void* q;
+  int64_t q_token, q_head;
+  void* out;
+  float* lse;
+  const void *k_cache, *v_cache;
+  int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+  int64_t pages;
+  const int32_t* page_table;
+  int64_t page_table_ld, max_pages;
+  const int32_t *seq_lens, *q_starts;
+  const void* mask;
+  int64_t mask_ld;
+  const float *k_scale, *v_scale;
+  int64_t tokens, sequences;
+  int q_heads, kv_heads, dim, dtype;
+  int page_size, cache_dtype, mask_width, k_scales, v_scales;
+  float scale;
+} b200_tree_attention_args;
+size_t b200_tree_attention_workspace_bytes(const b200_tree_attention_args* args);
+int b200_tree_attention(const b200_tree_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,7 @@ from .topk import (  # noqa: F401,E402
 )
 from .int8_kernel import int8_scaled_mm, per_token_quant_int8, w8a8_int8_linear  # noqa: F401,E402
 from .layernorm import rmsnorm_quant_fp8, rmsnorm_quant_int8  # noqa: F401,E402
+from .attention import tree_attention  # noqa: F401,E402
 from .rotary import append_paged_kv, qk_norm_rope, qk_norm_rope_append  # noqa: F401,E402
 from . import fp8  # noqa: F401,E402
 from . import int8  # noqa: F401,E402

@@ -145,6 +145,8 @@ SIGNATURES = {
          c_void_p],
     ),
     "b200_qk_norm_rope": (c_int, [c_void_p, c_void_p]),
+    "b200_tree_attention_workspace_bytes": (c_size_t, [c_void_p]),
+    "b200_tree_attention": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "b200_route_topk_softmax_capped": (
         c_int,
         [c_void_p, c_int, c_float, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],

@@ -19,7 +19,7 @@ OUT_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(OUT_DIR, "libb200_blockfp8.so")
 HOST_EXT = os.path.join(OUT_DIR, "_host.so")  # CPython extension: the operators' host path (csrc/host_ext.cpp)
 SOURCES = ["status.cu", "quant.cu", "align.cu", "gemm.cu", "moe.cu", "topk.cu", "comm.cu", "ep.cu",
-           "row_quant.cu", "int8_gemm.cu", "rotary.cu"]
+           "row_quant.cu", "int8_gemm.cu", "rotary.cu", "tree_attention.cu"]
 
 NVCC_FLAGS = [
     "-std=c++17",
