@@ -66,7 +66,7 @@ def args(**fields):
 
 
 def call(**fields):
-    return N.load().b200_tree_attention(ctypes.addressof(args(**fields)), None, 0, None)
+    return N.load().b200_tree_attention(ctypes.byref(args(**fields)), None, 0, None)
 
 
 def test_abi_refuses_before_a_launch():
@@ -84,7 +84,7 @@ def test_abi_refuses_before_a_launch():
 
 
 def test_workspace():
-    size = lambda **f: N.load().b200_tree_attention_workspace_bytes(ctypes.addressof(args(**f)))  # noqa: E731
+    size = lambda **f: N.load().b200_tree_attention_workspace_bytes(ctypes.byref(args(**f)))  # noqa: E731
     assert size() > 0 and size(tokens=0) == 0 and size(dim=100) == 0
     # two pieces of at most 128 rows for each of at most 148 CTAs
     big = size(tokens=10000, sequences=10000, max_pages=10000, pages=10000)
