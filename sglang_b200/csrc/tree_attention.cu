@@ -1,12 +1,13 @@
 // Attention of the newest tokens of every sequence (one, or a tree of drafted ones) over a paged cache:
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale * k_scale * log2(e),  m near the largest exponent so far
-// Query row r of a kv head is (token r / G, head r % G of the G query heads that share it); 128 rows are a tile of the tensor core's lanes, so that a
-// softmax row belongs to one thread and needs no exchange, and few rows cost no more than the lanes they leave idle: bound by the cache's
-// bytes, a tile of keys has more time than its two products and its exponentials take.
-//   S [128, keys] = Q K^T        Q and K in shared memory, S in TMEM, two buffers
-//   O [128, D]   += P V          P in TMEM over its own S, in the input's 16-bit type, V in shared memory as it lies in the cache
+// The G query heads of a kv head times the new tokens are the rows of one problem, NT of them a tile. 128 keys fill the lanes of the tensor core's
+// tile and the rows are its columns, so that few rows cost little:
+//   S^T [128 keys, NT] = K Q^T     K and Q in shared memory, S^T in TMEM, two buffers
+//   O^T [D, NT]       += V^T P^T   V as it lies in the cache (its rows are the product's depth), P^T [keys, NT] in shared memory
+// A thread of the softmax has one key and NT columns. It takes its exponentials against a reference per row that is moved only when a score exceeds
+// it by 2^8, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end.
 // Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies (an FP8 cache through registers, where codes become
-// 16-bit values, exactly). All tiles of all (sequence, kv head, row tile) form one line that is cut into equal pieces, one per CTA, so that ragged
+// fp16 values, exactly). All tiles of all (sequence, kv head, row tile) form one line that is cut into equal pieces, one per CTA, so that ragged
 // lengths leave no SM idle; rows whose keys were cut leave partial sums in a workspace, which a second kernel joins in the line's order.
 #include "gemm_host.cuh"
 #include "int8_round.cuh"
@@ -14,8 +15,8 @@
 namespace b200 {
 namespace ptx {
 
-// D (+)= A B with 16-bit operands, fp32 sums; A in shared memory, or in TMEM (two elements a column)
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// D (+)= A B with 16-bit operands in shared memory, fp32 sums
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
@@ -25,27 +26,18 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t desc_a, uint64_t
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "}" ::"r"(d),
-      "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Instruction descriptor for kind::f16, fp32 sums: bits 4-5 D format (1 = f32), 7-9 / 10-12 A / B format (0 = f16, 1 = bf16), 16 B is MN-major,
-// 17-22 N >> 3, 24-28 M >> 4
-__host__ __device__ constexpr uint32_t idesc_f16_f32(bool bf16, bool b_mn_major, int M, int N) {
-  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+// Instruction descriptor for kind::f16, fp32 sums: bits 4-5 D format (1 = f32), 7-9 / 10-12 A / B format (0 = f16, 1 = bf16), 15 / 16 rows of A / B are
+// the depth, 17-22 N >> 3, 24-28 M >> 4
+__host__ __device__ constexpr uint32_t idesc_f16_f32(bool bf16, bool depth_rows, int M, int N) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((depth_rows ? 3u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
 }
-// Operand whose rows are k and whose 128-byte rows are 64 elements of N, 128-byte swizzle: 8-row groups 1024 bytes apart, the next 64 elements of N
-// `block` bytes further
-__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t block) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
+// Operand of 16-bit elements whose rows are the product's depth: rows of ROW bytes (32, 64 or 128: that swizzle), groups of eight rows one behind the
+// other, the next ROW / 2 elements across `block` bytes further
+template <int ROW>
+__device__ __forceinline__ uint64_t smem_desc_depth_rows(uint32_t addr, uint32_t block) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(8 * ROW >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)(ROW == 128 ? 2 : ROW == 64 ? 4 : 6) << 61);
 }
 // 16 columns of this thread's lane
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -73,6 +65,26 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// true in all `threads` threads of barrier `id` if it is in one
+__device__ __forceinline__ bool any_of(int id, int threads, bool mine) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"((uint32_t)mine)
+      : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
 }  // namespace ptx
 
 // Rows whose keys were cut between CTAs: from the CTA where they begin, to the last one with a piece of them. parts == 0: none begin here.
@@ -93,17 +105,29 @@ struct AttnParams {
   int* status;
 };
 
-template <int D, bool FP8>
+constexpr int kKeys = 128;  // of a tile
+
+template <int D, int NT, bool FP8>
 struct AttnCfg {
-  static constexpr int kKeys = D > 128 ? 64 : 128;      // of a tile
-  static constexpr int kStage = kKeys * D * 2;          // bytes of a tile of keys or values
-  static constexpr int kQBytes = 128 * D * 2;
-  static constexpr int kStages = D == 64 ? 10 : D == 128 ? 6 : 5;
-  static constexpr int kAhead = 3;                      // stages whose copies are under way when the one before them is handed over
-  static constexpr int kSoftmaxWarps = 4, kMmaWarp = 4, kQWarp = 5, kProducerWarp = 6, kProducerWarps = 4;
+  static constexpr int kWidth = D < 128 ? D : 128, kParts = D / kWidth;  // elements of a head in a stage; stages of a tile of keys, or of values
+  static constexpr int kStage = kKeys * kWidth * 2;
+  static constexpr int kGroups = NT <= 32 ? 1 : 2;  // softmax warps per 32 keys, each with some of the columns
+  static constexpr int kCols = NT / kGroups;
+  static constexpr int kPBufs = NT * D < 64 * 256 ? 2 : 1;
+  static constexpr int kQBytes = NT * D * 2, kPBytes = kKeys * NT * 2;
+  static constexpr int kTables = NT * 4 * (2 + 1 + 1 + 4);  // scales of two segments' rows, references, factors, and a value per warp and column
+  static constexpr int kFixed = kQBytes + kPBufs * kPBytes + kTables + 1024 + 512;
+  static constexpr int kFit = (232448 - kFixed) / kStage;
+  static constexpr int kStages = kFit < 12 ? kFit : 12;
+  // Stages whose copies are under way when the one before them is handed over. The scores of a tile are asked for before the tile ahead of it gives
+  // its values' stages back, so that its last stage of keys has to be handed over with those still taken.
+  static constexpr int kAhead = kStages - 2 * kParts < 8 ? kStages - 2 * kParts : 8;
+  static constexpr int kSoftmaxWarps = 4 * kGroups, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 2, kProducerWarps = 4;
   static constexpr int kThreads = (kProducerWarp + kProducerWarps) * 32;
-  static constexpr int kTmemO = 256;                    // columns: S 0 .. 2 kKeys, O from here
-  static constexpr size_t kSmemBytes = (size_t)kQBytes + (size_t)kStages * kStage + 1024 + 512;
+  static constexpr int kTmemO = 2 * NT, kTmemUsed = (2 + kParts) * NT;  // columns: S^T twice, O^T from here
+  static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
+  static constexpr size_t kSmemBytes = (size_t)kFixed + (size_t)kStages * kStage;
+  static_assert(kAhead >= 1 && kTmemUsed <= 512, "a tile of keys and one of values fit");
 };
 
 // Sequence b as the kernel takes it: whatever the index tensors hold, tokens and keys stay inside q and the page table.
@@ -111,7 +135,7 @@ struct Seq {
   int start, n, len, row_tiles, key_tiles;
   __device__ __forceinline__ int64_t tiles(int heads) const { return n > 0 ? (int64_t)heads * row_tiles * key_tiles : 0; }
 };
-template <int KEYS>
+template <int NT>
 __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
   const b200_tree_attention_args& a = p.a;
   Seq s;
@@ -125,13 +149,13 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
   }
   s.n = end - s.start;
   s.len = (int)min((int64_t)max(ld_operand(a.seq_lens + b), 0), p.capacity);
-  s.row_tiles = (s.n * p.group + 127) >> 7;
-  s.key_tiles = max(1, (s.len + KEYS - 1) / KEYS);
+  s.row_tiles = (s.n * p.group + NT - 1) / NT;
+  s.key_tiles = max(1, (s.len + kKeys - 1) / kKeys);
   return s;
 }
 
 // A CTA's piece of the line, one (sequence, head, row tile) at a time
-template <int KEYS>
+template <int NT>
 struct Walk {
   const AttnParams& p;
   int b, h, qt, t0, t1;
@@ -141,7 +165,7 @@ struct Walk {
     h = qt = t0 = t1 = 0;
     s = {};
     if (left <= 0) return;
-    s = seq_of<KEYS>(p, b);
+    s = seq_of<NT>(p, b);
     const int64_t per_head = (int64_t)s.row_tiles * s.key_tiles;
     h = (int)(offset / per_head);
     const int rest = (int)(offset - h * per_head);
@@ -159,7 +183,7 @@ struct Walk {
       if (++h == p.a.kv_heads) {
         h = 0;
         do {
-          s = seq_of<KEYS>(p, ++b);
+          s = seq_of<NT>(p, ++b);
         } while (s.n == 0 && b + 1 < p.a.sequences);
       }
     }
@@ -167,17 +191,10 @@ struct Walk {
   }
 };
 
-// Two E4M3 codes as 16-bit values: exact, both types hold all of them
-template <typename T>
+// Two E4M3 codes as fp16 values: exact
 __device__ __forceinline__ uint32_t widen2(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
-  if constexpr (std::is_same_v<T, __half>) {
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
-  } else {
-    const float2 f = __half22float2(__half2(h));
-    const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -190,31 +207,68 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// References of the exponents may lie this far (in powers of two) below the largest: the sums stay exact to fp32 and P far from the 16-bit types'
-// limits, and O is rescaled a few times per row instead of once per tile.
+// A score may exceed its row's reference by this much (in powers of two) before the reference moves: sums stay exact to fp32 and weights far from the
+// 16-bit types' limits, and most rows move theirs in the first tile alone.
 constexpr float kSlack = 8.f;
 
-template <typename T, int D, bool FP8>
-__global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_kernel(const __grid_constant__ AttnParams p) {
-  using Cfg = AttnCfg<D, FP8>;
-  constexpr int S = Cfg::kStages, KEYS = Cfg::kKeys;
+// Value i of lane l, N <= 32 of them in each of 32 lanes -> lane l has the result over all lanes of value l % N. Each step halves the values that a
+// lane still has, N - 1 exchanges and 5 - log2 N more.
+template <int N, int BIT = 1, typename F>
+__device__ __forceinline__ float across_lanes(const float (&v)[N], F op) {
+  if constexpr (BIT == 32) {
+    return v[0];
+  } else if constexpr (N == 1) {
+    const float next[1] = {op(v[0], __shfl_xor_sync(0xffffffffu, v[0], BIT))};
+    return across_lanes<1, BIT * 2>(next, op);
+  } else {
+    const bool upper = (threadIdx.x & BIT) != 0;
+    float next[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? v[2 * i] : v[2 * i + 1], BIT);
+      next[i] = op(upper ? v[2 * i + 1] : v[2 * i], other);
+    }
+    return across_lanes<N / 2, BIT * 2>(next, op);
+  }
+}
+
+__device__ __forceinline__ bool not_finite16(uint32_t two, uint32_t exponent) {  // either of two 16-bit values
+  return (two & exponent) == exponent || ((two >> 16) & exponent) == exponent;
+}
+
+template <typename T, int D, int NT, bool FP8>
+__global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attention_kernel(const __grid_constant__ AttnParams p) {
+  using Cfg = AttnCfg<D, NT, FP8>;
+  // An FP8 cache is multiplied in fp16, which holds its codes, whatever the queries' type: a code is converted by one instruction for two, and weights keep
+  // 11 bits. bf16 queries become fp16 behind a power of two per row that brings their largest element to 2^7 .. 2^8; what then lies below fp16's
+  // normal range is 2^-21 of it.
+  using M = std::conditional_t<FP8, __half, T>;
+  constexpr bool kRowScales = FP8 && std::is_same_v<T, __nv_bfloat16>, kBf16 = std::is_same_v<M, __nv_bfloat16>;
+  constexpr uint32_t kExponent = kBf16 ? 0x7f80u : 0x7c00u;
+  constexpr int S = Cfg::kStages, kParts = Cfg::kParts, kCols = Cfg::kCols;
   const b200_tree_attention_args& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-  const uint32_t sQ = smem_base, sKV = smem_base + Cfg::kQBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + Cfg::kQBytes + S * Cfg::kStage);
+  constexpr uint32_t kRing = S * Cfg::kStage;
+  const uint32_t sKV = smem_base, sQ = smem_base + kRing, sP = sQ + Cfg::kQBytes;
+  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + Cfg::kPBufs * Cfg::kPBytes);  // [2][NT]: of a segment's rows
+  float* minus_ref = row_scale + 2 * NT;                                                                    // [NT]
+  float* factor = minus_ref + NT;                                                                           // [NT]
+  float* by_warp = factor + NT;                                                                             // [4][NT]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(by_warp + 4 * NT);
   const uint32_t bar0 = ptx::smem_u32(bars);
-  auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
-  const uint32_t q_full = bar0 + 8u * (2 * S), q_empty = q_full + 8u, o_done = q_full + 16u;
-  auto s_full = [&](int i) { return q_full + 24u + 8u * i; };
-  auto p_full = [&](int i) { return q_full + 40u + 8u * i; };
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 7);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 8);
+  auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (S + s); };
+  const uint32_t q_full = bar0 + 8u * (2 * S), q_empty = q_full + 8u;
+  auto o_done = [&](uint32_t i) { return q_full + 16u + 8u * (i & 1); };  // products with the values of tiles i, i + 2, ..
+  auto s_full = [&](uint32_t i) { return q_full + 32u + 8u * (i & 1); };
+  auto p_full = [&](uint32_t i) { return q_full + 48u + 8u * (i & 1); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 9);
   volatile int* begin_seq = abort_flag + 1;
-  volatile int64_t* line = reinterpret_cast<volatile int64_t*>(bars + 2 * S + 9);  // offset within the first sequence, tiles of this CTA, of every CTA
-  volatile int64_t* sums = line + 3;                                               // of each warp
+  volatile int64_t* line = reinterpret_cast<volatile int64_t*>(bars + 2 * S + 10);  // offset within the first sequence, tiles of this CTA, of every CTA
+  volatile int64_t* sums = line + 3;                                                // of each warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -224,8 +278,8 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
     }
     ptx::mbar_init(q_full, 1);
     ptx::mbar_init(q_empty, 1);
-    ptx::mbar_init(o_done, 1);
     for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(o_done(i), 1);
       ptx::mbar_init(s_full(i), 1);
       ptx::mbar_init(p_full(i), Cfg::kSoftmaxWarps);
     }
@@ -236,7 +290,7 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
     ptx::fence_mbar_init();
   }
   if (warp == Cfg::kMmaWarp) {
-    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
@@ -250,7 +304,7 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
     const int per = (int)((a.sequences + Cfg::kThreads - 1) / Cfg::kThreads);
     const int b0 = min((int)threadIdx.x * per, (int)a.sequences), b1 = min(b0 + per, (int)a.sequences);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_of<KEYS>(p, b).tiles(a.kv_heads);
+    for (int b = b0; b < b1; ++b) mine += seq_of<NT>(p, b).tiles(a.kv_heads);
     int64_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -269,7 +323,7 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
     const int64_t chunk = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1), begin = blockIdx.x * chunk;
     if (begin >= before && begin < before + mine) {
       for (int b = b0; b < b1; ++b) {
-        const int64_t n = seq_of<KEYS>(p, b).tiles(a.kv_heads);
+        const int64_t n = seq_of<NT>(p, b).tiles(a.kv_heads);
         if (begin < before + n) {
           *begin_seq = b;
           line[0] = begin - before;
@@ -282,28 +336,27 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
     }
     __syncthreads();
   }
-  Walk<KEYS> w(p, *begin_seq, line[0], line[1]);
-  const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+  Walk<NT> w(p, *begin_seq, line[0], line[1]);
   bool ok = true;
 
   if (warp >= Cfg::kProducerWarp) {
-    // ------------------------------------------------------------------ keys and values into the ring: K, V, K, V, ..
-    constexpr int kRows = KEYS / Cfg::kProducerWarps;  // keys of a tile that this warp copies
+    // ------------------------------------------------------------------ keys and values into the ring, a tile's keys, then its values
+    constexpr int kRows = kKeys / Cfg::kProducerWarps;  // keys of a tile that this warp copies, lane l the l-th
+    static_assert(kRows == 32, "a lane per key");
     const int row0 = (warp - Cfg::kProducerWarp) * kRows;
-    constexpr int kPerKey = FP8 ? D / 16 : D / 8;      // 16-byte pieces of a key in the cache
-    constexpr int kSteps = kRows * kPerKey / 32;
-    constexpr int64_t kAbsent = -1, kUnknown = -2;     // no key; a page that the cache does not have
-    const int es = FP8 ? 1 : 2;
-    // lane l: key row0 + l
-    auto entry_of = [&](const Walk<KEYS>& at, int t) {
-      const int j = t * KEYS + row0 + lane;
-      if (!at.more() || lane >= kRows || j >= at.s.len) return -1;
+    constexpr int kPieces = Cfg::kWidth / (FP8 ? 16 : 8);  // of 16 bytes, of a key's part in the cache
+    constexpr int kSteps = kRows * kPieces / 32;
+    constexpr int64_t kAbsent = -1, kUnknown = -2;         // no key; a page that the cache does not have
+    constexpr int es = FP8 ? 1 : 2;
+    auto entry_of = [&](const Walk<NT>& at, int t) {
+      const int j = t * kKeys + row0 + lane;
+      if (!at.more() || j >= at.s.len) return -1;
       return (int)ld_operand(a.page_table + (int64_t)at.b * a.page_table_ld + fast_div(j, p.page_div));
     };
     int64_t off[2];
-    auto offsets = [&](const Walk<KEYS>& at, int t, int entry) {
-      const int j = t * KEYS + row0 + lane;
-      if (lane >= kRows || j >= at.s.len) {
+    auto offsets = [&](const Walk<NT>& at, int t, int entry) {
+      const int j = t * kKeys + row0 + lane;
+      if (j >= at.s.len) {
         off[0] = off[1] = kAbsent;
       } else if (entry < 0 || entry >= a.pages) {
         off[0] = kUnknown;
@@ -314,7 +367,6 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
         off[1] = (entry * a.v_page + in_page * a.v_token + at.h * a.v_head) * es;
       }
     };
-    const uint32_t nan2 = 0x7fff7fffu;
     uint32_t it = 0;
     auto ready = [&](uint32_t stage) {  // this thread's part of the stage is in shared memory
       ptx::fence_proxy_async_smem();
@@ -322,30 +374,35 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
       if (lane == 0) ptx::mbar_arrive(full_bar(stage % S));
     };
     int t = w.t0, entry = entry_of(w, t);
+    auto next_tile = [&] {
+      offsets(w, t, entry);
+      if (++t == w.t1) {
+        w.next();
+        t = w.t0;
+      }
+      entry = entry_of(w, t);
+    };
     if constexpr (!FP8) {
+      const uint32_t nan2 = 0x7fff7fffu;
       while (w.more() && ok) {
-        offsets(w, t, entry);
-        if (++t == w.t1) {
-          w.next();
-          t = w.t0;
-        }
-        entry = entry_of(w, t);
+        next_tile();
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++it) {
-          const int s = it % S;
+        for (int part = 0; part < 2 * kParts; ++part, ++it) {
+          const int kv = part / kParts;
+          const uint32_t s = it % S;
           ok = ok && ptx::mbar_wait(empty_bar(s), ((it / S) & 1) ^ 1, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
-          const uint8_t* src = static_cast<const uint8_t*>(kv ? a.v_cache : a.k_cache);
+          const uint8_t* src = static_cast<const uint8_t*>(kv ? a.v_cache : a.k_cache) + (part % kParts) * 256;
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) {
-            const int piece = i * 32 + lane, r = piece / kPerKey, c = piece % kPerKey, row = row0 + r;
+            const int piece = i * 32 + lane, r = piece / kPieces, c = piece % kPieces, row = row0 + r;
             const int64_t o = __shfl_sync(0xffffffffu, off[kv], r);
-            const uint32_t dst = sKV + s * Cfg::kStage + (c >> 3) * (KEYS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            const uint32_t dst = sKV + s * Cfg::kStage + (c >> 3) * (kKeys * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
             if (o == kUnknown) ptx::st_shared_16(dst, make_uint4(nan2, nan2, nan2, nan2));
-            else ptx::cp_async_16(dst, src + (o < 0 ? 0 : o + c * 16), o < 0 ? 0u : 16u);
+            else ptx::cp_async_16(dst, o < 0 ? static_cast<const void*>(a.k_cache) : src + o + c * 16, o < 0 ? 0u : 16u);
           }
           ptx::cp_async_commit();
           if (it >= Cfg::kAhead) {
@@ -359,27 +416,21 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
         for (uint32_t s = it > Cfg::kAhead ? it - Cfg::kAhead : 0; s < it; ++s) ready(s);
     } else {
       // Codes pass through registers: the pieces of kDepth stages are under way, the oldest is widened and stored
-      constexpr int kDepth = 3;
+      constexpr int kDepth = NT <= 32 ? 3 : 2;
       uint4 raw[kDepth][kSteps];
-      const uint32_t total = 2 * (uint32_t)line[1];
-      uint32_t asked = 0;
+      const uint32_t total = 2 * kParts * (uint32_t)line[1];
+      uint32_t asked = 0, part = 0;
       auto request = [&](uint4 (&to)[kSteps]) {
-        const int kv = asked & 1;
         if (asked >= total) return;
-        if (kv == 0) {
-          offsets(w, t, entry);
-          if (++t == w.t1) {
-            w.next();
-            t = w.t0;
-          }
-          entry = entry_of(w, t);
-        }
-        ++asked;
-        const uint8_t* src = static_cast<const uint8_t*>(kv ? a.v_cache : a.k_cache);
+        if (part == 0) next_tile();
+        const int kv = part / kParts;
+        const uint8_t* src = static_cast<const uint8_t*>(kv ? a.v_cache : a.k_cache) + (part % kParts) * 128;
         const int64_t mine = kv ? off[1] : off[0];
+        ++asked;
+        part = part + 1 == 2 * kParts ? 0 : part + 1;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-          const int piece = i * 32 + lane, r = piece / kPerKey, c = piece % kPerKey;
+          const int piece = i * 32 + lane, r = piece / kPieces, c = piece % kPieces;
           const int64_t o = __shfl_sync(0xffffffffu, mine, r);
           const uint32_t fill = o == kUnknown ? 0x7f7f7f7fu : 0u;
           to[i] = make_uint4(fill, fill, fill, fill);
@@ -392,7 +443,7 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
 #pragma unroll
         for (int u = 0; u < kDepth; ++u) {
           if (it >= total) break;
-          const int s = it % S;
+          const uint32_t s = it % S;
           ok = ok && ptx::mbar_wait(empty_bar(s), ((it / S) & 1) ^ 1, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
@@ -400,15 +451,15 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
           }
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) {
-            const int piece = i * 32 + lane, r = piece / kPerKey, row = row0 + r;
+            const int piece = i * 32 + lane, r = piece / kPieces, row = row0 + r;
             const uint32_t words[4] = {raw[u][i].x, raw[u][i].y, raw[u][i].z, raw[u][i].w};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const int c = (piece % kPerKey) * 2 + half;
+              const int c = (piece % kPieces) * 2 + half;
               uint32_t o[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) o[k] = widen2<T>((words[half * 2 + (k >> 1)] >> (16 * (k & 1))) & 0xffffu);
-              ptx::st_shared_16(sKV + s * Cfg::kStage + (c >> 3) * (KEYS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+              for (int k = 0; k < 4; ++k) o[k] = widen2(words[half * 2 + (k >> 1)] >> (16 * (k & 1)));
+              ptx::st_shared_16(sKV + s * Cfg::kStage + (c >> 3) * (kKeys * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
                                 make_uint4(o[0], o[1], o[2], o[3]));
             }
           }
@@ -420,20 +471,37 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
     }
     grid_launch_dependents();
   } else if (warp == Cfg::kQWarp) {
-    // ------------------------------------------------------------------ query rows
+    // ------------------------------------------------------------------ query rows, those behind the last one as zeros
     for (int seg = 0; w.more() && ok; w.next(), ++seg) {
       ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
-      const int rows = min(128, w.s.n * p.group - w.qt * 128);
+      const int rows = w.s.n * p.group - w.qt * NT;
       constexpr int kPerRow = D / 8;
-#pragma unroll 8
-      for (int i = lane; i < rows * kPerRow; i += 32) {
-        const int r = i / kPerRow, c = i % kPerRow, at = w.qt * 128 + r, token = fast_div(at, p.group_div);
-        const T* src = static_cast<const T*>(a.q) + (int64_t)(w.s.start + token) * a.q_token + (w.h * p.group + at - token * p.group) * a.q_head;
-        ptx::st_shared_16(sQ + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), ld_stream_16(src + c * 8));
+#pragma unroll 4
+      for (int i = lane; i < NT * kPerRow; i += 32) {
+        const int r = i / kPerRow, c = i % kPerRow, at = w.qt * NT + r, token = fast_div(at, p.group_div);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows)
+          v = ld_stream_16(static_cast<const T*>(a.q) + (int64_t)(w.s.start + token) * a.q_token + (w.h * p.group + at - token * p.group) * a.q_head + c * 8);
+        if constexpr (kRowScales) {
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&v);
+          float top = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(x[k])), fabsf(__high2float(x[k]))));
+#pragma unroll
+          for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
+          const float by = __uint_as_float((uint32_t)(127 + e) << 23);
+          if (c == 0) row_scale[(seg & 1) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = pack2<__half>(__low2float(x[k]) * by, __high2float(x[k]) * by);
+          v = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        ptx::st_shared_16(sQ + (c >> 3) * (NT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v);
       }
       ptx::fence_proxy_async_smem();
       __syncwarp();
@@ -442,38 +510,44 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
   } else if (warp == Cfg::kMmaWarp) {
     // ------------------------------------------------------------------ both products
     if (ptx::elect_one()) {
-      constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
-      constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kBf16, false, 128, KEYS), idesc_o = ptx::idesc_f16_f32(kBf16, true, 128, D);
+      constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kBf16, false, 128, NT), idesc_o = ptx::idesc_f16_f32(kBf16, true, 128, NT);
+      constexpr int kPRow = NT >= 64 ? 128 : NT * 2;
+      // heads of 64 fill half of the lanes: the other half repeats them
+      constexpr uint32_t kNextV = D == 64 ? 0u : kKeys * 128u;
       uint32_t it = 0, g = 0;  // stages and tiles of this CTA so far
-      // stages of the ring: keys of tile x in 2 x, its values in 2 x + 1
       auto scores = [&](uint32_t x, bool last) {
-        const uint32_t st = it + 2 * x, s = st % S;
-        if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
-        ptx::tc_fence_after();
-        const uint32_t d = tmem_base + ((g + x) & 1) * KEYS;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = (k & 3) * 32;
-          ptx::mma_f16_ss(d, ptx::smem_desc_sw128(sQ + (k >> 2) * (128 * 128) + at),
-                          ptx::smem_desc_sw128(sKV + s * Cfg::kStage + (k >> 2) * (KEYS * 128) + at), idesc_s, k > 0);
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t st = it + 2 * kParts * x + part, s = st % S;
+          if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < Cfg::kWidth / 16; ++k) {
+            const uint32_t in_row = (k & 3) * 32, block = k >> 2;
+            ptx::mma_f16(tmem_base + ((g + x) & 1) * NT, ptx::smem_desc_sw128(sKV + s * Cfg::kStage + block * (kKeys * 128) + in_row),
+                         ptx::smem_desc_sw128(sQ + (part * 2 + block) * (NT * 128) + in_row), idesc_s, part > 0 || k > 0);
+          }
+          ptx::mma_commit(empty_bar(s));
         }
-        ptx::mma_commit(empty_bar(s));
-        ptx::mma_commit(s_full((g + x) & 1));
+        ptx::mma_commit(s_full(g + x));
         if (last) ptx::mma_commit(q_empty);
         return true;
       };
       auto output = [&](uint32_t x) {
-        const uint32_t st = it + 2 * x + 1, s = st % S;
-        if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
-        if (!ptx::mbar_wait(p_full((g + x) & 1), ((g + x) >> 1) & 1, abort_flag)) return false;
-        ptx::tc_fence_after();
-        const uint32_t pt = tmem_base + ((g + x) & 1) * KEYS;
+        if (!ptx::mbar_wait(p_full(g + x), ((g + x) >> 1) & 1, abort_flag)) return false;
+        const uint32_t weights = sP + ((g + x) % Cfg::kPBufs) * Cfg::kPBytes;
 #pragma unroll
-        for (int k = 0; k < KEYS / 16; ++k)
-          ptx::mma_f16_ts(tmem_base + Cfg::kTmemO, pt + k * 8, ptx::smem_desc_mn_sw128(sKV + s * Cfg::kStage + k * 2048, KEYS * 128), idesc_o,
-                          x > 0 || k > 0);
-        ptx::mma_commit(empty_bar(s));
-        ptx::mma_commit(o_done);
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t st = it + 2 * kParts * x + kParts + part, s = st % S;
+          if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            ptx::mma_f16(tmem_base + Cfg::kTmemO + part * NT, ptx::smem_desc_depth_rows<128>(sKV + s * Cfg::kStage + k * 2048, kNextV),
+                         ptx::smem_desc_depth_rows<kPRow>(weights + k * 16 * kPRow, kKeys * 128), idesc_o, x > 0 || k > 0);
+          ptx::mma_commit(empty_bar(s));
+        }
+        ptx::mma_commit(o_done(g + x));
         return true;
       };
       for (int seg = 0; w.more() && ok; w.next(), ++seg) {
@@ -484,155 +558,225 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
           if (ok && x > 0) ok = output(x - 1);
         }
         ok = ok && output(n - 1);
-        it += 2 * n;
+        it += 2 * kParts * n;
         g += n;
       }
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax: a thread per row
-    const int r = threadIdx.x;
+    // ------------------------------------------------------------------ softmax: a thread per key, and per element of the heads for O^T
+    // What a warp decides alone would leave the others at a barrier: after a wait that may have failed all threads of a group decide together.
+    const int group = warp >> 2, r = threadIdx.x & 127, n0 = group * kCols, bar = 1 + group;
+    const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    constexpr int kChunk = kCols < 32 ? kCols : 32;  // columns in registers
+    auto load = [&](uint32_t at, uint32_t (&v)[32]) {
+      if constexpr (kChunk == 16) {
+        ptx::tmem_ld16(at, v);
+        ptx::tmem_ld_wait16(v);
+      } else {
+        ptx::tmem_ld32(at, v);
+        ptx::tmem_ld_wait(v);
+      }
+    };
     SplitRows begun = {0, 0, 0, 0, 0};
     uint32_t g = 0;
-    for (; w.more() && ok; w.next()) {
+    for (int seg = 0; w.more() && ok; w.next(), ++seg) {
       const Seq& s = w.s;
-      const int rows = min(128, s.n * p.group - w.qt * 128);
-      const bool busy = (warp * 32) < rows;  // the same for the whole warp
-      const int at = w.qt * 128 + min(r, rows - 1), token = fast_div(at, p.group_div), head = w.h * p.group + at - token * p.group;
-      const int first_token = fast_div(w.qt * 128, p.group_div), prefix = s.len - s.n;
+      const int rows = min(NT, s.n * p.group - w.qt * NT), prefix = s.len - s.n;
+      const int first_token = fast_div(w.qt * NT, p.group_div);
       float c = p.scale_log2;
       if (FP8 && a.k_scale) c *= ld_operand(a.k_scale + (a.k_scales > 1 ? w.h : 0));
-      float m = -INFINITY, l = 0.f;  // reference of the exponents; sum
+      const float* scales = row_scale + (seg & 1) * NT + n0;
+      float l[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) l[i] = 0.f;
+      if (r < kCols) minus_ref[n0 + r] = INFINITY;  // no reference yet
+      bool odd_values = false;                      // this thread met a value that is not finite among the sequence's own
       for (int t = w.t0; t < w.t1; ++t, ++g) {
-        ok = ptx::mbar_wait(s_full(g & 1), (g >> 1) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
+        ok = ok && ptx::mbar_wait(s_full(g), (g >> 1) & 1, abort_flag);
+        ptx::tc_fence_after();
+        const uint32_t ts = lane_base + (g & 1) * NT + n0;
+        const int j = t * kKeys + r;  // this thread's key
+        const bool own = j >= prefix && j < s.len;
+        // the tile's keys that not every row sees
+        const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
+        uint32_t v[32];
+        auto scores = [&](int k) {  // chunk k as exponents, without their reference
+          load(ts + k * kChunk, v);
+          if constexpr (kRowScales) {
+#pragma unroll
+            for (int i = 0; i < kChunk; i += 4) {
+              const float4 by = ld_shared_f4(scales + k * kChunk + i);
+              v[i] = __float_as_uint(__uint_as_float(v[i]) * (by.x * c)), v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) * (by.y * c));
+              v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) * (by.z * c)), v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) * (by.w * c));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * c);
+          }
+          if (masked && j >= prefix) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+              const int token = fast_div(w.qt * NT + n0 + k * kChunk + i, p.group_div);
+              bool sees = own && token < s.n;
+              if (sees)
+                sees = a.mask ? j - prefix < a.mask_width &&
+                                    static_cast<const volatile uint8_t*>(a.mask)[(int64_t)(s.start + token) * a.mask_ld + j - prefix] != 0
+                              : j - prefix <= token;
+              if (!sees) v[i] = 0xff800000u;
+            }
+          }
+        };
+        float above = -INFINITY;  // largest exponent over its reference
+#pragma unroll
+        for (int k = 0; k < kCols / kChunk; ++k) {
+          scores(k);
+#pragma unroll
+          for (int i = 0; i < kChunk; i += 4) {
+            const float4 m = ld_shared_f4(minus_ref + n0 + k * kChunk + i);
+            above = fmaxf(above, fmaxf(fmaxf(__uint_as_float(v[i]) + m.x, __uint_as_float(v[i + 1]) + m.y),
+                                       fmaxf(__uint_as_float(v[i + 2]) + m.z, __uint_as_float(v[i + 3]) + m.w)));
+          }
         }
-        if (busy) {
-          ptx::tc_fence_after();
-          const uint32_t ts = lane_base + (g & 1) * KEYS;
-          uint32_t v[KEYS / 32][32];
+        if (ptx::any_of(bar, 128, above > kSlack || t == w.t0 || !ok)) {
+          // Rows whose largest score lies too far above their reference take it as the new one
 #pragma unroll
-          for (int k = 0; k < KEYS / 32; ++k) ptx::tmem_ld32(ts + k * 32, v[k]);
+          for (int k = 0; k < kCols / kChunk; ++k) {
+            if (kCols > kChunk) scores(k);
+            float top[kChunk];
 #pragma unroll
-          for (int k = 0; k < KEYS / 32; ++k) ptx::tmem_ld_wait(v[k]);
-          const int j0 = t * KEYS;
-          // keys that every row of the tile sees need no mask
-          if (j0 + KEYS > (a.mask ? prefix : prefix + first_token + 1)) {
-#pragma unroll
-            for (int k = 0; k < KEYS / 32; ++k) {
-              const int j = j0 + k * 32, sees = (a.mask ? prefix : min(s.len, prefix + token + 1)) - j;  // keys seen of these 32
-              uint32_t bits = sees >= 32 ? 0xffffffffu : sees <= 0 ? 0u : (1u << sees) - 1u;
-              if (a.mask) {
-                const volatile uint8_t* line_of_mask = static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + token) * a.mask_ld;
-                const int end = min(min(32, s.len - j), a.mask_width + prefix - j);
-                for (int i = max(sees, 0); i < end; ++i) bits |= (line_of_mask[j + i - prefix] ? 1u : 0u) << i;
-              }
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[k][i] = (bits >> i) & 1u ? v[k][i] : 0xff800000u;
-            }
+            for (int i = 0; i < kChunk; ++i) top[i] = __uint_as_float(v[i]);
+            const float of_lane = across_lanes(top, [](float x, float y) { return fmaxf(x, y); });
+            if (lane < kChunk) by_warp[(warp & 3) * NT + n0 + k * kChunk + lane] = of_lane;
           }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int k = 0; k < KEYS / 32; ++k)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[k][i]));
-          const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-          const bool move = largest > m + kSlack;
-          const float m_new = move ? largest : m, factor = move ? ptx::ex2(m - m_new) : 1.f, minus_m = m_new == -INFINITY ? 0.f : -m_new;
-          l *= factor;
-          m = m_new;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < KEYS / 32; ++k) {
-            uint32_t out[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e0 = ptx::ex2(fmaf(__uint_as_float(v[k][2 * i]), c, minus_m)), e1 = ptx::ex2(fmaf(__uint_as_float(v[k][2 * i + 1]), c, minus_m));
-              out[i] = pack2<T>(e0, e1);
-              if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-                // the weights as they are multiplied: a row that one key rules comes out as that key's value, without the rounding of its weight
-                sum[i & 3] += __uint_as_float(out[i] << 16);
-                sum[i & 3] += __uint_as_float(out[i] & 0xffff0000u);
-              } else {
-                sum[i & 3] += e0;
-                sum[i & 3] += e1;
-              }
-            }
-            ptx::tmem_st16(ts + k * 16, out);  // over scores that are in registers
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          // O of the tiles before this one is complete: waited for in every tile, so that the barrier is never two phases ahead
-          if (g > 0) ok = ptx::mbar_wait(o_done, (g - 1) & 1, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) {
+          const bool moves = t > w.t0;
+          if (moves) ok = ok && ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
+          if (ptx::any_of(bar, 128, !ok)) {
             ok = false;
             break;
           }
-          if (t > w.t0 && __any_sync(0xffffffffu, move)) {
+          if (r < kCols) {
+            const int n = n0 + r;
+            const float top = fmaxf(fmaxf(by_warp[n], by_warp[NT + n]), fmaxf(by_warp[2 * NT + n], by_warp[3 * NT + n])), old = -minus_ref[n];
+            const bool move = top > old + kSlack;
+            factor[n] = move ? ptx::ex2(old - top) : 1.f;
+            if (move) minus_ref[n] = -top;
+          }
+          ptx::any_of(bar, 128, false);
+          if (moves) {
+#pragma unroll
+            for (int i = 0; i < kCols; i += 4) {
+              const float4 f = ld_shared_f4(factor + n0 + i);
+              l[i] *= f.x, l[i + 1] *= f.y, l[i + 2] *= f.z, l[i + 3] *= f.w;
+            }
             ptx::tc_fence_after();
 #pragma unroll 1
-            for (int d = 0; d < D; d += 16) {
-              uint32_t o[32], n[16];
-              ptx::tmem_ld16(lane_base + Cfg::kTmemO + d, o);
+            for (int d = 0; d < kParts * kCols; d += 16) {
+              const int part = d / kCols, n = n0 + d - part * kCols;
+              uint32_t o[32], scaled[16];
+              ptx::tmem_ld16(lane_base + Cfg::kTmemO + part * NT + n, o);
               ptx::tmem_ld_wait16(o);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) n[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-              ptx::tmem_st16(lane_base + Cfg::kTmemO + d, n);
+              for (int i = 0; i < 16; i += 4) {
+                const float4 f = ld_shared_f4(factor + n + i);
+                scaled[i] = __float_as_uint(__uint_as_float(o[i]) * f.x), scaled[i + 1] = __float_as_uint(__uint_as_float(o[i + 1]) * f.y);
+                scaled[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * f.z), scaled[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * f.w);
+              }
+              ptx::tmem_st16(lane_base + Cfg::kTmemO + part * NT + n, scaled);
+            }
+            ptx::tmem_st_wait();
+          }
+        }
+        // the buffer of P^T is free when the product that read it is complete
+        if (g >= Cfg::kPBufs) ok = ok && ptx::mbar_wait(o_done(g - Cfg::kPBufs), ((g - Cfg::kPBufs) >> 1) & 1, abort_flag);
+#pragma unroll
+        for (int k = 0; k < kCols / kChunk; ++k) {
+          if (kCols > kChunk) scores(k);
+          uint32_t out[kChunk / 2];
+#pragma unroll
+          for (int i = 0; i < kChunk; i += 4) {
+            const float4 m = ld_shared_f4(minus_ref + n0 + k * kChunk + i);
+            // a row without a reference has seen nothing: its scores are all -infinity
+            const float e0 = ptx::ex2(__uint_as_float(v[i]) + (m.x < INFINITY ? m.x : 0.f)), e1 = ptx::ex2(__uint_as_float(v[i + 1]) + (m.y < INFINITY ? m.y : 0.f));
+            const float e2 = ptx::ex2(__uint_as_float(v[i + 2]) + (m.z < INFINITY ? m.z : 0.f)), e3 = ptx::ex2(__uint_as_float(v[i + 3]) + (m.w < INFINITY ? m.w : 0.f));
+            out[i / 2] = pack2<M>(e0, e1), out[i / 2 + 1] = pack2<M>(e2, e3);
+            const int n = k * kChunk + i;
+            if constexpr (kBf16) {
+              // the weights as they are multiplied: a row that one key rules comes out as that key's value, without the rounding of its weight
+              l[n] += __uint_as_float(out[i / 2] << 16), l[n + 1] += __uint_as_float(out[i / 2] & 0xffff0000u);
+              l[n + 2] += __uint_as_float(out[i / 2 + 1] << 16), l[n + 3] += __uint_as_float(out[i / 2 + 1] & 0xffff0000u);
+            } else {
+              l[n] += e0, l[n + 1] += e1, l[n + 2] += e2, l[n + 3] += e3;
             }
           }
-          ptx::tmem_st_wait();
-          ptx::tc_fence_before();
+          constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
+          const uint32_t row = sP + (g % Cfg::kPBufs) * Cfg::kPBytes + ((n0 + k * kChunk) / 64) * (kKeys * 128) + r * kRow;
+          const int piece0 = (n0 + k * kChunk) % 64 / 8;
+#pragma unroll
+          for (int q = 0; q < kChunk / 8; ++q) {
+            const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
+            if (ok) ptx::st_shared_16(row + (((piece0 + q) ^ swizzle) << 4), make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]));
+          }
         }
+        ptx::fence_proxy_async_smem();
+        ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_full(g & 1));
+        if (lane == 0) ptx::mbar_arrive(p_full(g));
       }
-      if (!ok) break;
+      if (!ok) break;  // (of the whole group: after its last barrier, or the same for every later one)
       const bool whole = w.t0 == 0 && w.t1 == s.key_tiles;
       if (!whole && w.t0 == 0)
         begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.key_tiles - w.t1 + line[2] - 1) / line[2])};
-      if (busy) {
-        ok = ptx::mbar_wait(o_done, (g - 1) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        if (whole) {
-          const float inv = l == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f) / l;
-          T* dst = static_cast<T*>(a.out) + ((int64_t)(s.start + token) * a.q_heads + head) * D;
-#pragma unroll 1
-          for (int d = 0; d < D; d += 16) {
-            uint32_t o[32], n[8];
-            ptx::tmem_ld16(lane_base + Cfg::kTmemO + d, o);
-            ptx::tmem_ld_wait16(o);
-            // a row that sees nothing is zero, whatever its weights of zero met
+      // sums of the weights: over this warp's keys, then over the warps
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              n[i] = l == 0.f ? 0u : pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-            if (r < rows) {
-              reinterpret_cast<uint4*>(dst + d)[0] = make_uint4(n[0], n[1], n[2], n[3]);
-              reinterpret_cast<uint4*>(dst + d)[1] = make_uint4(n[4], n[5], n[6], n[7]);
+      for (int k = 0; k < kCols / kChunk; ++k) {
+        float part[kChunk];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) part[i] = l[k * kChunk + i];
+        const float of_lane = across_lanes(part, [](float x, float y) { return x + y; });
+        if (lane < kChunk) by_warp[(warp & 3) * NT + n0 + k * kChunk + lane] = of_lane;
+      }
+      ok = ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
+      if (ptx::any_of(bar, 128, !ok)) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      const int64_t slot0 = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots;
+      if (r < kCols) {
+        const int n = n0 + r, at = w.qt * NT + n, token = fast_div(at, p.group_div);
+        const float sum = (by_warp[n] + by_warp[NT + n]) + (by_warp[2 * NT + n] + by_warp[3 * NT + n]), ref = -minus_ref[n];
+        factor[n] = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f) / sum;
+        if (n < rows) {
+          if (!whole) p.part_ml[slot0 + n] = make_float2(ref, sum);
+          else if (a.lse)
+            a.lse[(int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group] =
+                sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+        }
+      }
+      ptx::any_of(bar, 128, false);
+      if (r < Cfg::kWidth) {
+#pragma unroll 1
+        for (int d0 = 0; d0 < kParts * kCols; d0 += 16) {
+          const int part = d0 / kCols, first = n0 + d0 - part * kCols, d = part * 128 + r;
+          if (first >= rows) continue;  // the same for the whole group
+          uint32_t o[32];
+          ptx::tmem_ld16(lane_base + Cfg::kTmemO + part * NT + first, o);
+          ptx::tmem_ld_wait16(o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int n = first + i, at = w.qt * NT + n, token = fast_div(at, p.group_div);
+            if (n < rows) {
+              // a row that has seen nothing is zero, whatever its weights of zero met
+              const float f = factor[n], x = f == 0.f ? 0.f : __uint_as_float(o[i]);
+              if (whole) static_cast<T*>(a.out)[((int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group) * D + d] = from_f32<T>(x * f);
+              else p.part_o[(slot0 + n) * D + d] = x;
             }
           }
-          if (a.lse && r < rows) a.lse[(int64_t)(s.start + token) * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-        } else {
-          const int64_t slot = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots + r;
-          float* dst = p.part_o + slot * D;
-#pragma unroll 1
-          for (int d = 0; d < D; d += 16) {
-            uint32_t o[32];
-            ptx::tmem_ld16(lane_base + Cfg::kTmemO + d, o);
-            ptx::tmem_ld_wait16(o);
-            if (r < rows)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                reinterpret_cast<uint4*>(dst + d)[i] = l == 0.f ? make_uint4(0, 0, 0, 0) : make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-          if (r < rows) p.part_ml[slot] = make_float2(m, l);
         }
-        ptx::tc_fence_before();
       }
+      ptx::tc_fence_before();
+      ptx::any_of(bar, 128, false);  // the tables of this segment have been read
     }
     if (threadIdx.x == 0) p.split[blockIdx.x] = begun;
   }
@@ -646,12 +790,12 @@ __global__ void __launch_bounds__(AttnCfg<D, FP8>::kThreads, 1) tree_attention_k
   if (threadIdx.x == 0 && *abort_flag) atomicCAS(p.status, 0, 1);
   if (warp == Cfg::kMmaWarp) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem_base, 512);
+    ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
 }
 
 // Rows whose keys were cut: a warp per row adds up its pieces, in the order of the line.
-template <typename T, int D, bool FP8>
+template <typename T, int D, int NT, bool FP8>
 __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_constant__ AttnParams p) {
   const b200_tree_attention_args& a = p.a;
   grid_launch_dependents();
@@ -660,8 +804,8 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_c
   const volatile int* const from = reinterpret_cast<const volatile int*>(p.split + cta);
   const int parts = from[4];
   if (parts == 0) return;
-  const int start = from[0], qt = from[1], h = from[2], row = qt * 128 + r;
-  if (r >= 128 || row >= from[3]) return;
+  const int start = from[0], qt = from[1], h = from[2], row = qt * NT + r;
+  if (r >= NT || row >= from[3]) return;
   auto slot_of = [&](int i) { return (2 * (int64_t)(cta + i) + (i == 0 ? 1 : 0)) * p.row_slots + r; };
   auto ml_of = [&](int i) {
     const volatile float* ml = reinterpret_cast<const volatile float*>(p.part_ml + slot_of(i));
@@ -703,18 +847,23 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_c
   if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
 }
 
+// Rows of a tile: those of one sequence's new tokens, as far as the host knows their number (the mask's width, else their mean).
+inline int attention_rows(const b200_tree_attention_args& a) {
+  const int64_t n = a.q_starts == nullptr ? 1 : a.mask ? a.mask_width : cdiv(a.tokens, a.sequences);
+  const int64_t rows = (n < 1 ? 1 : n) * (a.q_heads / a.kv_heads);
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || a.dim > 128 ? 64 : 128;  // 128 rows of 256 leave no room for the ring
+}
 // CTAs of a call: no more than there can be tiles
 inline int64_t attention_grid(const b200_tree_attention_args& a) {
-  const int keys = a.dim > 128 ? 64 : 128;
-  const int64_t group = a.q_heads / a.kv_heads, row_tiles = cdiv(a.tokens * group, 128) + a.sequences;
-  const int64_t capacity = a.max_pages * a.page_size, key_tiles = capacity > 0 ? cdiv(capacity, keys) : 1;
+  const int64_t group = a.q_heads / a.kv_heads, row_tiles = cdiv(a.tokens * group, attention_rows(a)) + a.sequences;
+  const int64_t capacity = a.max_pages * a.page_size, key_tiles = capacity > 0 ? cdiv(capacity, kKeys) : 1;
   const double tiles = (double)row_tiles * a.kv_heads * key_tiles;
   const int sms = sm_count();
   return tiles < sms ? (int64_t)tiles : sms;
 }
 inline int attention_row_slots(const b200_tree_attention_args& a) {
-  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads);
-  return rows < 128 ? (int)rows : 128;
+  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads), tile = attention_rows(a);
+  return (int)(rows < tile ? rows : tile);
 }
 struct AttnWorkspace {
   size_t ml, split, total;  // byte offsets behind the partial sums
@@ -728,18 +877,29 @@ inline AttnWorkspace attention_workspace(const b200_tree_attention_args& a) {
   return w;
 }
 
-template <typename T, int D, bool FP8>
+template <typename T, int D, int NT, bool FP8>
 static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
-  using Cfg = AttnCfg<D, FP8>;
-  auto k = tree_attention_kernel<T, D, FP8>;
+  using Cfg = AttnCfg<D, NT, FP8>;
+  auto k = tree_attention_kernel<T, D, NT, FP8>;
   if (int rc = allow_smem(k, Cfg::kSmemBytes, "tree_attention_kernel")) return rc;
   if (int rc = launch_dependent(k, dim3((unsigned)grid), Cfg::kThreads, Cfg::kSmemBytes, st, 1, "tree_attention", p)) return rc;
-  return launch_dependent(tree_attention_join_kernel<T, D, FP8>, dim3((unsigned)grid, (unsigned)cdiv(p.row_slots, 8)), 256, 0, st, 1,
+  return launch_dependent(tree_attention_join_kernel<T, D, NT, FP8>, dim3((unsigned)grid, (unsigned)cdiv(p.row_slots, 8)), 256, 0, st, 1,
                           "tree_attention", p);
+}
+template <typename T, int D, int NT>
+static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
+  return p.a.cache_dtype == B200_E4M3 ? launch_attention<T, D, NT, true>(p, grid, st) : launch_attention<T, D, NT, false>(p, grid, st);
 }
 template <typename T, int D>
 static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
-  return p.a.cache_dtype == B200_E4M3 ? launch_attention<T, D, true>(p, grid, st) : launch_attention<T, D, false>(p, grid, st);
+  switch (attention_rows(p.a)) {
+    case 16: return launch_attention<T, D, 16>(p, grid, st);
+    case 32: return launch_attention<T, D, 32>(p, grid, st);
+    case 64: return launch_attention<T, D, 64>(p, grid, st);
+    default:
+      if constexpr (D <= 128) return launch_attention<T, D, 128>(p, grid, st);
+      return B200_E_UNSUPPORTED;
+  }
 }
 template <typename T>
 static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
