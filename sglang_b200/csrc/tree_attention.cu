@@ -52,18 +52,41 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// Arrives once all copies that this thread has issued so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void st_shared_16(uint32_t dst, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_byte(const uint8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Moves this warp's registers from what it was launched with to N a thread (all warps of its group of four do the same)
+template <int N, int LAUNCH>
+__device__ __forceinline__ void give_registers() {
+  if constexpr (N > LAUNCH) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  if constexpr (N < LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Two fp32 operations at once
+__device__ __forceinline__ void fma_two(float& a, float& b, float x0, float x1, float y0, float y1, float z0, float z1) {  // x y + z
+  asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x;}"
+      : "=f"(a), "=f"(b)
+      : "f"(x0), "f"(x1), "f"(y0), "f"(y1), "f"(z0), "f"(z1));
+}
+__device__ __forceinline__ void add_two(float& a, float& b, float x0, float x1) {  // a += x0, b += x1
+  asm("{.reg .b64 x, y; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %3}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}" : "+f"(a), "+f"(b) : "f"(x0), "f"(x1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // true in all `threads` threads of barrier `id` if it is in one
 __device__ __forceinline__ bool any_of(int id, int threads, bool mine) {
@@ -106,6 +129,7 @@ struct AttnParams {
 };
 
 constexpr int kKeys = 128;  // of a tile
+__device__ const uint4 not_a_number = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // in either 16-bit type
 
 template <int D, int NT, bool FP8>
 struct AttnCfg {
@@ -115,19 +139,24 @@ struct AttnCfg {
   static constexpr int kCols = NT / kGroups;
   static constexpr int kPBufs = NT * D < 64 * 256 ? 2 : 1;
   static constexpr int kQBytes = NT * D * 2, kPBytes = kKeys * NT * 2;
-  static constexpr int kTables = NT * 4 * (2 + 1 + 1 + 4);  // scales of two segments' rows, references, factors, and a value per warp and column
+  static constexpr int kTables = NT * 4 * (2 + 1 + 1 + 4 + 1 + 1);  // scales of two segments' rows, references, factors, a value per warp, tokens, rows of the output
   static constexpr int kFixed = kQBytes + kPBufs * kPBytes + kTables + 1024 + 512;
   static constexpr int kFit = (232448 - kFixed) / kStage;
   static constexpr int kStages = kFit < 12 ? kFit : 12;
-  // Stages whose copies are under way when the one before them is handed over. The scores of a tile are asked for before the tile ahead of it gives
-  // its values' stages back, so that its last stage of keys has to be handed over with those still taken.
-  static constexpr int kAhead = kStages - 2 * kParts < 8 ? kStages - 2 * kParts : 8;
-  static constexpr int kSoftmaxWarps = 4 * kGroups, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 2, kProducerWarps = 4;
-  static constexpr int kThreads = (kProducerWarp + kProducerWarps) * 32;
+  // Warps: softmax; products, queries and two idle ones; then four that bring keys and four values, with 128 rows four that bring both (registers)
+  static constexpr int kSoftmaxWarps = 4 * kGroups, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 4;
+  // (heads of 256 four that bring both, too: with two stages a tile, warps that run ahead of the others could take a stage's barrier for two phases older)
+  static constexpr bool kSplit = NT <= 64 && kParts == 1;
+  static constexpr int kThreads = (kProducerWarp + (kSplit ? 8 : 4)) * 32;
+  // Registers of a thread at launch, and of the three kinds of warps where two groups of softmax warps need more than that (0: as launched)
+  static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
+  static constexpr int kSoftmaxRegs = kGroups == 1 ? 0 : kSplit ? 112 : 160, kProducerRegs = kSplit ? 88 : 112, kOtherRegs = 80;
+  static_assert(kGroups == 1 || (8 * kSoftmaxRegs + 4 * kOtherRegs + (kSplit ? 8 : 4) * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
+                "the registers add up to no more than at launch");
   static constexpr int kTmemO = 2 * NT, kTmemUsed = (2 + kParts) * NT;  // columns: S^T twice, O^T from here
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static constexpr size_t kSmemBytes = (size_t)kFixed + (size_t)kStages * kStage;
-  static_assert(kAhead >= 1 && kTmemUsed <= 512, "a tile of keys and one of values fit");
+  static_assert(kStages >= 2 * kParts + 1 && kTmemUsed <= 512, "a tile of keys and one of values fit");
 };
 
 // Sequence b as the kernel takes it: whatever the index tensors hold, tokens and keys stay inside q and the page table.
@@ -191,10 +220,9 @@ struct Walk {
   }
 };
 
-// Two E4M3 codes as fp16 values: exact
-__device__ __forceinline__ uint32_t widen2(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four E4M3 codes as fp16 values: exact
+__device__ __forceinline__ void widen4(uint32_t codes, uint32_t& low, uint32_t& high) {
+  asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(low), "=r"(high) : "r"(codes));
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -210,6 +238,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // A score may exceed its row's reference by this much (in powers of two) before the reference moves: sums stay exact to fp32 and weights far from the
 // 16-bit types' limits, and most rows move theirs in the first tile alone.
 constexpr float kSlack = 8.f;
+constexpr float kNoRef = 3e38f;  // of a row that has seen nothing yet, negated like all references: any score exceeds it, and -infinity stays what it is
 
 // Value i of lane l, N <= 32 of them in each of 32 lanes -> lane l has the result over all lanes of value l % N. Each step halves the values that a
 // lane still has, N - 1 exchanges and 5 - log2 N more.
@@ -256,7 +285,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   float* minus_ref = row_scale + 2 * NT;                                                                    // [NT]
   float* factor = minus_ref + NT;                                                                           // [NT]
   float* by_warp = factor + NT;                                                                             // [4][NT]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(by_warp + 4 * NT);
+  int* token_of = reinterpret_cast<int*>(by_warp + 4 * NT);                                                 // [NT]
+  int* out_row = token_of + NT;                                                                             // [NT]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_row + NT);
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (S + s); };
@@ -273,10 +304,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      ptx::mbar_init(full_bar(s), Cfg::kProducerWarps);
+      ptx::mbar_init(full_bar(s), FP8 ? 4 : 128);  // warps that have stored, or threads whose copies have landed
       ptx::mbar_init(empty_bar(s), 1);
     }
-    ptx::mbar_init(q_full, 1);
+    ptx::mbar_init(q_full, 3);
     ptx::mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(o_done(i), 1);
@@ -341,175 +372,178 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 
   if (warp >= Cfg::kProducerWarp) {
     // ------------------------------------------------------------------ keys and values into the ring, a tile's keys, then its values
-    constexpr int kRows = kKeys / Cfg::kProducerWarps;  // keys of a tile that this warp copies, lane l the l-th
-    static_assert(kRows == 32, "a lane per key");
-    const int row0 = (warp - Cfg::kProducerWarp) * kRows;
+    if constexpr (Cfg::kGroups > 1) ptx::give_registers<Cfg::kProducerRegs, Cfg::kLaunchRegs>();
+    const int row0 = ((warp - Cfg::kProducerWarp) & 3) * 32;  // 32 keys of a tile, lane l has the addresses of the l-th
+    // stages of a tile that are this warp's
+    constexpr int kMine = Cfg::kSplit ? kParts : 2 * kParts;
+    const int first_part = Cfg::kSplit && warp >= Cfg::kProducerWarp + 4 ? kParts : 0;
     constexpr int kPieces = Cfg::kWidth / (FP8 ? 16 : 8);  // of 16 bytes, of a key's part in the cache
-    constexpr int kSteps = kRows * kPieces / 32;
-    constexpr int64_t kAbsent = -1, kUnknown = -2;         // no key; a page that the cache does not have
+    constexpr int kKeysAtOnce = 32 / kPieces;              // of a load of the warp
+    constexpr int kSteps = kPieces;
     constexpr int es = FP8 ? 1 : 2;
     auto entry_of = [&](const Walk<NT>& at, int t) {
       const int j = t * kKeys + row0 + lane;
       if (!at.more() || j >= at.s.len) return -1;
       return (int)ld_operand(a.page_table + (int64_t)at.b * a.page_table_ld + fast_div(j, p.page_div));
     };
-    int64_t off[2];
-    auto offsets = [&](const Walk<NT>& at, int t, int entry) {
-      const int j = t * kKeys + row0 + lane;
-      if (j >= at.s.len) {
-        off[0] = off[1] = kAbsent;
-      } else if (entry < 0 || entry >= a.pages) {
-        off[0] = kUnknown;
-        off[1] = kAbsent;
-      } else {
-        const int in_page = j - fast_div(j, p.page_div) * a.page_size;
-        off[0] = (entry * a.k_page + in_page * a.k_token + at.h * a.k_head) * es;
-        off[1] = (entry * a.v_page + in_page * a.v_token + at.h * a.v_head) * es;
-      }
-    };
-    uint32_t it = 0;
-    auto ready = [&](uint32_t stage) {  // this thread's part of the stage is in shared memory
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(full_bar(stage % S));
-    };
+    const uint8_t* from[2];       // this lane's key and its value; something readable where there is none
+    uint32_t absent, unknown;     // a bit per lane: no key there; a page that the cache does not have
     int t = w.t0, entry = entry_of(w, t);
     auto next_tile = [&] {
-      offsets(w, t, entry);
+      const int j = t * kKeys + row0 + lane, in_page = j - fast_div(j, p.page_div) * a.page_size;
+      const bool key = j < w.s.len, page = entry >= 0 && entry < a.pages;
+      absent = __ballot_sync(0xffffffffu, !key);
+      unknown = __ballot_sync(0xffffffffu, key && !page);
+      from[0] = from[1] = static_cast<const uint8_t*>(a.q);
+      if (key && page) {
+        from[0] = static_cast<const uint8_t*>(a.k_cache) + (entry * a.k_page + in_page * a.k_token + w.h * a.k_head) * es;
+        from[1] = static_cast<const uint8_t*>(a.v_cache) + (entry * a.v_page + in_page * a.v_token + w.h * a.v_head) * es;
+      }
       if (++t == w.t1) {
         w.next();
         t = w.t0;
       }
       entry = entry_of(w, t);
     };
+    const uint32_t total = kMine * (uint32_t)line[1];  // stages of this warp
+    auto stage_of = [&](uint32_t n) { return (n / kMine) * 2 * kParts + first_part + n % kMine; };
+    // Step i of a stage: key i * kKeysAtOnce + lane / kPieces of this warp's, piece lane % kPieces
+    const int my_key = lane / kPieces, my_piece = lane % kPieces;
+    auto address = [&](const uint8_t* mine, int i) {
+      return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i * kKeysAtOnce + my_key)) + my_piece * 16;
+    };
+    // where 16 bytes of 16-bit elements go, piece c of the key: 128-byte rows, 128-byte swizzle (the key's low bits are those of i and of my_key, apart)
+    auto slot = [&](uint32_t base, int c, int i) {
+      return base + (c >> 3) * (kKeys * 128) + my_key * 128 + (((uint32_t)((c & 7) ^ my_key) << 4) ^ (((i * kKeysAtOnce) & 7) << 4)) + i * kKeysAtOnce * 128;
+    };
     if constexpr (!FP8) {
-      const uint32_t nan2 = 0x7fff7fffu;
-      while (w.more() && ok) {
-        next_tile();
+      for (uint32_t n = 0; n < total; ++n) {
+        const int part = first_part + n % kMine, kv = part / kParts;
+        if (n % kMine == 0) next_tile();
+        const uint32_t st = stage_of(n), s = st % S;
+        ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const uint8_t* mine = kv ? from[1] : from[0];
+        const uint32_t base = sKV + s * Cfg::kStage + row0 * 128;
+        if ((absent | unknown) == 0) {
 #pragma unroll
-        for (int part = 0; part < 2 * kParts; ++part, ++it) {
-          const int kv = part / kParts;
-          const uint32_t s = it % S;
-          ok = ok && ptx::mbar_wait(empty_bar(s), ((it / S) & 1) ^ 1, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          const uint8_t* src = static_cast<const uint8_t*>(kv ? a.v_cache : a.k_cache) + (part % kParts) * 256;
-#pragma unroll
+          for (int i = 0; i < kSteps; ++i) ptx::cp_async_16(slot(base, my_piece, i), address(mine, i) + (part % kParts) * 256, 16u);
+        } else {
+#pragma unroll 1
           for (int i = 0; i < kSteps; ++i) {
-            const int piece = i * 32 + lane, r = piece / kPieces, c = piece % kPieces, row = row0 + r;
-            const int64_t o = __shfl_sync(0xffffffffu, off[kv], r);
-            const uint32_t dst = sKV + s * Cfg::kStage + (c >> 3) * (kKeys * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-            if (o == kUnknown) ptx::st_shared_16(dst, make_uint4(nan2, nan2, nan2, nan2));
-            else ptx::cp_async_16(dst, o < 0 ? static_cast<const void*>(a.k_cache) : src + o + c * 16, o < 0 ? 0u : 16u);
-          }
-          ptx::cp_async_commit();
-          if (it >= Cfg::kAhead) {
-            ptx::cp_async_wait<Cfg::kAhead>();
-            ready(it - Cfg::kAhead);
+            const uint8_t* src = address(mine, i) + (part % kParts) * 256;
+            const int key = i * kKeysAtOnce + my_key;
+            const bool none = (absent >> key) & 1u, nan = (unknown >> key) & 1u;
+            ptx::cp_async_16(slot(base, my_piece, i), nan ? reinterpret_cast<const uint8_t*>(&not_a_number) : none ? static_cast<const uint8_t*>(a.q) : src,
+                             none || (nan && kv) ? 0u : 16u);
           }
         }
+        ptx::cp_async_arrive(full_bar(s));  // when they have landed
       }
-      ptx::cp_async_wait<0>();
-      if (ok)
-        for (uint32_t s = it > Cfg::kAhead ? it - Cfg::kAhead : 0; s < it; ++s) ready(s);
+      ptx::cp_async_wait_all();
     } else {
-      // Codes pass through registers: the pieces of kDepth stages are under way, the oldest is widened and stored
-      constexpr int kDepth = NT <= 32 ? 3 : 2;
+      // Codes pass through registers: the pieces of kDepth stages are under way, the oldest is widened and stored. Where there is no key to load, something
+      // that exists is, and replaced when it is stored: a load behind a branch would be waited for there.
+      constexpr int kDepth = 2;
       uint4 raw[kDepth][kSteps];
-      const uint32_t total = 2 * kParts * (uint32_t)line[1];
-      uint32_t asked = 0, part = 0;
-      auto request = [&](uint4 (&to)[kSteps]) {
+      uint32_t no_key[kDepth], no_page[kDepth], asked = 0;
+      auto request = [&](uint4 (&to)[kSteps], uint32_t& missing, uint32_t& lost) {
         if (asked >= total) return;
-        if (part == 0) next_tile();
-        const int kv = part / kParts;
-        const uint8_t* src = static_cast<const uint8_t*>(kv ? a.v_cache : a.k_cache) + (part % kParts) * 128;
-        const int64_t mine = kv ? off[1] : off[0];
+        const int part = first_part + asked % kMine, kv = part / kParts;
+        if (asked % kMine == 0) next_tile();
         ++asked;
-        part = part + 1 == 2 * kParts ? 0 : part + 1;
+        missing = absent | unknown;
+        lost = kv ? 0u : unknown;
+        const uint8_t* mine = kv ? from[1] : from[0];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int piece = i * 32 + lane, r = piece / kPieces, c = piece % kPieces;
-          const int64_t o = __shfl_sync(0xffffffffu, mine, r);
-          const uint32_t fill = o == kUnknown ? 0x7f7f7f7fu : 0u;
-          to[i] = make_uint4(fill, fill, fill, fill);
-          if (o >= 0) to[i] = ld_stream_16(src + o + c * 16);
-        }
+        for (int i = 0; i < kSteps; ++i) to[i] = ld_stream_16(address(mine, i) + (part % kParts) * 128);
       };
 #pragma unroll
-      for (int u = 0; u < kDepth; ++u) request(raw[u]);
-      while (it < total && ok) {
+      for (int u = 0; u < kDepth; ++u) request(raw[u], no_key[u], no_page[u]);
+      uint32_t n = 0;
+      while (n < total && ok) {
 #pragma unroll
         for (int u = 0; u < kDepth; ++u) {
-          if (it >= total) break;
-          const uint32_t s = it % S;
-          ok = ok && ptx::mbar_wait(empty_bar(s), ((it / S) & 1) ^ 1, abort_flag);
+          if (n >= total) break;
+          const uint32_t st = stage_of(n), s = st % S;
+          ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
+          if (no_key[u]) {
 #pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            const int piece = i * 32 + lane, r = piece / kPieces, row = row0 + r;
-            const uint32_t words[4] = {raw[u][i].x, raw[u][i].y, raw[u][i].z, raw[u][i].w};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int c = (piece % kPieces) * 2 + half;
-              uint32_t o[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) o[k] = widen2(words[half * 2 + (k >> 1)] >> (16 * (k & 1)));
-              ptx::st_shared_16(sKV + s * Cfg::kStage + (c >> 3) * (kKeys * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4),
-                                make_uint4(o[0], o[1], o[2], o[3]));
+            for (int i = 0; i < kSteps; ++i) {
+              const int key = i * kKeysAtOnce + my_key;
+              const uint32_t fill = (no_page[u] >> key) & 1u ? 0x7f7f7f7fu : 0u;
+              if ((no_key[u] >> key) & 1u) raw[u][i] = make_uint4(fill, fill, fill, fill);
             }
           }
-          ready(it);
-          ++it;
-          request(raw[u]);
+          const uint32_t base = sKV + s * Cfg::kStage + row0 * 128;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            uint4 lo, hi;
+            widen4(raw[u][i].x, lo.x, lo.y);
+            widen4(raw[u][i].y, lo.z, lo.w);
+            widen4(raw[u][i].z, hi.x, hi.y);
+            widen4(raw[u][i].w, hi.z, hi.w);
+            ptx::st_shared_16(slot(base, 2 * my_piece, i), lo);
+            ptx::st_shared_16(slot(base, 2 * my_piece + 1, i), hi);
+          }
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(full_bar(s));
+          ++n;
+          request(raw[u], no_key[u], no_page[u]);
         }
       }
     }
     grid_launch_dependents();
-  } else if (warp == Cfg::kQWarp) {
-    // ------------------------------------------------------------------ query rows, those behind the last one as zeros
-    for (int seg = 0; w.more() && ok; w.next(), ++seg) {
-      ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      const int rows = w.s.n * p.group - w.qt * NT;
-      constexpr int kPerRow = D / 8;
-#pragma unroll 4
-      for (int i = lane; i < NT * kPerRow; i += 32) {
-        const int r = i / kPerRow, c = i % kPerRow, at = w.qt * NT + r, token = fast_div(at, p.group_div);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows)
-          v = ld_stream_16(static_cast<const T*>(a.q) + (int64_t)(w.s.start + token) * a.q_token + (w.h * p.group + at - token * p.group) * a.q_head + c * 8);
-        if constexpr (kRowScales) {
-          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&v);
-          float top = 0.f;
+  } else if (warp >= Cfg::kMmaWarp) {
+    if constexpr (Cfg::kGroups > 1) ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
+    // ------------------------------------------------------------------ query rows, those behind the last one as zeros: three warps
+    if (warp != Cfg::kMmaWarp) {
+      constexpr int kPerRow = D / 8, kAtOnce = 8, kLanes = 96;
+      const int first = (warp - Cfg::kQWarp) * 32 + lane;
+      for (int seg = 0; w.more(); w.next(), ++seg) {
+        ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int rows = min(NT, w.s.n * p.group - w.qt * NT);
+#pragma unroll 1
+        for (int i0 = first; i0 - lane < NT * kPerRow; i0 += kAtOnce * kLanes) {
+          uint4 v[kAtOnce];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(x[k])), fabsf(__high2float(x[k]))));
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kLanes, r = min(i / kPerRow, rows - 1), c = i % kPerRow, at = w.qt * NT + r, token = fast_div(at, p.group_div);
+            v[u] = ld_stream_16(static_cast<const T*>(a.q) + (int64_t)(w.s.start + token) * a.q_token + (w.h * p.group + at - token * p.group) * a.q_head + c * 8);
+          }
 #pragma unroll
-          for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
-          const float by = __uint_as_float((uint32_t)(127 + e) << 23);
-          if (c == 0) row_scale[(seg & 1) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
-          uint32_t o[4];
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * kLanes, r = i / kPerRow, c = i % kPerRow;
+            if (r >= rows) v[u] = make_uint4(0, 0, 0, 0);
+            if constexpr (kRowScales) {
+              const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&v[u]);
+              float top = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = pack2<__half>(__low2float(x[k]) * by, __high2float(x[k]) * by);
-          v = make_uint4(o[0], o[1], o[2], o[3]);
+              for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(x[k])), fabsf(__high2float(x[k]))));
+#pragma unroll
+              for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
+              const float by = __uint_as_float((uint32_t)(127 + e) << 23);
+              if (c == 0 && r < NT) row_scale[(seg & 1) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
+              v[u] = make_uint4(pack2<__half>(__low2float(x[0]) * by, __high2float(x[0]) * by), pack2<__half>(__low2float(x[1]) * by, __high2float(x[1]) * by),
+                                pack2<__half>(__low2float(x[2]) * by, __high2float(x[2]) * by), pack2<__half>(__low2float(x[3]) * by, __high2float(x[3]) * by));
+            }
+            if (r < NT) ptx::st_shared_16(sQ + (c >> 3) * (NT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[u]);
+          }
         }
-        ptx::st_shared_16(sQ + (c >> 3) * (NT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(q_full);
       }
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(q_full);
     }
-  } else if (warp == Cfg::kMmaWarp) {
     // ------------------------------------------------------------------ both products
-    if (ptx::elect_one()) {
+    // Operands come by ordinary stores and small copies of other threads. What orders them before the products is this thread's fence behind its wait: a
+    // fence of the threads that bring keys would wait for everything that they have under way (FP8 cache, 64 x 16384: 620 us).
+    if (warp == Cfg::kMmaWarp && ptx::elect_one()) {
       constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kBf16, false, 128, NT), idesc_o = ptx::idesc_f16_f32(kBf16, true, 128, NT);
       constexpr int kPRow = NT >= 64 ? 128 : NT * 2;
       // heads of 64 fill half of the lanes: the other half repeats them
@@ -520,6 +554,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         for (int part = 0; part < kParts; ++part) {
           const uint32_t st = it + 2 * kParts * x + part, s = st % S;
           if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
+          ptx::fence_proxy_async_smem();
           ptx::tc_fence_after();
 #pragma unroll
           for (int k = 0; k < Cfg::kWidth / 16; ++k) {
@@ -540,6 +575,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         for (int part = 0; part < kParts; ++part) {
           const uint32_t st = it + 2 * kParts * x + kParts + part, s = st % S;
           if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
+          ptx::fence_proxy_async_smem();
           ptx::tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
@@ -566,21 +602,13 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   } else {
     // ------------------------------------------------------------------ softmax: a thread per key, and per element of the heads for O^T
     // What a warp decides alone would leave the others at a barrier: after a wait that may have failed all threads of a group decide together.
+    if constexpr (Cfg::kGroups > 1) ptx::give_registers<Cfg::kSoftmaxRegs, Cfg::kLaunchRegs>();
     const int group = warp >> 2, r = threadIdx.x & 127, n0 = group * kCols, bar = 1 + group;
     const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-    constexpr int kChunk = kCols < 32 ? kCols : 32;  // columns in registers
-    auto load = [&](uint32_t at, uint32_t (&v)[32]) {
-      if constexpr (kChunk == 16) {
-        ptx::tmem_ld16(at, v);
-        ptx::tmem_ld_wait16(v);
-      } else {
-        ptx::tmem_ld32(at, v);
-        ptx::tmem_ld_wait(v);
-      }
-    };
     SplitRows begun = {0, 0, 0, 0, 0};
     uint32_t g = 0;
-    for (int seg = 0; w.more() && ok; w.next(), ++seg) {
+    bool stop = false;
+    for (int seg = 0; w.more(); w.next(), ++seg) {
       const Seq& s = w.s;
       const int rows = min(NT, s.n * p.group - w.qt * NT), prefix = s.len - s.n;
       const int first_token = fast_div(w.qt * NT, p.group_div);
@@ -590,71 +618,96 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       float l[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) l[i] = 0.f;
-      if (r < kCols) minus_ref[n0 + r] = INFINITY;  // no reference yet
-      bool odd_values = false;                      // this thread met a value that is not finite among the sequence's own
+      if (r < kCols) {
+        minus_ref[n0 + r] = kNoRef;
+        const int at = w.qt * NT + n0 + r, token = fast_div(at, p.group_div);
+        token_of[n0 + r] = token;
+        out_row[n0 + r] = (s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
+      }
+      ptx::any_of(bar, 128, false);
       for (int t = w.t0; t < w.t1; ++t, ++g) {
         ok = ok && ptx::mbar_wait(s_full(g), (g >> 1) & 1, abort_flag);
         ptx::tc_fence_after();
         const uint32_t ts = lane_base + (g & 1) * NT + n0;
         const int j = t * kKeys + r;  // this thread's key
-        const bool own = j >= prefix && j < s.len;
         // the tile's keys that not every row sees
         const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
-        uint32_t v[32];
-        auto scores = [&](int k) {  // chunk k as exponents, without their reference
-          load(ts + k * kChunk, v);
-          if constexpr (kRowScales) {
+        // bit i: this thread's key, one of the sequence's own, is seen by token first_of_group + i
+        const int first_of_group = fast_div(w.qt * NT + n0, p.group_div);
+        uint64_t seen = 0;
+        if (masked) {
+          const int at = j - prefix, tokens = min(s.n - 1, fast_div(w.qt * NT + n0 + kCols - 1, p.group_div)) - first_of_group + 1;
+          const bool known = at >= 0 && j < s.len && (!a.mask || at < a.mask_width);
+          const uint8_t* column = static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + first_of_group) * a.mask_ld + at;
+          for (int i0 = 0; i0 < tokens; i0 += 8) {
+            uint32_t bit[8];
 #pragma unroll
-            for (int i = 0; i < kChunk; i += 4) {
-              const float4 by = ld_shared_f4(scales + k * kChunk + i);
-              v[i] = __float_as_uint(__uint_as_float(v[i]) * (by.x * c)), v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) * (by.y * c));
-              v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) * (by.z * c)), v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) * (by.w * c));
+            for (int i = 0; i < 8; ++i) {  // (a load behind a branch would be waited for before the next)
+              const bool here = known && i0 + i < tokens;
+              bit[i] = a.mask ? (ptx::ld_byte(here ? column + (i0 + i) * a.mask_ld : static_cast<const uint8_t*>(a.q)) != 0 && here)
+                              : here && at <= first_of_group + i0 + i;
             }
-          } else {
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * c);
+            for (int i = 0; i < 8; ++i) seen |= (uint64_t)bit[i] << (i0 + i);
+          }
+        }
+        float x[kCols];
+        auto exponents = [&](bool over_ref) {  // of this thread's key, with or without their reference
+          if constexpr (kCols == 16) {
+            uint32_t v[32];
+            ptx::tmem_ld16(ts, v);
+            ptx::tmem_ld_wait16(v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(v[i]);
+          } else {
+            uint32_t v[kCols / 32][32];
+#pragma unroll
+            for (int k = 0; k < kCols / 32; ++k) ptx::tmem_ld32(ts + k * 32, v[k]);
+#pragma unroll
+            for (int k = 0; k < kCols / 32; ++k) ptx::tmem_ld_wait(v[k]);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) x[i] = __uint_as_float(v[i / 32][i % 32]);
+          }
+#pragma unroll
+          for (int i = 0; i < kCols; i += 4) {
+            const float4 m = over_ref ? ld_shared_f4(minus_ref + n0 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float4 by = make_float4(c, c, c, c);
+            if constexpr (kRowScales) {
+              by = ld_shared_f4(scales + i);
+              by.x *= c, by.y *= c, by.z *= c, by.w *= c;
+            }
+            ptx::fma_two(x[i], x[i + 1], x[i], x[i + 1], by.x, by.y, m.x, m.y);
+            ptx::fma_two(x[i + 2], x[i + 3], x[i + 2], x[i + 3], by.z, by.w, m.z, m.w);
           }
           if (masked && j >= prefix) {
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-              const int token = fast_div(w.qt * NT + n0 + k * kChunk + i, p.group_div);
-              bool sees = own && token < s.n;
-              if (sees)
-                sees = a.mask ? j - prefix < a.mask_width &&
-                                    static_cast<const volatile uint8_t*>(a.mask)[(int64_t)(s.start + token) * a.mask_ld + j - prefix] != 0
-                              : j - prefix <= token;
-              if (!sees) v[i] = 0xff800000u;
-            }
+            for (int i = 0; i < kCols; ++i)
+              if (!((seen >> (token_of[n0 + i] - first_of_group)) & 1)) x[i] = -INFINITY;
           }
         };
-        float above = -INFINITY;  // largest exponent over its reference
+        exponents(true);
+        float above[2] = {-INFINITY, -INFINITY};  // largest of them
 #pragma unroll
-        for (int k = 0; k < kCols / kChunk; ++k) {
-          scores(k);
-#pragma unroll
-          for (int i = 0; i < kChunk; i += 4) {
-            const float4 m = ld_shared_f4(minus_ref + n0 + k * kChunk + i);
-            above = fmaxf(above, fmaxf(fmaxf(__uint_as_float(v[i]) + m.x, __uint_as_float(v[i + 1]) + m.y),
-                                       fmaxf(__uint_as_float(v[i + 2]) + m.z, __uint_as_float(v[i + 3]) + m.w)));
-          }
+        for (int i = 0; i < kCols; i += 4) {
+          above[0] = ptx::max3(above[0], x[i], x[i + 1]);
+          above[1] = ptx::max3(above[1], x[i + 2], x[i + 3]);
         }
-        if (ptx::any_of(bar, 128, above > kSlack || t == w.t0 || !ok)) {
+        if (ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == w.t0 || !ok)) {
           // Rows whose largest score lies too far above their reference take it as the new one
+          exponents(false);
+          constexpr int kAtOnce = kCols < 32 ? kCols : 32;
 #pragma unroll
-          for (int k = 0; k < kCols / kChunk; ++k) {
-            if (kCols > kChunk) scores(k);
-            float top[kChunk];
+          for (int k = 0; k < kCols; k += kAtOnce) {
+            float top[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) top[i] = __uint_as_float(v[i]);
+            for (int i = 0; i < kAtOnce; ++i) top[i] = x[k + i];
             const float of_lane = across_lanes(top, [](float x, float y) { return fmaxf(x, y); });
-            if (lane < kChunk) by_warp[(warp & 3) * NT + n0 + k * kChunk + lane] = of_lane;
+            if (lane < kAtOnce) by_warp[(warp & 3) * NT + n0 + k + lane] = of_lane;
           }
           const bool moves = t > w.t0;
           if (moves) ok = ok && ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
-          if (ptx::any_of(bar, 128, !ok)) {
-            ok = false;
-            break;
-          }
+          stop = ptx::any_of(bar, 128, !ok);
+          if (stop) break;
           if (r < kCols) {
             const int n = n0 + r;
             const float top = fmaxf(fmaxf(by_warp[n], by_warp[NT + n]), fmaxf(by_warp[2 * NT + n], by_warp[3 * NT + n])), old = -minus_ref[n];
@@ -663,6 +716,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             if (move) minus_ref[n] = -top;
           }
           ptx::any_of(bar, 128, false);
+          exponents(true);
           if (moves) {
 #pragma unroll
             for (int i = 0; i < kCols; i += 4) {
@@ -689,69 +743,49 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         }
         // the buffer of P^T is free when the product that read it is complete
         if (g >= Cfg::kPBufs) ok = ok && ptx::mbar_wait(o_done(g - Cfg::kPBufs), ((g - Cfg::kPBufs) >> 1) & 1, abort_flag);
+        constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
+        const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
+        const uint32_t row = sP + (g % Cfg::kPBufs) * Cfg::kPBytes + (n0 / 64) * (kKeys * 128) + r * kRow;
 #pragma unroll
-        for (int k = 0; k < kCols / kChunk; ++k) {
-          if (kCols > kChunk) scores(k);
-          uint32_t out[kChunk / 2];
+        for (int i = 0; i < kCols; i += 8) {
+          uint32_t out[4];
 #pragma unroll
-          for (int i = 0; i < kChunk; i += 4) {
-            const float4 m = ld_shared_f4(minus_ref + n0 + k * kChunk + i);
-            // a row without a reference has seen nothing: its scores are all -infinity
-            const float e0 = ptx::ex2(__uint_as_float(v[i]) + (m.x < INFINITY ? m.x : 0.f)), e1 = ptx::ex2(__uint_as_float(v[i + 1]) + (m.y < INFINITY ? m.y : 0.f));
-            const float e2 = ptx::ex2(__uint_as_float(v[i + 2]) + (m.z < INFINITY ? m.z : 0.f)), e3 = ptx::ex2(__uint_as_float(v[i + 3]) + (m.w < INFINITY ? m.w : 0.f));
-            out[i / 2] = pack2<M>(e0, e1), out[i / 2 + 1] = pack2<M>(e2, e3);
-            const int n = k * kChunk + i;
-            if constexpr (kBf16) {
-              // the weights as they are multiplied: a row that one key rules comes out as that key's value, without the rounding of its weight
-              l[n] += __uint_as_float(out[i / 2] << 16), l[n + 1] += __uint_as_float(out[i / 2] & 0xffff0000u);
-              l[n + 2] += __uint_as_float(out[i / 2 + 1] << 16), l[n + 3] += __uint_as_float(out[i / 2 + 1] & 0xffff0000u);
-            } else {
-              l[n] += e0, l[n + 1] += e1, l[n + 2] += e2, l[n + 3] += e3;
-            }
+          for (int k = 0; k < 8; k += 2) {
+            const float e0 = ptx::ex2(x[i + k]), e1 = ptx::ex2(x[i + k + 1]);
+            ptx::add_two(l[i + k], l[i + k + 1], e0, e1);
+            out[k / 2] = pack2<M>(e0, e1);
           }
-          constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
-          const uint32_t row = sP + (g % Cfg::kPBufs) * Cfg::kPBytes + ((n0 + k * kChunk) / 64) * (kKeys * 128) + r * kRow;
-          const int piece0 = (n0 + k * kChunk) % 64 / 8;
-#pragma unroll
-          for (int q = 0; q < kChunk / 8; ++q) {
-            const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
-            if (ok) ptx::st_shared_16(row + (((piece0 + q) ^ swizzle) << 4), make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]));
-          }
+          if (ok) ptx::st_shared_16(row + ((((n0 % 64 + i) / 8) ^ swizzle) << 4), make_uint4(out[0], out[1], out[2], out[3]));
         }
-        ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_full(g));
       }
-      if (!ok) break;  // (of the whole group: after its last barrier, or the same for every later one)
+      if (stop) break;
       const bool whole = w.t0 == 0 && w.t1 == s.key_tiles;
       if (!whole && w.t0 == 0)
         begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.key_tiles - w.t1 + line[2] - 1) / line[2])};
       // sums of the weights: over this warp's keys, then over the warps
+      constexpr int kAtOnce = kCols < 32 ? kCols : 32;
 #pragma unroll
-      for (int k = 0; k < kCols / kChunk; ++k) {
-        float part[kChunk];
+      for (int k = 0; k < kCols; k += kAtOnce) {
+        float part[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) part[i] = l[k * kChunk + i];
+        for (int i = 0; i < kAtOnce; ++i) part[i] = l[k + i];
         const float of_lane = across_lanes(part, [](float x, float y) { return x + y; });
-        if (lane < kChunk) by_warp[(warp & 3) * NT + n0 + k * kChunk + lane] = of_lane;
+        if (lane < kAtOnce) by_warp[(warp & 3) * NT + n0 + k + lane] = of_lane;
       }
-      ok = ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
-      if (ptx::any_of(bar, 128, !ok)) {
-        ok = false;
-        break;
-      }
+      ok = ok && ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
+      if (ptx::any_of(bar, 128, !ok)) break;
       ptx::tc_fence_after();
       const int64_t slot0 = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots;
       if (r < kCols) {
-        const int n = n0 + r, at = w.qt * NT + n, token = fast_div(at, p.group_div);
+        const int n = n0 + r;
         const float sum = (by_warp[n] + by_warp[NT + n]) + (by_warp[2 * NT + n] + by_warp[3 * NT + n]), ref = -minus_ref[n];
         factor[n] = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f) / sum;
         if (n < rows) {
           if (!whole) p.part_ml[slot0 + n] = make_float2(ref, sum);
-          else if (a.lse)
-            a.lse[(int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group] =
-                sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+          else if (a.lse) a.lse[out_row[n]] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
         }
       }
       ptx::any_of(bar, 128, false);
@@ -763,14 +797,22 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           uint32_t o[32];
           ptx::tmem_ld16(lane_base + Cfg::kTmemO + part * NT + first, o);
           ptx::tmem_ld_wait16(o);
+          T* const out = static_cast<T*>(a.out) + d;
+          float* const partial = p.part_o + (slot0 + first) * D + d;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int n = first + i, at = w.qt * NT + n, token = fast_div(at, p.group_div);
-            if (n < rows) {
-              // a row that has seen nothing is zero, whatever its weights of zero met
-              const float f = factor[n], x = f == 0.f ? 0.f : __uint_as_float(o[i]);
-              if (whole) static_cast<T*>(a.out)[((int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group) * D + d] = from_f32<T>(x * f);
-              else p.part_o[(slot0 + n) * D + d] = x;
+          for (int i = 0; i < 16; i += 4) {
+            const float4 f = ld_shared_f4(factor + first + i);
+            const int4 to = *reinterpret_cast<const int4*>(out_row + first + i);
+            // a row that has seen nothing is zero, whatever its weights of zero met
+            const float x[4] = {f.x == 0.f ? 0.f : __uint_as_float(o[i]), f.y == 0.f ? 0.f : __uint_as_float(o[i + 1]),
+                                f.z == 0.f ? 0.f : __uint_as_float(o[i + 2]), f.w == 0.f ? 0.f : __uint_as_float(o[i + 3])};
+            const float by[4] = {f.x, f.y, f.z, f.w};
+            const int rows_to[4] = {to.x, to.y, to.z, to.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (first + i + k >= rows) continue;
+              if (whole) out[(int64_t)rows_to[k] * D] = from_f32<T>(x[k] * by[k]);
+              else partial[(i + k) * D] = x[k];
             }
           }
         }
@@ -794,57 +836,119 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   }
 }
 
-// Rows whose keys were cut: a warp per row adds up its pieces, in the order of the line.
+// Rows whose keys were cut: adds up their pieces, in the order of the line. Every block reads the list of cut tiles and takes its share of their rows: eight at a
+// time, a warp each, or where a tile was cut into many pieces one at a time, each warp with some of them.
+constexpr int kManyParts = 8, kJoinBlocks = 296;
 template <typename T, int D, int NT, bool FP8>
-__global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_constant__ AttnParams p, int ctas) {
   const b200_tree_attention_args& a = p.a;
+  constexpr int kPer = D / 32;  // elements per lane
+  __shared__ int ends[256];     // units of work up to each CTA's tile
+  __shared__ int warp_sum[8];
+  __shared__ float part_acc[8][D], part_m[8], part_sum[8];
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, cta = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const volatile int* const from = reinterpret_cast<const volatile int*>(p.split + cta);
-  const int parts = from[4];
-  if (parts == 0) return;
-  const int start = from[0], qt = from[1], h = from[2], row = qt * NT + r;
-  if (r >= NT || row >= from[3]) return;
-  auto slot_of = [&](int i) { return (2 * (int64_t)(cta + i) + (i == 0 ? 1 : 0)) * p.row_slots + r; };
-  auto ml_of = [&](int i) {
-    const volatile float* ml = reinterpret_cast<const volatile float*>(p.part_ml + slot_of(i));
-    return make_float2(ml[0], ml[1]);
-  };
-  float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml_of(i).x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-  constexpr int kPer = D / 32;
-  float sum = 0.f, acc[kPer];
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    float weight = 0.f;
-    if (i0 + lane < parts) {
-      const float2 ml = ml_of(i0 + lane);
-      weight = ptx::ex2(ml.x - ref);
-      sum = fmaf(ml.y, weight, sum);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto field = [&](int cta, int i) { return ld_operand(reinterpret_cast<const int32_t*>(p.split + cta) + i); };
+  auto rows_of = [&](int rows, int qt) { return min(NT, rows - qt * NT); };
+  {
+    int units = 0;
+    if ((int)threadIdx.x < ctas) {
+      const int parts = field(threadIdx.x, 4), rows = rows_of(field(threadIdx.x, 3), field(threadIdx.x, 1));
+      units = parts == 0 ? 0 : parts > kManyParts ? rows : (rows + 7) / 8;
     }
-    const int n = min(32, parts - i0);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float f = __shfl_sync(0xffffffffu, weight, i);
-      const volatile float* src = p.part_o + slot_of(i0 + i) * D + lane * kPer;
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[k] = fmaf(src[k], f, acc[k]);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, units, o);
+      if (lane >= o) units += other;
     }
+    if (lane == 31) warp_sum[warp] = units;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) units += warp_sum[i];
+    ends[threadIdx.x] = units;
+    __syncthreads();
   }
+  const int total = ends[255];
+  for (int unit = blockIdx.x; unit < total; unit += gridDim.x) {
+    int cta = 0;  // the first whose end lies behind the unit
+    for (int step = 128; step > 0; step >>= 1)
+      if (ends[cta + step - 1] <= unit) cta += step;
+    const int index = unit - (cta ? ends[cta - 1] : 0);
+    const int start = field(cta, 0), qt = field(cta, 1), h = field(cta, 2), all = field(cta, 3), parts = field(cta, 4);
+    const bool many = parts > kManyParts;
+    const int r = many ? index : index * 8 + warp;
+    const bool here = r < rows_of(all, qt);
+    const int step = many ? 8 : 1, begin = many ? warp : 0;  // pieces begin, begin + step, ..
+    auto slot_of = [&](int i) { return (2 * (int64_t)(cta + i) + (i == 0 ? 1 : 0)) * p.row_slots + r; };
+    float m = -kNoRef, sum = 0.f, acc[kPer];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const int token = fast_div(row, p.group_div), head = h * p.group + row - token * p.group;
-  const int64_t to = (int64_t)(start + token) * a.q_heads + head;
-  const float inv = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? h : 0)) : 1.f) / sum;
-  T* dst = static_cast<T*>(a.out) + to * D + lane * kPer;
+    for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+    const int mine = here && begin < parts ? (parts - begin + step - 1) / step : 0;
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+      float ref = -kNoRef, l = 0.f;
+      if (i0 + lane < mine) {
+        const float* ml = reinterpret_cast<const float*>(p.part_ml + slot_of(begin + (i0 + lane) * step));
+        ref = ld_operand(ml);
+        l = ld_operand(ml + 1);
+      }
+      float top = fmaxf(ref, m);
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) dst[k] = from_f32<T>(acc[k] * inv);
-  if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float old = ptx::ex2(m - top), weight = ptx::ex2(ref - top);
+      m = top;
+      sum = fmaf(sum, old, l * weight);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] *= old;
+      const int n = min(32, mine - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float f = __shfl_sync(0xffffffffu, weight, i);
+        const float* src = p.part_o + slot_of(begin + (i0 + i) * step) * D + lane * kPer;
+        float x[kPer];
+        if constexpr (kPer == 2) {
+          x[0] = ld_operand(src), x[1] = ld_operand(src + 1);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kPer; k += 4) {
+            const float4 v = ld_operand(reinterpret_cast<const float4*>(src + k));
+            x[k] = v.x, x[k + 1] = v.y, x[k + 2] = v.z, x[k + 3] = v.w;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(x[k], f, acc[k]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (many) {  // over the warps
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) part_acc[warp][lane * kPer + k] = acc[k];
+      if (lane == 0) part_m[warp] = m, part_sum[warp] = sum;
+      __syncthreads();
+      if (warp == 0) {
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, part_m[i]);
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const float f = ptx::ex2(part_m[i] - m);
+          sum = fmaf(part_sum[i], f, sum);
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) acc[k] = fmaf(part_acc[i][lane * kPer + k], f, acc[k]);
+        }
+      }
+    }
+    if (here && (!many || warp == 0)) {
+      const int row = qt * NT + r, token = fast_div(row, p.group_div), head = h * p.group + row - token * p.group;
+      const int64_t to = (int64_t)(start + token) * a.q_heads + head;
+      const float inv = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? h : 0)) : 1.f) / sum;
+      T* dst = static_cast<T*>(a.out) + to * D + lane * kPer;
+#pragma unroll
+      for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
+      if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+    }
+    if (many) __syncthreads();  // the tables have been read
+  }
 }
 
 // Rows of a tile: those of one sequence's new tokens, as far as the host knows their number (the mask's width, else their mean).
@@ -858,7 +962,7 @@ inline int64_t attention_grid(const b200_tree_attention_args& a) {
   const int64_t group = a.q_heads / a.kv_heads, row_tiles = cdiv(a.tokens * group, attention_rows(a)) + a.sequences;
   const int64_t capacity = a.max_pages * a.page_size, key_tiles = capacity > 0 ? cdiv(capacity, kKeys) : 1;
   const double tiles = (double)row_tiles * a.kv_heads * key_tiles;
-  const int sms = sm_count();
+  const int sms = sm_count() < 256 ? sm_count() : 256;  // (as many as the joining kernel has threads)
   return tiles < sms ? (int64_t)tiles : sms;
 }
 inline int attention_row_slots(const b200_tree_attention_args& a) {
@@ -883,8 +987,7 @@ static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
   auto k = tree_attention_kernel<T, D, NT, FP8>;
   if (int rc = allow_smem(k, Cfg::kSmemBytes, "tree_attention_kernel")) return rc;
   if (int rc = launch_dependent(k, dim3((unsigned)grid), Cfg::kThreads, Cfg::kSmemBytes, st, 1, "tree_attention", p)) return rc;
-  return launch_dependent(tree_attention_join_kernel<T, D, NT, FP8>, dim3((unsigned)grid, (unsigned)cdiv(p.row_slots, 8)), 256, 0, st, 1,
-                          "tree_attention", p);
+  return launch_dependent(tree_attention_join_kernel<T, D, NT, FP8>, dim3(kJoinBlocks), 256, 0, st, 1, "tree_attention", p, grid);
 }
 template <typename T, int D, int NT>
 static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
