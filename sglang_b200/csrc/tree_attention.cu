@@ -4,7 +4,8 @@
 // tile and the rows are its columns, so that few rows cost little:
 //   S^T [128 keys, NT] = K Q^T     K and Q in shared memory, S^T in TMEM, two buffers
 //   O^T [D, NT]       += V^T P^T   V as it lies in the cache (its rows are the product's depth), P^T [keys, NT] in shared memory
-// A thread of the softmax has one key and NT columns. It takes its exponentials against a reference per row that is moved only when a score exceeds
+// (More than 64 rows: the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: softmax rows are a
+// thread's own, and P needs no shared memory.) A thread of the softmax has one key and NT columns. It takes its exponentials against a reference per row that is moved only when a score exceeds
 // it by 2^8, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end.
 // Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies (an FP8 cache through registers, where codes become
 // fp16 values, exactly). All tiles of all (sequence, kv head, row tile) form one line that is cut into equal pieces, one per CTA, so that ragged
@@ -26,10 +27,21 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t desc_a, uint64_t de
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same with A in TMEM, two elements a column
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}" ::"r"(d),
+      "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // Instruction descriptor for kind::f16, fp32 sums: bits 4-5 D format (1 = f32), 7-9 / 10-12 A / B format (0 = f16, 1 = bf16), 15 / 16 rows of A / B are
-// the depth, 17-22 N >> 3, 24-28 M >> 4
-__host__ __device__ constexpr uint32_t idesc_f16_f32(bool bf16, bool depth_rows, int M, int N) {
-  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((depth_rows ? 3u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) |
+// the depth (depth_rows: 1, 2), 17-22 N >> 3, 24-28 M >> 4
+__host__ __device__ constexpr uint32_t idesc_f16_f32(bool bf16, uint32_t depth_rows, int M, int N) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | (depth_rows << 15) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
 }
 // Operand of 16-bit elements whose rows are the product's depth: rows of ROW bytes (32, 64 or 128: that swizzle), groups of eight rows one behind the
@@ -135,28 +147,29 @@ template <int D, int NT, bool FP8>
 struct AttnCfg {
   static constexpr int kWidth = D < 128 ? D : 128, kParts = D / kWidth;  // elements of a head in a stage; stages of a tile of keys, or of values
   static constexpr int kStage = kKeys * kWidth * 2;
-  static constexpr int kGroups = NT <= 32 ? 1 : 2;  // softmax warps per 32 keys, each with some of the columns
-  static constexpr int kCols = NT / kGroups;
-  static constexpr int kPBufs = NT * D < 64 * 256 ? 2 : 1;
-  static constexpr int kQBytes = NT * D * 2, kPBytes = kKeys * NT * 2;
-  static constexpr int kTables = NT * 4 * (2 + 1 + 1 + 4 + 1 + 1);  // scales of two segments' rows, references, factors, a value per warp, tokens, rows of the output
-  static constexpr int kFixed = kQBytes + kPBufs * kPBytes + kTables + 1024 + 512;
+  static constexpr bool kRowsInLanes = NT == 128;  // rows in the lanes, keys in the columns, P in TMEM over its own S
+  static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
+  // fp32 words per row: scales of two segments' rows, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
+  static constexpr int kTables = NT * 4 * (kRowsInLanes ? 2 + 2 + 2 + 8 : 2 + 2 + 2 + 8 + 2 + 1);
+  static constexpr int kFixed = kQBytes + 2 * kPBytes + kTables + 1024 + 512;
   static constexpr int kFit = (232448 - kFixed) / kStage;
   static constexpr int kStages = kFit < 12 ? kFit : 12;
-  // Warps: softmax; products, queries and two idle ones; then four that bring keys and four values, with 128 rows four that bring both (registers)
-  static constexpr int kSoftmaxWarps = 4 * kGroups, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 4;
-  // (heads of 256 four that bring both, too: with two stages a tile, warps that run ahead of the others could take a stage's barrier for two phases older)
-  static constexpr bool kSplit = NT <= 64 && kParts == 1;
+  // Warps: two groups of four for the softmax; products and queries; then four that bring keys and four values, or four that bring both (registers; and with
+  // two stages a tile, warps that run ahead of the others could take a stage's barrier for two phases older)
+  static constexpr int kSoftmaxWarps = 8, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 4;
+  static constexpr bool kSplit = NT <= 32 && kParts == 1;
   static constexpr int kThreads = (kProducerWarp + (kSplit ? 8 : 4)) * 32;
-  // Registers of a thread at launch, and of the three kinds of warps where two groups of softmax warps need more than that (0: as launched)
+  // Registers of a thread at launch, and of the three kinds of warps
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-  static constexpr int kSoftmaxRegs = kGroups == 1 ? 0 : kSplit ? 112 : 160, kProducerRegs = kSplit ? 88 : 112, kOtherRegs = 80;
-  static_assert(kGroups == 1 || (8 * kSoftmaxRegs + 4 * kOtherRegs + (kSplit ? 8 : 4) * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
+  static constexpr int kSoftmaxRegs = kSplit ? 112 : 160, kProducerRegs = kSplit ? 88 : 112, kOtherRegs = 80;
+  static_assert((8 * kSoftmaxRegs + 4 * kOtherRegs + (kSplit ? 8 : 4) * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
                 "the registers add up to no more than at launch");
-  static constexpr int kTmemO = 2 * NT, kTmemUsed = (2 + kParts) * NT;  // columns: S^T twice, O^T from here
+  // TMEM columns: the scores of two tiles, then an O for each of the two groups
+  static constexpr int kSCols = kRowsInLanes ? kKeys : NT, kOCols = kRowsInLanes ? D : kParts * NT, kTmemO = 2 * kSCols;
+  static constexpr int kTmemUsed = 2 * kSCols + 2 * kOCols;
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static constexpr size_t kSmemBytes = (size_t)kFixed + (size_t)kStages * kStage;
-  static_assert(kStages >= 2 * kParts + 1 && kTmemUsed <= 512, "a tile of keys and one of values fit");
+  static_assert(kStages >= 2 * kParts && kTmemUsed <= 512, "a tile of values and the keys of the next one fit");
 };
 
 // Sequence b as the kernel takes it: whatever the index tensors hold, tokens and keys stay inside q and the page table.
@@ -261,10 +274,6 @@ __device__ __forceinline__ float across_lanes(const float (&v)[N], F op) {
   }
 }
 
-__device__ __forceinline__ bool not_finite16(uint32_t two, uint32_t exponent) {  // either of two 16-bit values
-  return (two & exponent) == exponent || ((two >> 16) & exponent) == exponent;
-}
-
 template <typename T, int D, int NT, bool FP8>
 __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attention_kernel(const __grid_constant__ AttnParams p) {
   using Cfg = AttnCfg<D, NT, FP8>;
@@ -274,20 +283,22 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   using M = std::conditional_t<FP8, __half, T>;
   constexpr bool kRowScales = FP8 && std::is_same_v<T, __nv_bfloat16>, kBf16 = std::is_same_v<M, __nv_bfloat16>;
   constexpr uint32_t kExponent = kBf16 ? 0x7f80u : 0x7c00u;
-  constexpr int S = Cfg::kStages, kParts = Cfg::kParts, kCols = Cfg::kCols;
+  constexpr int S = Cfg::kStages, kParts = Cfg::kParts;
   const b200_tree_attention_args& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
   constexpr uint32_t kRing = S * Cfg::kStage;
   const uint32_t sKV = smem_base, sQ = smem_base + kRing, sP = sQ + Cfg::kQBytes;
-  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + Cfg::kPBufs * Cfg::kPBytes);  // [2][NT]: of a segment's rows
-  float* minus_ref = row_scale + 2 * NT;                                                                    // [NT]
-  float* factor = minus_ref + NT;                                                                           // [NT]
-  float* by_warp = factor + NT;                                                                             // [4][NT]
-  int* token_of = reinterpret_cast<int*>(by_warp + 4 * NT);                                                 // [NT]
-  int* out_row = token_of + NT;                                                                             // [NT]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(out_row + NT);
+  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes);  // [2][NT]: of a segment's rows
+  float* minus_ref = row_scale + 2 * NT;                                                           // [2][NT]: of each group
+  float* factor = minus_ref + 2 * NT;                                                              // [2][NT]
+  float* by_warp = factor + 2 * NT;                                                                // [8][NT]
+  int* token_of = reinterpret_cast<int*>(by_warp + 8 * NT);                                        // [2][NT]
+  int* out_row = token_of + 2 * NT;                                                                // [NT]
+  uint32_t* seen_words = reinterpret_cast<uint32_t*>(factor);                                      // rows in lanes: [2][NT][4], behind [2][NT] sums
+  if (Cfg::kRowsInLanes) by_warp = factor, seen_words = reinterpret_cast<uint32_t*>(factor + 2 * NT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kTables);
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (S + s); };
@@ -312,7 +323,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(o_done(i), 1);
       ptx::mbar_init(s_full(i), 1);
-      ptx::mbar_init(p_full(i), Cfg::kSoftmaxWarps);
+      ptx::mbar_init(p_full(i), 4);
     }
     *abort_flag = 0;
     *begin_seq = 0;
@@ -372,7 +383,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 
   if (warp >= Cfg::kProducerWarp) {
     // ------------------------------------------------------------------ keys and values into the ring, a tile's keys, then its values
-    if constexpr (Cfg::kGroups > 1) ptx::give_registers<Cfg::kProducerRegs, Cfg::kLaunchRegs>();
+    ptx::give_registers<Cfg::kProducerRegs, Cfg::kLaunchRegs>();
     const int row0 = ((warp - Cfg::kProducerWarp) & 3) * 32;  // 32 keys of a tile, lane l has the addresses of the l-th
     // stages of a tile that are this warp's
     constexpr int kMine = Cfg::kSplit ? kParts : 2 * kParts;
@@ -499,7 +510,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     }
     grid_launch_dependents();
   } else if (warp >= Cfg::kMmaWarp) {
-    if constexpr (Cfg::kGroups > 1) ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
+    ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
     // ------------------------------------------------------------------ query rows, those behind the last one as zeros: three warps
     if (warp != Cfg::kMmaWarp) {
       constexpr int kPerRow = D / 8, kAtOnce = 8, kLanes = 96;
@@ -544,10 +555,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     // Operands come by ordinary stores and small copies of other threads. What orders them before the products is this thread's fence behind its wait: a
     // fence of the threads that bring keys would wait for everything that they have under way (FP8 cache, 64 x 16384: 620 us).
     if (warp == Cfg::kMmaWarp && ptx::elect_one()) {
-      constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kBf16, false, 128, NT), idesc_o = ptx::idesc_f16_f32(kBf16, true, 128, NT);
+      // A tile's scores are asked for before the output of the tile ahead, whose weights its softmax group still computes
+      constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kBf16, 0, 128, Cfg::kSCols);
+      constexpr uint32_t idesc_o = Cfg::kRowsInLanes ? ptx::idesc_f16_f32(kBf16, 2, 128, D) : ptx::idesc_f16_f32(kBf16, 3, 128, NT);
       constexpr int kPRow = NT >= 64 ? 128 : NT * 2;
       // heads of 64 fill half of the lanes: the other half repeats them
-      constexpr uint32_t kNextV = D == 64 ? 0u : kKeys * 128u;
+      constexpr uint32_t kNextV = D == 64 && !Cfg::kRowsInLanes ? 0u : kKeys * 128u;
       uint32_t it = 0, g = 0;  // stages and tiles of this CTA so far
       auto scores = [&](uint32_t x, bool last) {
 #pragma unroll
@@ -559,8 +572,11 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 #pragma unroll
           for (int k = 0; k < Cfg::kWidth / 16; ++k) {
             const uint32_t in_row = (k & 3) * 32, block = k >> 2;
-            ptx::mma_f16(tmem_base + ((g + x) & 1) * NT, ptx::smem_desc_sw128(sKV + s * Cfg::kStage + block * (kKeys * 128) + in_row),
-                         ptx::smem_desc_sw128(sQ + (part * 2 + block) * (NT * 128) + in_row), idesc_s, part > 0 || k > 0);
+            const uint64_t keys = ptx::smem_desc_sw128(sKV + s * Cfg::kStage + block * (kKeys * 128) + in_row);
+            const uint64_t queries = ptx::smem_desc_sw128(sQ + (part * 2 + block) * (NT * 128) + in_row);
+            const uint32_t d = tmem_base + ((g + x) & 1) * Cfg::kSCols;
+            if (Cfg::kRowsInLanes) ptx::mma_f16(d, queries, keys, idesc_s, part > 0 || k > 0);
+            else ptx::mma_f16(d, keys, queries, idesc_s, part > 0 || k > 0);
           }
           ptx::mma_commit(empty_bar(s));
         }
@@ -569,8 +585,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         return true;
       };
       auto output = [&](uint32_t x) {
-        if (!ptx::mbar_wait(p_full(g + x), ((g + x) >> 1) & 1, abort_flag)) return false;
-        const uint32_t weights = sP + ((g + x) % Cfg::kPBufs) * Cfg::kPBytes;
+        const uint32_t own = (g + x) & 1;
+        if (!ptx::mbar_wait(p_full(own), ((g + x) >> 1) & 1, abort_flag)) return false;
+        const uint32_t weights = sP + own * Cfg::kPBytes, o = tmem_base + Cfg::kTmemO + own * Cfg::kOCols;
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
           const uint32_t st = it + 2 * kParts * x + kParts + part, s = st % S;
@@ -578,12 +595,14 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            ptx::mma_f16(tmem_base + Cfg::kTmemO + part * NT, ptx::smem_desc_depth_rows<128>(sKV + s * Cfg::kStage + k * 2048, kNextV),
-                         ptx::smem_desc_depth_rows<kPRow>(weights + k * 16 * kPRow, kKeys * 128), idesc_o, x > 0 || k > 0);
+          for (int k = 0; k < kKeys / 16; ++k) {
+            const uint64_t values = ptx::smem_desc_depth_rows<128>(sKV + s * Cfg::kStage + k * 2048, kNextV);
+            if (Cfg::kRowsInLanes) ptx::mma_f16_ts(o, tmem_base + own * Cfg::kSCols + k * 8, values, idesc_o, x > 1 || k > 0);
+            else ptx::mma_f16(o + part * NT, values, ptx::smem_desc_depth_rows<kPRow>(weights + k * 16 * kPRow, kKeys * 128), idesc_o, x > 1 || k > 0);
+          }
           ptx::mma_commit(empty_bar(s));
         }
-        ptx::mma_commit(o_done(g + x));
+        ptx::mma_commit(o_done(own));
         return true;
       };
       for (int seg = 0; w.more() && ok; w.next(), ++seg) {
@@ -600,225 +619,421 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax: a thread per key, and per element of the heads for O^T
-    // What a warp decides alone would leave the others at a barrier: after a wait that may have failed all threads of a group decide together.
-    if constexpr (Cfg::kGroups > 1) ptx::give_registers<Cfg::kSoftmaxRegs, Cfg::kLaunchRegs>();
-    const int group = warp >> 2, r = threadIdx.x & 127, n0 = group * kCols, bar = 1 + group;
+    // ------------------------------------------------------------------ softmax: two groups of four warps take the tiles in turn, each with references, sums and an
+    // O of its own, so that one computes while the other waits for its products; the two are joined behind a segment's last tile.
+    // What a warp decided alone would leave the others at a barrier: where a wait may have failed, all threads of a group, or all, decide together.
+    ptx::give_registers<Cfg::kSoftmaxRegs, Cfg::kLaunchRegs>();
+    const int group = warp >> 2, r = threadIdx.x & 127, bar = 1 + group;
+    constexpr int kBoth = 3;  // barrier of both groups
     const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_own = lane_base + group * Cfg::kSCols, o_own = lane_base + Cfg::kTmemO + group * Cfg::kOCols;
     SplitRows begun = {0, 0, 0, 0, 0};
-    uint32_t g = 0;
-    bool stop = false;
+    uint32_t g = 0, k = 0;  // tiles of this CTA so far, tiles of this group
     for (int seg = 0; w.more(); w.next(), ++seg) {
       const Seq& s = w.s;
       const int rows = min(NT, s.n * p.group - w.qt * NT), prefix = s.len - s.n;
-      const int first_token = fast_div(w.qt * NT, p.group_div);
+      const int first_token = fast_div(w.qt * NT, p.group_div), last_token = fast_div(w.qt * NT + rows - 1, p.group_div);
+      const float* scales = row_scale + (seg & 1) * NT;
       float c = p.scale_log2;
       if (FP8 && a.k_scale) c *= ld_operand(a.k_scale + (a.k_scales > 1 ? w.h : 0));
-      const float* scales = row_scale + (seg & 1) * NT + n0;
-      float l[kCols];
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) l[i] = 0.f;
-      if (r < kCols) {
-        minus_ref[n0 + r] = kNoRef;
-        const int at = w.qt * NT + n0 + r, token = fast_div(at, p.group_div);
-        token_of[n0 + r] = token;
-        out_row[n0 + r] = (s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
-      }
-      ptx::any_of(bar, 128, false);
-      for (int t = w.t0; t < w.t1; ++t, ++g) {
-        ok = ok && ptx::mbar_wait(s_full(g), (g >> 1) & 1, abort_flag);
-        ptx::tc_fence_after();
-        const uint32_t ts = lane_base + (g & 1) * NT + n0;
-        const int j = t * kKeys + r;  // this thread's key
-        // the tile's keys that not every row sees
-        const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
-        // bit i: this thread's key, one of the sequence's own, is seen by token first_of_group + i
-        const int first_of_group = fast_div(w.qt * NT + n0, p.group_div);
-        uint64_t seen = 0;
-        if (masked) {
-          const int at = j - prefix, tokens = min(s.n - 1, fast_div(w.qt * NT + n0 + kCols - 1, p.group_div)) - first_of_group + 1;
-          const bool known = at >= 0 && j < s.len && (!a.mask || at < a.mask_width);
-          const uint8_t* column = static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + first_of_group) * a.mask_ld + at;
-          for (int i0 = 0; i0 < tokens; i0 += 8) {
-            uint32_t bit[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // (a load behind a branch would be waited for before the next)
-              const bool here = known && i0 + i < tokens;
-              bit[i] = a.mask ? (ptx::ld_byte(here ? column + (i0 + i) * a.mask_ld : static_cast<const uint8_t*>(a.q)) != 0 && here)
-                              : here && at <= first_of_group + i0 + i;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) seen |= (uint64_t)bit[i] << (i0 + i);
-          }
-        }
-        float x[kCols];
-        auto exponents = [&](bool over_ref) {  // of this thread's key, with or without their reference
-          if constexpr (kCols == 16) {
-            uint32_t v[32];
-            ptx::tmem_ld16(ts, v);
-            ptx::tmem_ld_wait16(v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(v[i]);
-          } else {
-            uint32_t v[kCols / 32][32];
-#pragma unroll
-            for (int k = 0; k < kCols / 32; ++k) ptx::tmem_ld32(ts + k * 32, v[k]);
-#pragma unroll
-            for (int k = 0; k < kCols / 32; ++k) ptx::tmem_ld_wait(v[k]);
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) x[i] = __uint_as_float(v[i / 32][i % 32]);
-          }
-#pragma unroll
-          for (int i = 0; i < kCols; i += 4) {
-            const float4 m = over_ref ? ld_shared_f4(minus_ref + n0 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            float4 by = make_float4(c, c, c, c);
-            if constexpr (kRowScales) {
-              by = ld_shared_f4(scales + i);
-              by.x *= c, by.y *= c, by.z *= c, by.w *= c;
-            }
-            ptx::fma_two(x[i], x[i + 1], x[i], x[i + 1], by.x, by.y, m.x, m.y);
-            ptx::fma_two(x[i + 2], x[i + 3], x[i + 2], x[i + 3], by.z, by.w, m.z, m.w);
-          }
-          if (masked && j >= prefix) {
-#pragma unroll
-            for (int i = 0; i < kCols; ++i)
-              if (!((seen >> (token_of[n0 + i] - first_of_group)) & 1)) x[i] = -INFINITY;
-          }
-        };
-        exponents(true);
-        float above[2] = {-INFINITY, -INFINITY};  // largest of them
-#pragma unroll
-        for (int i = 0; i < kCols; i += 4) {
-          above[0] = ptx::max3(above[0], x[i], x[i + 1]);
-          above[1] = ptx::max3(above[1], x[i + 2], x[i + 3]);
-        }
-        if (ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == w.t0 || !ok)) {
-          // Rows whose largest score lies too far above their reference take it as the new one
-          exponents(false);
-          constexpr int kAtOnce = kCols < 32 ? kCols : 32;
-#pragma unroll
-          for (int k = 0; k < kCols; k += kAtOnce) {
-            float top[kAtOnce];
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) top[i] = x[k + i];
-            const float of_lane = across_lanes(top, [](float x, float y) { return fmaxf(x, y); });
-            if (lane < kAtOnce) by_warp[(warp & 3) * NT + n0 + k + lane] = of_lane;
-          }
-          const bool moves = t > w.t0;
-          if (moves) ok = ok && ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
-          stop = ptx::any_of(bar, 128, !ok);
-          if (stop) break;
-          if (r < kCols) {
-            const int n = n0 + r;
-            const float top = fmaxf(fmaxf(by_warp[n], by_warp[NT + n]), fmaxf(by_warp[2 * NT + n], by_warp[3 * NT + n])), old = -minus_ref[n];
-            const bool move = top > old + kSlack;
-            factor[n] = move ? ptx::ex2(old - top) : 1.f;
-            if (move) minus_ref[n] = -top;
-          }
-          ptx::any_of(bar, 128, false);
-          exponents(true);
-          if (moves) {
-#pragma unroll
-            for (int i = 0; i < kCols; i += 4) {
-              const float4 f = ld_shared_f4(factor + n0 + i);
-              l[i] *= f.x, l[i + 1] *= f.y, l[i + 2] *= f.z, l[i + 3] *= f.w;
-            }
-            ptx::tc_fence_after();
+      const bool whole = w.t0 == 0 && w.t1 == s.key_tiles;
+      if (!whole && w.t0 == 0) begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.key_tiles - w.t1 + line[2] - 1) / line[2])};
+      const int64_t slot0 = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots;
+      const float v_scale = FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f;
+      const int mine = w.t0 + (int)((g ^ (uint32_t)group) & 1);  // this group's first tile
+      bool odd_values = false;  // this thread met a value that is not finite among the sequence's own
+
+      // Before the values of tile t are multiplied. Their product with a weight of zero would be NaN where a value is not finite. Those before the sequence's own
+      // tokens every row sees; of its own, which some rows do not, such elements are taken out here and added where they are seen, at the end.
+      auto check_values = [&](int t) {
+        const int j = t * kKeys + r;
+        const uint32_t x = g + (t - w.t0);
 #pragma unroll 1
-            for (int d = 0; d < kParts * kCols; d += 16) {
-              const int part = d / kCols, n = n0 + d - part * kCols;
-              uint32_t o[32], scaled[16];
-              ptx::tmem_ld16(lane_base + Cfg::kTmemO + part * NT + n, o);
-              ptx::tmem_ld_wait16(o);
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t st = 2 * kParts * x + kParts + part;
+          ok = ok && ptx::mbar_wait(full_bar(st % S), (st / S) & 1, abort_flag);
+          if (!ok || j < prefix || j >= s.len) continue;
+#pragma unroll 1
+          for (int c8 = 0; c8 < Cfg::kWidth / 8; ++c8) {
+            const uint32_t at = sKV + (st % S) * Cfg::kStage + (c8 >> 3) * (kKeys * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
+            uint4 v = ptx::ld_shared_16(at);
+            uint32_t word[4] = {v.x, v.y, v.z, v.w}, odd = 0;
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const float4 f = ld_shared_f4(factor + n + i);
-                scaled[i] = __float_as_uint(__uint_as_float(o[i]) * f.x), scaled[i + 1] = __float_as_uint(__uint_as_float(o[i + 1]) * f.y);
-                scaled[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * f.z), scaled[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * f.w);
+            for (int i = 0; i < 4; ++i) {
+              const bool low = (word[i] & kExponent) == kExponent, high = (word[i] >> 16 & kExponent) == kExponent;
+              odd |= low || high;
+              word[i] &= (low ? 0xffff0000u : 0xffffffffu) & (high ? 0xffffu : 0xffffffffu);
+            }
+            if (odd) {
+              odd_values = true;
+              ptx::st_shared_16(at, make_uint4(word[0], word[1], word[2], word[3]));
+            }
+          }
+        }
+      };
+      // Bit i of byte loads: does token first + i see this thread's key j, one of the sequence's own or behind its last
+      auto seen_by = [&](int j, int first, int count) {
+        uint64_t seen = 0;
+        const int at = j - prefix;
+        const bool known = at >= 0 && j < s.len && (!a.mask || at < a.mask_width);
+        const uint8_t* column = static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + first) * a.mask_ld + at;
+        for (int i0 = 0; i0 < count; i0 += 8) {
+          uint32_t bit[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // (a load behind a branch would be waited for before the next)
+            const bool here = known && i0 + i < count;
+            bit[i] = a.mask ? (ptx::ld_byte(here ? column + (i0 + i) * a.mask_ld : static_cast<const uint8_t*>(a.q)) != 0 && here)
+                            : here && at <= first + i0 + i;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) seen |= (uint64_t)bit[i] << (i0 + i);
+        }
+        return seen;
+      };
+
+      if constexpr (!Cfg::kRowsInLanes) {
+        float* const refs = minus_ref + group * NT;  // of this group's references, negated
+        float* const factors = factor + group * NT;
+        float* const warps = by_warp + group * 4 * NT;
+        int* const tokens = token_of + group * NT;
+        constexpr int kChunk = NT < 32 ? NT : 32;  // columns in registers
+        float l[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) l[i] = 0.f;
+        if (r < NT) {
+          refs[r] = kNoRef;
+          tokens[r] = fast_div(w.qt * NT + r, p.group_div);
+        }
+        ptx::any_of(bar, 128, false);
+        for (int t = mine; t < w.t1; t += 2, ++k) {
+          ok = ok && ptx::mbar_wait(s_full(group), k & 1, abort_flag);
+          ptx::tc_fence_after();
+          const int j = t * kKeys + r;  // this thread's key
+          // the tile's keys that not every row sees
+          const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
+          uint64_t seen = 0;
+          if (masked) {
+            seen = seen_by(j, first_token, last_token - first_token + 1);
+            if (s.n > 1 || a.mask) check_values(t);
+          }
+          float x[kChunk];
+          auto exponents = [&](int n0, bool over_ref) {  // of this thread's key and rows n0 .., with or without their reference
+            uint32_t v[32];
+            if constexpr (kChunk == 16) {
+              ptx::tmem_ld16(s_own + n0, v);
+              ptx::tmem_ld_wait16(v);
+            } else {
+              ptx::tmem_ld32(s_own + n0, v);
+              ptx::tmem_ld_wait(v);
+            }
+#pragma unroll
+            for (int i = 0; i < kChunk; i += 4) {
+              const float4 m = over_ref ? ld_shared_f4(refs + n0 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+              float4 by = make_float4(c, c, c, c);
+              if constexpr (kRowScales) {
+                by = ld_shared_f4(scales + n0 + i);
+                by.x *= c, by.y *= c, by.z *= c, by.w *= c;
               }
-              ptx::tmem_st16(lane_base + Cfg::kTmemO + part * NT + n, scaled);
+              ptx::fma_two(x[i], x[i + 1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]), by.x, by.y, m.x, m.y);
+              ptx::fma_two(x[i + 2], x[i + 3], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]), by.z, by.w, m.z, m.w);
+            }
+            if (masked && j >= prefix) {
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i)
+                if (!((seen >> (tokens[n0 + i] - first_token)) & 1)) x[i] = -INFINITY;
+            }
+          };
+          float above[2] = {-INFINITY, -INFINITY};  // largest of them
+#pragma unroll
+          for (int n0 = 0; n0 < NT; n0 += kChunk) {
+            exponents(n0, true);
+#pragma unroll
+            for (int i = 0; i < kChunk; i += 4) {
+              above[0] = ptx::max3(above[0], x[i], x[i + 1]);
+              above[1] = ptx::max3(above[1], x[i + 2], x[i + 3]);
+            }
+          }
+          // the product that read this group's P^T is complete
+          if (k > 0) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+          if (ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == mine || !ok)) {
+            if (ptx::any_of(bar, 128, !ok)) {
+              ok = false;
+              break;
+            }
+            // Rows whose largest score lies too far above their reference take it as the new one
+#pragma unroll
+            for (int n0 = 0; n0 < NT; n0 += kChunk) {
+              exponents(n0, false);
+              const float of_lane = across_lanes(x, [](float x, float y) { return fmaxf(x, y); });
+              if (lane < kChunk) warps[(warp & 3) * NT + n0 + lane] = of_lane;
+            }
+            ptx::any_of(bar, 128, false);
+            if (r < NT) {
+              const float top = fmaxf(fmaxf(warps[r], warps[NT + r]), fmaxf(warps[2 * NT + r], warps[3 * NT + r])), old = -refs[r];
+              const bool move = top > old + kSlack;
+              factors[r] = move ? ptx::ex2(old - top) : 1.f;
+              if (move) refs[r] = -top;
+            }
+            ptx::any_of(bar, 128, false);
+            if (t > mine) {
+#pragma unroll
+              for (int i = 0; i < NT; i += 4) {
+                const float4 f = ld_shared_f4(factors + i);
+                l[i] *= f.x, l[i + 1] *= f.y, l[i + 2] *= f.z, l[i + 3] *= f.w;
+              }
+              ptx::tc_fence_after();
+#pragma unroll 1
+              for (int d = 0; d < kParts * NT; d += 16) {
+                uint32_t o[32], scaled[16];
+                ptx::tmem_ld16(o_own + d, o);
+                ptx::tmem_ld_wait16(o);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                  const float4 f = ld_shared_f4(factors + d % NT + i);
+                  scaled[i] = __float_as_uint(__uint_as_float(o[i]) * f.x), scaled[i + 1] = __float_as_uint(__uint_as_float(o[i + 1]) * f.y);
+                  scaled[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * f.z), scaled[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * f.w);
+                }
+                ptx::tmem_st16(o_own + d, scaled);
+              }
+              ptx::tmem_st_wait();
+            }
+            if (NT == kChunk) exponents(0, true);
+          }
+          constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
+          const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
+          const uint32_t row = sP + group * Cfg::kPBytes + r * kRow;
+#pragma unroll
+          for (int n0 = 0; n0 < NT; n0 += kChunk) {
+            if (NT > kChunk) exponents(n0, true);
+#pragma unroll
+            for (int i = 0; i < kChunk; i += 8) {
+              uint32_t out[4];
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) {
+                const float e0 = ptx::ex2(x[i + e]), e1 = ptx::ex2(x[i + e + 1]);
+                ptx::add_two(l[n0 + i + e], l[n0 + i + e + 1], e0, e1);
+                out[e / 2] = pack2<M>(e0, e1);
+              }
+              ptx::st_shared_16(row + ((((n0 + i) / 8) ^ swizzle) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+            }
+          }
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(p_full(group));
+        }
+        // sums of the weights: over this warp's keys, then over the warps
+#pragma unroll
+        for (int n0 = 0; n0 < NT; n0 += kChunk) {
+          float part[kChunk];
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) part[i] = l[n0 + i];
+          const float of_lane = across_lanes(part, [](float x, float y) { return x + y; });
+          if (lane < kChunk) warps[(warp & 3) * NT + n0 + lane] = of_lane;
+        }
+        if (mine < w.t1) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+        if (ptx::any_of(kBoth, 256, !ok)) break;
+        ptx::tc_fence_after();
+        if (threadIdx.x < NT) {  // both groups' rows on the larger reference
+          const int n = threadIdx.x, at = w.qt * NT + n, token = fast_div(at, p.group_div);
+          const float* b = by_warp + n;
+          const float sum0 = (b[0] + b[NT]) + (b[2 * NT] + b[3 * NT]), sum1 = (b[4 * NT] + b[5 * NT]) + (b[6 * NT] + b[7 * NT]);
+          const float ref0 = -minus_ref[n], ref1 = -minus_ref[NT + n], ref = fmaxf(ref0, ref1);
+          const float f0 = sum0 == 0.f ? 0.f : ptx::ex2(ref0 - ref), f1 = sum1 == 0.f ? 0.f : ptx::ex2(ref1 - ref);
+          const float sum = sum0 * f0 + sum1 * f1, by = whole ? (sum == 0.f ? 0.f : v_scale / sum) : 1.f;
+          factor[n] = f0 * by;
+          factor[NT + n] = f1 * by;
+          out_row[n] = (s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
+          if (n < rows) {
+            if (!whole) p.part_ml[slot0 + n] = make_float2(ref, sum);
+            else if (a.lse) a.lse[out_row[n]] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+          }
+        }
+        ptx::any_of(kBoth, 256, false);
+        if (r < Cfg::kWidth) {
+#pragma unroll 1
+          for (int d0 = group * 16; d0 < kParts * NT; d0 += 32) {  // the groups take every second 16 columns
+            const int part = d0 / NT, first = d0 - part * NT, d = part * 128 + r;
+            if (first >= rows) continue;  // the same for the whole group
+            uint32_t o0[32], o1[32];
+            ptx::tmem_ld16(lane_base + Cfg::kTmemO + d0, o0);
+            ptx::tmem_ld16(lane_base + Cfg::kTmemO + Cfg::kOCols + d0, o1);
+            ptx::tmem_ld_wait16(o0);
+            ptx::tmem_ld_wait16(o1);
+            T* const out = static_cast<T*>(a.out) + d;
+            float* const partial = p.part_o + (slot0 + first) * D + d;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 f0 = ld_shared_f4(factor + first + i), f1 = ld_shared_f4(factor + NT + first + i);
+              const int4 to = *reinterpret_cast<const int4*>(out_row + first + i);
+              // a group that has seen nothing of a row adds nothing, whatever its O holds
+              auto both = [&](uint32_t x0, float y0, uint32_t x1, float y1) {
+                return (y0 == 0.f ? 0.f : __uint_as_float(x0) * y0) + (y1 == 0.f ? 0.f : __uint_as_float(x1) * y1);
+              };
+              const float x[4] = {both(o0[i], f0.x, o1[i], f1.x), both(o0[i + 1], f0.y, o1[i + 1], f1.y), both(o0[i + 2], f0.z, o1[i + 2], f1.z),
+                                  both(o0[i + 3], f0.w, o1[i + 3], f1.w)};
+              const int rows_to[4] = {to.x, to.y, to.z, to.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (first + i + e >= rows) continue;
+                if (whole) out[(int64_t)rows_to[e] * D] = from_f32<T>(x[e]);
+                else partial[(i + e) * D] = x[e];
+              }
+            }
+          }
+        }
+      } else {
+        // A thread per row, 128 keys in its registers: reference and sum are its own
+        const bool busy = (warp & 3) * 32 < rows;  // the same for the whole warp
+        const int at = w.qt * NT + min(r, rows - 1), token = fast_div(at, p.group_div);
+        const int64_t to = (int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
+        uint32_t* const words = seen_words + group * NT * 4;
+        float m = -kNoRef, l = 0.f, scale = c;
+        for (int t = mine; t < w.t1; t += 2, ++k) {
+          ok = ok && ptx::mbar_wait(s_full(group), k & 1, abort_flag);
+          ptx::tc_fence_after();
+          if (kRowScales && t == mine) scale = c * scales[min(r, rows - 1)];
+          const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
+          if (masked) {  // thread r finds out who sees key r; a word per token and 32 keys
+            const int j = t * kKeys + r;
+            for (int i0 = 0; i0 <= last_token - first_token; i0 += 64) {
+              const int count = min(64, last_token - first_token + 1 - i0);
+              const uint64_t seen = seen_by(j, first_token + i0, count);
+              for (int i = 0; i < count; ++i) {
+                const uint32_t word = __ballot_sync(0xffffffffu, j < prefix || ((seen >> i) & 1));
+                if (lane == 0) words[(i0 + i) * 4 + (warp & 3)] = word;
+              }
+            }
+            if (s.n > 1 || a.mask) check_values(t);
+            ptx::any_of(bar, 128, false);
+          }
+          uint32_t v[4][32];
+          if (busy) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ptx::tmem_ld32(s_own + i * 32, v[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ptx::tmem_ld_wait(v[i]);
+            if (masked) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint32_t word = words[(token - first_token) * 4 + q];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[q][i] = (word >> i) & 1u ? v[q][i] : 0xff800000u;
+              }
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = ptx::max3(top[(i >> 1) & 3], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+            const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+            const bool move = largest > m + kSlack;
+            const float old = m;
+            if (move) m = largest;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t out[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float e0, e1;
+                ptx::fma_two(e0, e1, __uint_as_float(v[q][2 * i]), __uint_as_float(v[q][2 * i + 1]), scale, scale, -m, -m);
+                e0 = ptx::ex2(e0), e1 = ptx::ex2(e1);
+                ptx::add_two(sum[(i & 1) * 2], sum[(i & 1) * 2 + 1], e0, e1);
+                out[i] = pack2<M>(e0, e1);
+              }
+              ptx::tmem_st16(s_own + q * 16, out);  // over scores that are in registers
+            }
+            if (k > 0) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+            const float f = move ? ptx::ex2(old - m) : 1.f;
+            l = l * f + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (t > mine && __any_sync(0xffffffffu, move)) {
+              ptx::tc_fence_after();
+#pragma unroll 1
+              for (int d = 0; d < D; d += 16) {
+                uint32_t o[32], scaled[16];
+                ptx::tmem_ld16(o_own + d, o);
+                ptx::tmem_ld_wait16(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) scaled[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                ptx::tmem_st16(o_own + d, scaled);
+              }
             }
             ptx::tmem_st_wait();
           }
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(p_full(group));
         }
-        // the buffer of P^T is free when the product that read it is complete
-        if (g >= Cfg::kPBufs) ok = ok && ptx::mbar_wait(o_done(g - Cfg::kPBufs), ((g - Cfg::kPBufs) >> 1) & 1, abort_flag);
-        constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
-        const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
-        const uint32_t row = sP + (g % Cfg::kPBufs) * Cfg::kPBytes + (n0 / 64) * (kKeys * 128) + r * kRow;
-#pragma unroll
-        for (int i = 0; i < kCols; i += 8) {
-          uint32_t out[4];
-#pragma unroll
-          for (int k = 0; k < 8; k += 2) {
-            const float e0 = ptx::ex2(x[i + k]), e1 = ptx::ex2(x[i + k + 1]);
-            ptx::add_two(l[i + k], l[i + k + 1], e0, e1);
-            out[k / 2] = pack2<M>(e0, e1);
+        if (mine < w.t1) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+        minus_ref[group * NT + r] = m;
+        by_warp[group * NT + r] = l;
+        if (ptx::any_of(kBoth, 256, !ok)) break;
+        ptx::tc_fence_after();
+        if (busy) {
+          const float ref0 = minus_ref[r], ref1 = minus_ref[NT + r], ref = fmaxf(ref0, ref1), sum0 = by_warp[r], sum1 = by_warp[NT + r];
+          float f0 = sum0 == 0.f ? 0.f : ptx::ex2(ref0 - ref), f1 = sum1 == 0.f ? 0.f : ptx::ex2(ref1 - ref);
+          const float sum = sum0 * f0 + sum1 * f1;
+          if (group == 0 && r < rows) {
+            if (!whole) p.part_ml[slot0 + r] = make_float2(ref, sum);
+            else if (a.lse) a.lse[to] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
           }
-          if (ok) ptx::st_shared_16(row + ((((n0 % 64 + i) / 8) ^ swizzle) << 4), make_uint4(out[0], out[1], out[2], out[3]));
-        }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_full(g));
-      }
-      if (stop) break;
-      const bool whole = w.t0 == 0 && w.t1 == s.key_tiles;
-      if (!whole && w.t0 == 0)
-        begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.key_tiles - w.t1 + line[2] - 1) / line[2])};
-      // sums of the weights: over this warp's keys, then over the warps
-      constexpr int kAtOnce = kCols < 32 ? kCols : 32;
-#pragma unroll
-      for (int k = 0; k < kCols; k += kAtOnce) {
-        float part[kAtOnce];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) part[i] = l[k + i];
-        const float of_lane = across_lanes(part, [](float x, float y) { return x + y; });
-        if (lane < kAtOnce) by_warp[(warp & 3) * NT + n0 + k + lane] = of_lane;
-      }
-      ok = ok && ptx::mbar_wait(o_done(g - 1), ((g - 1) >> 1) & 1, abort_flag);
-      if (ptx::any_of(bar, 128, !ok)) break;
-      ptx::tc_fence_after();
-      const int64_t slot0 = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots;
-      if (r < kCols) {
-        const int n = n0 + r;
-        const float sum = (by_warp[n] + by_warp[NT + n]) + (by_warp[2 * NT + n] + by_warp[3 * NT + n]), ref = -minus_ref[n];
-        factor[n] = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f) / sum;
-        if (n < rows) {
-          if (!whole) p.part_ml[slot0 + n] = make_float2(ref, sum);
-          else if (a.lse) a.lse[out_row[n]] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
-        }
-      }
-      ptx::any_of(bar, 128, false);
-      if (r < Cfg::kWidth) {
+          const float by = whole ? (sum == 0.f ? 0.f : v_scale / sum) : 1.f;
+          f0 *= by, f1 *= by;
+          T* const out = static_cast<T*>(a.out) + to * D;
+          float* const partial = p.part_o + (slot0 + r) * D;
 #pragma unroll 1
-        for (int d0 = 0; d0 < kParts * kCols; d0 += 16) {
-          const int part = d0 / kCols, first = n0 + d0 - part * kCols, d = part * 128 + r;
-          if (first >= rows) continue;  // the same for the whole group
-          uint32_t o[32];
-          ptx::tmem_ld16(lane_base + Cfg::kTmemO + part * NT + first, o);
-          ptx::tmem_ld_wait16(o);
-          T* const out = static_cast<T*>(a.out) + d;
-          float* const partial = p.part_o + (slot0 + first) * D + d;
+          for (int d = group * (D / 2); d < (group + 1) * (D / 2); d += 16) {  // half of the row each
+            uint32_t o0[32], o1[32];
+            ptx::tmem_ld16(lane_base + Cfg::kTmemO + d, o0);
+            ptx::tmem_ld16(lane_base + Cfg::kTmemO + Cfg::kOCols + d, o1);
+            ptx::tmem_ld_wait16(o0);
+            ptx::tmem_ld_wait16(o1);
+            float x[16];
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 f = ld_shared_f4(factor + first + i);
-            const int4 to = *reinterpret_cast<const int4*>(out_row + first + i);
-            // a row that has seen nothing is zero, whatever its weights of zero met
-            const float x[4] = {f.x == 0.f ? 0.f : __uint_as_float(o[i]), f.y == 0.f ? 0.f : __uint_as_float(o[i + 1]),
-                                f.z == 0.f ? 0.f : __uint_as_float(o[i + 2]), f.w == 0.f ? 0.f : __uint_as_float(o[i + 3])};
-            const float by[4] = {f.x, f.y, f.z, f.w};
-            const int rows_to[4] = {to.x, to.y, to.z, to.w};
+            for (int i = 0; i < 16; ++i)  // a group that has seen nothing of the row adds nothing, whatever its O holds
+              x[i] = (f0 == 0.f ? 0.f : __uint_as_float(o0[i]) * f0) + (f1 == 0.f ? 0.f : __uint_as_float(o1[i]) * f1);
+            if (r < rows) {
+              if (whole) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (first + i + k >= rows) continue;
-              if (whole) out[(int64_t)rows_to[k] * D] = from_f32<T>(x[k] * by[k]);
-              else partial[(i + k) * D] = x[k];
+                for (int i = 0; i < 16; i += 8)
+                  *reinterpret_cast<uint4*>(out + d + i) =
+                      make_uint4(pack2<T>(x[i], x[i + 1]), pack2<T>(x[i + 2], x[i + 3]), pack2<T>(x[i + 4], x[i + 5]), pack2<T>(x[i + 6], x[i + 7]));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(partial + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+              }
             }
           }
         }
       }
       ptx::tc_fence_before();
-      ptx::any_of(bar, 128, false);  // the tables of this segment have been read
+      // (the barrier also says that this segment's tables have been read)
+      if (ptx::any_of(kBoth, 256, odd_values)) {
+        // Values that were taken out go to the rows that see them: NaN and infinities, whatever their weight
+        const int j1 = min(s.len, w.t1 * kKeys);
+        for (int j = max(max(prefix, 0), w.t0 * kKeys); j < j1; ++j) {
+          const int entry = ld_operand(a.page_table + (int64_t)w.b * a.page_table_ld + fast_div(j, p.page_div));
+          if (entry < 0 || entry >= a.pages) continue;
+          const int in_page = j - fast_div(j, p.page_div) * a.page_size;
+          const int64_t value = entry * a.v_page + in_page * a.v_token + w.h * a.v_head;
+          for (int d = threadIdx.x; d < D; d += 256) {
+            float v;
+            if constexpr (FP8) v = (static_cast<const volatile uint8_t*>(a.v_cache)[value + d] & 0x7f) == 0x7f ? NAN : 0.f;
+            else v = to_f32<T>(static_cast<const T*>(a.v_cache)[value + d]);
+            if (v - v == 0.f) continue;  // finite
+            for (int n = 0; n < rows; ++n) {
+              const int at = w.qt * NT + n, token = fast_div(at, p.group_div), own = j - prefix;
+              if (a.mask ? own >= a.mask_width || ptx::ld_byte(static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + token) * a.mask_ld + own) == 0 : own > token)
+                continue;
+              const int64_t head = (int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
+              if (whole) static_cast<T*>(a.out)[head * D + d] = from_f32<T>(to_f32<T>(static_cast<T*>(a.out)[head * D + d]) + v);
+              else p.part_o[(slot0 + n) * D + d] += v;
+            }
+          }
+        }
+        ptx::any_of(kBoth, 256, false);
+      }
+      g += w.t1 - w.t0;
     }
     if (threadIdx.x == 0) p.split[blockIdx.x] = begun;
   }

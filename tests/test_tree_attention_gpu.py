@@ -343,3 +343,39 @@ def test_device_status_is_clean():
     from sglang_b200 import _native as N
 
     assert N.read_device_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("held", [None, FP8])
+@pytest.mark.parametrize("lens, counts, heads", [([140], [12], 1), ([300, 9], [20, 9], 8), ([70, 1300], [5, 130], 2)])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(lens, counts, heads, held, dim):
+    """A drafted token whose value has NaN or infinities: rows whose mask hides it are what they were, the others get those elements alone."""
+    for mask in (True, False):
+        c = Case(lens, counts, 2 * heads, 2, dim, BF, held, 16, mask)
+        want, lse = c(return_lse=True)
+        for b, (length, n) in enumerate(zip(lens, counts)):
+            own = n - 2  # (its index among the new tokens)
+            j = length - n + own
+            row = c.vc[int(c.table[b, j // 16]), j % 16, 1]
+            if held:
+                row.view(torch.uint8)[5], row.view(torch.uint8)[dim - 1] = 0x7F, 0xFF
+            else:
+                row[5], row[dim - 1], row[8] = math.nan, math.inf, -math.inf
+        got, lse2 = c(return_lse=True)
+        assert torch.equal(lse, lse2)
+        for b, (length, n) in enumerate(zip(lens, counts)):
+            at, own = int(c.starts[b]), n - 2
+            sees = c.visible(b)[:, length - n + own]
+            for i in range(n):
+                g, w = got[at + i], want[at + i]
+                assert torch.equal(g[:heads], w[:heads])  # the other kv head's
+                odd = torch.zeros(dim, dtype=torch.bool, device="cuda")
+                if sees[i]:
+                    odd[[5, dim - 1] if held else [5, dim - 1, 8]] = True
+                    assert torch.isnan(g[heads:, 5]).all()
+                    if not held:
+                        assert (g[heads:, dim - 1] == math.inf).all() and (g[heads:, 8] == -math.inf).all()
+                    else:
+                        assert torch.isnan(g[heads:, dim - 1]).all()
+                # the other elements lose nothing but what the taken-out ones did not add
+                assert torch.equal(g[heads:, ~odd], w[heads:, ~odd])
