@@ -7,8 +7,8 @@
 // (More than 64 rows: the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: softmax rows are a
 // thread's own, and P needs no shared memory.) A thread of the softmax has one key and NT columns. It takes its exponentials against a reference per row that is moved only when a score exceeds
 // it by 2^8, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end.
-// Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies (an FP8 cache through registers, where codes become
-// fp16 values, exactly). All tiles of all (sequence, kv head, row tile) form one line that is cut into equal pieces, one per CTA, so that ragged
+// Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies (of an FP8 cache into a ring of codes, which become
+// fp16 values, exactly, on their way into the ring of tiles). All tiles of all (sequence, kv head, row tile) form one line that is cut into equal pieces, one per CTA, so that ragged
 // lengths leave no SM idle; rows whose keys were cut leave partial sums in a workspace, which a second kernel joins in the line's order.
 #include "gemm_host.cuh"
 #include "int8_round.cuh"
@@ -16,26 +16,46 @@
 namespace b200 {
 namespace ptx {
 
+// Descriptor of an operand in shared memory whose upper half is known at compile time: it takes one register, and steps are 32-bit additions.
+struct Operand {
+  uint32_t low, high;
+  __device__ __forceinline__ Operand at(uint32_t bytes) const { return {low + (bytes >> 4), high}; }
+};
+// Rows of 128 bytes along the depth (K-major), 128-byte swizzle, groups of eight rows one behind the other
+__device__ __forceinline__ Operand operand_sw128(uint32_t addr) {
+  return {(addr >> 4) | (1u << 16), (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29)};
+}
+// Rows that are the depth: ROW bytes (32, 64 or 128: that swizzle) across, groups of eight rows one behind the other, the next ROW / 2 elements across `block`
+// bytes further
+template <int ROW>
+__device__ __forceinline__ Operand operand_depth_rows(uint32_t addr, uint32_t block) {
+  return {(addr >> 4) | ((block >> 4) << 16), (uint32_t)(8 * ROW >> 4) | (1u << 14) | ((ROW == 128 ? 2u : ROW == 64 ? 4u : 6u) << 29)};
+}
 // D (+)= A B with 16-bit operands in shared memory, fp32 sums
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16(uint32_t d, Operand a, Operand b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 a, {%1, %2};\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
       "}" ::"r"(d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      "r"(a.low), "r"(a.high), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // The same with A in TMEM, two elements a column
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, Operand b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      ".reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t"
       "}" ::"r"(d),
-      "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      "r"(a), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // Instruction descriptor for kind::f16, fp32 sums: bits 4-5 D format (1 = f32), 7-9 / 10-12 A / B format (0 = f16, 1 = bf16), 15 / 16 rows of A / B are
@@ -43,13 +63,6 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t desc
 __host__ __device__ constexpr uint32_t idesc_f16_f32(bool bf16, uint32_t depth_rows, int M, int N) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | (depth_rows << 15) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
-}
-// Operand of 16-bit elements whose rows are the product's depth: rows of ROW bytes (32, 64 or 128: that swizzle), groups of eight rows one behind the
-// other, the next ROW / 2 elements across `block` bytes further
-template <int ROW>
-__device__ __forceinline__ uint64_t smem_desc_depth_rows(uint32_t addr, uint32_t block) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(8 * ROW >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)(ROW == 128 ? 2 : ROW == 64 ? 4 : 6) << 61);
 }
 // 16 columns of this thread's lane
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -66,6 +79,11 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint3
 }
 // Arrives once all copies that this thread has issued so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void st_shared_16(uint32_t dst, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -141,7 +159,8 @@ struct AttnParams {
 };
 
 constexpr int kKeys = 128;  // of a tile
-__device__ const uint4 not_a_number = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // in either 16-bit type
+__device__ const uint4 not_a_number16 = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // in either 16-bit type
+__device__ const uint4 not_a_number8 = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
 
 template <int D, int NT, bool FP8>
 struct AttnCfg {
@@ -151,25 +170,31 @@ struct AttnCfg {
   static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
   // fp32 words per row: scales of two segments' rows, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
   static constexpr int kTables = NT * 4 * (kRowsInLanes ? 2 + 2 + 2 + 8 : 2 + 2 + 2 + 8 + 2 + 1);
-  static constexpr int kFixed = kQBytes + 2 * kPBytes + kTables + 1024 + 512;
-  static constexpr int kFit = (232448 - kFixed) / kStage;
-  static constexpr int kStages = kFit < 12 ? kFit : 12;
-  // Warps: two groups of four for the softmax; products and queries; then four that bring keys and four values, or four that bring both (registers; and with
-  // two stages a tile, warps that run ahead of the others could take a stage's barrier for two phases older)
+  // Warps: two groups of four for the softmax; products and queries; then four that bring keys and four values, or, with two stages a tile, four that bring
+  // both (warps that run ahead of the others could take a stage's barrier for two phases older)
   static constexpr int kSoftmaxWarps = 8, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 4;
-  static constexpr bool kSplit = NT <= 32 && kParts == 1;
-  static constexpr int kThreads = (kProducerWarp + (kSplit ? 8 : 4)) * 32;
+  static constexpr bool kSplit = kParts == 1;
+  static constexpr int kProducerWarps = kSplit ? 8 : 4, kThreads = (kProducerWarp + kProducerWarps) * 32;
+  // FP8: codes land in a ring of each producer's own, kRaw stages deep, and go from there into the ring of 16-bit tiles
+  static constexpr int kRawStage = 32 * kWidth, kRaw = !FP8 ? 0 : NT <= 32 ? 2 : 3, kRawBytes = kProducerWarps * kRaw * kRawStage;
+  static constexpr int kFixed = kQBytes + 2 * kPBytes + kRawBytes + kTables + 1024 + 512;
+  static constexpr int kFit = (232448 - kFixed) / kStage;
+  // A wait for a stage's place tells its phase from the one two before it, which has to be over: with keys and values brought by different warps that holds
+  // where each have places of their own (an even number), or from five on, where a warp cannot be that far ahead.
+  static constexpr int kStages = kFit >= 12 ? 12 : FP8 && kSplit ? kFit / 2 * 2 : kFit;
+  static_assert(!kSplit || kStages % 2 == 0 || kStages >= 5, "phases are told apart");
   // Registers of a thread at launch, and of the three kinds of warps
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-  static constexpr int kSoftmaxRegs = kSplit ? 112 : 160, kProducerRegs = kSplit ? 88 : 112, kOtherRegs = 80;
-  static_assert((8 * kSoftmaxRegs + 4 * kOtherRegs + (kSplit ? 8 : 4) * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
+  static constexpr int kSoftmaxRegs = !kSplit ? 160 : NT <= 32 ? 112 : NT == 64 ? 144 : 152;
+  static constexpr int kProducerRegs = !kSplit ? 112 : NT <= 32 ? 72 : 56, kOtherRegs = !kSplit ? 80 : NT <= 32 ? 112 : NT == 64 ? 80 : 64;
+  static_assert((8 * kSoftmaxRegs + 4 * kOtherRegs + kProducerWarps * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
                 "the registers add up to no more than at launch");
   // TMEM columns: the scores of two tiles, then an O for each of the two groups
   static constexpr int kSCols = kRowsInLanes ? kKeys : NT, kOCols = kRowsInLanes ? D : kParts * NT, kTmemO = 2 * kSCols;
   static constexpr int kTmemUsed = 2 * kSCols + 2 * kOCols;
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static constexpr size_t kSmemBytes = (size_t)kFixed + (size_t)kStages * kStage;
-  static_assert(kStages >= 2 * kParts && kTmemUsed <= 512, "a tile of values and the keys of the next one fit");
+  static_assert(kStages >= 2 * kParts && kTmemUsed <= 512 && kSmemBytes <= 232448, "a tile of values and the keys of the next one fit");
 };
 
 // Sequence b as the kernel takes it: whatever the index tensors hold, tokens and keys stay inside q and the page table.
@@ -289,8 +314,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
   constexpr uint32_t kRing = S * Cfg::kStage;
-  const uint32_t sKV = smem_base, sQ = smem_base + kRing, sP = sQ + Cfg::kQBytes;
-  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes);  // [2][NT]: of a segment's rows
+  const uint32_t sKV = smem_base, sQ = smem_base + kRing, sP = sQ + Cfg::kQBytes, sRaw = sP + 2 * Cfg::kPBytes;
+  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kRawBytes);  // [2][NT]: of a segment's rows
   float* minus_ref = row_scale + 2 * NT;                                                           // [2][NT]: of each group
   float* factor = minus_ref + 2 * NT;                                                              // [2][NT]
   float* by_warp = factor + 2 * NT;                                                                // [8][NT]
@@ -298,7 +323,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   int* out_row = token_of + 2 * NT;                                                                // [NT]
   uint32_t* seen_words = reinterpret_cast<uint32_t*>(factor);                                      // rows in lanes: [2][NT][4], behind [2][NT] sums
   if (Cfg::kRowsInLanes) by_warp = factor, seen_words = reinterpret_cast<uint32_t*>(factor + 2 * NT);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kTables);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kRawBytes + Cfg::kTables);
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (S + s); };
@@ -427,93 +452,70 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     auto slot = [&](uint32_t base, int c, int i) {
       return base + (c >> 3) * (kKeys * 128) + my_key * 128 + (((uint32_t)((c & 7) ^ my_key) << 4) ^ (((i * kKeysAtOnce) & 7) << 4)) + i * kKeysAtOnce * 128;
     };
+    // Asks for stage n: into its place in the ring, or as codes into this warp's own
+    auto request = [&](uint32_t n, uint32_t base) {
+      const int part = first_part + n % kMine, kv = part / kParts;
+      if (n % kMine == 0) next_tile();
+      const uint8_t* mine = kv ? from[1] : from[0];
+      const int beside = (part % kParts) * Cfg::kWidth * es;
+      auto to = [&](int i) { return FP8 ? base + i * 512 + lane * 16 : slot(base, my_piece, i); };
+      if ((absent | unknown) == 0) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) ptx::cp_async_16(to(i), address(mine, i) + beside, 16u);
+      } else {
+        const uint8_t* lost = reinterpret_cast<const uint8_t*>(FP8 ? &not_a_number8 : &not_a_number16);
+#pragma unroll 1
+        for (int i = 0; i < kSteps; ++i) {
+          const uint8_t* src = address(mine, i) + beside;
+          const int key = i * kKeysAtOnce + my_key;
+          const bool none = (absent >> key) & 1u, nan = (unknown >> key) & 1u;
+          ptx::cp_async_16(to(i), nan ? lost : none ? static_cast<const uint8_t*>(a.q) : src, none || (nan && kv) ? 0u : 16u);
+        }
+      }
+    };
     if constexpr (!FP8) {
       for (uint32_t n = 0; n < total; ++n) {
-        const int part = first_part + n % kMine, kv = part / kParts;
-        if (n % kMine == 0) next_tile();
         const uint32_t st = stage_of(n), s = st % S;
         ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const uint8_t* mine = kv ? from[1] : from[0];
-        const uint32_t base = sKV + s * Cfg::kStage + row0 * 128;
-        if ((absent | unknown) == 0) {
-#pragma unroll
-          for (int i = 0; i < kSteps; ++i) ptx::cp_async_16(slot(base, my_piece, i), address(mine, i) + (part % kParts) * 256, 16u);
-        } else {
-#pragma unroll 1
-          for (int i = 0; i < kSteps; ++i) {
-            const uint8_t* src = address(mine, i) + (part % kParts) * 256;
-            const int key = i * kKeysAtOnce + my_key;
-            const bool none = (absent >> key) & 1u, nan = (unknown >> key) & 1u;
-            ptx::cp_async_16(slot(base, my_piece, i), nan ? reinterpret_cast<const uint8_t*>(&not_a_number) : none ? static_cast<const uint8_t*>(a.q) : src,
-                             none || (nan && kv) ? 0u : 16u);
-          }
-        }
+        request(n, sKV + s * Cfg::kStage + row0 * 128);
         ptx::cp_async_arrive(full_bar(s));  // when they have landed
       }
-      ptx::cp_async_wait_all();
     } else {
-      // Codes pass through registers: the pieces of kDepth stages are under way, the oldest is widened and stored. Where there is no key to load, something
-      // that exists is, and replaced when it is stored: a load behind a branch would be waited for there.
-      constexpr int kDepth = 2;
-      uint4 raw[kDepth][kSteps];
-      uint32_t no_key[kDepth], no_page[kDepth], asked = 0;
-      auto request = [&](uint4 (&to)[kSteps], uint32_t& missing, uint32_t& lost) {
-        if (asked >= total) return;
-        const int part = first_part + asked % kMine, kv = part / kParts;
-        if (asked % kMine == 0) next_tile();
-        ++asked;
-        missing = absent | unknown;
-        lost = kv ? 0u : unknown;
-        const uint8_t* mine = kv ? from[1] : from[0];
+      // Every lane reads back what it has copied itself. (Codes held in registers on their way took so many that few bytes were under way.)
+      constexpr uint32_t kAhead = Cfg::kRaw - 1;
+      const uint32_t raw = sRaw + (warp - Cfg::kProducerWarp) * Cfg::kRaw * Cfg::kRawStage;
+      for (uint32_t m = 0; m < total + kAhead; ++m) {
+        if (m < total) request(m, raw + m % Cfg::kRaw * Cfg::kRawStage);
+        ptx::cp_async_commit();
+        if (m < kAhead) continue;
+        const uint32_t n = m - kAhead, st = stage_of(n), s = st % S;
+        ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        ptx::cp_async_wait<kAhead>();
+        const uint32_t base = sKV + s * Cfg::kStage + row0 * 128, codes = raw + n % Cfg::kRaw * Cfg::kRawStage + lane * 16;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) to[i] = ld_stream_16(address(mine, i) + (part % kParts) * 128);
-      };
-#pragma unroll
-      for (int u = 0; u < kDepth; ++u) request(raw[u], no_key[u], no_page[u]);
-      uint32_t n = 0;
-      while (n < total && ok) {
-#pragma unroll
-        for (int u = 0; u < kDepth; ++u) {
-          if (n >= total) break;
-          const uint32_t st = stage_of(n), s = st % S;
-          ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          if (no_key[u]) {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-              const int key = i * kKeysAtOnce + my_key;
-              const uint32_t fill = (no_page[u] >> key) & 1u ? 0x7f7f7f7fu : 0u;
-              if ((no_key[u] >> key) & 1u) raw[u][i] = make_uint4(fill, fill, fill, fill);
-            }
-          }
-          const uint32_t base = sKV + s * Cfg::kStage + row0 * 128;
-#pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            uint4 lo, hi;
-            widen4(raw[u][i].x, lo.x, lo.y);
-            widen4(raw[u][i].y, lo.z, lo.w);
-            widen4(raw[u][i].z, hi.x, hi.y);
-            widen4(raw[u][i].w, hi.z, hi.w);
-            ptx::st_shared_16(slot(base, 2 * my_piece, i), lo);
-            ptx::st_shared_16(slot(base, 2 * my_piece + 1, i), hi);
-          }
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(full_bar(s));
-          ++n;
-          request(raw[u], no_key[u], no_page[u]);
+        for (int i = 0; i < kSteps; ++i) {
+          const uint4 v = ptx::ld_shared_16(codes + i * 512);
+          uint4 lo, hi;
+          widen4(v.x, lo.x, lo.y);
+          widen4(v.y, lo.z, lo.w);
+          widen4(v.z, hi.x, hi.y);
+          widen4(v.w, hi.z, hi.w);
+          ptx::st_shared_16(slot(base, 2 * my_piece, i), lo);
+          ptx::st_shared_16(slot(base, 2 * my_piece + 1, i), hi);
         }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(full_bar(s));
       }
     }
+    ptx::cp_async_wait_all();
     grid_launch_dependents();
   } else if (warp >= Cfg::kMmaWarp) {
     ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
     // ------------------------------------------------------------------ query rows, those behind the last one as zeros: three warps
     if (warp != Cfg::kMmaWarp) {
-      constexpr int kPerRow = D / 8, kAtOnce = 8, kLanes = 96;
+      constexpr int kPerRow = D / 8, kAtOnce = 4, kLanes = 96;
       const int first = (warp - Cfg::kQWarp) * 32 + lane;
       for (int seg = 0; w.more(); w.next(), ++seg) {
         ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
@@ -569,14 +571,14 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_after();
+          const ptx::Operand keys = ptx::operand_sw128(sKV + s * Cfg::kStage), queries = ptx::operand_sw128(sQ + part * 2 * (NT * 128));
+          const uint32_t d = tmem_base + ((g + x) & 1) * Cfg::kSCols;
 #pragma unroll
           for (int k = 0; k < Cfg::kWidth / 16; ++k) {
             const uint32_t in_row = (k & 3) * 32, block = k >> 2;
-            const uint64_t keys = ptx::smem_desc_sw128(sKV + s * Cfg::kStage + block * (kKeys * 128) + in_row);
-            const uint64_t queries = ptx::smem_desc_sw128(sQ + (part * 2 + block) * (NT * 128) + in_row);
-            const uint32_t d = tmem_base + ((g + x) & 1) * Cfg::kSCols;
-            if (Cfg::kRowsInLanes) ptx::mma_f16(d, queries, keys, idesc_s, part > 0 || k > 0);
-            else ptx::mma_f16(d, keys, queries, idesc_s, part > 0 || k > 0);
+            const ptx::Operand kk = keys.at(block * (kKeys * 128) + in_row), qq = queries.at(block * (NT * 128) + in_row);
+            if (Cfg::kRowsInLanes) ptx::mma_f16(d, qq, kk, idesc_s, part > 0 || k > 0);
+            else ptx::mma_f16(d, kk, qq, idesc_s, part > 0 || k > 0);
           }
           ptx::mma_commit(empty_bar(s));
         }
@@ -587,18 +589,19 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       auto output = [&](uint32_t x) {
         const uint32_t own = (g + x) & 1;
         if (!ptx::mbar_wait(p_full(own), ((g + x) >> 1) & 1, abort_flag)) return false;
-        const uint32_t weights = sP + own * Cfg::kPBytes, o = tmem_base + Cfg::kTmemO + own * Cfg::kOCols;
+        const uint32_t o = tmem_base + Cfg::kTmemO + own * Cfg::kOCols;
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
           const uint32_t st = it + 2 * kParts * x + kParts + part, s = st % S;
           if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_after();
+          const ptx::Operand values = ptx::operand_depth_rows<128>(sKV + s * Cfg::kStage, kNextV);
+          const ptx::Operand weights = ptx::operand_depth_rows<kPRow>(sP + own * Cfg::kPBytes, kKeys * 128);
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) {
-            const uint64_t values = ptx::smem_desc_depth_rows<128>(sKV + s * Cfg::kStage + k * 2048, kNextV);
-            if (Cfg::kRowsInLanes) ptx::mma_f16_ts(o, tmem_base + own * Cfg::kSCols + k * 8, values, idesc_o, x > 1 || k > 0);
-            else ptx::mma_f16(o + part * NT, values, ptx::smem_desc_depth_rows<kPRow>(weights + k * 16 * kPRow, kKeys * 128), idesc_o, x > 1 || k > 0);
+            if (Cfg::kRowsInLanes) ptx::mma_f16_ts(o, tmem_base + own * Cfg::kSCols + k * 8, values.at(k * 2048), idesc_o, x > 1 || k > 0);
+            else ptx::mma_f16(o + part * NT, values.at(k * 2048), weights.at(k * 16 * kPRow), idesc_o, x > 1 || k > 0);
           }
           ptx::mma_commit(empty_bar(s));
         }
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         float* const factors = factor + group * NT;
         float* const warps = by_warp + group * 4 * NT;
         int* const tokens = token_of + group * NT;
-        constexpr int kChunk = NT < 32 ? NT : 32;  // columns in registers
+        constexpr int kChunk = NT == 64 ? 32 : 16;  // columns in registers
         float l[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) l[i] = 0.f;
@@ -1170,7 +1173,7 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_c
 inline int attention_rows(const b200_tree_attention_args& a) {
   const int64_t n = a.q_starts == nullptr ? 1 : a.mask ? a.mask_width : cdiv(a.tokens, a.sequences);
   const int64_t rows = (n < 1 ? 1 : n) * (a.q_heads / a.kv_heads);
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || a.dim > 128 ? 64 : 128;  // 128 rows of 256 leave no room for the ring
+  return rows <= 16 ? 16 : rows <= 32 || a.dim > 128 ? 32 : rows <= 64 ? 64 : 128;  // more rows of 256 leave no room for the ring
 }
 // CTAs of a call: no more than there can be tiles
 inline int64_t attention_grid(const b200_tree_attention_args& a) {
@@ -1213,7 +1216,9 @@ static int launch_attention(const AttnParams& p, int grid, cudaStream_t st) {
   switch (attention_rows(p.a)) {
     case 16: return launch_attention<T, D, 16>(p, grid, st);
     case 32: return launch_attention<T, D, 32>(p, grid, st);
-    case 64: return launch_attention<T, D, 64>(p, grid, st);
+    case 64:
+      if constexpr (D <= 128) return launch_attention<T, D, 64>(p, grid, st);
+      return B200_E_UNSUPPORTED;
     default:
       if constexpr (D <= 128) return launch_attention<T, D, 128>(p, grid, st);
       return B200_E_UNSUPPORTED;
