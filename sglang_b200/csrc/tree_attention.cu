@@ -186,7 +186,7 @@ struct AttnCfg {
   // Registers of a thread at launch, and of the three kinds of warps
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
   static constexpr int kSoftmaxRegs = !kSplit ? 160 : NT <= 32 ? 112 : NT == 64 ? 144 : 152;
-  static constexpr int kProducerRegs = !kSplit ? 112 : NT <= 32 ? 72 : 56, kOtherRegs = !kSplit ? 80 : NT <= 32 ? 112 : NT == 64 ? 80 : 64;
+  static constexpr int kProducerRegs = !kSplit ? 112 : NT <= 32 ? 88 : 56, kOtherRegs = !kSplit ? 80 : NT <= 64 ? 80 : 64;
   static_assert((8 * kSoftmaxRegs + 4 * kOtherRegs + kProducerWarps * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
                 "the registers add up to no more than at launch");
   // TMEM columns: the scores of two tiles, then an O for each of the two groups
