@@ -166,7 +166,11 @@ template <int D, int NT, bool FP8>
 struct AttnCfg {
   static constexpr int kWidth = D < 128 ? D : 128, kParts = D / kWidth;  // elements of a head in a stage; stages of a tile of keys, or of values
   static constexpr int kStage = kKeys * kWidth * 2;
-  static constexpr bool kRowsInLanes = NT == 128;  // rows in the lanes, keys in the columns, P in TMEM over its own S
+  // What the two groups of softmax warps share: up to 32 rows they take the tiles in turn, each with an O of its own, so that one computes while the other
+  // waits for its products; with 64 each has half of the rows of every tile; with 128 the rows are in the lanes, P lies in TMEM over its own S, and each has
+  // half of the keys of every tile, for all rows, and an O of its own.
+  static constexpr bool kRowsInLanes = NT == 128, kTurns = NT <= 32, kTwoO = NT != 64;
+  static constexpr int kCols = kTurns ? NT : NT / 2;  // columns of a softmax thread
   static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
   // fp32 words per row: scales of two segments' rows, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
   static constexpr int kTables = NT * 4 * (kRowsInLanes ? 2 + 2 + 2 + 8 : 2 + 2 + 2 + 8 + 2 + 1);
@@ -185,13 +189,12 @@ struct AttnCfg {
   static_assert(!kSplit || kStages % 2 == 0 || kStages >= 5, "phases are told apart");
   // Registers of a thread at launch, and of the three kinds of warps
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-  static constexpr int kSoftmaxRegs = !kSplit ? 160 : NT <= 32 ? 112 : NT == 64 ? 144 : 152;
-  static constexpr int kProducerRegs = !kSplit ? 112 : NT <= 32 ? 88 : 56, kOtherRegs = !kSplit ? 80 : NT <= 64 ? 80 : 64;
+  static constexpr int kSoftmaxRegs = kSplit ? 112 : 160, kProducerRegs = kSplit ? 88 : 112, kOtherRegs = 80;
   static_assert((8 * kSoftmaxRegs + 4 * kOtherRegs + kProducerWarps * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
                 "the registers add up to no more than at launch");
   // TMEM columns: the scores of two tiles, then an O for each of the two groups
   static constexpr int kSCols = kRowsInLanes ? kKeys : NT, kOCols = kRowsInLanes ? D : kParts * NT, kTmemO = 2 * kSCols;
-  static constexpr int kTmemUsed = 2 * kSCols + 2 * kOCols;
+  static constexpr int kTmemUsed = 2 * kSCols + (kTwoO ? 2 : 1) * kOCols;
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static constexpr size_t kSmemBytes = (size_t)kFixed + (size_t)kStages * kStage;
   static_assert(kStages >= 2 * kParts && kTmemUsed <= 512 && kSmemBytes <= 232448, "a tile of values and the keys of the next one fit");
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(o_done(i), 1);
       ptx::mbar_init(s_full(i), 1);
-      ptx::mbar_init(p_full(i), 4);
+      ptx::mbar_init(p_full(i), Cfg::kTurns ? 4 : 8);
     }
     *abort_flag = 0;
     *begin_seq = 0;
@@ -422,7 +425,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       if (!at.more() || j >= at.s.len) return -1;
       return (int)ld_operand(a.page_table + (int64_t)at.b * a.page_table_ld + fast_div(j, p.page_div));
     };
-    const uint8_t* from[2];       // this lane's key and its value; something readable where there is none
+    // this lane's key and its value; something readable where there is none. Warps that bring one of them know that one alone.
+    const uint8_t* from[Cfg::kSplit ? 1 : 2];
+    const bool values = Cfg::kSplit && first_part > 0;
     uint32_t absent, unknown;     // a bit per lane: no key there; a page that the cache does not have
     int t = w.t0, entry = entry_of(w, t);
     auto next_tile = [&] {
@@ -430,11 +435,13 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       const bool key = j < w.s.len, page = entry >= 0 && entry < a.pages;
       absent = __ballot_sync(0xffffffffu, !key);
       unknown = __ballot_sync(0xffffffffu, key && !page);
-      from[0] = from[1] = static_cast<const uint8_t*>(a.q);
-      if (key && page) {
-        from[0] = static_cast<const uint8_t*>(a.k_cache) + (entry * a.k_page + in_page * a.k_token + w.h * a.k_head) * es;
-        from[1] = static_cast<const uint8_t*>(a.v_cache) + (entry * a.v_page + in_page * a.v_token + w.h * a.v_head) * es;
-      }
+      const uint8_t* const some = static_cast<const uint8_t*>(a.q);
+      const bool have = key && page;
+      from[0] = have ? static_cast<const uint8_t*>(values ? a.v_cache : a.k_cache) +
+                           (entry * (values ? a.v_page : a.k_page) + in_page * (values ? a.v_token : a.k_token) + w.h * (values ? a.v_head : a.k_head)) * es
+                     : some;
+      if constexpr (!Cfg::kSplit)
+        from[1] = have ? static_cast<const uint8_t*>(a.v_cache) + (entry * a.v_page + in_page * a.v_token + w.h * a.v_head) * es : some;
       if (++t == w.t1) {
         w.next();
         t = w.t0;
@@ -443,8 +450,11 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     };
     const uint32_t total = kMine * (uint32_t)line[1];  // stages of this warp
     auto stage_of = [&](uint32_t n) { return (n / kMine) * 2 * kParts + first_part + n % kMine; };
-    // Step i of a stage: key i * kKeysAtOnce + lane / kPieces of this warp's, piece lane % kPieces
-    const int my_key = lane / kPieces, my_piece = lane % kPieces;
+    // Step i of a stage: key i * kKeysAtOnce + my_key of this warp's, piece my_piece. (Eight codes of a piece become 16 bytes and go to every second place of a
+    // 128-byte row: eight lanes store to all of the banks if they have four pieces of two keys.)
+    constexpr bool kInterleave = FP8 && kPieces == 8;
+    const int my_key = kInterleave ? ((lane >> 2) & 1) | (lane >> 4 << 1) : lane / kPieces;
+    const int my_piece = kInterleave ? (lane & 3) | ((lane >> 3) & 1) << 2 : lane % kPieces;
     auto address = [&](const uint8_t* mine, int i) {
       return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i * kKeysAtOnce + my_key)) + my_piece * 16;
     };
@@ -456,7 +466,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     auto request = [&](uint32_t n, uint32_t base) {
       const int part = first_part + n % kMine, kv = part / kParts;
       if (n % kMine == 0) next_tile();
-      const uint8_t* mine = kv ? from[1] : from[0];
+      const uint8_t* mine = from[0];
+      if constexpr (!Cfg::kSplit) mine = kv ? from[1] : from[0];
       const int beside = (part % kParts) * Cfg::kWidth * es;
       auto to = [&](int i) { return FP8 ? base + i * 512 + lane * 16 : slot(base, my_piece, i); };
       if ((absent | unknown) == 0) {
@@ -589,7 +600,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       auto output = [&](uint32_t x) {
         const uint32_t own = (g + x) & 1;
         if (!ptx::mbar_wait(p_full(own), ((g + x) >> 1) & 1, abort_flag)) return false;
-        const uint32_t o = tmem_base + Cfg::kTmemO + own * Cfg::kOCols;
+        const uint32_t o = tmem_base + Cfg::kTmemO + (Cfg::kTurns ? own * Cfg::kOCols : 0);
+        const uint32_t before = x > (Cfg::kTurns ? 1 : 0);  // O holds earlier tiles
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
           const uint32_t st = it + 2 * kParts * x + kParts + part, s = st % S;
@@ -600,8 +612,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           const ptx::Operand weights = ptx::operand_depth_rows<kPRow>(sP + own * Cfg::kPBytes, kKeys * 128);
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) {
-            if (Cfg::kRowsInLanes) ptx::mma_f16_ts(o, tmem_base + own * Cfg::kSCols + k * 8, values.at(k * 2048), idesc_o, x > 1 || k > 0);
-            else ptx::mma_f16(o + part * NT, values.at(k * 2048), weights.at(k * 16 * kPRow), idesc_o, x > 1 || k > 0);
+            if (Cfg::kRowsInLanes)  // each half of the keys into its own O
+              ptx::mma_f16_ts(o + (k >> 2) * Cfg::kOCols, tmem_base + own * Cfg::kSCols + (k >> 2) * 64 + (k & 3) * 8, values.at(k * 2048), idesc_o, before || (k & 3));
+            else ptx::mma_f16(o + part * NT, values.at(k * 2048), weights.at(k * 16 * kPRow), idesc_o, before || k > 0);
           }
           ptx::mma_commit(empty_bar(s));
         }
@@ -622,16 +635,16 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax: two groups of four warps take the tiles in turn, each with references, sums and an
-    // O of its own, so that one computes while the other waits for its products; the two are joined behind a segment's last tile.
+    // ------------------------------------------------------------------ softmax: two groups of four warps
     // What a warp decided alone would leave the others at a barrier: where a wait may have failed, all threads of a group, or all, decide together.
     ptx::give_registers<Cfg::kSoftmaxRegs, Cfg::kLaunchRegs>();
     const int group = warp >> 2, r = threadIdx.x & 127, bar = 1 + group;
     constexpr int kBoth = 3;  // barrier of both groups
+    constexpr int kStep = Cfg::kTurns ? 2 : 1, kCols = Cfg::kCols;
     const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_own = lane_base + group * Cfg::kSCols, o_own = lane_base + Cfg::kTmemO + group * Cfg::kOCols;
+    const uint32_t o_own = lane_base + Cfg::kTmemO + (Cfg::kTwoO ? group * Cfg::kOCols : group * kCols);
     SplitRows begun = {0, 0, 0, 0, 0};
-    uint32_t g = 0, k = 0;  // tiles of this CTA so far, tiles of this group
+    uint32_t g = 0;  // tiles of this CTA so far
     for (int seg = 0; w.more(); w.next(), ++seg) {
       const Seq& s = w.s;
       const int rows = min(NT, s.n * p.group - w.qt * NT), prefix = s.len - s.n;
@@ -643,7 +656,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       if (!whole && w.t0 == 0) begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.key_tiles - w.t1 + line[2] - 1) / line[2])};
       const int64_t slot0 = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots;
       const float v_scale = FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f;
-      const int mine = w.t0 + (int)((g ^ (uint32_t)group) & 1);  // this group's first tile
+      const int mine = w.t0 + (Cfg::kTurns ? (int)((g ^ (uint32_t)group) & 1) : 0);  // this group's first tile
       bool odd_values = false;  // this thread met a value that is not finite among the sequence's own
 
       // Before the values of tile t are multiplied. Their product with a weight of zero would be NaN where a value is not finite. Those before the sequence's own
@@ -651,6 +664,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       auto check_values = [&](int t) {
         const int j = t * kKeys + r;
         const uint32_t x = g + (t - w.t0);
+        if (!Cfg::kTurns && group != 0) return;  // one group looks at a tile
 #pragma unroll 1
         for (int part = 0; part < kParts; ++part) {
           const uint32_t st = 2 * kParts * x + kParts + part;
@@ -694,22 +708,30 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         return seen;
       };
 
+      auto wait_for_output = [&] {  // the products with this segment's last tiles
+        const uint32_t last = g + (w.t1 - w.t0) - 1;
+        if (last >= 1 && w.t1 - w.t0 > 1) ok = ok && ptx::mbar_wait(o_done(last - 1), ((last - 1) >> 1) & 1, abort_flag);
+        ok = ok && ptx::mbar_wait(o_done(last), (last >> 1) & 1, abort_flag);
+      };
+
       if constexpr (!Cfg::kRowsInLanes) {
-        float* const refs = minus_ref + group * NT;  // of this group's references, negated
-        float* const factors = factor + group * NT;
-        float* const warps = by_warp + group * 4 * NT;
-        int* const tokens = token_of + group * NT;
-        constexpr int kChunk = NT == 64 ? 32 : 16;  // columns in registers
-        float l[NT];
+        float* const refs = minus_ref + group * kCols;  // of this group's references, negated
+        float* const factors = factor + group * kCols;
+        float* const warps = by_warp + group * 4 * kCols;
+        int* const tokens = token_of + group * kCols;
+        const int n0 = Cfg::kTurns ? 0 : group * kCols;  // this group's first row
+        float l[kCols];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) l[i] = 0.f;
-        if (r < NT) {
+        for (int i = 0; i < kCols; ++i) l[i] = 0.f;
+        if (r < kCols) {
           refs[r] = kNoRef;
-          tokens[r] = fast_div(w.qt * NT + r, p.group_div);
+          tokens[r] = fast_div(w.qt * NT + n0 + r, p.group_div);
         }
         ptx::any_of(bar, 128, false);
-        for (int t = mine; t < w.t1; t += 2, ++k) {
-          ok = ok && ptx::mbar_wait(s_full(group), k & 1, abort_flag);
+        for (int t = mine; t < w.t1; t += kStep) {
+          const uint32_t x_tile = g + (t - w.t0), own = x_tile & 1, phase = x_tile >> 1;
+          const uint32_t s_own = lane_base + own * Cfg::kSCols + n0;
+          ok = ok && ptx::mbar_wait(s_full(own), phase & 1, abort_flag);
           ptx::tc_fence_after();
           const int j = t * kKeys + r;  // this thread's key
           // the tile's keys that not every row sees
@@ -719,19 +741,19 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             seen = seen_by(j, first_token, last_token - first_token + 1);
             if (s.n > 1 || a.mask) check_values(t);
           }
-          float x[kChunk];
-          auto exponents = [&](int n0, bool over_ref) {  // of this thread's key and rows n0 .., with or without their reference
+          float x[kCols];
+          auto exponents = [&](bool over_ref) {  // of this thread's key and this group's rows, with or without their reference
             uint32_t v[32];
-            if constexpr (kChunk == 16) {
-              ptx::tmem_ld16(s_own + n0, v);
+            if constexpr (kCols == 16) {
+              ptx::tmem_ld16(s_own, v);
               ptx::tmem_ld_wait16(v);
             } else {
-              ptx::tmem_ld32(s_own + n0, v);
+              ptx::tmem_ld32(s_own, v);
               ptx::tmem_ld_wait(v);
             }
 #pragma unroll
-            for (int i = 0; i < kChunk; i += 4) {
-              const float4 m = over_ref ? ld_shared_f4(refs + n0 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < kCols; i += 4) {
+              const float4 m = over_ref ? ld_shared_f4(refs + i) : make_float4(0.f, 0.f, 0.f, 0.f);
               float4 by = make_float4(c, c, c, c);
               if constexpr (kRowScales) {
                 by = ld_shared_f4(scales + n0 + i);
@@ -742,105 +764,94 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             }
             if (masked && j >= prefix) {
 #pragma unroll
-              for (int i = 0; i < kChunk; ++i)
-                if (!((seen >> (tokens[n0 + i] - first_token)) & 1)) x[i] = -INFINITY;
+              for (int i = 0; i < kCols; ++i)
+                if (!((seen >> (tokens[i] - first_token)) & 1)) x[i] = -INFINITY;
             }
           };
+          exponents(true);
           float above[2] = {-INFINITY, -INFINITY};  // largest of them
 #pragma unroll
-          for (int n0 = 0; n0 < NT; n0 += kChunk) {
-            exponents(n0, true);
-#pragma unroll
-            for (int i = 0; i < kChunk; i += 4) {
-              above[0] = ptx::max3(above[0], x[i], x[i + 1]);
-              above[1] = ptx::max3(above[1], x[i + 2], x[i + 3]);
-            }
+          for (int i = 0; i < kCols; i += 4) {
+            above[0] = ptx::max3(above[0], x[i], x[i + 1]);
+            above[1] = ptx::max3(above[1], x[i + 2], x[i + 3]);
           }
-          // the product that read this group's P^T is complete
-          if (k > 0) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+          // the product that read this buffer of P^T is complete (with tiles in turn it is the last one that this group's O was in)
+          if (x_tile >= 2) ok = ok && ptx::mbar_wait(o_done(own), (phase - 1) & 1, abort_flag);
           if (ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == mine || !ok)) {
+            // Rows whose largest score lies too far above their reference take it as the new one
+            const bool moves = t > mine;
+            if (moves && !Cfg::kTurns) ok = ok && ptx::mbar_wait(o_done(own ^ 1), ((x_tile - 1) >> 1) & 1, abort_flag);
             if (ptx::any_of(bar, 128, !ok)) {
               ok = false;
               break;
             }
-            // Rows whose largest score lies too far above their reference take it as the new one
-#pragma unroll
-            for (int n0 = 0; n0 < NT; n0 += kChunk) {
-              exponents(n0, false);
-              const float of_lane = across_lanes(x, [](float x, float y) { return fmaxf(x, y); });
-              if (lane < kChunk) warps[(warp & 3) * NT + n0 + lane] = of_lane;
-            }
+            exponents(false);
+            const float of_lane = across_lanes(x, [](float x, float y) { return fmaxf(x, y); });
+            if (lane < kCols) warps[(warp & 3) * kCols + lane] = of_lane;
             ptx::any_of(bar, 128, false);
-            if (r < NT) {
-              const float top = fmaxf(fmaxf(warps[r], warps[NT + r]), fmaxf(warps[2 * NT + r], warps[3 * NT + r])), old = -refs[r];
+            if (r < kCols) {
+              const float top = fmaxf(fmaxf(warps[r], warps[kCols + r]), fmaxf(warps[2 * kCols + r], warps[3 * kCols + r])), old = -refs[r];
               const bool move = top > old + kSlack;
               factors[r] = move ? ptx::ex2(old - top) : 1.f;
               if (move) refs[r] = -top;
             }
             ptx::any_of(bar, 128, false);
-            if (t > mine) {
+            if (moves) {
 #pragma unroll
-              for (int i = 0; i < NT; i += 4) {
+              for (int i = 0; i < kCols; i += 4) {
                 const float4 f = ld_shared_f4(factors + i);
                 l[i] *= f.x, l[i + 1] *= f.y, l[i + 2] *= f.z, l[i + 3] *= f.w;
               }
               ptx::tc_fence_after();
 #pragma unroll 1
-              for (int d = 0; d < kParts * NT; d += 16) {
+              for (int d = 0; d < kParts * kCols; d += 16) {
+                const int part = d / kCols, n = d - part * kCols;
                 uint32_t o[32], scaled[16];
-                ptx::tmem_ld16(o_own + d, o);
+                ptx::tmem_ld16(o_own + part * NT + n, o);
                 ptx::tmem_ld_wait16(o);
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                  const float4 f = ld_shared_f4(factors + d % NT + i);
+                  const float4 f = ld_shared_f4(factors + n + i);
                   scaled[i] = __float_as_uint(__uint_as_float(o[i]) * f.x), scaled[i + 1] = __float_as_uint(__uint_as_float(o[i + 1]) * f.y);
                   scaled[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * f.z), scaled[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * f.w);
                 }
-                ptx::tmem_st16(o_own + d, scaled);
+                ptx::tmem_st16(o_own + part * NT + n, scaled);
               }
               ptx::tmem_st_wait();
             }
-            if (NT == kChunk) exponents(0, true);
+            exponents(true);
           }
           constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
           const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
-          const uint32_t row = sP + group * Cfg::kPBytes + r * kRow;
+          const uint32_t row = sP + own * Cfg::kPBytes + r * kRow;
 #pragma unroll
-          for (int n0 = 0; n0 < NT; n0 += kChunk) {
-            if (NT > kChunk) exponents(n0, true);
+          for (int i = 0; i < kCols; i += 8) {
+            uint32_t out[4];
 #pragma unroll
-            for (int i = 0; i < kChunk; i += 8) {
-              uint32_t out[4];
-#pragma unroll
-              for (int e = 0; e < 8; e += 2) {
-                const float e0 = ptx::ex2(x[i + e]), e1 = ptx::ex2(x[i + e + 1]);
-                ptx::add_two(l[n0 + i + e], l[n0 + i + e + 1], e0, e1);
-                out[e / 2] = pack2<M>(e0, e1);
-              }
-              ptx::st_shared_16(row + ((((n0 + i) / 8) ^ swizzle) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+            for (int e = 0; e < 8; e += 2) {
+              const float e0 = ptx::ex2(x[i + e]), e1 = ptx::ex2(x[i + e + 1]);
+              ptx::add_two(l[i + e], l[i + e + 1], e0, e1);
+              out[e / 2] = pack2<M>(e0, e1);
             }
+            ptx::st_shared_16(row + ((((n0 + i) / 8) ^ swizzle) << 4), make_uint4(out[0], out[1], out[2], out[3]));
           }
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(p_full(group));
+          if (lane == 0) ptx::mbar_arrive(p_full(own));
         }
         // sums of the weights: over this warp's keys, then over the warps
-#pragma unroll
-        for (int n0 = 0; n0 < NT; n0 += kChunk) {
-          float part[kChunk];
-#pragma unroll
-          for (int i = 0; i < kChunk; ++i) part[i] = l[n0 + i];
-          const float of_lane = across_lanes(part, [](float x, float y) { return x + y; });
-          if (lane < kChunk) warps[(warp & 3) * NT + n0 + lane] = of_lane;
-        }
-        if (mine < w.t1) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+        const float of_lane = across_lanes(l, [](float x, float y) { return x + y; });
+        if (lane < kCols) warps[(warp & 3) * kCols + lane] = of_lane;
+        wait_for_output();
         if (ptx::any_of(kBoth, 256, !ok)) break;
         ptx::tc_fence_after();
-        if (threadIdx.x < NT) {  // both groups' rows on the larger reference
+        if (threadIdx.x < NT) {  // with tiles in turn, both groups' sums on the larger reference
           const int n = threadIdx.x, at = w.qt * NT + n, token = fast_div(at, p.group_div);
-          const float* b = by_warp + n;
-          const float sum0 = (b[0] + b[NT]) + (b[2 * NT] + b[3 * NT]), sum1 = (b[4 * NT] + b[5 * NT]) + (b[6 * NT] + b[7 * NT]);
-          const float ref0 = -minus_ref[n], ref1 = -minus_ref[NT + n], ref = fmaxf(ref0, ref1);
+          const float* b = by_warp + (Cfg::kTurns ? n : n / kCols * 4 * kCols + n % kCols);
+          const float sum0 = (b[0] + b[kCols]) + (b[2 * kCols] + b[3 * kCols]), ref0 = -minus_ref[n];
+          float sum1 = 0.f, ref1 = ref0;
+          if constexpr (Cfg::kTurns) sum1 = (b[4 * NT] + b[5 * NT]) + (b[6 * NT] + b[7 * NT]), ref1 = -minus_ref[NT + n];
+          const float ref = fmaxf(ref0, ref1);
           const float f0 = sum0 == 0.f ? 0.f : ptx::ex2(ref0 - ref), f1 = sum1 == 0.f ? 0.f : ptx::ex2(ref1 - ref);
           const float sum = sum0 * f0 + sum1 * f1, by = whole ? (sum == 0.f ? 0.f : v_scale / sum) : 1.f;
           factor[n] = f0 * by;
@@ -859,9 +870,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             if (first >= rows) continue;  // the same for the whole group
             uint32_t o0[32], o1[32];
             ptx::tmem_ld16(lane_base + Cfg::kTmemO + d0, o0);
-            ptx::tmem_ld16(lane_base + Cfg::kTmemO + Cfg::kOCols + d0, o1);
+            if constexpr (Cfg::kTwoO) ptx::tmem_ld16(lane_base + Cfg::kTmemO + Cfg::kOCols + d0, o1);
             ptx::tmem_ld_wait16(o0);
-            ptx::tmem_ld_wait16(o1);
+            if constexpr (Cfg::kTwoO) ptx::tmem_ld_wait16(o1);
             T* const out = static_cast<T*>(a.out) + d;
             float* const partial = p.part_o + (slot0 + first) * D + d;
 #pragma unroll
@@ -869,11 +880,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
               const float4 f0 = ld_shared_f4(factor + first + i), f1 = ld_shared_f4(factor + NT + first + i);
               const int4 to = *reinterpret_cast<const int4*>(out_row + first + i);
               // a group that has seen nothing of a row adds nothing, whatever its O holds
-              auto both = [&](uint32_t x0, float y0, uint32_t x1, float y1) {
-                return (y0 == 0.f ? 0.f : __uint_as_float(x0) * y0) + (y1 == 0.f ? 0.f : __uint_as_float(x1) * y1);
+              auto both = [&](int e, float y0, float y1) {
+                float sum = y0 == 0.f ? 0.f : __uint_as_float(o0[e]) * y0;
+                if constexpr (Cfg::kTwoO) sum += y1 == 0.f ? 0.f : __uint_as_float(o1[e]) * y1;
+                return sum;
               };
-              const float x[4] = {both(o0[i], f0.x, o1[i], f1.x), both(o0[i + 1], f0.y, o1[i + 1], f1.y), both(o0[i + 2], f0.z, o1[i + 2], f1.z),
-                                  both(o0[i + 3], f0.w, o1[i + 3], f1.w)};
+              const float x[4] = {both(i, f0.x, f1.x), both(i + 1, f0.y, f1.y), both(i + 2, f0.z, f1.z), both(i + 3, f0.w, f1.w)};
               const int rows_to[4] = {to.x, to.y, to.z, to.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -885,18 +897,20 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           }
         }
       } else {
-        // A thread per row, 128 keys in its registers: reference and sum are its own
+        // A thread per row, 64 keys of a tile in its registers: reference and sum are its own
         const bool busy = (warp & 3) * 32 < rows;  // the same for the whole warp
         const int at = w.qt * NT + min(r, rows - 1), token = fast_div(at, p.group_div);
         const int64_t to = (int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
         uint32_t* const words = seen_words + group * NT * 4;
         float m = -kNoRef, l = 0.f, scale = c;
-        for (int t = mine; t < w.t1; t += 2, ++k) {
-          ok = ok && ptx::mbar_wait(s_full(group), k & 1, abort_flag);
+        for (int t = mine; t < w.t1; ++t) {
+          const uint32_t x_tile = g + (t - w.t0), own = x_tile & 1, phase = x_tile >> 1;
+          const uint32_t s_own = lane_base + own * Cfg::kSCols + group * 64;
+          ok = ok && ptx::mbar_wait(s_full(own), phase & 1, abort_flag);
           ptx::tc_fence_after();
           if (kRowScales && t == mine) scale = c * scales[min(r, rows - 1)];
           const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
-          if (masked) {  // thread r finds out who sees key r; a word per token and 32 keys
+          if (masked) {  // thread r finds out who sees key r; a word per token and 32 keys. (Each group for itself: they need not be at the same tile.)
             const int j = t * kKeys + r;
             for (int i0 = 0; i0 <= last_token - first_token; i0 += 64) {
               const int count = min(64, last_token - first_token + 1 - i0);
@@ -909,47 +923,36 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             if (s.n > 1 || a.mask) check_values(t);
             ptx::any_of(bar, 128, false);
           }
-          uint32_t v[4][32];
+          // the product that was in this buffer before is complete: waited for in every tile, so that a wait is never for a phase two ahead
+          if (x_tile >= 2) ok = ok && ptx::mbar_wait(o_done(own), (phase - 1) & 1, abort_flag);
           if (busy) {
+            uint32_t v[2][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ptx::tmem_ld32(s_own + i * 32, v[i]);
+            for (int i = 0; i < 2; ++i) ptx::tmem_ld32(s_own + i * 32, v[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ptx::tmem_ld_wait(v[i]);
+            for (int i = 0; i < 2; ++i) ptx::tmem_ld_wait(v[i]);
             if (masked) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint32_t word = words[(token - first_token) * 4 + q];
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t word = words[(token - first_token) * 4 + group * 2 + q];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[q][i] = (word >> i) & 1u ? v[q][i] : 0xff800000u;
               }
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
               for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = ptx::max3(top[(i >> 1) & 3], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
             const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
             const bool move = largest > m + kSlack;
-            const float old = m;
-            if (move) m = largest;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t out[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float e0, e1;
-                ptx::fma_two(e0, e1, __uint_as_float(v[q][2 * i]), __uint_as_float(v[q][2 * i + 1]), scale, scale, -m, -m);
-                e0 = ptx::ex2(e0), e1 = ptx::ex2(e1);
-                ptx::add_two(sum[(i & 1) * 2], sum[(i & 1) * 2 + 1], e0, e1);
-                out[i] = pack2<M>(e0, e1);
-              }
-              ptx::tmem_st16(s_own + q * 16, out);  // over scores that are in registers
-            }
-            if (k > 0) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
-            const float f = move ? ptx::ex2(old - m) : 1.f;
-            l = l * f + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-            if (t > mine && __any_sync(0xffffffffu, move)) {
+            if (t == mine) {
+              if (move) m = largest;
+            } else if (__any_sync(0xffffffffu, move)) {
+              const float f = move ? ptx::ex2(m - largest) : 1.f;
+              if (move) m = largest;
+              l *= f;
+              ok = ok && ptx::mbar_wait(o_done(own ^ 1), ((x_tile - 1) >> 1) & 1, abort_flag);
               ptx::tc_fence_after();
 #pragma unroll 1
               for (int d = 0; d < D; d += 16) {
@@ -961,13 +964,28 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
                 ptx::tmem_st16(o_own + d, scaled);
               }
             }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t out[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float e0, e1;
+                ptx::fma_two(e0, e1, __uint_as_float(v[q][2 * i]), __uint_as_float(v[q][2 * i + 1]), scale, scale, -m, -m);
+                e0 = ptx::ex2(e0), e1 = ptx::ex2(e1);
+                ptx::add_two(sum[(i & 1) * 2], sum[(i & 1) * 2 + 1], e0, e1);
+                out[i] = pack2<M>(e0, e1);
+              }
+              ptx::tmem_st16(s_own + q * 16, out);  // over scores that are in registers
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             ptx::tmem_st_wait();
           }
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(p_full(group));
+          if (lane == 0) ptx::mbar_arrive(p_full(own));
         }
-        if (mine < w.t1) ok = ok && ptx::mbar_wait(o_done(group), (k - 1) & 1, abort_flag);
+        wait_for_output();
         minus_ref[group * NT + r] = m;
         by_warp[group * NT + r] = l;
         if (ptx::any_of(kBoth, 256, !ok)) break;
