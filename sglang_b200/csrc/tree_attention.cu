@@ -174,13 +174,14 @@ struct AttnCfg {
   static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
   // fp32 words per row: scales of two segments' rows, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
   static constexpr int kTables = NT * 4 * (kRowsInLanes ? 2 + 2 + 2 + 8 : 2 + 2 + 2 + 8 + 2 + 1);
-  // Warps: two groups of four for the softmax; products and queries; then four that bring keys and four values, or, with two stages a tile, four that bring
-  // both (warps that run ahead of the others could take a stage's barrier for two phases older)
+  // Warps: two groups of four for the softmax; products and queries; then four that bring keys and four values, or all bring both: eight where an FP8 cache's
+  // ring is short, so that a stage is soon widened, four with two stages a tile (where warps ahead of others could take a barrier's phase for one two older)
   static constexpr int kSoftmaxWarps = 8, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 4;
-  static constexpr bool kSplit = kParts == 1;
-  static constexpr int kProducerWarps = kSplit ? 8 : 4, kThreads = (kProducerWarp + kProducerWarps) * 32;
+  static constexpr bool kSplit = kParts == 1 && (!FP8 || NT <= 32);
+  static constexpr int kProducerWarps = kParts == 1 ? 8 : 4, kWarpKeys = kParts == 1 && !kSplit ? 16 : 32;  // keys of a stage that a warp brings
+  static constexpr int kThreads = (kProducerWarp + kProducerWarps) * 32;
   // FP8: codes land in a ring of each producer's own, kRaw stages deep, and go from there into the ring of 16-bit tiles
-  static constexpr int kRawStage = 32 * kWidth, kRaw = !FP8 ? 0 : NT <= 32 ? 2 : 3, kRawBytes = kProducerWarps * kRaw * kRawStage;
+  static constexpr int kRawStage = kWarpKeys * kWidth, kRaw = !FP8 ? 0 : kSplit ? 2 : 3, kRawBytes = kProducerWarps * kRaw * kRawStage;
   static constexpr int kFixed = kQBytes + 2 * kPBytes + kRawBytes + kTables + 1024 + 512;
   static constexpr int kFit = (232448 - kFixed) / kStage;
   // A wait for a stage's place tells its phase from the one two before it, which has to be over: with keys and values brought by different warps that holds
@@ -189,7 +190,7 @@ struct AttnCfg {
   static_assert(!kSplit || kStages % 2 == 0 || kStages >= 5, "phases are told apart");
   // Registers of a thread at launch, and of the three kinds of warps
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-  static constexpr int kSoftmaxRegs = kSplit ? 112 : 160, kProducerRegs = kSplit ? 88 : 112, kOtherRegs = 80;
+  static constexpr int kSoftmaxRegs = kParts == 1 ? 112 : 160, kProducerRegs = kParts == 1 ? 88 : 112, kOtherRegs = 80;
   static_assert((8 * kSoftmaxRegs + 4 * kOtherRegs + kProducerWarps * kProducerRegs) * 32 <= kThreads * kLaunchRegs,
                 "the registers add up to no more than at launch");
   // TMEM columns: the scores of two tiles, then an O for each of the two groups
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      ptx::mbar_init(full_bar(s), FP8 ? 4 : 128);  // warps that have stored, or threads whose copies have landed
+      ptx::mbar_init(full_bar(s), FP8 ? 128 / Cfg::kWarpKeys : 128);  // warps that have stored, or threads whose copies have landed
       ptx::mbar_init(empty_bar(s), 1);
     }
     ptx::mbar_init(q_full, 3);
@@ -412,17 +413,18 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   if (warp >= Cfg::kProducerWarp) {
     // ------------------------------------------------------------------ keys and values into the ring, a tile's keys, then its values
     ptx::give_registers<Cfg::kProducerRegs, Cfg::kLaunchRegs>();
-    const int row0 = ((warp - Cfg::kProducerWarp) & 3) * 32;  // 32 keys of a tile, lane l has the addresses of the l-th
+    constexpr int kWarpKeys = Cfg::kWarpKeys;
+    const int row0 = (warp - Cfg::kProducerWarp) * kWarpKeys % kKeys;  // this warp's keys of a tile, lane l has the addresses of the l-th
     // stages of a tile that are this warp's
     constexpr int kMine = Cfg::kSplit ? kParts : 2 * kParts;
     const int first_part = Cfg::kSplit && warp >= Cfg::kProducerWarp + 4 ? kParts : 0;
     constexpr int kPieces = Cfg::kWidth / (FP8 ? 16 : 8);  // of 16 bytes, of a key's part in the cache
     constexpr int kKeysAtOnce = 32 / kPieces;              // of a load of the warp
-    constexpr int kSteps = kPieces;
+    constexpr int kSteps = kPieces * kWarpKeys / 32;
     constexpr int es = FP8 ? 1 : 2;
     auto entry_of = [&](const Walk<NT>& at, int t) {
       const int j = t * kKeys + row0 + lane;
-      if (!at.more() || j >= at.s.len) return -1;
+      if (!at.more() || j >= at.s.len || lane >= kWarpKeys) return -1;
       return (int)ld_operand(a.page_table + (int64_t)at.b * a.page_table_ld + fast_div(j, p.page_div));
     };
     // this lane's key and its value; something readable where there is none. Warps that bring one of them know that one alone.
@@ -432,8 +434,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     int t = w.t0, entry = entry_of(w, t);
     auto next_tile = [&] {
       const int j = t * kKeys + row0 + lane, in_page = j - fast_div(j, p.page_div) * a.page_size;
-      const bool key = j < w.s.len, page = entry >= 0 && entry < a.pages;
-      absent = __ballot_sync(0xffffffffu, !key);
+      const bool key = j < w.s.len && lane < kWarpKeys, page = entry >= 0 && entry < a.pages;
+      absent = __ballot_sync(0xffffffffu, !key && lane < kWarpKeys);
       unknown = __ballot_sync(0xffffffffu, key && !page);
       const uint8_t* const some = static_cast<const uint8_t*>(a.q);
       const bool have = key && page;
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       if constexpr (!Cfg::kSplit) mine = kv ? from[1] : from[0];
       const int beside = (part % kParts) * Cfg::kWidth * es;
       auto to = [&](int i) { return FP8 ? base + i * 512 + lane * 16 : slot(base, my_piece, i); };
-      if ((absent | unknown) == 0) {
+      if (__builtin_expect((absent | unknown) == 0, 1)) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) ptx::cp_async_16(to(i), address(mine, i) + beside, 16u);
       } else {
@@ -737,12 +739,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           // the tile's keys that not every row sees
           const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
           uint64_t seen = 0;
-          if (masked) {
+          if (__builtin_expect(masked, 0)) {
             seen = seen_by(j, first_token, last_token - first_token + 1);
             if (s.n > 1 || a.mask) check_values(t);
           }
-          float x[kCols];
-          auto exponents = [&](bool over_ref) {  // of this thread's key and this group's rows, with or without their reference
+          float x[kCols];  // exponents of this thread's key and this group's rows, without their reference
+          {
             uint32_t v[32];
             if constexpr (kCols == 16) {
               ptx::tmem_ld16(s_own, v);
@@ -753,31 +755,35 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             }
 #pragma unroll
             for (int i = 0; i < kCols; i += 4) {
-              const float4 m = over_ref ? ld_shared_f4(refs + i) : make_float4(0.f, 0.f, 0.f, 0.f);
               float4 by = make_float4(c, c, c, c);
               if constexpr (kRowScales) {
                 by = ld_shared_f4(scales + n0 + i);
                 by.x *= c, by.y *= c, by.z *= c, by.w *= c;
               }
-              ptx::fma_two(x[i], x[i + 1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]), by.x, by.y, m.x, m.y);
-              ptx::fma_two(x[i + 2], x[i + 3], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]), by.z, by.w, m.z, m.w);
+              x[i] = __uint_as_float(v[i]) * by.x, x[i + 1] = __uint_as_float(v[i + 1]) * by.y;
+              x[i + 2] = __uint_as_float(v[i + 2]) * by.z, x[i + 3] = __uint_as_float(v[i + 3]) * by.w;
             }
-            if (masked && j >= prefix) {
+          }
+          if (__builtin_expect(masked && j >= prefix, 0)) {
 #pragma unroll
-              for (int i = 0; i < kCols; ++i)
-                if (!((seen >> (tokens[i] - first_token)) & 1)) x[i] = -INFINITY;
+            for (int i = 0; i < kCols; i += 4) {
+              const int4 token = *reinterpret_cast<const int4*>(tokens + i);
+              if (!((seen >> (token.x - first_token)) & 1)) x[i] = -INFINITY;
+              if (!((seen >> (token.y - first_token)) & 1)) x[i + 1] = -INFINITY;
+              if (!((seen >> (token.z - first_token)) & 1)) x[i + 2] = -INFINITY;
+              if (!((seen >> (token.w - first_token)) & 1)) x[i + 3] = -INFINITY;
             }
-          };
-          exponents(true);
-          float above[2] = {-INFINITY, -INFINITY};  // largest of them
+          }
+          float above[2] = {-INFINITY, -INFINITY};  // largest of them over its reference
 #pragma unroll
           for (int i = 0; i < kCols; i += 4) {
-            above[0] = ptx::max3(above[0], x[i], x[i + 1]);
-            above[1] = ptx::max3(above[1], x[i + 2], x[i + 3]);
+            const float4 m = ld_shared_f4(refs + i);
+            above[0] = ptx::max3(above[0], x[i] + m.x, x[i + 1] + m.y);
+            above[1] = ptx::max3(above[1], x[i + 2] + m.z, x[i + 3] + m.w);
           }
           // the product that read this buffer of P^T is complete (with tiles in turn it is the last one that this group's O was in)
           if (x_tile >= 2) ok = ok && ptx::mbar_wait(o_done(own), (phase - 1) & 1, abort_flag);
-          if (ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == mine || !ok)) {
+          if (__builtin_expect(ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == mine || !ok), 0)) {
             // Rows whose largest score lies too far above their reference take it as the new one
             const bool moves = t > mine;
             if (moves && !Cfg::kTurns) ok = ok && ptx::mbar_wait(o_done(own ^ 1), ((x_tile - 1) >> 1) & 1, abort_flag);
@@ -785,7 +791,6 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
               ok = false;
               break;
             }
-            exponents(false);
             const float of_lane = across_lanes(x, [](float x, float y) { return fmaxf(x, y); });
             if (lane < kCols) warps[(warp & 3) * kCols + lane] = of_lane;
             ptx::any_of(bar, 128, false);
@@ -819,7 +824,6 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
               }
               ptx::tmem_st_wait();
             }
-            exponents(true);
           }
           constexpr int kRow = NT >= 64 ? 128 : NT * 2;  // bytes of a key's row of P^T
           const int swizzle = kRow == 128 ? r & 7 : kRow == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
@@ -827,6 +831,11 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 #pragma unroll
           for (int i = 0; i < kCols; i += 8) {
             uint32_t out[4];
+            const float4 m0 = ld_shared_f4(refs + i), m1 = ld_shared_f4(refs + i + 4);
+            ptx::add_two(x[i], x[i + 1], m0.x, m0.y);
+            ptx::add_two(x[i + 2], x[i + 3], m0.z, m0.w);
+            ptx::add_two(x[i + 4], x[i + 5], m1.x, m1.y);
+            ptx::add_two(x[i + 6], x[i + 7], m1.z, m1.w);
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
               const float e0 = ptx::ex2(x[i + e]), e1 = ptx::ex2(x[i + e + 1]);
@@ -910,7 +919,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           ptx::tc_fence_after();
           if (kRowScales && t == mine) scale = c * scales[min(r, rows - 1)];
           const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
-          if (masked) {  // thread r finds out who sees key r; a word per token and 32 keys. (Each group for itself: they need not be at the same tile.)
+          if (__builtin_expect(masked, 0)) {  // thread r finds out who sees key r; a word per token and 32 keys. (Each group for itself: they need not be at the same tile.)
             const int j = t * kKeys + r;
             for (int i0 = 0; i0 <= last_token - first_token; i0 += 64) {
               const int count = min(64, last_token - first_token + 1 - i0);
@@ -931,7 +940,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             for (int i = 0; i < 2; ++i) ptx::tmem_ld32(s_own + i * 32, v[i]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) ptx::tmem_ld_wait(v[i]);
-            if (masked) {
+            if (__builtin_expect(masked, 0)) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const uint32_t word = words[(token - first_token) * 4 + group * 2 + q];
@@ -948,7 +957,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             const bool move = largest > m + kSlack;
             if (t == mine) {
               if (move) m = largest;
-            } else if (__any_sync(0xffffffffu, move)) {
+            } else if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
               const float f = move ? ptx::ex2(m - largest) : 1.f;
               if (move) m = largest;
               l *= f;
@@ -1029,7 +1038,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       }
       ptx::tc_fence_before();
       // (the barrier also says that this segment's tables have been read)
-      if (ptx::any_of(kBoth, 256, odd_values)) {
+      if (__builtin_expect(ptx::any_of(kBoth, 256, odd_values), 0)) {
         // Values that were taken out go to the rows that see them: NaN and infinities, whatever their weight
         const int j1 = min(s.len, w.t1 * kKeys);
         for (int j = max(max(prefix, 0), w.t0 * kKeys); j < j1; ++j) {
