@@ -174,9 +174,9 @@ struct AttnCfg {
   static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
   // fp32 words per row: scales of two segments' rows, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
   static constexpr int kTables = NT * 4 * (kRowsInLanes ? 2 + 2 + 2 + 8 : 2 + 2 + 2 + 8 + 2 + 1);
-  // Warps: two groups of four for the softmax; products and queries; then four that bring keys and four values, or all bring both: eight where an FP8 cache's
-  // ring is short, so that a stage is soon widened, four with two stages a tile (where warps ahead of others could take a barrier's phase for one two older)
-  static constexpr int kSoftmaxWarps = 8, kMmaWarp = kSoftmaxWarps, kQWarp = kMmaWarp + 1, kProducerWarp = kMmaWarp + 4;
+  // Warps: two groups of four for the softmax; one issues the output's products, two bring queries, one issues the scores' products; then four that bring keys
+  // and four values, or all bring both: eight where an FP8 cache's ring is short, so that a stage is soon widened, four with two stages a tile
+  static constexpr int kSoftmaxWarps = 8, kOutputWarp = kSoftmaxWarps, kQWarp = kOutputWarp + 1, kScoreWarp = kOutputWarp + 3, kProducerWarp = kOutputWarp + 4;
   static constexpr bool kSplit = kParts == 1 && (!FP8 || NT <= 32);
   static constexpr int kProducerWarps = kParts == 1 ? 8 : 4, kWarpKeys = kParts == 1 && !kSplit ? 16 : 32;  // keys of a stage that a warp brings
   static constexpr int kThreads = (kProducerWarp + kProducerWarps) * 32;
@@ -184,10 +184,8 @@ struct AttnCfg {
   static constexpr int kRawStage = kWarpKeys * kWidth, kRaw = !FP8 ? 0 : kSplit ? 2 : 3, kRawBytes = kProducerWarps * kRaw * kRawStage;
   static constexpr int kFixed = kQBytes + 2 * kPBytes + kRawBytes + kTables + 1024 + 512;
   static constexpr int kFit = (232448 - kFixed) / kStage;
-  // A wait for a stage's place tells its phase from the one two before it, which has to be over: with keys and values brought by different warps that holds
-  // where each have places of their own (an even number), or from five on, where a warp cannot be that far ahead.
-  static constexpr int kStages = kFit >= 12 ? 12 : FP8 && kSplit ? kFit / 2 * 2 : kFit;
-  static_assert(!kSplit || kStages % 2 == 0 || kStages >= 5, "phases are told apart");
+  // places for keys and for values: each have a ring of their own, so that a wait for a place is never for a phase two ahead
+  static constexpr int kStages = kFit < 12 ? kFit : 12, kPlacesK = kStages / 2, kPlacesV = kStages - kPlacesK;
   // Registers of a thread at launch, and of the three kinds of warps
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
   static constexpr int kSoftmaxRegs = kParts == 1 ? 112 : 160, kProducerRegs = kParts == 1 ? 88 : 112, kOtherRegs = 80;
@@ -198,7 +196,7 @@ struct AttnCfg {
   static constexpr int kTmemUsed = 2 * kSCols + (kTwoO ? 2 : 1) * kOCols;
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
   static constexpr size_t kSmemBytes = (size_t)kFixed + (size_t)kStages * kStage;
-  static_assert(kStages >= 2 * kParts && kTmemUsed <= 512 && kSmemBytes <= 232448, "a tile of values and the keys of the next one fit");
+  static_assert(kPlacesK >= 1 && kTmemUsed <= 512 && kSmemBytes <= 232448, "the rings fit");
 };
 
 // Sequence b as the kernel takes it: whatever the index tensors hold, tokens and keys stay inside q and the page table.
@@ -331,6 +329,13 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (S + s); };
+  struct Place {
+    uint32_t at, phase;
+  };
+  auto place_of = [](int values, uint32_t n) {  // of the n-th stage of keys, or of values
+    constexpr uint32_t kK = Cfg::kPlacesK, kV = Cfg::kPlacesV;
+    return values ? Place{kK + n % kV, n / kV} : Place{n % kK, n / kK};
+  };
   const uint32_t q_full = bar0 + 8u * (2 * S), q_empty = q_full + 8u;
   auto o_done = [&](uint32_t i) { return q_full + 16u + 8u * (i & 1); };  // products with the values of tiles i, i + 2, ..
   auto s_full = [&](uint32_t i) { return q_full + 32u + 8u * (i & 1); };
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       ptx::mbar_init(full_bar(s), FP8 ? 128 / Cfg::kWarpKeys : 128);  // warps that have stored, or threads whose copies have landed
       ptx::mbar_init(empty_bar(s), 1);
     }
-    ptx::mbar_init(q_full, 3);
+    ptx::mbar_init(q_full, 2);
     ptx::mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(o_done(i), 1);
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     line[2] = 1;
     ptx::fence_mbar_init();
   }
-  if (warp == Cfg::kMmaWarp) {
+  if (warp == Cfg::kOutputWarp) {
     ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
     ptx::tmem_relinquish();
   }
@@ -451,7 +456,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       entry = entry_of(w, t);
     };
     const uint32_t total = kMine * (uint32_t)line[1];  // stages of this warp
-    auto stage_of = [&](uint32_t n) { return (n / kMine) * 2 * kParts + first_part + n % kMine; };
+    auto place = [&](uint32_t n) {  // of this warp's n-th stage
+      const int part = first_part + n % kMine;
+      return place_of(part / kParts, n / kMine * kParts + part % kParts);
+    };
     // Step i of a stage: key i * kKeysAtOnce + my_key of this warp's, piece my_piece. (Eight codes of a piece become 16 bytes and go to every second place of a
     // 128-byte row: eight lanes store to all of the banks if they have four pieces of two keys.)
     constexpr bool kInterleave = FP8 && kPieces == 8;
@@ -488,11 +496,11 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     };
     if constexpr (!FP8) {
       for (uint32_t n = 0; n < total; ++n) {
-        const uint32_t st = stage_of(n), s = st % S;
-        ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
+        const Place to = place(n);
+        ok = ptx::mbar_wait(empty_bar(to.at), (to.phase & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
-        request(n, sKV + s * Cfg::kStage + row0 * 128);
-        ptx::cp_async_arrive(full_bar(s));  // when they have landed
+        request(n, sKV + to.at * Cfg::kStage + row0 * 128);
+        ptx::cp_async_arrive(full_bar(to.at));  // when they have landed
       }
     } else {
       // Every lane reads back what it has copied itself. (Codes held in registers on their way took so many that few bytes were under way.)
@@ -502,11 +510,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         if (m < total) request(m, raw + m % Cfg::kRaw * Cfg::kRawStage);
         ptx::cp_async_commit();
         if (m < kAhead) continue;
-        const uint32_t n = m - kAhead, st = stage_of(n), s = st % S;
-        ok = ptx::mbar_wait(empty_bar(s), ((st / S) & 1) ^ 1, abort_flag);
+        const uint32_t n = m - kAhead;
+        const Place to = place(n);
+        ok = ptx::mbar_wait(empty_bar(to.at), (to.phase & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
         ptx::cp_async_wait<kAhead>();
-        const uint32_t base = sKV + s * Cfg::kStage + row0 * 128, codes = raw + n % Cfg::kRaw * Cfg::kRawStage + lane * 16;
+        const uint32_t base = sKV + to.at * Cfg::kStage + row0 * 128, codes = raw + n % Cfg::kRaw * Cfg::kRawStage + lane * 16;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
           const uint4 v = ptx::ld_shared_16(codes + i * 512);
@@ -519,16 +528,16 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           ptx::st_shared_16(slot(base, 2 * my_piece + 1, i), hi);
         }
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(full_bar(s));
+        if (lane == 0) ptx::mbar_arrive(full_bar(to.at));
       }
     }
     ptx::cp_async_wait_all();
     grid_launch_dependents();
-  } else if (warp >= Cfg::kMmaWarp) {
+  } else if (warp >= Cfg::kOutputWarp) {
     ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
-    // ------------------------------------------------------------------ query rows, those behind the last one as zeros: three warps
-    if (warp != Cfg::kMmaWarp) {
-      constexpr int kPerRow = D / 8, kAtOnce = 4, kLanes = 96;
+    // ------------------------------------------------------------------ query rows, those behind the last one as zeros: two warps
+    if (warp == Cfg::kQWarp || warp == Cfg::kQWarp + 1) {
+      constexpr int kPerRow = D / 8, kAtOnce = 4, kLanes = 64;
       const int first = (warp - Cfg::kQWarp) * 32 + lane;
       for (int seg = 0; w.more(); w.next(), ++seg) {
         ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
@@ -566,73 +575,73 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         if (lane == 0) ptx::mbar_arrive(q_full);
       }
     }
-    // ------------------------------------------------------------------ both products
-    // Operands come by ordinary stores and small copies of other threads. What orders them before the products is this thread's fence behind its wait: a
-    // fence of the threads that bring keys would wait for everything that they have under way (FP8 cache, 64 x 16384: 620 us).
-    if (warp == Cfg::kMmaWarp && ptx::elect_one()) {
-      // A tile's scores are asked for before the output of the tile ahead, whose weights its softmax group still computes
-      constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kBf16, 0, 128, Cfg::kSCols);
-      constexpr uint32_t idesc_o = Cfg::kRowsInLanes ? ptx::idesc_f16_f32(kBf16, 2, 128, D) : ptx::idesc_f16_f32(kBf16, 3, 128, NT);
-      constexpr int kPRow = NT >= 64 ? 128 : NT * 2;
+    // ------------------------------------------------------------------ the products, each issued by a thread of its own: the scores of the next tiles do not
+    // wait for the weights of this one
+    // Operands come by ordinary stores and small copies of other threads. What orders them before the products is the issuing thread's fence behind its wait:
+    // a fence of the threads that bring keys would wait for everything that they have under way (FP8 cache, 64 x 16384: 620 us).
+    constexpr int kPRow = NT >= 64 ? 128 : NT * 2;
+    if (warp == Cfg::kScoreWarp && ptx::elect_one()) {
+      constexpr uint32_t idesc = ptx::idesc_f16_f32(kBf16, 0, 128, Cfg::kSCols);
+      uint32_t x = 0, stage = 0;  // tiles and stages of keys so far
+      for (int seg = 0; w.more() && ok; w.next(), ++seg) {
+        ok = ptx::mbar_wait(q_full, seg & 1, abort_flag);
+        for (int t = w.t0; t < w.t1 && ok; ++t, ++x) {
+          // the scores that were in this buffer have been read, or the weights that took their place multiplied
+          if (x >= 2) ok = ptx::mbar_wait(Cfg::kRowsInLanes ? o_done(x) : p_full(x), ((x >> 1) - 1) & 1, abort_flag);
+#pragma unroll
+          for (int part = 0; part < kParts && ok; ++part, ++stage) {
+            const Place from = place_of(0, stage);
+            ok = ptx::mbar_wait(full_bar(from.at), from.phase & 1, abort_flag);
+            if (!ok) break;
+            ptx::fence_proxy_async_smem();
+            ptx::tc_fence_after();
+            const ptx::Operand keys = ptx::operand_sw128(sKV + from.at * Cfg::kStage), queries = ptx::operand_sw128(sQ + part * 2 * (NT * 128));
+            const uint32_t d = tmem_base + (x & 1) * Cfg::kSCols;
+#pragma unroll
+            for (int k = 0; k < Cfg::kWidth / 16; ++k) {
+              const uint32_t in_row = (k & 3) * 32, block = k >> 2;
+              const ptx::Operand kk = keys.at(block * (kKeys * 128) + in_row), qq = queries.at(block * (NT * 128) + in_row);
+              if (Cfg::kRowsInLanes) ptx::mma_f16(d, qq, kk, idesc, part > 0 || k > 0);
+              else ptx::mma_f16(d, kk, qq, idesc, part > 0 || k > 0);
+            }
+            ptx::mma_commit(empty_bar(from.at));
+          }
+          if (ok) ptx::mma_commit(s_full(x));
+        }
+        if (ok) ptx::mma_commit(q_empty);
+      }
+    }
+    if (warp == Cfg::kOutputWarp && ptx::elect_one()) {
+      constexpr uint32_t idesc = Cfg::kRowsInLanes ? ptx::idesc_f16_f32(kBf16, 2, 128, D) : ptx::idesc_f16_f32(kBf16, 3, 128, NT);
       // heads of 64 fill half of the lanes: the other half repeats them
       constexpr uint32_t kNextV = D == 64 && !Cfg::kRowsInLanes ? 0u : kKeys * 128u;
-      uint32_t it = 0, g = 0;  // stages and tiles of this CTA so far
-      auto scores = [&](uint32_t x, bool last) {
+      uint32_t x = 0, stage = 0;  // tiles and stages of values so far
+      for (; w.more() && ok; w.next()) {
+        for (int t = w.t0; t < w.t1 && ok; ++t, ++x) {
+          const uint32_t own = x & 1;
+          ok = ptx::mbar_wait(p_full(own), (x >> 1) & 1, abort_flag);
+          const uint32_t o = tmem_base + Cfg::kTmemO + (Cfg::kTurns ? own * Cfg::kOCols : 0);
+          const uint32_t before = t - w.t0 > (Cfg::kTurns ? 1 : 0);  // O holds earlier tiles
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-          const uint32_t st = it + 2 * kParts * x + part, s = st % S;
-          if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
-          ptx::fence_proxy_async_smem();
-          ptx::tc_fence_after();
-          const ptx::Operand keys = ptx::operand_sw128(sKV + s * Cfg::kStage), queries = ptx::operand_sw128(sQ + part * 2 * (NT * 128));
-          const uint32_t d = tmem_base + ((g + x) & 1) * Cfg::kSCols;
+          for (int part = 0; part < kParts && ok; ++part, ++stage) {
+            const Place from = place_of(1, stage);
+            ok = ptx::mbar_wait(full_bar(from.at), from.phase & 1, abort_flag);
+            if (!ok) break;
+            ptx::fence_proxy_async_smem();
+            ptx::tc_fence_after();
+            const ptx::Operand values = ptx::operand_depth_rows<128>(sKV + from.at * Cfg::kStage, kNextV);
+            const ptx::Operand weights = ptx::operand_depth_rows<kPRow>(sP + own * Cfg::kPBytes, kKeys * 128);
 #pragma unroll
-          for (int k = 0; k < Cfg::kWidth / 16; ++k) {
-            const uint32_t in_row = (k & 3) * 32, block = k >> 2;
-            const ptx::Operand kk = keys.at(block * (kKeys * 128) + in_row), qq = queries.at(block * (NT * 128) + in_row);
-            if (Cfg::kRowsInLanes) ptx::mma_f16(d, qq, kk, idesc_s, part > 0 || k > 0);
-            else ptx::mma_f16(d, kk, qq, idesc_s, part > 0 || k > 0);
+            for (int k = 0; k < kKeys / 16; ++k) {
+              if (Cfg::kRowsInLanes)  // each half of the keys into its own O
+                ptx::mma_f16_ts(o + (k >> 2) * Cfg::kOCols, tmem_base + own * Cfg::kSCols + (k >> 2) * 64 + (k & 3) * 8, values.at(k * 2048), idesc,
+                                before || (k & 3));
+              else ptx::mma_f16(o + part * NT, values.at(k * 2048), weights.at(k * 16 * kPRow), idesc, before || k > 0);
+            }
+            ptx::mma_commit(empty_bar(from.at));
           }
-          ptx::mma_commit(empty_bar(s));
+          if (ok) ptx::mma_commit(o_done(own));
         }
-        ptx::mma_commit(s_full(g + x));
-        if (last) ptx::mma_commit(q_empty);
-        return true;
-      };
-      auto output = [&](uint32_t x) {
-        const uint32_t own = (g + x) & 1;
-        if (!ptx::mbar_wait(p_full(own), ((g + x) >> 1) & 1, abort_flag)) return false;
-        const uint32_t o = tmem_base + Cfg::kTmemO + (Cfg::kTurns ? own * Cfg::kOCols : 0);
-        const uint32_t before = x > (Cfg::kTurns ? 1 : 0);  // O holds earlier tiles
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-          const uint32_t st = it + 2 * kParts * x + kParts + part, s = st % S;
-          if (!ptx::mbar_wait(full_bar(s), (st / S) & 1, abort_flag)) return false;
-          ptx::fence_proxy_async_smem();
-          ptx::tc_fence_after();
-          const ptx::Operand values = ptx::operand_depth_rows<128>(sKV + s * Cfg::kStage, kNextV);
-          const ptx::Operand weights = ptx::operand_depth_rows<kPRow>(sP + own * Cfg::kPBytes, kKeys * 128);
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k) {
-            if (Cfg::kRowsInLanes)  // each half of the keys into its own O
-              ptx::mma_f16_ts(o + (k >> 2) * Cfg::kOCols, tmem_base + own * Cfg::kSCols + (k >> 2) * 64 + (k & 3) * 8, values.at(k * 2048), idesc_o, before || (k & 3));
-            else ptx::mma_f16(o + part * NT, values.at(k * 2048), weights.at(k * 16 * kPRow), idesc_o, before || k > 0);
-          }
-          ptx::mma_commit(empty_bar(s));
-        }
-        ptx::mma_commit(o_done(own));
-        return true;
-      };
-      for (int seg = 0; w.more() && ok; w.next(), ++seg) {
-        const uint32_t n = w.t1 - w.t0;
-        ok = ptx::mbar_wait(q_full, seg & 1, abort_flag);
-        for (uint32_t x = 0; x < n && ok; ++x) {
-          ok = scores(x, x + 1 == n);
-          if (ok && x > 0) ok = output(x - 1);
-        }
-        ok = ok && output(n - 1);
-        it += 2 * kParts * n;
-        g += n;
       }
     }
     __syncwarp();
@@ -669,12 +678,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         if (!Cfg::kTurns && group != 0) return;  // one group looks at a tile
 #pragma unroll 1
         for (int part = 0; part < kParts; ++part) {
-          const uint32_t st = 2 * kParts * x + kParts + part;
-          ok = ok && ptx::mbar_wait(full_bar(st % S), (st / S) & 1, abort_flag);
+          const Place from = place_of(1, kParts * x + part);
+          ok = ok && ptx::mbar_wait(full_bar(from.at), from.phase & 1, abort_flag);
           if (!ok || j < prefix || j >= s.len) continue;
 #pragma unroll 1
           for (int c8 = 0; c8 < Cfg::kWidth / 8; ++c8) {
-            const uint32_t at = sKV + (st % S) * Cfg::kStage + (c8 >> 3) * (kKeys * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
+            const uint32_t at = sKV + from.at * Cfg::kStage + (c8 >> 3) * (kKeys * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
             uint4 v = ptx::ld_shared_16(at);
             uint32_t word[4] = {v.x, v.y, v.z, v.w}, odd = 0;
 #pragma unroll
@@ -1075,7 +1084,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   ptx::tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) atomicCAS(p.status, 0, 1);
-  if (warp == Cfg::kMmaWarp) {
+  if (warp == Cfg::kOutputWarp) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
