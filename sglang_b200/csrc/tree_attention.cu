@@ -202,8 +202,13 @@ struct AttnCfg {
 // Sequence b as the kernel takes it: whatever the index tensors hold, tokens and keys stay inside q and the page table.
 struct Seq {
   int start, n, len, row_tiles, key_tiles;
-  __device__ __forceinline__ int64_t tiles(int heads) const { return n > 0 ? (int64_t)heads * row_tiles * key_tiles : 0; }
+  // A row tile's length on the line: its tiles of keys, and as many more as its queries, masks and output cost (16 x 16384 keys, 8 tokens: without them the
+  // CTAs with the short sequences took 156 us where others took 94)
+  __device__ __forceinline__ int units(int extra) const { return key_tiles + extra; }
+  __device__ __forceinline__ int64_t length(int heads, int extra) const { return n > 0 ? (int64_t)heads * row_tiles * units(extra) : 0; }
 };
+template <int NT>
+constexpr int kExtraTiles = NT <= 32 ? 2 : 3;
 template <int NT>
 __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
   const b200_tree_attention_args& a = p.a;
@@ -227,36 +232,49 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
 template <int NT>
 struct Walk {
   const AttnParams& p;
-  int b, h, qt, t0, t1;
-  int64_t left;
+  int b, h, qt, t0, t1;  // sequence, kv head, row tile; its tiles of keys t0 .. t1 - 1
+  int at, end;           // the piece's part of the row tile's length
+  int64_t left;          // of the piece
   Seq s;
-  __device__ __forceinline__ Walk(const AttnParams& p_, int b0, int64_t offset, int64_t count) : p(p_), b(b0), left(count) {
-    h = qt = t0 = t1 = 0;
+  __device__ __forceinline__ Walk(const AttnParams& p_, int b0, int64_t offset, int64_t length) : p(p_), b(b0), left(length) {
+    h = qt = t0 = t1 = at = end = 0;
     s = {};
     if (left <= 0) return;
     s = seq_of<NT>(p, b);
-    const int64_t per_head = (int64_t)s.row_tiles * s.key_tiles;
+    const int units = s.units(kExtraTiles<NT>);
+    const int64_t per_head = (int64_t)s.row_tiles * units;
     h = (int)(offset / per_head);
     const int rest = (int)(offset - h * per_head);
-    qt = rest / s.key_tiles;
-    t0 = rest - qt * s.key_tiles;
-    t1 = (int)min((int64_t)s.key_tiles, t0 + left);
+    qt = rest / units;
+    at = rest - qt * units;
+    settle();
   }
   __device__ __forceinline__ bool more() const { return left > 0; }
   __device__ __forceinline__ void next() {
-    left -= t1 - t0;
-    if (left <= 0) return;
-    t0 = 0;
-    if (++qt == s.row_tiles) {
-      qt = 0;
-      if (++h == p.a.kv_heads) {
-        h = 0;
-        do {
-          s = seq_of<NT>(p, ++b);
-        } while (s.n == 0 && b + 1 < p.a.sequences);
-      }
+    leave();
+    settle();
+  }
+
+ private:
+  __device__ __forceinline__ void settle() {  // to the next row tile of which the piece has keys
+    while (left > 0) {
+      end = (int)min((int64_t)s.units(kExtraTiles<NT>), at + left);
+      t0 = max(0, at - kExtraTiles<NT>);
+      t1 = max(0, end - kExtraTiles<NT>);
+      if (t1 > t0) return;
+      leave();
     }
-    t1 = (int)min((int64_t)s.key_tiles, left);
+  }
+  __device__ __forceinline__ void leave() {
+    left -= end - at;
+    at = 0;
+    if (left <= 0 || ++qt < s.row_tiles) return;
+    qt = 0;
+    if (++h < p.a.kv_heads) return;
+    h = 0;
+    do {
+      s = seq_of<NT>(p, ++b);
+    } while (s.n == 0 && b + 1 < p.a.sequences);
   }
 };
 
@@ -343,7 +361,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 2 * S + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * S + 9);
   volatile int* begin_seq = abort_flag + 1;
-  volatile int64_t* line = reinterpret_cast<volatile int64_t*>(bars + 2 * S + 10);  // offset within the first sequence, tiles of this CTA, of every CTA
+  volatile int64_t* line = reinterpret_cast<volatile int64_t*>(bars + 2 * S + 10);  // offset within the first sequence, length of this CTA's piece, of every piece
   volatile int64_t* sums = line + 3;                                                // of each warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -380,7 +398,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     const int per = (int)((a.sequences + Cfg::kThreads - 1) / Cfg::kThreads);
     const int b0 = min((int)threadIdx.x * per, (int)a.sequences), b1 = min(b0 + per, (int)a.sequences);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_of<NT>(p, b).tiles(a.kv_heads);
+    for (int b = b0; b < b1; ++b) mine += seq_of<NT>(p, b).length(a.kv_heads, kExtraTiles<NT>);
     int64_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -399,7 +417,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     const int64_t chunk = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1), begin = blockIdx.x * chunk;
     if (begin >= before && begin < before + mine) {
       for (int b = b0; b < b1; ++b) {
-        const int64_t n = seq_of<NT>(p, b).tiles(a.kv_heads);
+        const int64_t n = seq_of<NT>(p, b).length(a.kv_heads, kExtraTiles<NT>);
         if (begin < before + n) {
           *begin_seq = b;
           line[0] = begin - before;
@@ -455,7 +473,6 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       }
       entry = entry_of(w, t);
     };
-    const uint32_t total = kMine * (uint32_t)line[1];  // stages of this warp
     auto place = [&](uint32_t n) {  // of this warp's n-th stage
       const int part = first_part + n % kMine;
       return place_of(part / kParts, n / kMine * kParts + part % kParts);
@@ -495,7 +512,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       }
     };
     if constexpr (!FP8) {
-      for (uint32_t n = 0; n < total; ++n) {
+      for (uint32_t n = 0; n % kMine != 0 || w.more(); ++n) {
         const Place to = place(n);
         ok = ptx::mbar_wait(empty_bar(to.at), (to.phase & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -506,11 +523,16 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       // Every lane reads back what it has copied itself. (Codes held in registers on their way took so many that few bytes were under way.)
       constexpr uint32_t kAhead = Cfg::kRaw - 1;
       const uint32_t raw = sRaw + (warp - Cfg::kProducerWarp) * Cfg::kRaw * Cfg::kRawStage;
-      for (uint32_t m = 0; m < total + kAhead; ++m) {
-        if (m < total) request(m, raw + m % Cfg::kRaw * Cfg::kRawStage);
+      uint32_t asked = 0;
+      for (uint32_t m = 0;; ++m) {
+        if (asked % kMine != 0 || w.more()) {
+          request(asked, raw + asked % Cfg::kRaw * Cfg::kRawStage);
+          ++asked;
+        }
         ptx::cp_async_commit();
         if (m < kAhead) continue;
         const uint32_t n = m - kAhead;
+        if (n >= asked) break;
         const Place to = place(n);
         ok = ptx::mbar_wait(empty_bar(to.at), (to.phase & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -537,7 +559,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
     // ------------------------------------------------------------------ query rows, those behind the last one as zeros: two warps
     if (warp == Cfg::kQWarp || warp == Cfg::kQWarp + 1) {
-      constexpr int kPerRow = D / 8, kAtOnce = 4, kLanes = 64;
+      constexpr int kPerRow = D / 8, kAtOnce = 8, kLanes = 64;
       const int first = (warp - Cfg::kQWarp) * 32 + lane;
       for (int seg = 0; w.more(); w.next(), ++seg) {
         ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
@@ -664,7 +686,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       float c = p.scale_log2;
       if (FP8 && a.k_scale) c *= ld_operand(a.k_scale + (a.k_scales > 1 ? w.h : 0));
       const bool whole = w.t0 == 0 && w.t1 == s.key_tiles;
-      if (!whole && w.t0 == 0) begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.key_tiles - w.t1 + line[2] - 1) / line[2])};
+      if (!whole && w.t0 == 0) begun = {s.start, w.qt, w.h, s.n * p.group, 1 + (int)((s.units(kExtraTiles<NT>) - w.end + line[2] - 1) / line[2])};
       const int64_t slot0 = (2 * (int64_t)blockIdx.x + (w.t0 == 0 ? 1 : 0)) * p.row_slots;
       const float v_scale = FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? w.h : 0)) : 1.f;
       const int mine = w.t0 + (Cfg::kTurns ? (int)((g ^ (uint32_t)group) & 1) : 0);  // this group's first tile
@@ -681,7 +703,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           const Place from = place_of(1, kParts * x + part);
           ok = ok && ptx::mbar_wait(full_bar(from.at), from.phase & 1, abort_flag);
           if (!ok || j < prefix || j >= s.len) continue;
-#pragma unroll 1
+#pragma unroll 4
           for (int c8 = 0; c8 < Cfg::kWidth / 8; ++c8) {
             const uint32_t at = sKV + from.at * Cfg::kStage + (c8 >> 3) * (kKeys * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
             uint4 v = ptx::ld_shared_16(at);
