@@ -177,6 +177,9 @@ struct AttnCfg {
   // Warps: two groups of four for the softmax; one issues the output's products, two bring queries, one issues the scores' products; then four that bring keys
   // and four values, or all bring both: eight where an FP8 cache's ring is short, so that a stage is soon widened, four with two stages a tile
   static constexpr int kSoftmaxWarps = 8, kOutputWarp = kSoftmaxWarps, kQWarp = kOutputWarp + 1, kScoreWarp = kOutputWarp + 3, kProducerWarp = kOutputWarp + 4;
+  // (Up to 32 rows the queries of the next row tile are brought while this one ends; more rows take so many loads that the softmax warps, which have
+  // nothing to do until then, bring them themselves: 128 rows 14 thousand clocks by three warps)
+  static constexpr bool kQueryWarps = NT <= 32;
   static constexpr bool kSplit = kParts == 1 && (!FP8 || NT <= 32);
   static constexpr int kProducerWarps = kParts == 1 ? 8 : 4, kWarpKeys = kParts == 1 && !kSplit ? 16 : 32;  // keys of a stage that a warp brings
   static constexpr int kThreads = (kProducerWarp + kProducerWarps) * 32;
@@ -208,7 +211,7 @@ struct Seq {
   __device__ __forceinline__ int64_t length(int heads, int extra) const { return n > 0 ? (int64_t)heads * row_tiles * units(extra) : 0; }
 };
 template <int NT>
-constexpr int kExtraTiles = NT <= 32 ? 2 : 3;
+constexpr int kExtraTiles = NT <= 32 ? 1 : 7;
 template <int NT>
 __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
   const b200_tree_attention_args& a = p.a;
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       ptx::mbar_init(full_bar(s), FP8 ? 128 / Cfg::kWarpKeys : 128);  // warps that have stored, or threads whose copies have landed
       ptx::mbar_init(empty_bar(s), 1);
     }
-    ptx::mbar_init(q_full, 2);
+    ptx::mbar_init(q_full, Cfg::kQueryWarps ? 2 : Cfg::kSoftmaxWarps);
     ptx::mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(o_done(i), 1);
@@ -432,6 +435,40 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   }
   Walk<NT> w(p, *begin_seq, line[0], line[1]);
   bool ok = true;
+
+  // Query rows of the present row tile, those behind the last one as zeros; this warp's share of `lanes` threads begins at `first`
+  auto load_queries = [&](int first, int lanes, int seg) {
+    constexpr int kPerRow = D / 8, kAtOnce = Cfg::kQueryWarps ? 4 : 8;
+    const int rows = min(NT, w.s.n * p.group - w.qt * NT);
+#pragma unroll 1
+    for (int from = first; from < NT * kPerRow; from += kAtOnce * lanes) {
+      uint4 v[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = from + lane + u * lanes, r = min(i / kPerRow, rows - 1), c = i % kPerRow, at = w.qt * NT + r, token = fast_div(at, p.group_div);
+        v[u] = ld_stream_16(static_cast<const T*>(a.q) + (int64_t)(w.s.start + token) * a.q_token + (w.h * p.group + at - token * p.group) * a.q_head + c * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = from + lane + u * lanes, r = i / kPerRow, c = i % kPerRow;
+        if (r >= rows) v[u] = make_uint4(0, 0, 0, 0);
+        if constexpr (kRowScales) {
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&v[u]);
+          float top = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(x[k])), fabsf(__high2float(x[k]))));
+#pragma unroll
+          for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
+          const float by = __uint_as_float((uint32_t)(127 + e) << 23);
+          if (c == 0 && r < NT) row_scale[(seg & 1) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
+          v[u] = make_uint4(pack2<__half>(__low2float(x[0]) * by, __high2float(x[0]) * by), pack2<__half>(__low2float(x[1]) * by, __high2float(x[1]) * by),
+                            pack2<__half>(__low2float(x[2]) * by, __high2float(x[2]) * by), pack2<__half>(__low2float(x[3]) * by, __high2float(x[3]) * by));
+        }
+        if (r < NT) ptx::st_shared_16(sQ + (c >> 3) * (NT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[u]);
+      }
+    }
+  };
 
   if (warp >= Cfg::kProducerWarp) {
     // ------------------------------------------------------------------ keys and values into the ring, a tile's keys, then its values
@@ -557,42 +594,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     grid_launch_dependents();
   } else if (warp >= Cfg::kOutputWarp) {
     ptx::give_registers<Cfg::kOtherRegs, Cfg::kLaunchRegs>();  // the same instruction for the group's four warps
-    // ------------------------------------------------------------------ query rows, those behind the last one as zeros: two warps
-    if (warp == Cfg::kQWarp || warp == Cfg::kQWarp + 1) {
-      constexpr int kPerRow = D / 8, kAtOnce = 8, kLanes = 64;
-      const int first = (warp - Cfg::kQWarp) * 32 + lane;
+    // ------------------------------------------------------------------ queries ahead of their row tile: two warps
+    if (Cfg::kQueryWarps && (warp == Cfg::kQWarp || warp == Cfg::kQWarp + 1)) {
       for (int seg = 0; w.more(); w.next(), ++seg) {
         ok = ptx::mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const int rows = min(NT, w.s.n * p.group - w.qt * NT);
-#pragma unroll 1
-        for (int i0 = first; i0 - lane < NT * kPerRow; i0 += kAtOnce * kLanes) {
-          uint4 v[kAtOnce];
-#pragma unroll
-          for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kLanes, r = min(i / kPerRow, rows - 1), c = i % kPerRow, at = w.qt * NT + r, token = fast_div(at, p.group_div);
-            v[u] = ld_stream_16(static_cast<const T*>(a.q) + (int64_t)(w.s.start + token) * a.q_token + (w.h * p.group + at - token * p.group) * a.q_head + c * 8);
-          }
-#pragma unroll
-          for (int u = 0; u < kAtOnce; ++u) {
-            const int i = i0 + u * kLanes, r = i / kPerRow, c = i % kPerRow;
-            if (r >= rows) v[u] = make_uint4(0, 0, 0, 0);
-            if constexpr (kRowScales) {
-              const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&v[u]);
-              float top = 0.f;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(x[k])), fabsf(__high2float(x[k]))));
-#pragma unroll
-              for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
-              const float by = __uint_as_float((uint32_t)(127 + e) << 23);
-              if (c == 0 && r < NT) row_scale[(seg & 1) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
-              v[u] = make_uint4(pack2<__half>(__low2float(x[0]) * by, __high2float(x[0]) * by), pack2<__half>(__low2float(x[1]) * by, __high2float(x[1]) * by),
-                                pack2<__half>(__low2float(x[2]) * by, __high2float(x[2]) * by), pack2<__half>(__low2float(x[3]) * by, __high2float(x[3]) * by));
-            }
-            if (r < NT) ptx::st_shared_16(sQ + (c >> 3) * (NT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[u]);
-          }
-        }
+        load_queries((warp - Cfg::kQWarp) * 32, 64, seg);
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(q_full);
       }
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           }
           if (ok) ptx::mma_commit(s_full(x));
         }
-        if (ok) ptx::mma_commit(q_empty);
+        if (ok && Cfg::kQueryWarps) ptx::mma_commit(q_empty);
       }
     }
     if (warp == Cfg::kOutputWarp && ptx::elect_one()) {
@@ -680,6 +687,12 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     uint32_t g = 0;  // tiles of this CTA so far
     for (int seg = 0; w.more(); w.next(), ++seg) {
       const Seq& s = w.s;
+      if constexpr (!Cfg::kQueryWarps) {  // (the last scores of the row tile before have been read)
+        load_queries(warp * 32, 256, seg);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(q_full);
+        if (kRowScales) ptx::any_of(kBoth, 256, false);
+      }
       const int rows = min(NT, s.n * p.group - w.qt * NT), prefix = s.len - s.n;
       const int first_token = fast_div(w.qt * NT, p.group_div), last_token = fast_div(w.qt * NT + rows - 1, p.group_div);
       const float* scales = row_scale + (seg & 1) * NT;
@@ -1041,7 +1054,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           const float by = whole ? (sum == 0.f ? 0.f : v_scale / sum) : 1.f;
           f0 *= by, f1 *= by;
           T* const out = static_cast<T*>(a.out) + to * D;
-          float* const partial = p.part_o + (slot0 + r) * D;
+          float* const partial = p.part_o + slot0 * D + r * 4;  // [D / 4][rows][4]: the lanes of a warp store side by side
 #pragma unroll 1
           for (int d = group * (D / 2); d < (group + 1) * (D / 2); d += 16) {  // half of the row each
             uint32_t o0[32], o1[32];
@@ -1061,7 +1074,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
                       make_uint4(pack2<T>(x[i], x[i + 1]), pack2<T>(x[i + 2], x[i + 3]), pack2<T>(x[i + 4], x[i + 5]), pack2<T>(x[i + 6], x[i + 7]));
               } else {
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(partial + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(partial + (d + i) * p.row_slots) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
               }
             }
           }
@@ -1088,7 +1101,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
                 continue;
               const int64_t head = (int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
               if (whole) static_cast<T*>(a.out)[head * D + d] = from_f32<T>(to_f32<T>(static_cast<T*>(a.out)[head * D + d]) + v);
-              else p.part_o[(slot0 + n) * D + d] += v;
+              else p.part_o[Cfg::kRowsInLanes ? slot0 * D + ((d >> 2) * p.row_slots + n) * 4 + (d & 3) : (slot0 + n) * D + d] += v;
             }
           }
         }
@@ -1179,8 +1192,10 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_c
 #pragma unroll 4
       for (int i = 0; i < n; ++i) {
         const float f = __shfl_sync(0xffffffffu, weight, i);
-        const float* src = p.part_o + slot_of(begin + (i0 + i) * step) * D + lane * kPer;
+        const int64_t slot = slot_of(begin + (i0 + i) * step);
         float x[kPer];
+        constexpr bool kRowsInLanes = AttnCfg<D, NT, FP8>::kRowsInLanes;
+        const float* src = p.part_o + (kRowsInLanes ? (slot - r) * D + (lane * kPer / 4 * p.row_slots + r) * 4 + lane * kPer % 4 : slot * D + lane * kPer);
         if constexpr (kPer == 2) {
           x[0] = ld_operand(src), x[1] = ld_operand(src + 1);
         } else {
