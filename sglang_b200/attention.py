@@ -57,6 +57,10 @@ def tree_attention(
     last sequence are not written: they keep what ``out`` held. A page that the cache does not have makes the rows that see it NaN; lengths
     past the page table are cut. Heads of q and of the caches start at multiples of 16 bytes."""
     N.load()
+    if not return_lse:
+        got = N.host.attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, tree_mask, scale, k_scale, v_scale, out)
+        if got is not None:
+            return got
     assert q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16), "q is [tokens, heads, dim], bfloat16 or float16"
     T, heads, dim = q.shape
     assert heads > 0 and dim > 0 and q.stride(2) == 1, "elements of a head are contiguous"

@@ -12,6 +12,7 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <cmath>
 #include <list>
 #include <mutex>
 #include <vector>
@@ -51,6 +52,9 @@ struct Abi {
   decltype(&b200_int8_scaled_mm) int8_mm;
   decltype(&b200_w8a8_int8_linear_workspace_bytes) int8_linear_ws;
   decltype(&b200_w8a8_int8_linear) int8_linear;
+  decltype(&b200_qk_norm_rope) rope;
+  decltype(&b200_tree_attention_workspace_bytes) attention_ws;
+  decltype(&b200_tree_attention) attention;
 } abi;
 
 PyObject* fail(int status, const char* what) {
@@ -544,6 +548,221 @@ PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------ between the qkv and the o_proj linear
+int index_code(at::ScalarType t) { return t == at::kInt ? B200_I32 : t == at::kLong ? B200_I64 : -1; }
+bool optional(PyObject* o, int dev, const Tensor*& t) {  // None, or a plain tensor
+  t = o == Py_None ? nullptr : plain(o, dev);
+  return o == Py_None || t;
+}
+
+// positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved at args[0 .. 4]; a.rows and a.dim are set
+bool rotation(b200_rope_args& a, PyObject* const* args, int dev) {
+  const Tensor *positions, *table;
+  if (!optional(args[0], dev, positions) || !optional(args[1], dev, table) || !positions != !table) return false;
+  if (!positions) return args[3] == Py_None;
+  if (table->dim() != 2 || table->scalar_type() != at::kFloat || table->stride(1) != 1 || table->size(1) > a.dim || table->size(1) % 2) return false;
+  a.rotated = (int)table->size(1);
+  a.positions_dtype = index_code(positions->scalar_type());
+  a.axes = 1;
+  if (args[3] != Py_None) {
+    if (!PyList_CheckExact(args[3]) || PyList_GET_SIZE(args[3]) < 1 || PyList_GET_SIZE(args[3]) > 4) return false;
+    a.sections_interleaved = args[4] == Py_True;
+    if (!a.sections_interleaved && args[4] != Py_False) return false;
+    a.axes = (int)PyList_GET_SIZE(args[3]);
+    int64_t pairs = 0;
+    for (int k = 0; k < a.axes; ++k) {
+      PyObject* n = PyList_GET_ITEM(args[3], k);
+      const long v = PyLong_CheckExact(n) ? PyLong_AsLong(n) : -1;
+      if (v < 0 || v > 256) return false;
+      if (a.sections_interleaved && k > 0 && v > 0 && (v - 1) * a.axes + k >= a.rotated / 2) return false;
+      a.sections[k] = (int)v;
+      pairs += v;
+    }
+    if (pairs != a.rotated / 2 || positions->dim() != 2 || positions->size(0) != a.axes || positions->size(1) != a.rows) return false;
+    a.positions_ld = positions->stride(0);
+  } else if (positions->dim() != 1 || positions->size(0) != a.rows) {
+    return false;
+  }
+  if (a.positions_dtype < 0 || (a.rows > 1 && positions->stride(-1) != 1)) return false;
+  a.positions = positions->data_ptr();
+  a.cos_sin = table->data_ptr<float>();
+  a.cos_sin_ld = table->stride(0);
+  a.table_rows = table->size(0);
+  a.neox = args[2] == Py_True;
+  return args[2] == Py_True || args[2] == Py_False;
+}
+
+// One element or one per kv head; no scale is fine
+bool cache_scale(const Tensor* t, int kv_heads, bool fp8, const float*& p, int& count) {
+  if (!t) return true;
+  if (!fp8 || t->scalar_type() != at::kFloat || !t->is_contiguous() || (t->numel() != 1 && t->numel() != kv_heads)) return false;
+  p = t->data_ptr<float>();
+  count = (int)t->numel();
+  return true;
+}
+bool is_cache(const Tensor& t, int64_t kv_heads, int64_t dim) {
+  return t.dim() == 4 && t.size(0) > 0 && t.size(1) > 0 && t.size(1) <= 0x7fffffff && t.size(2) == kv_heads && t.size(3) == dim && t.stride(3) == 1;
+}
+
+// k_cache, v_cache, slots, k_scale, v_scale; a.rows, a.kv_heads and a.dim are set
+bool caches(b200_rope_args& a, at::ScalarType type, PyObject* const* cache, PyObject* const* scale, int dev) {
+  const Tensor *k = plain(cache[0], dev), *v = plain(cache[1], dev), *slots = plain(cache[2], dev), *ks, *vs;
+  if (!k || !v || !slots || !optional(scale[0], dev, ks) || !optional(scale[1], dev, vs) || !is_cache(*k, a.kv_heads, a.dim) ||
+      !is_cache(*v, a.kv_heads, a.dim) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type())
+    return false;
+  const bool fp8 = k->scalar_type() == kFp8;
+  if ((!fp8 && k->scalar_type() != type) || slots->dim() != 1 || slots->size(0) != a.rows || (a.rows > 1 && slots->stride(0) != 1) ||
+      !cache_scale(ks, a.kv_heads, fp8, a.k_scale, a.k_scales) || !cache_scale(vs, a.kv_heads, fp8, a.v_scale, a.v_scales))
+    return false;
+  a.k_cache = k->data_ptr(), a.v_cache = v->data_ptr();
+  a.k_cache_page = k->stride(0), a.k_cache_token = k->stride(1), a.k_cache_head = k->stride(2);
+  a.v_cache_page = v->stride(0), a.v_cache_token = v->stride(1), a.v_cache_head = v->stride(2);
+  a.pages = k->size(0);
+  a.page_size = (int)k->size(1);
+  a.cache_dtype = fp8 ? B200_E4M3 : dtype_code(type);
+  a.slots = slots->data_ptr();
+  a.slots_dtype = index_code(slots->scalar_type());
+  return a.slots_dtype >= 0;
+}
+
+// qkv_rope(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved, q_weight, k_weight, eps[, k_cache, v_cache,
+// slots, k_scale, v_scale]) -> (q, k), or q where there is a cache
+PyObject* qkv_rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if ((nargs != 11 && nargs != 16) || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor* x = plain(args[0], dev);
+  const long q_heads = PyLong_AsLong(args[1]), kv_heads = PyLong_AsLong(args[2]);
+  const double eps = PyFloat_AsDouble(args[10]);
+  const Tensor *wq, *wk;
+  if (PyErr_Occurred() || !x || !optional(args[8], dev, wq) || !optional(args[9], dev, wk)) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (q_heads <= 0 || kv_heads <= 0 || q_heads > 0x10000 || kv_heads > 0x10000) Py_RETURN_NONE;
+  const int64_t heads = q_heads + 2 * kv_heads;
+  const auto type = x->scalar_type();
+  b200_rope_args a = {};
+  a.dtype = dtype_code(type);
+  if (a.dtype < 0 || x->dim() != 2 || x->size(0) == 0 || x->size(1) == 0 || x->size(1) % heads || x->stride(1) != 1) Py_RETURN_NONE;
+  const int64_t dim = x->size(1) / heads, ld = x->size(0) > 1 ? x->stride(0) : x->size(1);
+  if (dim > 0x10000) Py_RETURN_NONE;
+  a.rows = x->size(0);
+  a.q_heads = (int)q_heads, a.kv_heads = (int)kv_heads, a.dim = (int)dim, a.eps = (float)eps;
+  for (const Tensor* w : {wq, wk})
+    if (w && (w->scalar_type() != type || w->dim() != 1 || w->size(0) != dim || !w->is_contiguous())) Py_RETURN_NONE;
+  if (!rotation(a, args + 3, dev)) Py_RETURN_NONE;
+  const char* base = static_cast<const char*>(x->data_ptr());
+  const int64_t es = (int64_t)x->element_size();
+  a.q = base, a.k = base + q_heads * dim * es;
+  a.q_token = a.k_token = ld, a.q_head = a.k_head = dim;
+  a.q_weight = wq ? wq->data_ptr() : nullptr, a.k_weight = wk ? wk->data_ptr() : nullptr;
+  const bool cached = nargs == 16;
+  if (cached) {
+    a.v = base + (q_heads + kv_heads) * dim * es;
+    a.v_token = ld, a.v_head = dim;
+    if (!caches(a, type, args + 11, args + 14, dev)) Py_RETURN_NONE;
+  }
+  Tensor q, k;
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    q = empty_on(dev, {a.rows, q_heads, dim}, type);
+    if (!cached) k = empty_on(dev, {a.rows, kv_heads, dim}, type);
+    a.q_out = q.data_ptr(), a.k_out = cached ? nullptr : k.data_ptr();
+    rc = abi.rope(&a, stream_of(dev));
+  }
+  if (rc) return fail(rc, cached ? "qk_norm_rope_append" : "qk_norm_rope");
+  if (cached) return THPVariable_Wrap(std::move(q));
+  return pair(std::move(q), std::move(k));
+  END_HANDLE_TH_ERRORS
+}
+
+// append_kv(k, v, k_cache, v_cache, slots, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved, k_scale, v_scale) -> True
+PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 12 || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor *k = plain(args[0], dev), *v = plain(args[1], dev);
+  if (!k || !v || k->dim() != 3 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || k->numel() == 0 || k->stride(2) != 1 ||
+      v->stride(2) != 1 || k->size(1) > 0x10000 || k->size(2) > 0x10000)
+    Py_RETURN_NONE;
+  b200_rope_args a = {};
+  a.dtype = dtype_code(k->scalar_type());
+  a.rows = k->size(0), a.kv_heads = (int)k->size(1), a.dim = (int)k->size(2);
+  if (a.dtype < 0 || !rotation(a, args + 5, dev) || !caches(a, k->scalar_type(), args + 2, args + 10, dev)) Py_RETURN_NONE;
+  a.k = k->data_ptr(), a.k_token = k->stride(0), a.k_head = k->stride(1);
+  a.v = v->data_ptr(), a.v_token = v->stride(0), a.v_head = v->stride(1);
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    rc = abi.rope(&a, stream_of(dev));
+  }
+  if (rc) return fail(rc, "append_paged_kv");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, tree_mask, scale or None, k_scale, v_scale, out or None) -> out. The partial sums live in a
+// block of the caching allocator, not in the stream's scratch: calls captured into two graphs may be replayed at the same time.
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11 || !is_cuda(args[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  const Tensor *q = plain(args[0], dev), *k = plain(args[1], dev), *v = plain(args[2], dev), *pages = plain(args[3], dev, at::kInt),
+               *lens = plain(args[4], dev, at::kInt), *starts, *mask, *ks, *vs, *given;
+  if (!q || !k || !v || !pages || !lens || !optional(args[5], dev, starts) || !optional(args[6], dev, mask) || !optional(args[8], dev, ks) ||
+      !optional(args[9], dev, vs) || !optional(args[10], dev, given))
+    Py_RETURN_NONE;
+  b200_tree_attention_args a = {};
+  const auto type = q->scalar_type();
+  a.dtype = dtype_code(type);
+  if ((a.dtype != B200_BF16 && a.dtype != B200_F16) || q->dim() != 3 || q->numel() == 0 || q->stride(2) != 1 || pages->dim() != 2 || lens->dim() != 1)
+    Py_RETURN_NONE;
+  const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), sequences = pages->size(0);
+  if (heads > 0x10000 || k->dim() != 4 || k->size(2) <= 0 || heads % k->size(2) || !is_cache(*k, k->size(2), dim) || !is_cache(*v, k->size(2), dim) ||
+      k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || sequences == 0 || pages->size(1) == 0 || lens->size(0) != sequences)
+    Py_RETURN_NONE;
+  const bool fp8 = k->scalar_type() == kFp8;
+  if ((!fp8 && k->scalar_type() != type) || (!starts && tokens != sequences) ||
+      (starts && (starts->scalar_type() != at::kInt || starts->dim() != 1 || starts->size(0) != sequences + 1 || !starts->is_contiguous())) ||
+      (mask && (mask->scalar_type() != at::kBool || mask->dim() != 2 || mask->size(0) != tokens || mask->size(1) == 0 || mask->size(1) > 0x7fffffff ||
+                mask->stride(1) != 1)) ||
+      (given && (given->scalar_type() != type || given->sizes() != q->sizes() || !given->is_contiguous())))
+    Py_RETURN_NONE;
+  a.scale = args[7] == Py_None ? (float)(1.0 / std::sqrt((double)dim)) : (float)PyFloat_AsDouble(args[7]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  a.kv_heads = (int)k->size(2);
+  if (!cache_scale(ks, a.kv_heads, fp8, a.k_scale, a.k_scales) || !cache_scale(vs, a.kv_heads, fp8, a.v_scale, a.v_scales)) Py_RETURN_NONE;
+  a.q = q->data_ptr(), a.q_token = q->stride(0), a.q_head = q->stride(1);
+  a.k_cache = k->data_ptr(), a.v_cache = v->data_ptr();
+  a.k_page = k->stride(0), a.k_token = k->stride(1), a.k_head = k->stride(2);
+  a.v_page = v->stride(0), a.v_token = v->stride(1), a.v_head = v->stride(2);
+  a.pages = k->size(0), a.page_size = (int)k->size(1);
+  a.page_table = pages->data_ptr<int32_t>(), a.page_table_ld = pages->stride(0), a.max_pages = pages->size(1);
+  a.seq_lens = lens->data_ptr<int32_t>(), a.q_starts = starts ? starts->data_ptr<int32_t>() : nullptr;
+  if (mask) a.mask = mask->data_ptr(), a.mask_ld = mask->stride(0), a.mask_width = (int)mask->size(1);
+  a.tokens = tokens, a.sequences = sequences;
+  a.q_heads = (int)heads, a.dim = (int)dim, a.cache_dtype = fp8 ? B200_E4M3 : a.dtype;
+  Tensor out;
+  int rc;
+  {
+    WithoutInterpreterLock unlocked;
+    out = given ? *given : empty_on(dev, {tokens, heads, dim}, type);
+    a.out = out.data_ptr();
+    const size_t need = abi.attention_ws(&a);
+    const Tensor ws = need ? empty_on(dev, {(int64_t)need}, at::kByte) : Tensor();
+    rc = abi.attention(&a, need ? ws.data_ptr() : nullptr, need, stream_of(dev));
+  }
+  if (rc) return fail(rc, "tree_attention");
+  if (given) return Py_NewRef(args[10]);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // scratch(device, bytes): the current stream's scratch buffer as a uint8 tensor of at least that size
 PyObject* scratch_tensor(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -621,6 +840,9 @@ PyObject* bind(PyObject*, PyObject* arg) {
   get(abi.int8_mm, "b200_int8_scaled_mm");
   get(abi.int8_linear_ws, "b200_w8a8_int8_linear_workspace_bytes");
   get(abi.int8_linear, "b200_w8a8_int8_linear");
+  get(abi.rope, "b200_qk_norm_rope");
+  get(abi.attention_ws, "b200_tree_attention_workspace_bytes");
+  get(abi.attention, "b200_tree_attention");
   if (!ok) return PyErr_Format(PyExc_ImportError, "%s lacks a symbol of its header", path);
   Py_RETURN_NONE;
 }
@@ -634,6 +856,8 @@ PyMethodDef methods[] = {
     {"acquire", FAST(acquire), nullptr},      {"release", release, METH_O, nullptr},
     {"norm_quant", FAST(norm_quant), nullptr}, {"quant_int8", FAST(quant_int8), nullptr},
     {"int8_mm", FAST(int8_mm), nullptr},      {"int8_linear", FAST(int8_linear), nullptr},
+    {"qkv_rope", FAST(qkv_rope), nullptr},    {"append_kv", FAST(append_kv), nullptr},
+    {"attention", FAST(attention), nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the block-FP8 operators.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -153,6 +153,10 @@ def qk_norm_rope(
     lengths, or with ``mrope_interleaved`` in turn, pair ``j`` axis ``j % axes`` while that has pairs left (``j < axes * section``), else axis 0.
     All in fp32, rounded once. A position outside the table makes its pairs NaN. ``positions`` and ``cos_sin_cache`` None: no rotation."""
     N.load()
+    out = N.host.qkv_rope(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved, q_weight, k_weight,
+                          eps)
+    if out is not None:
+        return out
     a = _qkv_args(qkv, num_heads, num_kv_heads, q_weight, k_weight, eps)
     _set_rotation(a, a.dim, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved)
     N.require_cuda(qkv, positions, cos_sin_cache, q_weight, k_weight)
@@ -185,6 +189,10 @@ def qk_norm_rope_append(
     """``qk_norm_rope`` whose keys, with the values, go straight into a paged cache (``append_paged_kv``): what a layer calls behind its
     qkv linear. Returns q ``[T, num_heads, dim]``; a token without a slot has a q all the same."""
     N.load()
+    out = N.host.qkv_rope(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved, q_weight, k_weight,
+                          eps, k_cache, v_cache, slots, k_scale, v_scale)
+    if out is not None:
+        return out
     a = _qkv_args(qkv, num_heads, num_kv_heads, q_weight, k_weight, eps)
     _set_rotation(a, a.dim, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved)
     a.v, a.v_token, a.v_head = a.k + num_kv_heads * a.dim * qkv.element_size(), a.k_token, a.dim
@@ -220,6 +228,8 @@ def append_paged_kv(
     distinct. An FP8 cache holds ``e4m3(x / scale)``, the quotient and the rotation unrounded, saturated at 448; ``k_scale``, ``v_scale`` fp32 of one
     element or one per kv head (None: 1)."""
     N.load()
+    if N.host.append_kv(k, v, k_cache, v_cache, slots, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved, k_scale, v_scale):
+        return
     assert k.dtype in (torch.bfloat16, torch.float16, torch.float32), f"unsupported input dtype {k.dtype}"
     assert k.dim() == 3 and v.shape == k.shape and v.dtype == k.dtype, "k and v are [tokens, kv heads, dim], alike"
     rows, heads, dim = k.shape

@@ -86,7 +86,8 @@ def test_abi_refuses_before_a_launch():
 def test_workspace():
     size = lambda **f: N.load().b200_tree_attention_workspace_bytes(ctypes.byref(args(**f)))  # noqa: E731
     assert size() > 0 and size(tokens=0) == 0 and size(dim=100) == 0
-    # two pieces of at most 128 rows for each of at most 148 CTAs
-    big = size(tokens=10000, sequences=10000, max_pages=10000, pages=10000)
-    assert big == size(tokens=20000, sequences=20000, max_pages=20000, pages=10000)
-    assert 2 * 148 * 128 * (128 + 2) * 4 <= big < 2 * 148 * 128 * (128 + 2) * 4 + 16384
+    # two pieces of a row tile for each of at most 148 CTAs: 16 rows where a sequence has 4, 128 where it may have more than 64
+    for rows, f in ((16, {}), (128, dict(q_starts=64)), (32, dict(q_starts=64, mask=64, mask_width=7))):
+        big = size(tokens=100000, sequences=1000, max_pages=10000, pages=10000, **f)
+        assert big == size(tokens=200000, sequences=2000, max_pages=20000, pages=10000, **f)
+        assert 2 * 148 * rows * (128 + 2) * 4 <= big < 2 * 148 * rows * (128 + 2) * 4 + 16384
