@@ -5,6 +5,8 @@
 //           or 2j and 2j + 1; elements from R on pass. With several axes every pair takes the row of its own axis' position.
 //   hold    the cache's type, or e4m3(y / scale) by the IEEE quotient
 // All in fp32 from the 16-bit input to the one rounding of the result: a 16-bit value between norm and rotation would add its half step.
+#include <type_traits>
+
 #include "int8_round.cuh"
 
 namespace b200 {
@@ -13,6 +15,7 @@ struct RopeParams {
   b200_rope_args a;
   uint32_t axis_of[16];  // 2 bits per pair, 16 pairs a word
   int split;             // warps per token
+  FastDiv split_div;
   int per_warp;          // heads of one of them
   int page_shift;        // log2 of the page size, -1: not a power of two
 };
@@ -53,24 +56,59 @@ __device__ __forceinline__ float scaled(float x, float s, float r) {
 
 enum HeadKind { HEAD_Q = 0, HEAD_K = 1, HEAD_V = 2 };
 
-// Eight 16-bit elements
-template <typename T>
-struct Vec8 {
-  uint4 v;
-  __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T*>(&v)[i]); }
-  __device__ __forceinline__ void set(int i, float f) { reinterpret_cast<T*>(&v)[i] = from_f32<T>(f); }
+// Two fp32 values in one register pair, and the operations that take both at once: half the instructions of the norm and the rotation.
+struct Two {
+  uint64_t v;
+  __device__ __forceinline__ Two() = default;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
 };
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// Two 16-bit values of a word, lowest first, and back
+template <typename T>
+__device__ __forceinline__ Two widen(uint32_t w) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return Two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return Two(f.x, f.y);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow(Two t) {
+  const float2 f = t.get();
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
 
 // LANES lanes of a warp per head, two vectors of eight elements per lane. Elements j and j + R / 2 of a pair lie in the lane's two vectors
-// (NEOX), or pairs lie within a vector. A warp takes 32 / LANES heads of one token at a time, UNROLL times that are under way together; angles and
-// weights stay in its registers for all heads of the token.
+// (NEOX), or pairs lie within a vector. A warp takes 32 / LANES heads of one token at a time, UNROLL times that are under way together, first those of q, then
+// of k, then of v; the angles stay in its registers for all of them.
+// Bound by the latency between a token's position, its angles and its heads, so what counts are heads under way: 80 registers and two steps a warp hide more than
+// 124 and four (16384 x 72 heads of 128, three axes: 129 us, 4.75 TB/s, against 133; into an FP8 cache, 8192 x 48: 57 against 63), 64 registers or asking
+// for all steps of a batch after the last of the one before less (156, 150).
 template <typename T, int LANES, bool NEOX, int UNROLL>
-__global__ void __launch_bounds__(256) rope_heads_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(256, 3) rope_heads_kernel(const __grid_constant__ RopeParams p) {
   const b200_rope_args& a = p.a;
   grid_launch_dependents();
   const int64_t zero = grid_dependency_zero();
-  const int64_t warp = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t row = warp / p.split + zero;
+  const int warp = (int)(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5));
+  const int64_t row = fast_div(warp, p.split_div) + zero;
   if (row >= a.rows) return;
   constexpr int kTeams = 32 / LANES;
   const int lane = threadIdx.x % LANES, team = (threadIdx.x & 31) / LANES;
@@ -79,39 +117,19 @@ __global__ void __launch_bounds__(256) rope_heads_kernel(const __grid_constant__
   const int va = turned ? lane : lane + P, vb = turned ? lane + P : va + rest;
   const bool has_a = lane < P + rest, has_b = has_a && vb < nvec;
   const int nq = a.q ? a.q_heads : 0, nk = a.k ? a.kv_heads : 0, total = nq + nk + (a.v ? a.kv_heads : 0);
-  const int first = (int)(warp % p.split) * p.per_warp, last = min(first + p.per_warp, total);
+  const int first = (warp - (int)row * p.split) * p.per_warp, last = min(first + p.per_warp, total);
 
-  auto kind_of = [&](int h) { return h < nq ? HEAD_Q : h < nq + nk ? HEAD_K : HEAD_V; };
-  auto load = [&](int h, Vec8<T> (&x)[2]) {
-    x[0].v = x[1].v = make_uint4(0, 0, 0, 0);
-    if (h >= last) return;
-    const int kind = kind_of(h);
-    const T* src = kind == HEAD_Q   ? static_cast<const T*>(a.q) + row * a.q_token + h * a.q_head
-                   : kind == HEAD_K ? static_cast<const T*>(a.k) + row * a.k_token + (h - nq) * a.k_head
-                                    : static_cast<const T*>(a.v) + row * a.v_token + (h - nq - nk) * a.v_head;
-    if (has_a) x[0].v = ld_stream_16(src + va * 8);
-    if (has_b) x[1].v = ld_stream_16(src + vb * 8);
+  auto load = [&](const T* src, int h, int end, uint4 (&x)[2]) {
+    x[0] = x[1] = make_uint4(0, 0, 0, 0);
+    if (h < end && has_a) x[0] = ld_stream_16(src + va * 8);
+    if (h < end && has_b) x[1] = ld_stream_16(src + vb * 8);
   };
-  Vec8<T> x[UNROLL][2];
-#pragma unroll
-  for (int u = 0; u < UNROLL; ++u) load(first + u * kTeams + team, x[u]);
-
-  Vec8<T> w[2][2];
-  const bool norm_q = a.q_weight != nullptr, norm_k = a.k_weight != nullptr;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const T* src = static_cast<const T*>(k ? a.k_weight : a.q_weight) + zero;
-    w[k][0].v = w[k][1].v = make_uint4(0, 0, 0, 0);
-    if ((k ? norm_k : norm_q) && first < nq + nk) {
-      if (has_a) w[k][0].v = ld_again_16(src + va * 8);
-      if (has_b) w[k][1].v = ld_again_16(src + vb * 8);
-    }
-  }
   // NEOX: c, s of pairs 8 lane .. 8 lane + 7; else of pairs 4 va .. and 4 vb ..
   float c[8], s[8];
+  auto load_angles = [&] {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
-  if (a.rotated > 0 && first < nq + nk) {
+    for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+    if (a.rotated == 0) return;
     const int pairs = a.rotated >> 1;
     const float* rows[4];
 #pragma unroll
@@ -141,85 +159,125 @@ __global__ void __launch_bounds__(256) rope_heads_kernel(const __grid_constant__
         }
       }
     }
-  }
+  };
   SlotAt at = {0, 0};
-  const bool cached = a.k_cache != nullptr, keep = cached && slot_at(p, row, at);
+  const bool cached = a.k_cache != nullptr;
+  bool keep = false, placed = false, angled = false;
 
-  auto finish = [&](int h, Vec8<T> (&x)[2]) {
-    const int kind = kind_of(h);
-    float f[16];
+  // The heads [lo, hi) of one kind that are this warp's
+  auto heads = [&](auto kind_of, const void* from, int64_t token, int64_t head, const void* norm, int lo, int hi) {
+    constexpr int kind = decltype(kind_of)::value;
+    if (lo >= hi) return;
+    const T* const src = static_cast<const T*>(from) + row * token + zero;
+    const bool normed = kind != HEAD_V && norm != nullptr;
+    uint4 x[UNROLL][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = x[0].get(i), f[8 + i] = x[1].get(i);
-    const bool norm = kind == HEAD_Q ? norm_q : kind == HEAD_K && norm_k;
-    if (norm_q || norm_k) {  // every lane of the warp takes part in the sums
-      float sum = 0.f;
+    for (int u = 0; u < UNROLL; ++u) load(src + (lo + u * kTeams + team) * head, lo + u * kTeams + team, hi, x[u]);
+    Two w[8];
+    if (normed) {
+      uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      const T* const weights = static_cast<const T*>(norm) + zero;
+      if (has_a) raw[0] = ld_again_16(weights + va * 8);
+      if (has_b) raw[1] = ld_again_16(weights + vb * 8);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum = fmaf(f[i], f[i], sum);
+      for (int i = 0; i < 8; ++i) w[i] = widen<T>(reinterpret_cast<const uint32_t*>(raw)[i]);
+    }
+    if (kind != HEAD_V && !angled) {
+      load_angles();
+      angled = true;
+    }
+    if (kind != HEAD_Q && cached && !placed) {
+      keep = slot_at(p, row, at);
+      placed = true;
+    }
+    const bool to_cache = kind != HEAD_Q && cached;
+    const float* const scales = to_cache && a.cache_dtype == B200_E4M3 ? (kind == HEAD_K ? a.k_scale : a.v_scale) : nullptr;
+    const bool one_scale = (kind == HEAD_K ? a.k_scales : a.v_scales) <= 1;
+
+    auto finish = [&](int h, const uint4 (&v)[2]) {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(v);
+      if (kind == HEAD_V && !(to_cache && a.cache_dtype == B200_E4M3)) {  // copied
+        if (h >= hi || !has_a || !keep) return;
+        T* dst = static_cast<T*>(a.v_cache) + at.v + h * a.v_cache_head;
+        *reinterpret_cast<uint4*>(dst + va * 8) = v[0];
+        if (has_b) *reinterpret_cast<uint4*>(dst + vb * 8) = v[1];
+        return;
+      }
+      Two f[8];
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (norm) {
+      for (int i = 0; i < 8; ++i) f[i] = widen<T>(words[i]);
+      if (normed) {  // every lane of the warp takes part in the sums
+        Two sq = mul(f[0], f[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) sq = fma(f[i], f[i], sq);
+        const float2 both = sq.get();
+        float sum = both.x + both.y;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float r = rsqrtf(sum / (float)a.dim + a.eps);
+        const Two rr(r, r);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const Vec8<T>& wq = w[0][i >> 3];
-          const Vec8<T>& wk = w[1][i >> 3];
-          f[i] *= r * (kind == HEAD_Q ? wq.get(i & 7) : wk.get(i & 7));
+        for (int i = 0; i < 8; ++i) f[i] = mul(f[i], mul(rr, w[i]));
+      }
+      if (h >= hi || !has_a) return;
+      if (kind != HEAD_V) {
+        if constexpr (NEOX) {
+          if (turned) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const Two e = f[i], o = f[i + 4], cc(c[2 * i], c[2 * i + 1]), ss(s[2 * i], s[2 * i + 1]), minus(-s[2 * i], -s[2 * i + 1]);
+              f[i] = fma(o, minus, mul(e, cc));
+              f[i + 4] = fma(e, ss, mul(o, cc));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if ((i < 4 ? va : vb) * 8 >= a.rotated) continue;  // elements that pass keep their bits beside an infinity
+            const float2 e = f[i].get();
+            f[i] = Two(e.x * c[i] - e.y * s[i], e.y * c[i] + e.x * s[i]);
+          }
         }
       }
-    }
-    if (h >= last || !has_a) return;
-    if (kind != HEAD_V) {
+      if (to_cache && a.cache_dtype == B200_E4M3) {
+        if (!keep) return;
+        float y[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float& e = f[NEOX ? i : 2 * i];
-        float& o = f[NEOX ? i + 8 : 2 * i + 1];
-        if (NEOX ? turned : (i < 4 ? va : vb) * 8 < a.rotated) {  // elements that pass keep their bits beside an infinity
-          const float e0 = e, o0 = o;
-          e = e0 * c[i] - o0 * s[i];
-          o = o0 * c[i] + e0 * s[i];
+        for (int i = 0; i < 8; ++i) {
+          const float2 e = f[i].get();
+          y[2 * i] = e.x, y[2 * i + 1] = e.y;
         }
-      }
-    }
-    if (kind == HEAD_Q || !cached) {
+        if (scales) {
+          const float d = ld_operand(scales + (one_scale ? 0 : h)), r = __frcp_rn(d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[0].set(i, f[i]), x[1].set(i, f[8 + i]);
+          for (int i = 0; i < 16; ++i) y[i] = scaled(y[i], d, r);
+        }
+        uint8_t* dst = kind == HEAD_K ? static_cast<uint8_t*>(a.k_cache) + at.k + h * a.k_cache_head : static_cast<uint8_t*>(a.v_cache) + at.v + h * a.v_cache_head;
+        *reinterpret_cast<uint2*>(dst + va * 8) = make_uint2(pack4_e4m3(y[0], y[1], y[2], y[3]), pack4_e4m3(y[4], y[5], y[6], y[7]));
+        if (has_b)
+          *reinterpret_cast<uint2*>(dst + vb * 8) = make_uint2(pack4_e4m3(y[8], y[9], y[10], y[11]), pack4_e4m3(y[12], y[13], y[14], y[15]));
+        return;
+      }
+      if (to_cache && !keep) return;
       T* dst = kind == HEAD_Q ? static_cast<T*>(a.q_out) + (row * a.q_heads + h) * a.dim
-                              : static_cast<T*>(a.k_out) + (row * a.kv_heads + (h - nq)) * a.dim;
-      *reinterpret_cast<uint4*>(dst + va * 8) = x[0].v;
-      if (has_b) *reinterpret_cast<uint4*>(dst + vb * 8) = x[1].v;
-      return;
-    }
-    if (!keep) return;
-    const int g = kind == HEAD_K ? h - nq : h - nq - nk;
-    const int64_t to = kind == HEAD_K ? at.k + g * a.k_cache_head : at.v + g * a.v_cache_head;
-    if (a.cache_dtype != B200_E4M3) {
+               : to_cache     ? static_cast<T*>(a.k_cache) + at.k + h * a.k_cache_head
+                              : static_cast<T*>(a.k_out) + (row * a.kv_heads + h) * a.dim;
+      *reinterpret_cast<uint4*>(dst + va * 8) = make_uint4(narrow<T>(f[0]), narrow<T>(f[1]), narrow<T>(f[2]), narrow<T>(f[3]));
+      if (has_b) *reinterpret_cast<uint4*>(dst + vb * 8) = make_uint4(narrow<T>(f[4]), narrow<T>(f[5]), narrow<T>(f[6]), narrow<T>(f[7]));
+    };
+    // A head's place is asked for anew as soon as the one before it is done, so that UNROLL steps are always under way
+    for (int h0 = lo; h0 < hi; h0 += UNROLL * kTeams) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[0].set(i, f[i]), x[1].set(i, f[8 + i]);
-      T* dst = static_cast<T*>(kind == HEAD_K ? a.k_cache : a.v_cache) + to;
-      *reinterpret_cast<uint4*>(dst + va * 8) = x[0].v;
-      if (has_b) *reinterpret_cast<uint4*>(dst + vb * 8) = x[1].v;
-    } else {
-      const float* scales = kind == HEAD_K ? a.k_scale : a.v_scale;
-      if (scales) {
-        const float d = ld_operand(scales + ((kind == HEAD_K ? a.k_scales : a.v_scales) > 1 ? g : 0)), r = __frcp_rn(d);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = scaled(f[i], d, r);
+      for (int u = 0; u < UNROLL; ++u) {
+        const int h = h0 + u * kTeams + team, next = h + UNROLL * kTeams;
+        finish(h, x[u]);
+        load(src + next * head, next, hi, x[u]);
       }
-      uint8_t* dst = static_cast<uint8_t*>(kind == HEAD_K ? a.k_cache : a.v_cache) + to;
-      *reinterpret_cast<uint2*>(dst + va * 8) = make_uint2(pack4_e4m3(f[0], f[1], f[2], f[3]), pack4_e4m3(f[4], f[5], f[6], f[7]));
-      if (has_b)
-        *reinterpret_cast<uint2*>(dst + vb * 8) = make_uint2(pack4_e4m3(f[8], f[9], f[10], f[11]), pack4_e4m3(f[12], f[13], f[14], f[15]));
     }
   };
-
-  for (int h0 = first; h0 < last; h0 += UNROLL * kTeams) {
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) finish(h0 + u * kTeams + team, x[u]);
-    if (h0 + UNROLL * kTeams < last) {
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) load(h0 + (UNROLL + u) * kTeams + team, x[u]);
-    }
-  }
+  heads(std::integral_constant<int, HEAD_Q>(), a.q, a.q_token, a.q_head, a.q_weight, min(first, nq), min(last, nq));
+  heads(std::integral_constant<int, HEAD_K>(), a.k, a.k_token, a.k_head, a.k_weight, max(first - nq, 0), min(last - nq, nk));
+  heads(std::integral_constant<int, HEAD_V>(), a.v, a.v_token, a.v_head, nullptr, max(first - nq - nk, 0), last - nq - nk);
 }
 
 // Any width, alignment and type: a warp per head, an element per lane at a time, read twice (once for the norm).
@@ -296,7 +354,7 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ R
 
 template <typename T, int LANES>
 static int launch_heads(RopeParams& p, int total, cudaStream_t st) {
-  constexpr int kTeams = 32 / LANES, kUnroll = 4;
+  constexpr int kTeams = 32 / LANES, kUnroll = 2;
   // Few tokens: a warp for every step of heads, so that all loads leave at once; many: a warp keeps a token's angles for all of its heads
   const int64_t steps = cdiv(total, kTeams);
   int64_t split = cdiv(148 * 32, p.a.rows);
@@ -305,7 +363,8 @@ static int launch_heads(RopeParams& p, int total, cudaStream_t st) {
   p.split = (int)cdiv(total, p.per_warp);
   const unsigned threads = p.a.rows * p.split >= 148 * 8 ? 256 : 128;
   const int64_t blocks = cdiv(p.a.rows * p.split, threads / 32);
-  B200_UNSUPPORTED(blocks > 0x7fffffffLL, "rope: too many rows");
+  B200_UNSUPPORTED(p.a.rows * p.split > 0x7ffffff0LL, "qk_norm_rope: too many rows");
+  p.split_div = make_fastdiv(p.split);
   const dim3 grid((unsigned)blocks);
   return p.a.neox ? launch_dependent(rope_heads_kernel<T, LANES, true, kUnroll>, grid, threads, 0, st, 1, "qk_norm_rope", p)
                   : launch_dependent(rope_heads_kernel<T, LANES, false, kUnroll>, grid, threads, 0, st, 1, "qk_norm_rope", p);
@@ -334,7 +393,7 @@ static int launch_rope(RopeParams& p, cudaStream_t st) {
     }
   }
   const int64_t blocks = cdiv(a.rows * total, 8);
-  B200_UNSUPPORTED(blocks > 0x7fffffffLL, "rope: too many rows");
+  B200_UNSUPPORTED(blocks > 0x7fffffffLL, "qk_norm_rope: too many rows");
   return launch_dependent(rope_any_kernel<T>, dim3((unsigned)blocks), 256, 0, st, 1, "qk_norm_rope", p);
 }
 
