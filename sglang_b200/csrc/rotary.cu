@@ -214,10 +214,10 @@ __global__ void __launch_bounds__(256, 3) rope_heads_kernel(const __grid_constan
         float sum = both.x + both.y;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float r = rsqrtf(sum / (float)a.dim + a.eps);
+        const float r = __frsqrt_rn(sum / (float)a.dim + a.eps);
         const Two rr(r, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = mul(f[i], mul(rr, w[i]));
+        for (int i = 0; i < 8; ++i) f[i] = mul(mul(f[i], rr), w[i]);
       }
       if (h >= hi || !has_a) return;
       if (kind != HEAD_V) {
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ R
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    r = rsqrtf(sum / (float)a.dim + a.eps);
+    r = __frsqrt_rn(sum / (float)a.dim + a.eps);
   }
   SlotAt at = {0, 0};
   const bool cached = a.k_cache != nullptr && kind != HEAD_Q;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ R
   }
   auto normed = [&](int i) {
     const float f = element(x, i);
-    return w ? f * (r * element(w, i)) : f;
+    return w ? f * r * element(w, i) : f;
   };
   const int pairs = a.rotated >> 1;
   for (int i = lane; i < a.dim; i += 32) {
