@@ -18,9 +18,11 @@ from typing import List, Optional
 import torch
 
 from . import _native as N
+from . import attention as _attn
 from . import fp8_kernel as _q
 from . import int8_kernel as _i8
 from . import layernorm as _norm
+from . import rotary as _rope
 from . import topk as _topk
 from .fused_moe import fused_experts_impl as _experts
 from .moe_align_block_size import sgl_moe_align_block_size as _align_into
@@ -41,6 +43,16 @@ SCHEMAS = {
     "rmsnorm_quant_int8": "(Tensor x, Tensor weight, float eps, Tensor? residual=None) -> Tensor[]",
     "rmsnorm_quant_fp8": "(Tensor x, Tensor weight, int group_size, float eps, Tensor? residual=None, "
     "bool column_major_scales=False, bool scale_tma_aligned=False, bool scale_ue8m0=False) -> Tensor[]",
+    "qk_norm_rope": "(Tensor qkv, int num_heads, int num_kv_heads, Tensor? positions, Tensor? cos_sin_cache, Tensor? q_weight=None, "
+    "Tensor? k_weight=None, float eps=1e-6, bool is_neox=True, int[]? mrope_section=None, bool mrope_interleaved=False) -> (Tensor, Tensor)",
+    "qk_norm_rope_append": "(Tensor qkv, int num_heads, int num_kv_heads, Tensor? positions, Tensor? cos_sin_cache, Tensor(a!) k_cache, "
+    "Tensor(b!) v_cache, Tensor slots, Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-6, bool is_neox=True, "
+    "int[]? mrope_section=None, bool mrope_interleaved=False, Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor",
+    "append_paged_kv": "(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, Tensor? positions=None, "
+    "Tensor? cos_sin_cache=None, bool is_neox=True, int[]? mrope_section=None, bool mrope_interleaved=False, Tensor? k_scale=None, "
+    "Tensor? v_scale=None) -> ()",
+    "tree_attention": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor seq_lens, Tensor? q_starts=None, "
+    "Tensor? tree_mask=None, float? scale=None, Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor",
     "moe_align_block_size": "(Tensor topk_ids, int num_experts, int block_size, Tensor(a!) sorted_token_ids, "
     "Tensor(b!) experts_ids, Tensor(c!) num_tokens_post_pad, Tensor(d!) cumsum_buffer, bool pad_sorted_token_ids) "
     "-> ()",
@@ -221,6 +233,57 @@ def _norm_fp8_fake(x, weight, group_size, eps, residual=None, column_major_scale
            _q.create_per_token_group_quant_fp8_output_scale(x.shape, x.device, group_size, column_major_scales, scale_tma_aligned,
                                                             scale_ue8m0)]
     return out if residual is None else out + [x.new_empty(x.shape)]
+
+
+# ------------------------------------------------------------------- between the qkv and the o_proj linear
+
+@_impl("qk_norm_rope")
+def _qk_norm_rope(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, q_weight=None, k_weight=None, eps=1e-6, is_neox=True, mrope_section=None,
+                  mrope_interleaved=False):
+    return _rope.qk_norm_rope(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, q_weight, k_weight, eps, is_neox, mrope_section,
+                              mrope_interleaved)
+
+
+@_fake("qk_norm_rope")
+def _qk_norm_rope_fake(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, q_weight=None, k_weight=None, eps=1e-6, is_neox=True,
+                       mrope_section=None, mrope_interleaved=False):
+    dim = qkv.shape[1] // (num_heads + 2 * num_kv_heads)
+    return qkv.new_empty((qkv.shape[0], num_heads, dim)), qkv.new_empty((qkv.shape[0], num_kv_heads, dim))
+
+
+@_impl("qk_norm_rope_append")
+def _qk_norm_rope_append(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, k_cache, v_cache, slots, q_weight=None, k_weight=None, eps=1e-6,
+                         is_neox=True, mrope_section=None, mrope_interleaved=False, k_scale=None, v_scale=None):
+    return _rope.qk_norm_rope_append(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, k_cache, v_cache, slots, q_weight, k_weight, eps,
+                                     is_neox, mrope_section, mrope_interleaved, k_scale, v_scale)
+
+
+@_fake("qk_norm_rope_append")
+def _qk_norm_rope_append_fake(qkv, num_heads, num_kv_heads, positions, cos_sin_cache, k_cache, v_cache, slots, q_weight=None, k_weight=None,
+                              eps=1e-6, is_neox=True, mrope_section=None, mrope_interleaved=False, k_scale=None, v_scale=None):
+    return qkv.new_empty((qkv.shape[0], num_heads, qkv.shape[1] // (num_heads + 2 * num_kv_heads)))
+
+
+@_impl("append_paged_kv")
+def _append_paged_kv(k, v, k_cache, v_cache, slots, positions=None, cos_sin_cache=None, is_neox=True, mrope_section=None, mrope_interleaved=False,
+                     k_scale=None, v_scale=None):
+    _rope.append_paged_kv(k, v, k_cache, v_cache, slots, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved, k_scale, v_scale)
+
+
+@_fake("append_paged_kv")
+def _append_paged_kv_fake(k, v, k_cache, v_cache, slots, positions=None, cos_sin_cache=None, is_neox=True, mrope_section=None,
+                          mrope_interleaved=False, k_scale=None, v_scale=None):
+    return None
+
+
+@_impl("tree_attention")
+def _tree_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts=None, tree_mask=None, scale=None, k_scale=None, v_scale=None):
+    return _attn.tree_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, tree_mask, scale, k_scale, v_scale)
+
+
+@_fake("tree_attention")
+def _tree_attention_fake(q, k_cache, v_cache, page_table, seq_lens, q_starts=None, tree_mask=None, scale=None, k_scale=None, v_scale=None):
+    return q.new_empty(q.shape)
 
 
 # ------------------------------------------------------------------------------------------ align

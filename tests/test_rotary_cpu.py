@@ -105,3 +105,20 @@ def test_abi_refuses_before_a_launch():
     assert lib.b200_qk_norm_rope(ctypes.addressof(a), None) == bad
     a = RopeArgs(rows=0, q_heads=2, kv_heads=1, dim=64, dtype=N.BF16)
     assert lib.b200_qk_norm_rope(ctypes.addressof(a), None) == 0
+
+
+def test_fake_implementations_describe_the_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import sglang_b200.custom_ops  # noqa: F401
+
+    ops = torch.ops.sglang_b200
+    with FakeTensorMode():
+        x = torch.empty(5, 12 * 64, dtype=BF, device="cuda")
+        cache = torch.empty(4, 16, 2, 64, dtype=BF, device="cuda")
+        index = torch.empty(5, dtype=torch.int32, device="cuda")
+        q, k = ops.qk_norm_rope(x, 8, 2, None, None)
+        assert q.shape == (5, 8, 64) and k.shape == (5, 2, 64) and q.dtype == BF
+        assert ops.qk_norm_rope_append(x, 8, 2, None, None, cache, cache.clone(), index).shape == (5, 8, 64)
+        assert ops.append_paged_kv(k, k, cache, cache.clone(), index) is None
+        assert ops.tree_attention(q, cache, cache, torch.empty(5, 3, dtype=torch.int32, device="cuda"), index).shape == q.shape
