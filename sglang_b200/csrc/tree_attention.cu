@@ -976,8 +976,6 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             if (s.n > 1 || a.mask) check_values(t);
             ptx::any_of(bar, 128, false);
           }
-          // the product that was in this buffer before is complete: waited for in every tile, so that a wait is never for a phase two ahead
-          if (x_tile >= 2) ok = ok && ptx::mbar_wait(o_done(own), (phase - 1) & 1, abort_flag);
           if (busy) {
             uint32_t v[2][32];
 #pragma unroll
@@ -1005,6 +1003,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
               const float f = move ? ptx::ex2(m - largest) : 1.f;
               if (move) m = largest;
               l *= f;
+              // (not for a phase two ahead: the scores of the tile before were asked for behind the product before this one)
               ok = ok && ptx::mbar_wait(o_done(own ^ 1), ((x_tile - 1) >> 1) & 1, abort_flag);
               ptx::tc_fence_after();
 #pragma unroll 1
@@ -1127,24 +1126,26 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 
 // Rows whose keys were cut: adds up their pieces, in the order of the line. Every block reads the list of cut tiles and takes its share of their rows: eight at a
 // time, a warp each, or where a tile was cut into many pieces one at a time, each warp with some of them.
-constexpr int kManyParts = 8, kJoinBlocks = 296;
+constexpr int kManyParts = 8, kJoinBlocks = 740;  // (five to an SM)
 template <typename T, int D, int NT, bool FP8>
 __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_constant__ AttnParams p, int ctas) {
   const b200_tree_attention_args& a = p.a;
   constexpr int kPer = D / 32;  // elements per lane
   __shared__ int ends[256];     // units of work up to each CTA's tile
+  __shared__ SplitRows list[256];
   __shared__ int warp_sum[8];
   __shared__ float part_acc[8][D], part_m[8], part_sum[8];
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto field = [&](int cta, int i) { return ld_operand(reinterpret_cast<const int32_t*>(p.split + cta) + i); };
-  auto rows_of = [&](int rows, int qt) { return min(NT, rows - qt * NT); };
+  auto rows_of = [&](const SplitRows& t) { return min(NT, t.rows - t.qt * NT); };
   {
     int units = 0;
     if ((int)threadIdx.x < ctas) {
-      const int parts = field(threadIdx.x, 4), rows = rows_of(field(threadIdx.x, 3), field(threadIdx.x, 1));
-      units = parts == 0 ? 0 : parts > kManyParts ? rows : (rows + 7) / 8;
+      const int32_t* from = reinterpret_cast<const int32_t*>(p.split + threadIdx.x);
+      const SplitRows t = {ld_operand(from), ld_operand(from + 1), ld_operand(from + 2), ld_operand(from + 3), ld_operand(from + 4)};
+      list[threadIdx.x] = t;
+      units = t.parts == 0 ? 0 : t.parts > kManyParts ? rows_of(t) : (rows_of(t) + 7) / 8;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1163,10 +1164,11 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_c
     for (int step = 128; step > 0; step >>= 1)
       if (ends[cta + step - 1] <= unit) cta += step;
     const int index = unit - (cta ? ends[cta - 1] : 0);
-    const int start = field(cta, 0), qt = field(cta, 1), h = field(cta, 2), all = field(cta, 3), parts = field(cta, 4);
+    const SplitRows tile = list[cta];
+    const int parts = tile.parts;
     const bool many = parts > kManyParts;
     const int r = many ? index : index * 8 + warp;
-    const bool here = r < rows_of(all, qt);
+    const bool here = r < rows_of(tile);
     const int step = many ? 8 : 1, begin = many ? warp : 0;  // pieces begin, begin + step, ..
     auto slot_of = [&](int i) { return (2 * (int64_t)(cta + i) + (i == 0 ? 1 : 0)) * p.row_slots + r; };
     float m = -kNoRef, sum = 0.f, acc[kPer];
@@ -1230,9 +1232,9 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(const __grid_c
       }
     }
     if (here && (!many || warp == 0)) {
-      const int row = qt * NT + r, token = fast_div(row, p.group_div), head = h * p.group + row - token * p.group;
-      const int64_t to = (int64_t)(start + token) * a.q_heads + head;
-      const float inv = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? h : 0)) : 1.f) / sum;
+      const int row = tile.qt * NT + r, token = fast_div(row, p.group_div), head = tile.head * p.group + row - token * p.group;
+      const int64_t to = (int64_t)(tile.token + token) * a.q_heads + head;
+      const float inv = sum == 0.f ? 0.f : (FP8 && a.v_scale ? ld_operand(a.v_scale + (a.v_scales > 1 ? tile.head : 0)) : 1.f) / sum;
       T* dst = static_cast<T*>(a.out) + to * D + lane * kPer;
 #pragma unroll
       for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(acc[k] * inv, acc[k + 1] * inv);
