@@ -4,12 +4,18 @@
 // tile and the rows are its columns, so that few rows cost little:
 //   S^T [128 keys, NT] = K Q^T     K and Q in shared memory, S^T in TMEM, two buffers
 //   O^T [D, NT]       += V^T P^T   V as it lies in the cache (its rows are the product's depth), P^T [keys, NT] in shared memory
-// (More than 64 rows: the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: softmax rows are a
-// thread's own, and P needs no shared memory.) A thread of the softmax has one key and NT columns. It takes its exponentials against a reference per row that is moved only when a score exceeds
-// it by 2^8, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end.
-// Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies (of an FP8 cache into a ring of codes, which become
-// fp16 values, exactly, on their way into the ring of tiles). All tiles of all (sequence, kv head, row tile) form one line that is cut into equal pieces, one per CTA, so that ragged
-// lengths leave no SM idle; rows whose keys were cut leave partial sums in a workspace, which a second kernel joins in the line's order.
+// A thread of the softmax has one key and the rows' columns. It takes its exponentials against a reference per row that is moved only when a score
+// exceeds it by 2^8, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end. With more than
+// 64 rows the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: a softmax row is a thread's own,
+// and P needs no shared memory.
+// Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies; codes of an FP8 cache land in a ring of their own and
+// become fp16 values, exactly, on their way into the ring of tiles. All tiles of all (sequence, kv head, row tile) form one line that is cut into equal
+// pieces, one per CTA, so that ragged lengths leave no SM idle; rows whose keys were cut leave partial sums in a workspace, which a second kernel joins in
+// the line's order.
+// Few rows over a 16-bit cache are bound by its bytes: 128 sequences of up to 8192 tokens, 8 kv heads of 128, one token a page, 2.17 GB: 330 us, 6.6 TB/s; 16 of up
+// to 16384 with 8 drafted tokens, 64 query heads (64 rows), 597 MB: 127 us, 4.7 TB/s. An FP8 cache is bound by the way of its codes through the SM, copied,
+// read, widened and stored: 64 sequences of up to 16384, one token, 1.08 GB: 240 us, 4.5 TB/s. 128 rows by the exponentials, 16 a clock and SM, and by the latency of
+// the steps between two products: 61 sequences of up to 32768, 16 tokens, FP8, 264 MB: 117 us, 535 TFLOP/s.
 #include "gemm_host.cuh"
 #include "int8_round.cuh"
 
@@ -172,8 +178,8 @@ struct AttnCfg {
   static constexpr bool kRowsInLanes = NT == 128, kTurns = NT <= 32, kTwoO = NT != 64;
   static constexpr int kCols = kTurns ? NT : NT / 2;  // columns of a softmax thread
   static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
-  // fp32 words per row: scales of two segments' rows, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
-  static constexpr int kTables = NT * 4 * (kRowsInLanes ? 2 + 2 + 2 + 8 : 2 + 2 + 2 + 8 + 2 + 1);
+  // fp32 words per row: scales of the rows of four row tiles, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
+  static constexpr int kTables = NT * 4 * (kRowsInLanes ? 4 + 2 + 2 + 8 : 4 + 2 + 2 + 8 + 2 + 1);
   // Warps: two groups of four for the softmax; one issues the output's products, two bring queries, one issues the scores' products; then four that bring keys
   // and four values, or all bring both: eight where an FP8 cache's ring is short, so that a stage is soon widened, four with two stages a tile
   static constexpr int kSoftmaxWarps = 8, kOutputWarp = kSoftmaxWarps, kQWarp = kOutputWarp + 1, kScoreWarp = kOutputWarp + 3, kProducerWarp = kOutputWarp + 4;
@@ -338,8 +344,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   uint8_t* smem_al = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
   constexpr uint32_t kRing = S * Cfg::kStage;
   const uint32_t sKV = smem_base, sQ = smem_base + kRing, sP = sQ + Cfg::kQBytes, sRaw = sP + 2 * Cfg::kPBytes;
-  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kRawBytes);  // [2][NT]: of a segment's rows
-  float* minus_ref = row_scale + 2 * NT;                                                           // [2][NT]: of each group
+  float* row_scale = reinterpret_cast<float*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kRawBytes);  
+  // [4][NT]: of a row tile's rows. Queries are brought as soon as the last scores of the row tile before have been asked for, which may be while the softmax
+  // is still at the last tile of the one before that: three row tiles' scales are alive at a time
+  float* minus_ref = row_scale + 4 * NT;                                                           // [2][NT]: of each group
   float* factor = minus_ref + 2 * NT;                                                              // [2][NT]
   float* by_warp = factor + 2 * NT;                                                                // [8][NT]
   int* token_of = reinterpret_cast<int*>(by_warp + 8 * NT);                                        // [2][NT]
@@ -461,7 +469,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
           const float by = __uint_as_float((uint32_t)(127 + e) << 23);
-          if (c == 0 && r < NT) row_scale[(seg & 1) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
+          if (c == 0 && r < NT) row_scale[(seg & 3) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
           v[u] = make_uint4(pack2<__half>(__low2float(x[0]) * by, __high2float(x[0]) * by), pack2<__half>(__low2float(x[1]) * by, __high2float(x[1]) * by),
                             pack2<__half>(__low2float(x[2]) * by, __high2float(x[2]) * by), pack2<__half>(__low2float(x[3]) * by, __high2float(x[3]) * by));
         }
@@ -695,7 +703,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       }
       const int rows = min(NT, s.n * p.group - w.qt * NT), prefix = s.len - s.n;
       const int first_token = fast_div(w.qt * NT, p.group_div), last_token = fast_div(w.qt * NT + rows - 1, p.group_div);
-      const float* scales = row_scale + (seg & 1) * NT;
+      const float* scales = row_scale + (seg & 3) * NT;
       float c = p.scale_log2;
       if (FP8 && a.k_scale) c *= ld_operand(a.k_scale + (a.k_scales > 1 ? w.h : 0));
       const bool whole = w.t0 == 0 && w.t1 == s.key_tiles;

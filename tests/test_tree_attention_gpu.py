@@ -379,3 +379,15 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(lens, count
                         assert torch.isnan(g[heads:, dim - 1]).all()
                 # the other elements lose nothing but what the taken-out ones did not add
                 assert torch.equal(g[heads:, ~odd], w[heads:, ~odd])
+
+
+def test_short_sequences_of_very_different_queries():
+    """Row tiles of a single tile of keys one after the other, the power of two that scales their queries another for each."""
+    for group in (1, 4, 8):
+        lens = [20 + 7 * b % 110 for b in range(900)]
+        c = Case(lens, [1] * len(lens), 2 * group, 2, 128, BF, FP8)
+        c.q = (c.q.float() * torch.pow(4.0, (torch.arange(900, device="cuda") % 5 - 4).float())[:, None, None]).to(BF)
+        want = c()
+        c.check(want)
+        for _ in range(5):
+            assert torch.equal(c(), want)
