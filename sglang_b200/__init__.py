@@ -1,5 +1,5 @@
-"""sglang_b200: the block-FP8 W8A8 linear + fused-MoE hot path of SGLang on B200 (sm_100a), with the int8 W8A8 linear and the
-norms that feed either.
+"""sglang_b200: the block-FP8 W8A8 linear + fused-MoE hot path of SGLang on B200 (sm_100a), with the int8 W8A8 linear, the
+norms that feed either, and the operators between a layer's qkv and o_proj linears.
 
 Operators keep the reference's names and signatures; all compute is hand-written CUDA
 behind the C ABI of ``include/b200_blockfp8.h``."""

@@ -7,6 +7,8 @@
     python -m sglang_b200.profile_cases int8_mm M N K [calls]             (rotates over three weights)
     python -m sglang_b200.profile_cases quant_int8 M K plain|silu [calls]
     python -m sglang_b200.profile_cases norm M H int8|fp8 [calls]         (RMSNorm with the residual's addition)
+    python -m sglang_b200.profile_cases rope T heads kv_heads [calls]         (norms and rotation of heads of 128, three axes)
+    python -m sglang_b200.profile_cases attend B length tokens heads kv_heads bf16|fp8 [calls]  (heads of 128, pages of 64)
     python -m sglang_b200.profile_cases align T topk E [calls]
     python -m sglang_b200.profile_cases route T E topk grouped|softmax [calls]
     python -m sglang_b200.profile_cases moe deepseek|mixtral T [calls]
@@ -92,6 +94,23 @@ def main(argv) -> int:
                 out, *_ = S.rmsnorm_quant_int8(x, w, residual=r)
             else:
                 out, *_ = S.rmsnorm_quant_fp8(x, w, residual=r, column_major_scales=True)
+    elif case == "rope":
+        T, heads, kv = (int(a) for a in args[:3])
+        x = torch.randn(T, (heads + 2 * kv) * 128, device=dev, generator=g).bfloat16()
+        w = torch.ones(128, device=dev).bfloat16()
+        positions = torch.arange(T, device=dev).repeat(3, 1)
+        angles = torch.rand(T, 128, device=dev, generator=g)
+        for _ in range(calls(3)):
+            out, _ = S.qk_norm_rope(x, heads, kv, positions, angles, w, w, mrope_section=[16, 24, 24])
+    elif case == "attend":
+        B, length, tokens, heads, kv = (int(a) for a in args[:5])
+        pages = torch.arange(B * -(-length // 64), device=dev, dtype=torch.int32).view(B, -1)
+        cache = [torch.randn(pages.numel(), 64, kv, 128, device=dev, generator=g).to(fp8 if args[5] == "fp8" else torch.bfloat16) for _ in range(2)]
+        q = torch.randn(B * tokens, heads, 128, device=dev, generator=g).bfloat16()
+        lens = torch.full((B,), length, dtype=torch.int32, device=dev)
+        starts = torch.arange(B + 1, dtype=torch.int32, device=dev) * tokens
+        for _ in range(calls(6)):
+            out = S.tree_attention(q, *cache, pages, lens, starts)
     elif case == "align":
         T, topk, E = (int(a) for a in args[:3])
         ids = torch.randint(0, E, (T, topk), device=dev, generator=g, dtype=torch.int32)
