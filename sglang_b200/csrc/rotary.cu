@@ -374,6 +374,7 @@ template <typename T>
 static int launch_rope(RopeParams& p, cudaStream_t st) {
   const b200_rope_args& a = p.a;
   const int total = (a.q ? a.q_heads : 0) + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
+  if (total == 0) return B200_OK;
   // 16-byte vectors of elements and angles; pairs whose halves lie whole vectors apart
   auto rows16 = [](const void* q, int64_t token, int64_t head) { return !q || ((uintptr_t)q % 16 == 0 && token % 8 == 0 && head % 8 == 0); };
   const uintptr_t held = a.cache_dtype == B200_E4M3 ? 8 : 16;
@@ -410,7 +411,7 @@ extern "C" int b200_qk_norm_rope(const b200_rope_args* args, void* stream) {
   B200_CHECK_ARG(a.rotated >= 0 && a.rotated % 2 == 0 && a.rotated <= a.dim, "qk_norm_rope: %d of %d elements cannot rotate", a.rotated, a.dim);
   B200_UNSUPPORTED(a.rotated > 2 * kRopePairs, "qk_norm_rope: more than %d rotated elements", 2 * kRopePairs);
   B200_UNSUPPORTED(a.dim > (1 << 20) || a.q_heads > (1 << 20) || a.kv_heads > (1 << 20), "qk_norm_rope: heads of this size");
-  if (a.rows == 0 || a.dim == 0 || (a.q_heads == 0 && a.kv_heads == 0)) return B200_OK;
+  if (a.rows == 0 || a.dim == 0) return B200_OK;
   const bool cached = a.k_cache != nullptr;
   B200_CHECK_ARG((a.q == nullptr) == (a.q_out == nullptr) && (a.q || a.k) && (a.k == nullptr || cached || a.k_out),
                  "qk_norm_rope: null pointer");

@@ -107,6 +107,12 @@ def test_abi_refuses_before_a_launch():
     assert lib.b200_qk_norm_rope(ctypes.addressof(a), None) == 0
 
 
+def test_abi_has_nothing_to_do_without_heads():
+    for heads in (dict(q_heads=0, kv_heads=3, q=64, q_out=64), dict(q_heads=3, kv_heads=0, k=64, k_out=64), dict(q=64, k=64, q_out=64, k_out=64)):
+        a = RopeArgs(rows=3, dim=64, dtype=N.BF16, **heads)
+        assert N.load().b200_qk_norm_rope(ctypes.addressof(a), None) == 0
+
+
 def test_fake_implementations_describe_the_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
 
