@@ -532,7 +532,8 @@ int b200_qk_norm_rope(const b200_rope_args* args, void* stream);
  * Token i of a sequence sees every key before the sequence's own n, and of those key j where byte mask[(q_starts[b] + i) * mask_ld + j] is not 0 (j <
  * mask_width), or without a mask those up to itself. A token that sees nothing: o = 0, lse = -infinity. Tokens of no sequence keep what
  * out and lse held. A key of a page outside [0, pages) makes the rows that see it NaN; seq_lens are capped at max_pages * page_size.
- * Pointers of q, out and the caches and all strides: multiples of 16 bytes. Workspace: 16-byte aligned, contents immaterial, one per call under way. */
+ * Pointers of q, out and the caches and all strides that lead somewhere: multiples of 16 bytes. No output overlaps an input. Workspace: 16-byte
+ * aligned, contents immaterial, one per call under way. */
 typedef struct {
   const void* q;
   int64_t q_token, q_head;

@@ -54,7 +54,7 @@ def tree_attention(
     those where its row is True. ``scale`` is ``dim ** -0.5`` unless given, positive.
 
     Softmax in fp32, weights rounded to q's type for the product, results rounded once. A token that sees nothing gives 0 (lse -inf). Rows behind the
-    last sequence are not written: they keep what ``out`` held. A page that the cache does not have makes the rows that see it NaN; lengths
+    last sequence are not written: they keep what ``out`` (a tensor of its own) held. A page that the cache does not have makes the rows that see it NaN; lengths
     past the page table are cut. Heads of q and of the caches start at multiples of 16 bytes."""
     N.load()
     if not return_lse:

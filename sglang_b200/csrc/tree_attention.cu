@@ -1346,6 +1346,12 @@ extern "C" int b200_tree_attention(const b200_tree_attention_args* args, void* w
   const b200_tree_attention_args& a = p.a;
   if (int rc = check_attention(a)) return rc;
   if (a.tokens == 0 || a.sequences == 0) return B200_OK;
+  // The distance of one thing to the next that does not exist says nothing
+  if (a.tokens == 1) p.a.q_token = 0;
+  if (a.q_heads == 1) p.a.q_head = 0;
+  if (a.pages <= 1) p.a.k_page = p.a.v_page = 0;
+  if (a.page_size == 1) p.a.k_token = p.a.v_token = 0;
+  if (a.kv_heads == 1) p.a.k_head = p.a.v_head = 0;
   B200_CHECK_ARG(a.q && a.out && a.seq_lens && (a.max_pages == 0 || (a.page_table && (a.pages == 0 || (a.k_cache && a.v_cache)))),
                  "tree_attention: null pointer");
   const int per16 = a.cache_dtype == B200_E4M3 ? 16 : 8;  // elements of 16 bytes

@@ -2,7 +2,10 @@
 the cache, o_proj linear, for prompts, single tokens and trees of drafted ones; and under what a server does to a call.
 
 Link by link: every operator is tested on what the one before it gave, at that operator's own tolerance."""
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -157,3 +160,26 @@ def test_native_and_general_host_path_agree():
         for a, b in zip(S.qk_norm_rope(x, 8, 2, pos, cs, None, None, 1e-6, False, section, inter),
                         S.qk_norm_rope(sub, 8, 2, pos, cs, None, None, 1e-6, False, tuple(section), inter)):
             assert torch.equal(a, b)
+
+
+def test_a_first_call_may_be_a_captured_one():
+    """A process whose first calls of the operators are captured: what they set up once must not need the stream."""
+    code = """
+import torch, sglang_b200 as S
+x = torch.randn(5, 12 * 128, device='cuda').bfloat16()
+at = torch.arange(5, device='cuda', dtype=torch.int32)
+kc, vc = (torch.zeros(2, 16, 2, 128, device='cuda', dtype=torch.bfloat16) for _ in range(2))
+cs = torch.randn(9, 128, device='cuda')
+pages, lens, starts = (torch.tensor(t, device='cuda', dtype=torch.int32) for t in ([[0]], [5], [0, 5]))
+torch.cuda.synchronize()
+def step():
+    q = S.qk_norm_rope_append(x, 8, 2, at, cs, kc, vc, at)
+    return q, S.tree_attention(q, kc, vc, pages, lens, starts)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+got = [t.clone() for t in got]
+assert got[1].abs().sum() > 0 and all(torch.equal(a, b) for a, b in zip(got, step()))
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)

@@ -83,6 +83,11 @@ def test_abi_refuses_before_a_launch():
         assert call(**f) == N.E_UNSUPPORTED, f
 
 
+def test_distances_that_lead_nowhere_are_not_checked():
+    assert call(tokens=1, sequences=1, q_token=1028) == call(q_heads=1, kv_heads=1, q_head=1, k_head=3, v_head=5) == N.E_WORKSPACE
+    assert call(pages=1, k_page=1, v_page=3) == call(page_size=1, k_token=1, v_token=3) == N.E_WORKSPACE
+
+
 def test_workspace():
     size = lambda **f: N.load().b200_tree_attention_workspace_bytes(ctypes.byref(args(**f)))  # noqa: E731
     assert size() > 0 and size(tokens=0) == 0 and size(dim=100) == 0

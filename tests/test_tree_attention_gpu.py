@@ -249,6 +249,18 @@ def test_layouts():
     assert torch.equal(c(), want)
 
 
+def test_distances_that_lead_nowhere():
+    """One token of rows whose length is no multiple of 16 bytes, one kv head, one page of one token."""
+    c = Case([1], [1], 4, 1, 64, page=1)
+    c.kc, c.vc = c.kc[int(c.table[0, 0])][None], c.vc[int(c.table[0, 0])][None]
+    c.table = torch.zeros_like(c.table)
+    want = c()
+    c.check(want)
+    c.q = c.q.as_strided(c.q.shape, (4 * 64 + 3, 64, 1))
+    c.kc, c.vc = (t.as_strided(t.shape, (3, 5, 7, 1)) for t in (c.kc, c.vc))
+    assert c.q.stride(0) % 8 and torch.equal(c(), want) and torch.equal(c(return_lse=True)[0], want)
+
+
 def test_what_no_row_sees_does_not_matter():
     """Garbage behind the last key of a page, in pages of no sequence."""
     for held in (None, FP8):
