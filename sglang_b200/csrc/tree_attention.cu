@@ -178,8 +178,9 @@ struct AttnCfg {
   static constexpr bool kRowsInLanes = NT == 128, kTurns = NT <= 32, kTwoO = NT != 64;
   static constexpr int kCols = kTurns ? NT : NT / 2;  // columns of a softmax thread
   static constexpr int kQBytes = NT * D * 2, kPBytes = kRowsInLanes ? 0 : kKeys * NT * 2;
-  // fp32 words per row: scales of the rows of four row tiles, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys
-  static constexpr int kTables = NT * 4 * (kRowsInLanes ? 4 + 2 + 2 + 8 : 4 + 2 + 2 + 8 + 2 + 1);
+  // fp32 words per row: scales of the rows of four row tiles, references, factors, sums per warp, tokens, rows of the output; or bits per 32 keys, for both
+  // groups, of two tiles
+  static constexpr int kTables = NT * 4 * (kRowsInLanes ? 4 + 2 + 2 + 16 : 4 + 2 + 2 + 8 + 2 + 1);
   // Warps: two groups of four for the softmax; one issues the output's products, two bring queries, one issues the scores' products; then four that bring keys
   // and four values, or all bring both: eight where an FP8 cache's ring is short, so that a stage is soon widened, four with two stages a tile
   static constexpr int kSoftmaxWarps = 8, kOutputWarp = kSoftmaxWarps, kQWarp = kOutputWarp + 1, kScoreWarp = kOutputWarp + 3, kProducerWarp = kOutputWarp + 4;
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
   float* by_warp = factor + 2 * NT;                                                                // [8][NT]
   int* token_of = reinterpret_cast<int*>(by_warp + 8 * NT);                                        // [2][NT]
   int* out_row = token_of + 2 * NT;                                                                // [NT]
-  uint32_t* seen_words = reinterpret_cast<uint32_t*>(factor);                                      // rows in lanes: [2][NT][4], behind [2][NT] sums
+  uint32_t* seen_words = reinterpret_cast<uint32_t*>(factor);                                      // rows in lanes: [2][2][NT][4], behind [2][NT] sums
   if (Cfg::kRowsInLanes) by_warp = factor, seen_words = reinterpret_cast<uint32_t*>(factor + 2 * NT);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kRing + Cfg::kQBytes + 2 * Cfg::kPBytes + Cfg::kRawBytes + Cfg::kTables);
   const uint32_t bar0 = ptx::smem_u32(bars);
@@ -961,7 +962,6 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
         const bool busy = (warp & 3) * 32 < rows;  // the same for the whole warp
         const int at = w.qt * NT + min(r, rows - 1), token = fast_div(at, p.group_div);
         const int64_t to = (int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
-        uint32_t* const words = seen_words + group * NT * 4;
         float m = -kNoRef, l = 0.f, scale = c;
         for (int t = mine; t < w.t1; ++t) {
           const uint32_t x_tile = g + (t - w.t0), own = x_tile & 1, phase = x_tile >> 1;
@@ -970,6 +970,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           ptx::tc_fence_after();
           if (kRowScales && t == mine) scale = c * scales[min(r, rows - 1)];
           const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
+          // Every second tile has the same words: a warp may be at the next masked tile while the others still read those of this one, and it is past that
+          // tile's barrier, which they reach with them read, before it writes these again
+          uint32_t* const words = seen_words + (own * 2 + group) * NT * 4;
           if (__builtin_expect(masked, 0)) {  // thread r finds out who sees key r; a word per token and 32 keys. (Each group for itself: they need not be at the same tile.)
             const int j = t * kKeys + r;
             for (int i0 = 0; i0 <= last_token - first_token; i0 += 64) {

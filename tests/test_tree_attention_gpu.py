@@ -403,3 +403,30 @@ def test_short_sequences_of_very_different_queries():
         c.check(want)
         for _ in range(5):
             assert torch.equal(c(), want)
+
+
+@pytest.mark.parametrize("held", [None, FP8])
+@pytest.mark.parametrize("mask", [False, True])
+def test_many_masked_tiles_of_partly_filled_row_tiles(mask, held):
+    """Row tiles of 128 with 4, 20, 60 and 92 rows at the end of every sequence, up to eight tiles of keys that not every row sees one after the other in
+    the same CTA: the definition, and the same bits every time."""
+    counts = [288 + (b * 37) % 11 * 32 + [1, 5, 15, 23][b % 4] for b in range(64)]
+    assert {n * 4 % 128 for n in counts} == {4, 20, 60, 92} and max(counts) < 700
+    lens = [n + [0, 100, 61][b % 3] for b, n in enumerate(counts)]
+    c = Case(lens, counts, 8, 2, 128, BF, held, 16, mask)
+    want, lse = c(return_lse=True)
+    c.check(want, lse)
+    for _ in range(40):
+        assert torch.equal(c(), want)
+
+
+def test_masked_tiles_in_the_first_places_of_a_piece():
+    """Nothing but masked tiles: a drafted tree, or a chain, of 9 to 12 tokens of eight heads across a multiple of 128 keys."""
+    for mask in (False, True):
+        lens = [128 * (1 + b % 3) + 1 + b % 8 for b in range(296)]
+        counts = [9 + b % 4 for b in range(296)]
+        c = Case(lens, counts, 8, 1, 128, BF, FP8, 16, mask)
+        want, lse = c(return_lse=True)
+        c.check(want, lse)
+        for _ in range(100):
+            assert torch.equal(c(), want)
