@@ -238,6 +238,16 @@ __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b) {
   return s;
 }
 
+// Where an offset on a sequence's part of the line lies: kv head, row tile, place in that row tile's length. In 64 bits: the row tiles of one head may be
+// longer than 2^31 together.
+struct LinePlace {
+  int h, qt, at;
+};
+__host__ __device__ inline LinePlace line_place(int64_t offset, int row_tiles, int units) {
+  const int64_t tile = offset / units, head = tile / row_tiles;
+  return {(int)head, (int)(tile - head * row_tiles), (int)(offset - tile * units)};
+}
+
 // A CTA's piece of the line, one (sequence, head, row tile) at a time
 template <int NT>
 struct Walk {
@@ -251,12 +261,8 @@ struct Walk {
     s = {};
     if (left <= 0) return;
     s = seq_of<NT>(p, b);
-    const int units = s.units(kExtraTiles<NT>);
-    const int64_t per_head = (int64_t)s.row_tiles * units;
-    h = (int)(offset / per_head);
-    const int rest = (int)(offset - h * per_head);
-    qt = rest / units;
-    at = rest - qt * units;
+    const LinePlace place = line_place(offset, s.row_tiles, s.units(kExtraTiles<NT>));
+    h = place.h, qt = place.qt, at = place.at;
     settle();
   }
   __device__ __forceinline__ bool more() const { return left > 0; }
