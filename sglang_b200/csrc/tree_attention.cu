@@ -335,6 +335,78 @@ __device__ __forceinline__ float across_lanes(const float (&v)[N], F op) {
   }
 }
 
+constexpr int kBothGroups = 3;  // barrier of both groups of softmax warps
+
+// A piece of a row tile as its odd values need it: its sequence's own keys [j0, j1)
+struct OddPiece {
+  int b, h, qt, start, rows, prefix, j0, j1;
+  bool whole;
+  int64_t slot0;
+};
+// Values that are not finite and were taken out go to the rows that see them, whatever their weight. 32 keys at a time the warps find out which rows see each,
+// then a thread with an element of the head notes which rows take what of it, and each row's element is changed once at the end. (A change for every key
+// would cost keys times rows trips to memory, more than the other warps wait for where a long prompt's values are NaN. Apart from the kernel, whose registers
+// it would take.)
+template <typename T, int D, int NT, bool FP8>
+__device__ __noinline__ void add_odd_values(const AttnParams& p, const OddPiece& s, uint32_t* rows_of_key /* [32][kWords] */) {
+  const b200_tree_attention_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr uint32_t kExponent = std::is_same_v<T, __nv_bfloat16> && !FP8 ? 0x7f80u : 0x7c00u;
+  constexpr int kWords = NT <= 32 ? 1 : NT / 32, kPer = 4 * kWords;  // words of a key; keys that a warp looks at
+  uint32_t nan[kWords] = {}, plus[kWords] = {}, minus[kWords] = {};   // rows that take one
+  const int d = threadIdx.x, my_row = warp % kWords * 32 + lane, my_token = fast_div(s.qt * NT + min(my_row, s.rows - 1), p.group_div);
+  const uint8_t* const line_of_mask = static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + my_token) * a.mask_ld;
+#pragma unroll 1
+  for (int j0 = s.j0; j0 < s.j1; j0 += 32) {
+#pragma unroll 4
+    for (int i = 0; i < kPer; ++i) {
+      const int k = warp / kWords * kPer + i, own = j0 + k - s.prefix;
+      const bool sees = my_row < s.rows && j0 + k < s.j1 && (a.mask ? own < a.mask_width && ptx::ld_byte(line_of_mask + own) != 0 : own <= my_token);
+      const uint32_t all = __ballot_sync(0xffffffffu, sees);
+      if (lane == 0) rows_of_key[k * kWords + warp % kWords] = all;
+    }
+    int64_t my_value = -1;  // of key j0 + lane: where it begins, if the cache has its page
+    if (j0 + lane < s.j1) {
+      const int page = fast_div(j0 + lane, p.page_div), entry = ld_operand(a.page_table + (int64_t)s.b * a.page_table_ld + page);
+      if (entry >= 0 && entry < a.pages) my_value = entry * a.v_page + (j0 + lane - page * a.page_size) * a.v_token + s.h * a.v_head;
+    }
+    ptx::any_of(kBothGroups, 256, false);
+#pragma unroll 8
+    for (int k = 0; k < 32; ++k) {
+      const int64_t value = __shfl_sync(0xffffffffu, my_value, k);
+      uint32_t x = 0;
+      if (value >= 0 && d < D) {
+        if constexpr (FP8) x = (static_cast<const volatile uint8_t*>(a.v_cache)[value + d] & 0x7fu) == 0x7fu ? kExponent + 1 : 0u;
+        else x = static_cast<const volatile uint16_t*>(a.v_cache)[value + d];
+      }
+      if ((x & kExponent) != kExponent) continue;  // finite
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const uint32_t to = rows_of_key[k * kWords + i];
+        if ((x & 0x7fffu) > kExponent) nan[i] |= to;
+        else if (x & 0x8000u) minus[i] |= to;
+        else plus[i] |= to;
+      }
+    }
+    ptx::any_of(kBothGroups, 256, false);
+  }
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    const uint32_t take = nan[i] | plus[i] | minus[i], none = nan[i] | (plus[i] & minus[i]);
+    for (uint32_t left = take; left != 0; left &= left - 1) {
+      const int bit = __ffs(left) - 1, n = i * 32 + bit;
+      const float v = (none >> bit) & 1u ? NAN : (minus[i] >> bit) & 1u ? -INFINITY : INFINITY;
+      const int at = s.qt * NT + n, token = fast_div(at, p.group_div);
+      if (s.whole) {
+        T* const o = static_cast<T*>(a.out) + ((int64_t)(s.start + token) * a.q_heads + s.h * p.group + at - token * p.group) * D + d;
+        *o = from_f32<T>(to_f32<T>(*o) + v);
+      } else {
+        p.part_o[AttnCfg<D, NT, FP8>::kRowsInLanes ? s.slot0 * D + ((d >> 2) * p.row_slots + n) * 4 + (d & 3) : (s.slot0 + n) * D + d] += v;
+      }
+    }
+  }
+}
+
 template <typename T, int D, int NT, bool FP8>
 __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attention_kernel(const __grid_constant__ AttnParams p) {
   using Cfg = AttnCfg<D, NT, FP8>;
@@ -693,7 +765,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
     // What a warp decided alone would leave the others at a barrier: where a wait may have failed, all threads of a group, or all, decide together.
     ptx::give_registers<Cfg::kSoftmaxRegs, Cfg::kLaunchRegs>();
     const int group = warp >> 2, r = threadIdx.x & 127, bar = 1 + group;
-    constexpr int kBoth = 3;  // barrier of both groups
+    constexpr int kBoth = kBothGroups;
     constexpr int kStep = Cfg::kTurns ? 2 : 1, kCols = Cfg::kCols;
     const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t o_own = lane_base + Cfg::kTmemO + (Cfg::kTwoO ? group * Cfg::kOCols : group * kCols);
@@ -1098,28 +1170,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
       ptx::tc_fence_before();
       // (the barrier also says that this segment's tables have been read)
       if (__builtin_expect(ptx::any_of(kBoth, 256, odd_values), 0)) {
-        // Values that were taken out go to the rows that see them: NaN and infinities, whatever their weight
-        const int j1 = min(s.len, w.t1 * kKeys);
-        for (int j = max(max(prefix, 0), w.t0 * kKeys); j < j1; ++j) {
-          const int entry = ld_operand(a.page_table + (int64_t)w.b * a.page_table_ld + fast_div(j, p.page_div));
-          if (entry < 0 || entry >= a.pages) continue;
-          const int in_page = j - fast_div(j, p.page_div) * a.page_size;
-          const int64_t value = entry * a.v_page + in_page * a.v_token + w.h * a.v_head;
-          for (int d = threadIdx.x; d < D; d += 256) {
-            float v;
-            if constexpr (FP8) v = (static_cast<const volatile uint8_t*>(a.v_cache)[value + d] & 0x7f) == 0x7f ? NAN : 0.f;
-            else v = to_f32<T>(static_cast<const T*>(a.v_cache)[value + d]);
-            if (v - v == 0.f) continue;  // finite
-            for (int n = 0; n < rows; ++n) {
-              const int at = w.qt * NT + n, token = fast_div(at, p.group_div), own = j - prefix;
-              if (a.mask ? own >= a.mask_width || ptx::ld_byte(static_cast<const uint8_t*>(a.mask) + (int64_t)(s.start + token) * a.mask_ld + own) == 0 : own > token)
-                continue;
-              const int64_t head = (int64_t)(s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
-              if (whole) static_cast<T*>(a.out)[head * D + d] = from_f32<T>(to_f32<T>(static_cast<T*>(a.out)[head * D + d]) + v);
-              else p.part_o[Cfg::kRowsInLanes ? slot0 * D + ((d >> 2) * p.row_slots + n) * 4 + (d & 3) : (slot0 + n) * D + d] += v;
-            }
-          }
-        }
+        add_odd_values<T, D, NT, FP8>(p, {w.b, w.h, w.qt, s.start, rows, prefix, max(max(prefix, 0), w.t0 * kKeys), min(s.len, w.t1 * kKeys), whole, slot0},
+                                      reinterpret_cast<uint32_t*>(factor));
         ptx::any_of(kBoth, 256, false);
       }
       g += w.t1 - w.t0;

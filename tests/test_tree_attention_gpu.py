@@ -430,3 +430,65 @@ def test_masked_tiles_in_the_first_places_of_a_piece():
         c.check(want, lse)
         for _ in range(100):
             assert torch.equal(c(), want)
+
+
+@pytest.mark.parametrize("held", [None, FP8])
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("dim, group", [(64, 1), (128, 1), (128, 3), (128, 16), (256, 2)])
+def test_many_values_that_are_not_finite(dim, group, mask, held):
+    """A third of the own values are NaN or infinite: every row takes what it sees, the other elements keep their bits."""
+    lens, counts = [300, 40, 700], [150, 33, 21]
+    c = Case(lens, counts, 2 * group, 2, dim, BF, held, 16, mask)
+    if mask:
+        c.mask[torch.rand(c.mask.shape, device="cuda") < 0.7] = False
+    want = c()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    expected = []
+    for b, (length, n) in enumerate(zip(lens, counts)):
+        kind = torch.randint(0, 9, (n, 2, dim), generator=g, device="cuda")  # 0: NaN, 1, 2: infinities, others stay
+        j = torch.arange(length - n, length, device="cuda")
+        page = c.table[b].long()[j // 16]
+        v = c.vc[page, j % 16]
+        if held:
+            v = v.view(torch.uint8).masked_fill(kind < 3, 0x7F).view(FP8)
+        else:
+            v = v.masked_fill(kind == 0, math.nan).masked_fill(kind == 1, math.inf).masked_fill(kind == 2, -math.inf)
+        bits = torch.uint8 if held else torch.int16
+        c.vc.view(bits)[page, j % 16] = v.view(bits)
+        sees = c.visible(b)[:, length - n :].float()
+        met = [torch.einsum("ij,jhd->ihd", sees, (kind == k).float()) > 0 for k in range(3)]
+        nan = met[0] | met[1] | met[2] if held else met[0] | (met[1] & met[2])
+        expected.append(torch.where(nan, 3, torch.where(met[1], 1, torch.where(met[2], 2, 0))).repeat_interleave(group, 1))
+    got, kind = c(), torch.cat(expected)
+    assert torch.equal(torch.isnan(got), kind == 3)
+    assert torch.equal(got == math.inf, kind == 1) and torch.equal(got == -math.inf, kind == 2)
+    assert torch.equal(got[kind == 0], want[kind == 0])
+
+
+@pytest.mark.parametrize("held", [None, FP8])
+def test_a_long_prompt_of_values_that_are_not_finite(held):
+    """What they cost must stay below what the kernel's other warps wait for, whose waits end."""
+    from sglang_b200 import _native as N
+
+    n = 32768
+    c = Case([n], [n], 1, 1, 64, BF, held, 64)
+    want = c()
+    j = torch.arange(n, device="cuda")
+    rows = c.vc.view(torch.uint8 if held else BF)
+    page = c.table[0].long()[j // 64]
+    if held:
+        rows[page, j % 64, 0, 5] = 0x7F
+        rows[page[1000:], j[1000:] % 64, 0, 9] = 0xFF
+    else:
+        rows[page, j % 64, 0, 5] = math.nan
+        rows[page[1000:], j[1000:] % 64, 0, 9] = math.inf
+        rows[page[10], 10, 0, 12], rows[page[20000], 20000 % 64, 0, 12] = math.inf, -math.inf
+    got = c()[:, 0]
+    assert N.read_device_status() == 0
+    assert torch.isnan(got[:, 5]).all()
+    assert torch.equal(got[:1000, 9], want[:1000, 0, 9])
+    assert torch.isnan(got[1000:, 9]).all() if held else (got[1000:, 9] == math.inf).all()
+    if not held:
+        assert torch.equal(got[:10, 12], want[:10, 0, 12]) and (got[10:20000, 12] == math.inf).all() and torch.isnan(got[20000:, 12]).all()
+    others = [d for d in range(64) if d not in (5, 9, 12)]
+    assert torch.equal(got[:, others], want[:, 0, others])
