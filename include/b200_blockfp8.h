@@ -527,7 +527,9 @@ int b200_qk_norm_rope(const b200_rope_args* args, void* stream);
  * Sequence b has the tokens q_starts[b] .. q_starts[b+1] - 1 (n of them; NULL: token b) and seq_lens[b] keys, the last n of which are its own. Key j is
  * token j % page_size of page page_table[b * page_table_ld + j / page_size] of k_cache and v_cache, pages, tokens and heads k_page, k_token, k_head (v_*)
  * elements apart, of `dtype` or B200_E4M3 with scales as for b200_qk_norm_rope, positive. Head i reads kv head i / (q_heads / kv_heads).
- *   o = sum_j softmax_j(scale q . k_j k_scale) v_j v_scale over the keys that the token sees, rounded once; weights are multiplied in `dtype`
+ *   o = sum_j softmax_j(scale q . k_j k_scale) v_j v_scale over the keys that the token sees, rounded once; weights are multiplied
+ *   in the cache's 16-bit type, over an E4M3 cache in f16 (bf16 queries too, by a power of two per row); in f16 a weight is off by up to 2^-32 of the row's
+ *   largest, however small it is itself
  *   lse [tokens,q_heads] fp32 or NULL: the logarithm of the sum of the exponentials
  * Token i of a sequence sees every key before the sequence's own n, and of those key j where byte mask[(q_starts[b] + i) * mask_ld + j] is not 0 (j <
  * mask_width), or without a mask those up to itself. A token that sees nothing: o = 0, lse = -infinity. Tokens of no sequence keep what

@@ -53,7 +53,8 @@ def tree_attention(
     Every new token sees the keys before its sequence's new ones, and of those the ones up to itself, or with ``tree_mask`` (bool, ``[T, widest]``)
     those where its row is True. ``scale`` is ``dim ** -0.5`` unless given, positive.
 
-    Softmax in fp32, weights rounded to q's type for the product, results rounded once. A token that sees nothing gives 0 (lse -inf). Rows behind the
+    Softmax in fp32, results rounded once. Weights are rounded for the product with the values, to q's type over a 16-bit cache and to fp16 over an FP8 one
+    (bf16 queries too become fp16 there, by a power of two per row); in fp16 a weight is off by up to 2^-32 of the row's largest, however small it is itself. A token that sees nothing gives 0 (lse -inf). Rows behind the
     last sequence are not written: they keep what ``out`` (a tensor of its own) held. A page that the cache does not have makes the rows that see it NaN; lengths
     past the page table are cut. Heads of q and of the caches start at multiples of 16 bytes."""
     N.load()

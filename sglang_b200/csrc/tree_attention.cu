@@ -5,7 +5,7 @@
 //   S^T [128 keys, NT] = K Q^T     K and Q in shared memory, S^T in TMEM, two buffers
 //   O^T [D, NT]       += V^T P^T   V as it lies in the cache (its rows are the product's depth), P^T [keys, NT] in shared memory
 // A thread of the softmax has one key and the rows' columns. It takes its exponentials against a reference per row that is moved only when a score
-// exceeds it by 2^8, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end. With more than
+// lies 2^8 above the one it was taken from, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end. With more than
 // 64 rows the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: a softmax row is a thread's own,
 // and P needs no shared memory.
 // Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies; codes of an FP8 cache land in a ring of their own and
@@ -309,9 +309,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// A score may exceed its row's reference by this much (in powers of two) before the reference moves: sums stay exact to fp32 and weights far from the
-// 16-bit types' limits, and most rows move theirs in the first tile alone.
-constexpr float kSlack = 8.f;
+// A row's reference is taken this far below its largest score (in powers of two), and stays until a score exceeds it by kReach: most rows move theirs in the
+// first tile alone. Weights in fp16 reach from 2^15 down to steps of 2^-24, so the largest stands at 2^7 or higher, and what a long context's many small
+// weights lose is below 2^-32 of it each (with the reference at the largest score itself 2^-25: 131072 keys of 2^-26 each were lost, 2^-9 of the
+// sum, which is taken of the fp32 weights). bf16 has the range of the sums.
+template <typename M>
+constexpr float kBelow = std::is_same_v<M, __half> ? 7.f : 0.f;
+template <typename M>
+constexpr float kReach = kBelow<M> + 8.f;
 constexpr float kNoRef = 3e38f;  // of a row that has seen nothing yet, negated like all references: any score exceeds it, and -infinity stays what it is
 
 // Value i of lane l, N <= 32 of them in each of 32 lanes -> lane l has the result over all lanes of value l % N. Each step halves the values that a
@@ -410,6 +415,8 @@ __device__ __noinline__ void add_odd_values(const AttnParams& p, const OddPiece&
 template <typename T, int D, int NT, bool FP8>
 __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attention_kernel(const __grid_constant__ AttnParams p) {
   using Cfg = AttnCfg<D, NT, FP8>;
+  // Weights are rounded to the 16 bits that the tensor core multiplies with the values; their sum is taken of the fp32 ones. (An output so differs from that
+  // of fp32 weights by less than its own rounding: 2.2e-3 against 1.7e-3 off in bf16, root mean square.)
   // An FP8 cache is multiplied in fp16, which holds its codes, whatever the queries' type: a code is converted by one instruction for two, and weights keep
   // 11 bits. bf16 queries become fp16 behind a power of two per row that brings their largest element to 2^7 .. 2^8; what then lies below fp16's
   // normal range is 2^-21 of it.
@@ -913,7 +920,7 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           }
           // the product that read this buffer of P^T is complete (with tiles in turn it is the last one that this group's O was in)
           if (x_tile >= 2) ok = ok && ptx::mbar_wait(o_done(own), (phase - 1) & 1, abort_flag);
-          if (__builtin_expect(ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kSlack || t == mine || !ok), 0)) {
+          if (__builtin_expect(ptx::any_of(bar, 128, fmaxf(above[0], above[1]) > kReach<M> || t == mine || !ok), 0)) {
             // Rows whose largest score lies too far above their reference take it as the new one
             const bool moves = t > mine;
             if (moves && !Cfg::kTurns) ok = ok && ptx::mbar_wait(o_done(own ^ 1), ((x_tile - 1) >> 1) & 1, abort_flag);
@@ -926,9 +933,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             ptx::any_of(bar, 128, false);
             if (r < kCols) {
               const float top = fmaxf(fmaxf(warps[r], warps[kCols + r]), fmaxf(warps[2 * kCols + r], warps[3 * kCols + r])), old = -refs[r];
-              const bool move = top > old + kSlack;
-              factors[r] = move ? ptx::ex2(old - top) : 1.f;
-              if (move) refs[r] = -top;
+              const bool move = top > old + kReach<M>;
+              const float next = top - kBelow<M>;
+              factors[r] = move ? ptx::ex2(old - next) : 1.f;
+              if (move) refs[r] = -next;
             }
             ptx::any_of(bar, 128, false);
             if (moves) {
@@ -1084,12 +1092,13 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
 #pragma unroll
               for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = ptx::max3(top[(i >> 1) & 3], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
             const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-            const bool move = largest > m + kSlack;
+            const bool move = largest > m + kReach<M>;
+            const float next = largest - kBelow<M>;
             if (t == mine) {
-              if (move) m = largest;
+              if (move) m = next;
             } else if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
-              const float f = move ? ptx::ex2(m - largest) : 1.f;
-              if (move) m = largest;
+              const float f = move ? ptx::ex2(m - next) : 1.f;
+              if (move) m = next;
               l *= f;
               // (not for a phase two ahead: the scores of the tile before were asked for behind the product before this one)
               ok = ok && ptx::mbar_wait(o_done(own ^ 1), ((x_tile - 1) >> 1) & 1, abort_flag);

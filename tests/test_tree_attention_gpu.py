@@ -492,3 +492,51 @@ def test_a_long_prompt_of_values_that_are_not_finite(held):
         assert torch.equal(got[:10, 12], want[:10, 0, 12]) and (got[10:20000, 12] == math.inf).all() and torch.isnan(got[20000:, 12]).all()
     others = [d for d in range(64) if d not in (5, 9, 12)]
     assert torch.equal(got[:, others], want[:, 0, others])
+
+
+@pytest.mark.parametrize("dtype, held", [(BF, FP8), (HF, FP8), (HF, None), (BF, None)])
+@pytest.mark.parametrize("dim, group, n", [(64, 1, 1), (128, 8, 1), (128, 8, 4), (64, 8, 8), (128, 8, 16), (256, 4, 8)])
+def test_one_large_key_above_a_long_flat_context(dim, group, n, dtype, held):
+    """A key whose weight is 2^26 times that of every other, 131072 of them: together 2^-9 of the result, which fp16 weights of the largest key's
+    size would lose. The largest weight is 2^7 or more and steps are 2^-24, so a weight is off by 2^-32 of it at most."""
+    L = 131072
+    c = Case([L] * 3, [n] * 3, group, 1, dim, dtype, held, 64)
+    c.ks = c.vs = None
+    c.q.zero_()
+    c.q[:, :, 0] = dim**0.5  # 18 * 1.4427 = 25.97 powers of two for a key of 18
+    score = float(c.q[0, 0, 0]) * 18 * dim**-0.5  # (the query as its type holds it)
+    for t in (c.kc, c.vc):
+        t.view(torch.uint8 if held else torch.int16).zero_()
+    v = torch.tensor([1.0, -2.0, 0.5, 0.0], device="cuda").repeat(dim // 4)
+    c.vc.copy_(v.to(c.held).expand(c.vc.shape))
+    for b, j in enumerate((3, L // 2 + 77, L - n - 1)):
+        page = int(c.table[b, j // 64])
+        c.kc[page, j % 64, 0, 0] = 18.0
+        c.vc[page, j % 64] = torch.zeros(dim, device="cuda").to(c.held)
+    out, lse = c(return_lse=True)
+    half = torch.finfo(dtype).eps / 2
+    weight = math.exp(-score)
+    for b in range(3):
+        for i in range(n):
+            others = L - n + i  # (without the large one)
+            total = 1 + others * weight
+            want = others * weight / total * v.double()
+            got = out[b * n + i].double()
+            # one rounding of the result, twice the weights' and the exponentials' (scores are exact but for the scale: 2^-22 of 26), and what fp16 loses
+            bound = (3 * half + 2.0**-15) * want.abs() + L * 2.0**-32 * v.double().abs()
+            assert ((got - want).abs() <= bound).all(), (b, i, got[0, :4], want[:4])
+            assert (lse[b * n + i].double() - (score + math.log(total))).abs().max() <= 18 * 2.0**-21 + 2.0**-15
+
+
+def test_weights_at_the_top_of_fp16():
+    """Scores that rise by just less than what moves a reference: weights up to 2^15, and sums of them."""
+    for held in (None, FP8):
+        for group, n in ((1, 1), (8, 4), (8, 8), (8, 16)):
+            c = Case([3000], [n], group, 1, 64, HF, held)
+            c.ks = c.vs = None
+            c.q.zero_()
+            c.q[:, :, 0] = 8
+            c.kc.view(torch.uint8 if held else torch.int16).zero_()
+            j = torch.arange(3000, device="cuda")
+            c.kc[c.table[0].long()[j // 16], j % 16, 0, 0] = ((j >= 200).float() * 5.5).to(c.held)  # 7.93 powers of two
+            c.check(*c(return_lse=True))
