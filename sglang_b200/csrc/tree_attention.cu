@@ -553,7 +553,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(x[k])), fabsf(__high2float(x[k]))));
 #pragma unroll
           for (int o = kPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e = top > 0.f && top < INFINITY ? min(max(134 - (int)(__float_as_uint(top) >> 23), -100), 100) : 0;
+          // (134 - 254 at least; rows far below 1 have no score that is not 0, and the power's own inverse stays a normal number)
+          const int e = top > 0.f && top < INFINITY ? min(134 - (int)(__float_as_uint(top) >> 23), 100) : 0;
           const float by = __uint_as_float((uint32_t)(127 + e) << 23);
           if (c == 0 && r < NT) row_scale[(seg & 3) * NT + r] = __uint_as_float((uint32_t)(127 - e) << 23);
           v[u] = make_uint4(pack2<__half>(__low2float(x[0]) * by, __high2float(x[0]) * by), pack2<__half>(__low2float(x[1]) * by, __high2float(x[1]) * by),

@@ -540,3 +540,17 @@ def test_weights_at_the_top_of_fp16():
             j = torch.arange(3000, device="cuda")
             c.kc[c.table[0].long()[j // 16], j % 16, 0, 0] = ((j >= 200).float() * 5.5).to(c.held)  # 7.93 powers of two
             c.check(*c(return_lse=True))
+
+
+@pytest.mark.parametrize("group, n", [(1, 1), (8, 4), (8, 8), (8, 16)])
+@pytest.mark.parametrize("power", [115, 117, 121, 125])
+def test_queries_at_the_end_of_bf16_over_an_fp8_cache(power, group, n):
+    """Rows of up to 2^128 whose scores a small scale (a normal number even so) makes ordinary ones: the bits of rows of ordinary size."""
+    c = Case([700, 130], [n, n], 2 * group, 2, 64, BF, FP8)
+    c.kc = (c.kc.float() * 2.0**-10).to(FP8)
+    c.ks = torch.ones(1, device="cuda")
+    want = c(scale=2.0)
+    c.check(want, scale=2.0)
+    c.q = c.q * 2.0**power
+    assert torch.isfinite(c.q).all()
+    assert torch.equal(c(scale=2.0 * 2.0**-power), want)
