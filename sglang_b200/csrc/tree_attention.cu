@@ -16,6 +16,8 @@
 // to 16384 with 8 drafted tokens, 64 query heads (64 rows), 597 MB: 127 us, 4.7 TB/s. An FP8 cache is bound by the way of its codes through the SM, copied,
 // read, widened and stored: 64 sequences of up to 16384, one token, 1.08 GB: 240 us, 4.5 TB/s. 128 rows by the exponentials, 16 a clock and SM, and by the latency of
 // the steps between two products: 61 sequences of up to 32768, 16 tokens, FP8, 264 MB: 117 us, 535 TFLOP/s.
+#include <cfloat>
+
 #include "gemm_host.cuh"
 #include "int8_round.cuh"
 
@@ -1055,7 +1057,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           const uint32_t s_own = lane_base + own * Cfg::kSCols + group * 64;
           ok = ok && ptx::mbar_wait(s_full(own), phase & 1, abort_flag);
           ptx::tc_fence_after();
-          if (kRowScales && t == mine) scale = c * scales[min(r, rows - 1)];
+          if (t == mine) {
+            if (kRowScales) scale = c * scales[min(r, rows - 1)];
+            if (FP8 && scale == 0.f) scale = FLT_MIN;  // an underflow would make NaN of keys that are not seen, -infinity here already
+          }
           const bool masked = t * kKeys + kKeys > (a.mask ? prefix : prefix + first_token + 1);
           // Every second tile has the same words: a warp may be at the next masked tile while the others still read those of this one, and it is past that
           // tile's barrier, which they reach with them read, before it writes these again

@@ -554,3 +554,13 @@ def test_queries_at_the_end_of_bf16_over_an_fp8_cache(power, group, n):
     c.q = c.q * 2.0**power
     assert torch.isfinite(c.q).all()
     assert torch.equal(c(scale=2.0 * 2.0**-power), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("group, n", [(1, 1), (8, 4), (8, 8), (8, 16)])
+def test_scales_whose_product_is_nothing(group, n, dtype):
+    """Scores that vanish altogether: every key that a row sees counts alike, the others not at all."""
+    for mask in (False, True):
+        c = Case([700, n], [n, n], 2 * group, 2, 64, dtype, FP8, mask=mask)
+        c.ks = torch.full((2,), 1e-12, device="cuda")
+        c.check(*c(scale=1e-38, return_lse=True), scale=1e-38)
