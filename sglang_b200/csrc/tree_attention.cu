@@ -319,6 +319,7 @@ template <typename M>
 constexpr float kBelow = std::is_same_v<M, __half> ? 7.f : 0.f;
 template <typename M>
 constexpr float kReach = kBelow<M> + 8.f;
+constexpr float kNothing = -INFINITY;  // in the place of a group's factor for a row of which it has seen nothing
 constexpr float kNoRef = 3e38f;  // of a row that has seen nothing yet, negated like all references: any score exceeds it, and -infinity stays what it is
 
 // Value i of lane l, N <= 32 of them in each of 32 lanes -> lane l has the result over all lanes of value l % N. Each step halves the values that a
@@ -1004,8 +1005,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
           const float ref = fmaxf(ref0, ref1);
           const float f0 = sum0 == 0.f ? 0.f : ptx::ex2(ref0 - ref), f1 = sum1 == 0.f ? 0.f : ptx::ex2(ref1 - ref);
           const float sum = sum0 * f0 + sum1 * f1, by = whole ? (sum == 0.f ? 0.f : v_scale / sum) : 1.f;
-          factor[n] = f0 * by;
-          factor[NT + n] = f1 * by;
+          factor[n] = sum0 == 0.f ? kNothing : f0 * by;
+          factor[NT + n] = sum1 == 0.f ? kNothing : f1 * by;
           out_row[n] = (s.start + token) * a.q_heads + w.h * p.group + at - token * p.group;
           if (n < rows) {
             if (!whole) p.part_ml[slot0 + n] = make_float2(ref, sum);
@@ -1029,10 +1030,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             for (int i = 0; i < 16; i += 4) {
               const float4 f0 = ld_shared_f4(factor + first + i), f1 = ld_shared_f4(factor + NT + first + i);
               const int4 to = *reinterpret_cast<const int4*>(out_row + first + i);
-              // a group that has seen nothing of a row adds nothing, whatever its O holds
+              // a group that has seen nothing of a row adds nothing, whatever its O holds; one whose weights vanish beside the other's still adds a NaN
               auto both = [&](int e, float y0, float y1) {
-                float sum = y0 == 0.f ? 0.f : __uint_as_float(o0[e]) * y0;
-                if constexpr (Cfg::kTwoO) sum += y1 == 0.f ? 0.f : __uint_as_float(o1[e]) * y1;
+                float sum = y0 == kNothing ? 0.f : __uint_as_float(o0[e]) * y0;
+                if constexpr (Cfg::kTwoO) sum += y1 == kNothing ? 0.f : __uint_as_float(o1[e]) * y1;
                 return sum;
               };
               const float x[4] = {both(i, f0.x, f1.x), both(i + 1, f0.y, f1.y), both(i + 2, f0.z, f1.z), both(i + 3, f0.w, f1.w)};
@@ -1166,8 +1167,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT, FP8>::kThreads, 1) tree_attenti
             ptx::tmem_ld_wait16(o1);
             float x[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)  // a group that has seen nothing of the row adds nothing, whatever its O holds
-              x[i] = (f0 == 0.f ? 0.f : __uint_as_float(o0[i]) * f0) + (f1 == 0.f ? 0.f : __uint_as_float(o1[i]) * f1);
+            for (int i = 0; i < 16; ++i)  // a group that has seen nothing of the row adds nothing, whatever its O holds; a NaN of vanishing weight counts
+              x[i] = (sum0 == 0.f ? 0.f : __uint_as_float(o0[i]) * f0) + (sum1 == 0.f ? 0.f : __uint_as_float(o1[i]) * f1);
             if (r < rows) {
               if (whole) {
 #pragma unroll

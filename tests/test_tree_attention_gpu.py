@@ -564,3 +564,26 @@ def test_scales_whose_product_is_nothing(group, n, dtype):
         c = Case([700, n], [n, n], 2 * group, 2, 64, dtype, FP8, mask=mask)
         c.ks = torch.full((2,), 1e-12, device="cuda")
         c.check(*c(scale=1e-38, return_lse=True), scale=1e-38)
+
+
+@pytest.mark.parametrize("held", [None, FP8])
+@pytest.mark.parametrize("group, n", [(1, 1), (8, 4), (8, 8), (8, 16)])
+@pytest.mark.parametrize("sequences", [1, 300])
+def test_a_value_that_is_not_a_number_shows_whatever_its_weight(sequences, group, n, held):
+    """NaN among the values that every row sees, its key 2^230 below another: in the other group's tile, in the other half of a tile, in another piece."""
+    for bad, large in ((5, 130), (5, 70), (70, 5), (130, 5)):
+        c = Case([200 + n] * sequences, [n] * sequences, group, 1, 64, BF, held)
+        c.ks = c.vs = None
+        c.q.zero_()
+        c.q[:, :, 0] = 64
+        c.kc.view(torch.uint8 if held else torch.int16).zero_()
+        c.kc[c.table[:, large // 16].long(), large % 16, 0, 0] = 20.0
+        where = c.table[:, bad // 16].long(), torch.tensor(bad % 16, device="cuda"), torch.tensor(0, device="cuda"), torch.tensor(7, device="cuda")
+        want = c()
+        assert torch.isfinite(want).all()
+        bits = torch.uint8 if held else torch.int16
+        c.vc.view(bits)[where] = 0x7F if held else 0x7FC0
+        out = c()
+        assert torch.isnan(out[..., 7]).all(), (bad, large)
+        others = [d for d in range(64) if d != 7]
+        assert torch.equal(out[..., others], want[..., others])
