@@ -54,6 +54,9 @@ __device__ __forceinline__ float scaled(float x, float s, float r) {
   return fabsf(q) > 0.f ? q : x * r;
 }
 
+// The reciprocal of a scale this small may be infinite: divisor and dividend go up by kLift, exactly, or to an infinity that saturates like the quotient.
+constexpr float kSmallScale = 0x1p-60f, kLift = 0x1p64f;
+
 enum HeadKind { HEAD_Q = 0, HEAD_K = 1, HEAD_V = 2 };
 
 // Two fp32 values in one register pair, and the operations that take both at once: half the instructions of the norm and the rotation.
@@ -248,7 +251,13 @@ __global__ void __launch_bounds__(256, 3) rope_heads_kernel(const __grid_constan
           y[2 * i] = e.x, y[2 * i + 1] = e.y;
         }
         if (scales) {
-          const float d = ld_operand(scales + (one_scale ? 0 : h)), r = __frcp_rn(d);
+          float d = ld_operand(scales + (one_scale ? 0 : h));
+          if (fabsf(d) < kSmallScale) {
+            d *= kLift;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] *= kLift;
+          }
+          const float r = __frcp_rn(d);
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] = scaled(y[i], d, r);
         }
@@ -319,10 +328,12 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ R
   const bool cached = a.k_cache != nullptr && kind != HEAD_Q;
   if (cached && !slot_at(p, row, at)) return;
   const int64_t to = kind == HEAD_K ? at.k + g * a.k_cache_head : at.v + g * a.v_cache_head;
-  float d = 1.f, rd = 1.f;
+  float d = 1.f, rd = 1.f, lift = 1.f;
   const float* scales = !cached ? nullptr : kind == HEAD_K ? a.k_scale : a.v_scale;
   if (scales) {
     d = ld_operand(scales + ((kind == HEAD_K ? a.k_scales : a.v_scales) > 1 ? g : 0));
+    if (fabsf(d) < kSmallScale) lift = kLift;
+    d *= lift;
     rd = __frcp_rn(d);
   }
   auto normed = [&](int i) {
@@ -347,7 +358,7 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ R
       (static_cast<T*>(kind == HEAD_K ? a.k_cache : a.v_cache) + to)[i] = from_f32<T>(f);
     } else {
       (static_cast<uint8_t*>(kind == HEAD_K ? a.k_cache : a.v_cache) + to)[i] =
-          (uint8_t)__nv_cvt_float_to_fp8(scales ? scaled(f, d, rd) : f, __NV_SATFINITE, __NV_E4M3);
+          (uint8_t)__nv_cvt_float_to_fp8(scales ? scaled(f * lift, d, rd) : f, __NV_SATFINITE, __NV_E4M3);
     }
   }
 }

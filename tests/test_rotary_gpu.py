@@ -299,3 +299,20 @@ def test_tokens_behind_a_kernel_that_still_writes_them():
         z[:, 8 * 128 : 10 * 128] = k.flatten(1)
         torch.cuda.synchronize()
     assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("scale", [2.0**-60, 1.3e-19, 2.0**-126, 1.9e-38, 2.0**-129, 3e-39, 2.0**-140, 2.0**-149, 1.7e38])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_fp8_codes_of_any_scale(dtype, scale):
+    """Scales whose reciprocal is infinite or not a normal number, values from the smallest to the largest: the codes of the IEEE quotient."""
+    x = torch.arange(0x7F80, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = torch.cat([x, -x]).view(-1, 1, 128).to(dtype)
+    s = torch.tensor([scale], device="cuda")
+    assert s.item() > 0
+    # (the quotient in 64 bits, rounded to 32: PyTorch's own 32-bit division may flush what is not normal)
+    want = (x.double() / s.double()).float().clamp(-448, 448).to(FP8)
+    for pad in (0, 1):  # whole vectors, and elements one by one
+        kc, vc = (torch.zeros(x.shape[0], 1, 1, 128 + pad, device="cuda").to(FP8)[..., pad:] for _ in range(2))
+        S.append_paged_kv(x, x, kc, vc, torch.arange(x.shape[0], device="cuda"), k_scale=s, v_scale=s)
+        for c in (kc, vc):
+            assert torch.equal(bits(c[:, 0].contiguous()), bits(want))
