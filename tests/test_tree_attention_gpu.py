@@ -587,3 +587,29 @@ def test_a_value_that_is_not_a_number_shows_whatever_its_weight(sequences, group
         assert torch.isnan(out[..., 7]).all(), (bad, large)
         others = [d for d in range(64) if d != 7]
         assert torch.equal(out[..., others], want[..., others])
+
+
+@pytest.mark.parametrize("dtype, held", [(BF, FP8), (HF, FP8), (HF, None), (BF, None)])
+@pytest.mark.parametrize("dim, group, n", [(64, 1, 1), (128, 8, 1), (128, 8, 4), (64, 8, 8), (128, 8, 16), (256, 4, 8)])
+def test_one_large_key_in_front_of_a_long_flat_context(dim, group, n, dtype, held):
+    """As above, in so many sequences (over the same pages) that all keys of one are taken against the same reference: cut over many CTAs, only the piece
+    with the large key would lose its others."""
+    L, B = 131072, 300
+    c = Case([L], [n], group, 1, dim, dtype, held, 64)
+    c.q = (torch.zeros_like(c.q) + torch.eye(1, dim, dtype=dtype, device="cuda") * dim**0.5).repeat(B, 1, 1)
+    score = float(c.q[0, 0, 0]) * 18 * dim**-0.5
+    c.kc.view(torch.uint8 if held else torch.int16).zero_()
+    v = torch.tensor([1.0, -2.0, 0.5, 0.0], device="cuda").repeat(dim // 4)
+    c.vc.copy_(v.to(c.held).expand(c.vc.shape))
+    page = int(c.table[0, 0])
+    c.kc[page, 3, 0, 0] = 18.0
+    c.vc[page, 3] = torch.zeros(dim, device="cuda").to(c.held)
+    c.table, c.seq_lens = c.table.repeat(B, 1), c.seq_lens.repeat(B)
+    c.starts = torch.arange(B + 1, dtype=torch.int32, device="cuda") * n
+    c.ks = c.vs = None
+    out = c().view(B, n, group, dim).double()
+    half, weight = torch.finfo(dtype).eps / 2, math.exp(-score)
+    others = (L - n + torch.arange(n, device="cuda", dtype=torch.float64)).view(1, n, 1, 1)
+    want = others * weight / (1 + others * weight) * v.double()
+    bound = (3 * half + 2.0**-15) * want.abs() + L * 2.0**-32 * v.double().abs()
+    assert ((out - want).abs() <= bound).all(), (out[0, 0, 0, :4], want[0, 0, 0, :4])
