@@ -11,7 +11,7 @@ import torch
 
 from . import _native as N
 from .int8_kernel import same_device
-from .rotary import E4M3, check_caches, check_scale, fp8_dtype
+from .rotary import E4M3, check_caches, check_scale, check_sizes, fp8_dtype
 
 
 class TreeAttentionArgs(ctypes.Structure):
@@ -67,6 +67,7 @@ def tree_attention(
     assert heads > 0 and dim > 0 and q.stride(2) == 1, "elements of a head are contiguous"
     assert k_cache.dim() == 4 and k_cache.shape[2] > 0 and heads % k_cache.shape[2] == 0, "heads are a multiple of the cache's kv heads"
     kv_heads = k_cache.shape[2]
+    check_sizes(heads, dim, 0 if tree_mask is None else tree_mask.shape[-1])
     check_caches(k_cache, v_cache, kv_heads, dim)
     assert k_cache.dtype in (q.dtype, fp8_dtype), "the caches have q's type, or float8_e4m3fn"
     assert k_cache.shape[1] > 0, "pages without tokens"

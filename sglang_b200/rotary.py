@@ -35,6 +35,12 @@ class RopeArgs(ctypes.Structure):
     )
 
 
+def check_sizes(*sizes: int) -> None:
+    """Sizes that the C ABI holds in 32 bits: ctypes would take the low ones of a larger number."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise NotImplementedError("heads, head sizes, page sizes and mask widths from 2^31 on are not built")
+
+
 def check_index(t: torch.Tensor, what: str) -> None:
     assert t.dtype in (torch.int32, torch.int64), f"{what} are int32 or int64"
 
@@ -75,6 +81,7 @@ def check_caches(k_cache, v_cache, kv_heads, dim):
         assert t.dim() == 4 and t.shape[2:] == (kv_heads, dim), f"a cache is [pages, page size, {kv_heads}, {dim}]"
         assert t.stride(3) == 1 or dim <= 1, "elements of a head are contiguous in the cache"
     assert k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype, "the caches differ"
+    check_sizes(k_cache.shape[1])
 
 
 def check_scale(scale, kv_heads, cache_dtype, what):
@@ -113,6 +120,7 @@ def _qkv_args(qkv, num_heads, num_kv_heads, q_weight, k_weight, eps) -> RopeArgs
     heads = num_heads + 2 * num_kv_heads
     assert qkv.dim() == 2 and qkv.shape[1] % heads == 0 and qkv.shape[1] > 0, f"qkv is [tokens, {heads} * dim]"
     assert qkv.stride(1) == 1, "rows of qkv are contiguous"
+    check_sizes(num_heads, num_kv_heads, qkv.shape[1] // heads)
     a = RopeArgs(rows=qkv.shape[0], q_heads=num_heads, kv_heads=num_kv_heads, dim=qkv.shape[1] // heads, dtype=N.DTYPE_CODE[qkv.dtype], eps=eps)
     for w in (q_weight, k_weight):
         assert w is None or (w.shape == (a.dim,) and w.dtype == qkv.dtype and w.is_contiguous()), "norm weights are [dim], of qkv's type"
@@ -234,6 +242,7 @@ def append_paged_kv(
     assert k.dim() == 3 and v.shape == k.shape and v.dtype == k.dtype, "k and v are [tokens, kv heads, dim], alike"
     rows, heads, dim = k.shape
     assert dim > 0 and heads > 0, "heads without elements"
+    check_sizes(heads, dim)
     assert dim <= 1 or (k.stride(2) == 1 and v.stride(2) == 1), "elements of a head are contiguous"
     a = RopeArgs(rows=rows, kv_heads=heads, dim=dim, dtype=N.DTYPE_CODE[k.dtype])
     _set_rotation(a, dim, positions, cos_sin_cache, is_neox, mrope_section, mrope_interleaved)

@@ -128,3 +128,23 @@ def test_fake_implementations_describe_the_shapes():
         assert ops.qk_norm_rope_append(x, 8, 2, None, None, cache, cache.clone(), index).shape == (5, 8, 64)
         assert ops.append_paged_kv(k, k, cache, cache.clone(), index) is None
         assert ops.tree_attention(q, cache, cache, torch.empty(5, 3, dtype=torch.int32, device="cuda"), index).shape == q.shape
+
+
+FAR = (1 << 32) + 16  # 16 in 32 bits
+
+
+def test_sizes_past_32_bits_are_not_taken_for_their_low_bits():
+    a = good()
+    for n in ("k_cache", "v_cache"):
+        a[n] = torch.zeros(1, 1, 2, 64, dtype=BF).expand(4, FAR, 2, 64)
+    with pytest.raises(NotImplementedError):
+        S.qk_norm_rope_append(**a)
+    with pytest.raises(NotImplementedError):
+        S.append_paged_kv(torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF), a["k_cache"], a["v_cache"], torch.arange(3))
+    meta = dict(dtype=BF, device="meta")
+    for heads, kv, dim in ((FAR, 2, 1), (8, FAR, 1), (8, 2, FAR)):
+        with pytest.raises(NotImplementedError):
+            S.qk_norm_rope(torch.empty(3, (heads + 2 * kv) * dim, **meta), heads, kv, None, None)
+    k = torch.empty(3, FAR, 1, **meta)
+    with pytest.raises(NotImplementedError):
+        S.append_paged_kv(k, k, k, k, torch.arange(3))

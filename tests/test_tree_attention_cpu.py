@@ -96,3 +96,13 @@ def test_workspace():
         big = size(tokens=100000, sequences=1000, max_pages=10000, pages=10000, **f)
         assert big == size(tokens=200000, sequences=2000, max_pages=20000, pages=10000, **f)
         assert 2 * 148 * rows * (128 + 2) * 4 <= big < 2 * 148 * rows * (128 + 2) * 4 + 16384
+
+
+def test_sizes_past_32_bits_are_not_taken_for_their_low_bits():
+    far, meta = (1 << 32) + 64, dict(dtype=BF, device="meta")
+    cache = torch.zeros(1, 1, 2, 128, dtype=BF).expand(4, far, 2, 128)
+    for bad in (dict(k_cache=cache, v_cache=cache), dict(tree_mask=torch.empty(5, far, dtype=torch.bool, device="meta")),
+                dict(q=torch.empty(5, 8, far, **meta), k_cache=torch.empty(4, 16, 2, far, **meta), v_cache=torch.empty(4, 16, 2, far, **meta)),
+                dict(q=torch.empty(5, far, 128, **meta))):
+        with pytest.raises(NotImplementedError):
+            S.tree_attention(**{**good(), **bad})
