@@ -5,17 +5,17 @@
 //   S^T [128 keys, NT] = K Q^T     K and Q in shared memory, S^T in TMEM, two buffers
 //   O^T [D, NT]       += V^T P^T   V as it lies in the cache (its rows are the product's depth), P^T [keys, NT] in shared memory
 // A thread of the softmax has one key and the rows' columns. It takes its exponentials against a reference per row that is moved only when a score
-// lies 2^8 above the one it was taken from, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the end. With more than
-// 64 rows the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: a softmax row is a thread's own,
-// and P needs no shared memory.
+// lies 2^8 above the one it was taken from, so a tile needs one vote of the threads and no maxima over keys; sums over keys stay in registers until the
+// end. With more than 64 rows the rows fill the lanes and the keys are the columns, S [128, keys] and O [128, D], P in TMEM over its own S: a softmax row
+// is a thread's own, and P needs no shared memory.
 // Keys come by their pages' addresses, any page size, in 16-byte pieces by asynchronous copies; codes of an FP8 cache land in a ring of their own and
 // become fp16 values, exactly, on their way into the ring of tiles. All tiles of all (sequence, kv head, row tile) form one line that is cut into equal
 // pieces, one per CTA, so that ragged lengths leave no SM idle; rows whose keys were cut leave partial sums in a workspace, which a second kernel joins in
 // the line's order.
-// Few rows over a 16-bit cache are bound by its bytes: 128 sequences of up to 8192 tokens, 8 kv heads of 128, one token a page, 2.17 GB: 330 us, 6.6 TB/s; 16 of up
-// to 16384 with 8 drafted tokens, 64 query heads (64 rows), 597 MB: 127 us, 4.7 TB/s. An FP8 cache is bound by the way of its codes through the SM, copied,
-// read, widened and stored: 64 sequences of up to 16384, one token, 1.08 GB: 240 us, 4.5 TB/s. 128 rows by the exponentials, 16 a clock and SM, and by the latency of
-// the steps between two products: 61 sequences of up to 32768, 16 tokens, FP8, 264 MB: 117 us, 535 TFLOP/s.
+// Few rows over a 16-bit cache are bound by its bytes: 128 sequences of up to 8192 tokens, 8 kv heads of 128, one token a page, 2.17 GB: 333 us, 6.5 TB/s; 16 of up
+// to 16384 with 8 drafted tokens, 64 query heads (64 rows), 597 MB: 127 to 131 us, 4.6 TB/s. An FP8 cache is bound by the way of its codes through the SM, copied,
+// read, widened and stored: 64 sequences of up to 16384, one token, 1.08 GB: 238 to 242 us, 4.5 TB/s. 128 rows by the exponentials, 16 a clock and SM, and by the
+// latency of the steps between two products: 61 sequences of up to 32768, 16 tokens, FP8, 264 MB: 113 to 119 us, 540 TFLOP/s.
 #include <cfloat>
 
 #include "gemm_host.cuh"
