@@ -613,3 +613,30 @@ def test_one_large_key_in_front_of_a_long_flat_context(dim, group, n, dtype, hel
     want = others * weight / (1 + others * weight) * v.double()
     bound = (3 * half + 2.0**-15) * want.abs() + L * 2.0**-32 * v.double().abs()
     assert ((out - want).abs() <= bound).all(), (out[0, 0, 0, :4], want[0, 0, 0, :4])
+
+
+@pytest.mark.parametrize("held", [None, FP8])
+@pytest.mark.parametrize("group, n", [(4, 1), (8, 16)])
+def test_the_longest_line_of_a_page_table(group, n, held):
+    """2^31 - 256 keys, the most that a line may name: one page again and again, so the result is that page's. fp32 sums of up to 2^17 tiles a CTA may be off by
+    2^17 half steps, the weights' and the values' both."""
+    c = Case([256], [n], group, 1, 64, BF, held, 256)
+    page = c.table[:, :1].clone()
+    k, v = c.keys(0)
+    s = torch.einsum("thd,kd->thk", c.q.double(), k[:, 0]) * 64**-0.5
+    want = torch.softmax(s, -1) @ v[:, 0]
+    c.table, c.seq_lens = page.repeat(1, 0x7FFFFF00 // 256), torch.full_like(c.seq_lens, 2**31 - 1)
+    out, lse = c(return_lse=True)
+    size = torch.softmax(s, -1) @ v[:, 0].abs()
+    assert ((out.double() - want).abs() <= 2.0**-9 * want.abs() + (2 * 2.0**-7 + 2.0**-8 + 2.0**-12) * size).all()
+    assert ((lse.double() - (torch.logsumexp(s, -1) + math.log(0x7FFFFF00 / 256))).abs() <= 2.0**-7 + 2.0**-12).all()
+
+
+def test_nothing_to_attend_to():
+    c = Case([100], [2], 4, 2, 64)
+    assert S.tree_attention(c.q[:0], c.kc, c.vc, c.table, c.seq_lens, torch.zeros_like(c.starts)).shape == (0, 4, 64)
+    out = torch.full_like(c.q, 3)
+    got = S.tree_attention(c.q, c.kc, c.vc, c.table[:0], c.seq_lens[:0], c.starts[:1], out=out)
+    assert got is out and (out == 3).all()
+    got = S.tree_attention(c.q, c.kc, c.vc, c.table[:, :0], c.seq_lens, c.starts)  # no page at all
+    assert (got == 0).all()
